@@ -196,6 +196,37 @@ int ka_sample_ex(int dtype, const void *logits, int64_t batch, int64_t vocab, in
 int ka_sample_mass_fixed(const float *d, int64_t n, uint64_t *out, void *hip_stream);
 
 /*
+ * Verification of drafted tokens (speculative sampling).  target_logits [batch, max_draft + 1, vocab] scores the drafted
+ * positions and the one behind them, draft_logits [batch, max_draft, vocab] (same dtype, a KA_DTYPE_* code) are the logits the
+ * drafts were drawn from; null: drafts without probabilities, Q one-hot at the draft.  Strides are in elements; rows have
+ * unit stride along the vocabulary.  draft_ids [batch, max_draft]; draft_lens [batch] (null: max_draft for all; clamped to
+ * [0, max_draft]): rows and ids behind a request's drafts are not read.
+ * Both rows of a position go through temperature -> top-k -> top-p as in ka_sample_ex (scalars, or one value per request in
+ * the *_rows arrays), giving integer masses W and totals Z: P = W^p / Z^p, Q = W^q / Z^q.
+ *   position j accepts its draft d  iff  uniforms[b, j] * Q(d) < P(d)   (an id outside [0, vocab) has P = 0)
+ *   n = the first position that does not, or the number of drafts
+ *   out_ids[b, 0 .. n) = the drafts; out_ids[b, n] = first i, in index order, whose inclusive sum of R exceeds
+ *       floor(uniforms[b, max_draft] * sum R), R_i = max(P_i - Q_i, 0) if position n rejected, P_i if all were accepted
+ *       (or if sum R is 0, which takes P = Q and a draft with Q(d) = 0)
+ *   out_ids[b, n + 1 ..] = -1; out_accepted[b] = n
+ * decided exactly, on integers of up to 126 bits.  uniforms: fp32 [batch, max_draft + 1] in [0, 1).
+ * out_policy_logprob (optional, fp32 [batch, max_draft + 1]): log-probability of every emitted token under the unfiltered
+ * softmax of its target row (to 1e-5 what ka_logprob_* returns), 0 behind the last.
+ * Limits: max_draft <= KA_VERIFY_MAX_DRAFT, vocab < 2^22, batch <= 65535.  The workspace is 16-byte aligned, of
+ * ka_verify_workspace_bytes (0 for arguments the call refuses): 40 bytes per row and 16 per request and share of 1024
+ * 16-byte vectors.  Any alignment of the rows is taken.  No counterpart in the reference, whose sampler draws one token per
+ * forward pass (rl_engine/kernels/sampling.py:39-88).
+ */
+#define KA_VERIFY_MAX_DRAFT 64
+size_t ka_verify_workspace_bytes(int dtype, int64_t batch, int64_t max_draft, int64_t vocab);
+int ka_verify_draft(int dtype, const void *target_logits, int64_t target_batch_stride, int64_t target_pos_stride,
+                    const void *draft_logits, int64_t draft_batch_stride, int64_t draft_pos_stride, const int64_t *draft_ids,
+                    const int64_t *draft_lens, const float *uniforms, int64_t batch, int64_t max_draft, int64_t vocab,
+                    float temperature, const float *temperature_rows, int32_t top_k, const int32_t *top_k_rows, float top_p,
+                    const float *top_p_rows, int64_t *out_ids, int64_t *out_accepted, float *out_policy_logprob,
+                    void *workspace, size_t workspace_bytes, void *hip_stream);
+
+/*
  * Fused lm_head -> logprob without materialised logits:
  *     out[r] = h_r . W[ids[r]] - logsumexp_v(h_r . W[v])               (fp32)
  * hidden: bf16 [n_rows, hidden_dim] row-major; weight: bf16 [vocab, hidden_dim]

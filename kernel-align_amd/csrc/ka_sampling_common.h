@@ -320,17 +320,20 @@ constexpr int LSE_PER_THREAD = LSE_LANES / S_THREADS;
 struct PolicyLse {  // in LDS
     float wave_ml2[LSE_WAVES];  // maximum * log2(e) of the elements of each wavefront of the 1024-lane order
     float wave_s[LSE_WAVES];    // sum of 2^(x * log2(e) - wave_ml2)
-    // log-probability of element `hit` of the row (thread 0, after a barrier behind to_block)
-    template <typename T> __device__ __forceinline__ float finish(const typename T::raw_t *rp, int64_t hit, int vocab) const {
-        if (hit < 0 || hit >= vocab) return __builtin_nanf("");
+    // the log-sum-exp (after a barrier behind to_block)
+    __device__ __forceinline__ double value() const {
         float big = wave_ml2[0];
 #pragma unroll
         for (int w = 1; w < LSE_WAVES; ++w) big = fmaxf(big, wave_ml2[w]);
         float total = 0.0f;
 #pragma unroll
         for (int w = 0; w < LSE_WAVES; ++w) total += wave_s[w] * fast_exp2(wave_ml2[w] - big);
-        const double lse = (double(big) + log2(double(total))) * 0.693147180559945309417232;
-        return float(double(T::widen(rp[hit])) - lse);
+        return (double(big) + log2(double(total))) * 0.693147180559945309417232;
+    }
+    // log-probability of element `hit` of the row (thread 0, after a barrier behind to_block)
+    template <typename T> __device__ __forceinline__ float finish(const typename T::raw_t *rp, int64_t hit, int vocab) const {
+        if (hit < 0 || hit >= vocab) return __builtin_nanf("");
+        return float(double(T::widen(rp[hit])) - value());
     }
 };
 

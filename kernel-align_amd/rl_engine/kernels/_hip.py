@@ -52,6 +52,10 @@ SIGNATURES = {
     "ka_sample_ex": (c_int, [c_int, c_void_p, c_int64, c_int64, c_int64, c_float, c_void_p, c_int32, c_void_p, c_float,
                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_size_t, c_void_p]),
     "ka_sample_mass_fixed": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
+    "ka_verify_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64]),
+    "ka_verify_draft": (c_int, [c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                c_int64, c_int64, c_int64, c_float, c_void_p, c_int32, c_void_p, c_float, c_void_p,
+                                c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "ka_lmhead_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
     "ka_lmhead_logprob_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                        c_void_p, c_size_t, c_void_p]),

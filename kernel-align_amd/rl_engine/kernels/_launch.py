@@ -1,0 +1,37 @@
+"""What every operator does around a launch: the device check, the device guard and the stream lookup."""
+from __future__ import annotations
+
+import torch
+
+
+def _require_gpu(t: torch.Tensor, name: str) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on the GPU: rl_engine has no CPU path (got {t.device})")
+
+
+class _NoGuard:
+    """Stands in for torch.cuda.device(...) when the tensor's device is the current one already."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+def _on_device(device):
+    """A context manager that makes `device` current for the launch.  Entering torch.cuda.device() and asking
+    torch.cuda.current_stream() cost more host time than a small kernel runs, so the common case (the tensor lives
+    on the current device) takes neither."""
+    index = device.index
+    if index is None or index == torch._C._cuda_getDevice():
+        return _NO_GUARD
+    return torch.cuda.device(index)
+
+
+def _raw_stream() -> int:
+    """Handle of the current HIP stream of the current device (what torch.cuda.current_stream().cuda_stream returns)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())

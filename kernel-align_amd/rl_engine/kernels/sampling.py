@@ -14,7 +14,9 @@ import torch
 import torch.nn as nn
 
 from rl_engine.kernels import _hip
+from rl_engine.kernels._launch import _on_device, _raw_stream, _require_gpu
 from rl_engine.kernels.pool import PoolExhausted, WorkspacePool
+from rl_engine.kernels.speculative import SpeculativeOps
 from rl_engine.platforms.constants import constants
 from rl_engine.utils.logger import logger
 
@@ -38,39 +40,6 @@ _SAMPLE_FN = {torch.bfloat16: "ka_sample_topk_topp_bf16", torch.float16: "ka_sam
               torch.float32: "ka_sample_topk_topp_f32"}
 
 
-def _require_gpu(t: torch.Tensor, name: str) -> None:
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must live on the GPU: rl_engine has no CPU path (got {t.device})")
-
-
-class _NoGuard:
-    """Stands in for torch.cuda.device(...) when the tensor's device is the current one already."""
-
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NO_GUARD = _NoGuard()
-
-
-def _on_device(device):
-    """A context manager that makes `device` current for the launch.  Entering torch.cuda.device() and asking
-    torch.cuda.current_stream() cost more host time than a small kernel runs, so the common case (the tensor lives
-    on the current device) takes neither."""
-    index = device.index
-    if index is None or index == torch._C._cuda_getDevice():
-        return _NO_GUARD
-    return torch.cuda.device(index)
-
-
-def _raw_stream() -> int:
-    """Handle of the current HIP stream of the current device (what torch.cuda.current_stream().cuda_stream returns)."""
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
-
-
 def _chunk_rows(chunk_tokens, default=None) -> int:
     """Rows per launch of a chunked operator; anything below one row would make the launch loop empty."""
     chunk = (DEFAULT_CHUNK_TOKENS if default is None else default) if chunk_tokens is None else int(chunk_tokens)
@@ -90,7 +59,7 @@ def _rows_view(logits: torch.Tensor) -> torch.Tensor:
     return logits.contiguous().view(-1, vocab)
 
 
-class SamplerBackend(nn.Module):
+class SamplerBackend(SpeculativeOps, nn.Module):
     def __init__(self, pool_bytes: int | None = None):
         super().__init__()
         self.backend = self._detect_backend()

@@ -162,3 +162,29 @@ def test_missing_library_fails_loudly(monkeypatch, tmp_path):
 
     with pytest.raises(_hip.HipLibraryError):
         SamplerBackend()
+
+
+def test_verify_argument_checks_and_workspace_size():
+    lib = _hip.load()
+    p = ctypes.c_void_p(4096)
+    ws = lib.ka_verify_workspace_bytes
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    assert ws(0, 64, 4, 128256) == up(64 * 9 * 40) + up(64 * 8) + 64 * 16 * 16
+    assert ws(2, 3, 0, 4097) == up(3 * 40) + up(24) + 3 * 2 * 16
+    assert ws(0, 0, 4, 128256) == 0 and ws(0, 4, 65, 100) == 0 and ws(0, 4, 4, 1 << 22) == 0
+
+    def call(dtype=0, target=p, tb=500, tp=100, draft=p, db=400, dp=100, ids=p, lens=None, u=p, batch=2, k=4, vocab=100,
+             t=1.0, top_k=0, top_p=1.0, out=p, acc=p, ws_ptr=p, ws_bytes=1 << 20):
+        return lib.ka_verify_draft(dtype, target, tb, tp, draft, db, dp, ids, lens, u, batch, k, vocab, t, None, top_k, None,
+                                   top_p, None, out, acc, None, ws_ptr, ws_bytes, None)
+
+    assert call(batch=0, target=None) == _hip.KA_OK
+    assert call(dtype=3) == _hip.KA_ERR_BAD_ARG
+    for bad in (dict(target=None), dict(ids=None), dict(u=None), dict(out=None), dict(acc=None), dict(batch=-1), dict(k=-1),
+                dict(vocab=0), dict(t=0.0), dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.5), dict(tp=99), dict(tb=99),
+                dict(dp=99), dict(db=99), dict(ws_ptr=ctypes.c_void_p(4104)), dict(target=ctypes.c_void_p(4097))):
+        assert call(**bad) == _hip.KA_ERR_BAD_ARG, bad
+    for far in (dict(k=65), dict(vocab=1 << 22, tb=1 << 30, tp=1 << 23, db=1 << 30, dp=1 << 23), dict(batch=65536)):
+        assert call(**far) == _hip.KA_ERR_UNSUPPORTED, far
+    assert call(ws_bytes=ws(0, 2, 4, 100) - 1) == _hip.KA_ERR_WORKSPACE
+    assert call(ws_ptr=None) == _hip.KA_ERR_WORKSPACE and b"workspace" in lib.ka_last_error()
