@@ -227,6 +227,43 @@ int ka_verify_draft(int dtype, const void *target_logits, int64_t target_batch_s
                     void *workspace, size_t workspace_bytes, void *hip_stream);
 
 /*
+ * Low-rank adapters of many requests beside a shared projection:
+ *     u[n, :]   = s_a * hidden[n, :] . lora_a[a]^T          a = adapter_ids[n], s_a = scaling[a] (null: `scale` for all)
+ *     out[n, :] = base[n, :] + u[n, :] . lora_b[a]^T        rounded once; an id outside [0, n_adapters): out = base
+ * dtype is KA_DTYPE_BF16 or KA_DTYPE_F16, of base [n_tokens, out_dim] (the shared projection's output), hidden
+ * [n_tokens, in_dim], lora_a [n_adapters, rank, in_dim], lora_b [n_adapters, out_dim, rank] and out; row strides in
+ * elements, the adapters contiguous.  out may be base.  out_shrunk (optional, fp32 [n_tokens, rank]) receives u (0 without an
+ * adapter), which the backward takes; with out null it is all that is computed, and base and lora_b are not read.
+ * Accumulation and u are fp32; a token's results do not depend on the other tokens, bit for bit.
+ *
+ * ka_lora_linear_backward, with du[n, :] = s_a * grad_out[n, :] . lora_b[a]:
+ *     dhidden[n, :] = dhidden_base[n, :] + du[n, :] . lora_a[a]      (dhidden_base, the shared projection's own gradient, may
+ *                                                                     be null: 0, or dhidden itself)
+ *     dlora_a[a]    = sum over the adapter's tokens of du[n, :]^T hidden[n, :]          fp32 [n_adapters, rank, in_dim]
+ *     dlora_b[a]    = sum over the adapter's tokens of grad_out[n, :]^T u[n, :]         fp32 [n_adapters, out_dim, rank]
+ * Sums run in a fixed order (a function of the shapes and the ids); an adapter without tokens gets zeros.
+ *
+ * Any alignment and any rank, width and token count up to the limits; multiples of eight on 16-byte aligned rows take
+ * 16-byte accesses.  The workspace is 16-byte aligned, of ka_lora_workspace_bytes (0 for arguments the calls refuse).  No
+ * counterpart in the reference, which names no adapters.
+ */
+#define KA_LORA_MAX_RANK 128
+#define KA_LORA_MAX_ADAPTERS 1023
+#define KA_LORA_MAX_TOKENS (1 << 21)
+size_t ka_lora_workspace_bytes(int64_t n_tokens, int64_t in_dim, int64_t out_dim, int64_t rank, int64_t n_adapters,
+                               int backward);
+int ka_lora_linear(int dtype, const void *base, int64_t base_stride, const void *hidden, int64_t hidden_stride,
+                   const void *lora_a, const void *lora_b, const int64_t *adapter_ids, const float *scaling, float scale,
+                   void *out, int64_t out_stride, float *out_shrunk, int64_t n_tokens, int64_t in_dim, int64_t out_dim,
+                   int64_t rank, int64_t n_adapters, void *workspace, size_t workspace_bytes, void *hip_stream);
+int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t grad_stride, const void *hidden, int64_t hidden_stride,
+                            const void *lora_a, const void *lora_b, const int64_t *adapter_ids, const float *scaling,
+                            float scale, const float *shrunk, const void *dhidden_base, int64_t dhidden_base_stride,
+                            void *dhidden, int64_t dhidden_stride, float *dlora_a, float *dlora_b, int64_t n_tokens,
+                            int64_t in_dim, int64_t out_dim, int64_t rank, int64_t n_adapters, void *workspace,
+                            size_t workspace_bytes, void *hip_stream);
+
+/*
  * Fused lm_head -> logprob without materialised logits:
  *     out[r] = h_r . W[ids[r]] - logsumexp_v(h_r . W[v])               (fp32)
  * hidden: bf16 [n_rows, hidden_dim] row-major; weight: bf16 [vocab, hidden_dim]

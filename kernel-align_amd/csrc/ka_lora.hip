@@ -1,0 +1,1026 @@
+// Low-rank adapters of many requests beside a shared projection, forward and backward.
+//
+//   forward    u_n = s_a x_n A_a^T           y_n = base_n + u_n B_a^T             a = adapter_ids[n], none: y_n = base_n
+//   backward   du_n = s_a dy_n B_a           dx_n = dx_base_n + du_n A_a
+//              dA_a = sum_n du_n^T x_n       dB_a = sum_n dy_n^T u_n              over the tokens n of adapter a, in order
+//
+// x [N, H], base / y / dy [N, O], A [S, R, H], B [S, O, R], R <= 128.  The tokens are sorted by adapter on the device (a stable
+// counting sort, lora_plan) and worked on in tiles of one adapter each, so that every product is a small dense one on the
+// matrix cores (v_mfma_f32_16x16x32).  All of it is bound by memory: per token 2 H bytes in and 4 O bytes through for
+// 2 R (H + O) flop, 16 flop per byte at R = 16, against about 300 that the matrix cores could do.
+//
+// Numbers.  Products of two 16-bit matrices (x A^T, dy B) run in their own type with fp32 accumulation.  u and du are fp32 and
+// stay so: an operand of a product with them is split into bf16 parts, high + low (17 bits: for results that are rounded
+// to 16 bits) or high + middle + low (24 bits: for the fp32 gradients); an fp16 operand next to them is split into two bf16 (11 bits, exact).
+// Every sum runs in a fixed order: no atomics on floating-point values.
+#include <type_traits>
+
+#include "ka_common.h"
+
+namespace ka {
+namespace {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int MAX_RANK = KA_LORA_MAX_RANK;
+constexpr int MAX_ADAPTERS = KA_LORA_MAX_ADAPTERS;
+constexpr int THREADS = 256;
+constexpr int WAVES = THREADS / kWave;
+constexpr int FWD_TILE = 64;    // tokens per tile of the forward: four groups of sixteen
+constexpr int BWD_TILE_MAX = 1024;  // ... of the backward at most (a multiple of 32)
+
+struct LoraTile {
+    int32_t adapter;       // -1: tokens without one
+    int32_t start, count;  // in `order`
+    int32_t slot;          // backward: -1 writes the adapter's gradient, others this partial one
+};
+struct LoraPlan {          // device pointers into the workspace
+    int32_t *head;         // [0] = number of tiles
+    int32_t *order;        // [N] tokens sorted by adapter, those without one last
+    LoraTile *tiles;
+    int32_t *per_adapter;  // [2 S]: tiles of the adapter, its first partial slot
+    int32_t max_tiles;
+};
+
+// ---------------------------------------------------------------------------
+// lora_plan: one workgroup sorts the tokens.  Every wavefront takes a contiguous share of them: counts, a prefix over
+// (adapter, wavefront), then the ranks inside a step of 64 tokens from ballots.
+// ---------------------------------------------------------------------------
+constexpr int PLAN_THREADS = 512;
+constexpr int PLAN_WAVES = PLAN_THREADS / kWave;
+
+__global__ __launch_bounds__(PLAN_THREADS) void lora_plan(const int64_t *__restrict__ ids, int n, int s, int tile, LoraPlan plan) {
+    __shared__ int32_t at[PLAN_WAVES][MAX_ADAPTERS + 1];  // counts, then the next position of the wavefront's tokens
+    __shared__ int32_t wave_sum[PLAN_WAVES][3];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    for (int i = tid; i < PLAN_WAVES * (MAX_ADAPTERS + 1); i += PLAN_THREADS) (&at[0][0])[i] = 0;
+    __syncthreads();
+    const int steps = (n + kWave - 1) / kWave, per = (steps + PLAN_WAVES - 1) / PLAN_WAVES;
+    const int s0 = wave * per, s1 = s0 + per < steps ? s0 + per : steps;
+    auto adapter_of = [&](int i) {
+        const int64_t a = ids[i];
+        return a >= 0 && a < s ? int(a) : s;
+    };
+    for (int st = s0; st < s1; ++st) {
+        const int i = st * kWave + lane;
+        if (i < n) atomicAdd(&at[wave][adapter_of(i)], 1);
+    }
+    __syncthreads();
+    // thread t owns the adapters t * own .. : tokens, tiles and partial slots before its first
+    const int own = (s + 1 + PLAN_THREADS - 1) / PLAN_THREADS;
+    int mine[3] = {0, 0, 0};
+    for (int j = 0; j < own; ++j) {
+        const int a = tid * own + j;
+        if (a > s) break;
+        int c = 0;
+        for (int w = 0; w < PLAN_WAVES; ++w) c += at[w][a];
+        const int t = (c + tile - 1) / tile;
+        mine[0] += c;
+        mine[1] += t;
+        if (a < s && t > 1) mine[2] += t - 1;
+    }
+    int before[3];
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        int inc = mine[q];
+#pragma unroll
+        for (int off = 1; off < kWave; off <<= 1) {
+            const int o = __shfl_up(inc, off, kWave);
+            if (lane >= off) inc += o;
+        }
+        if (lane == kWave - 1) wave_sum[wave][q] = inc;
+        before[q] = inc - mine[q];
+    }
+    __syncthreads();
+    int total_tiles = 0;
+    for (int w = 0; w < PLAN_WAVES; ++w) {
+        if (w < wave) {
+#pragma unroll
+            for (int q = 0; q < 3; ++q) before[q] += wave_sum[w][q];
+        }
+        total_tiles += wave_sum[w][1];
+    }
+    for (int j = 0; j < own; ++j) {
+        const int a = tid * own + j;
+        if (a > s) break;
+        int c = 0;
+        for (int w = 0; w < PLAN_WAVES; ++w) {
+            const int x = at[w][a];
+            at[w][a] = before[0] + c;
+            c += x;
+        }
+        const int t = (c + tile - 1) / tile;
+        for (int k = 0; k < t; ++k) {
+            LoraTile lt;
+            lt.adapter = a < s ? a : -1;
+            lt.start = before[0] + k * tile;
+            lt.count = c - k * tile < tile ? c - k * tile : tile;
+            lt.slot = k == 0 ? -1 : before[2] + k - 1;
+            plan.tiles[before[1] + k] = lt;
+        }
+        if (a < s) {
+            plan.per_adapter[2 * a] = t;
+            plan.per_adapter[2 * a + 1] = before[2];
+        }
+        before[0] += c;
+        before[1] += t;
+        if (a < s && t > 1) before[2] += t - 1;
+    }
+    if (tid == 0) plan.head[0] = total_tiles;
+    __syncthreads();
+    for (int st = s0; st < s1; ++st) {
+        const int i = st * kWave + lane;
+        const int a = i < n ? adapter_of(i) : -1;
+        uint64_t left = __ballot(a >= 0);
+        while (left != 0) {  // one turn per adapter that occurs in the step
+            const int leader = __ffsll((long long)left) - 1;
+            const int want = __builtin_amdgcn_readlane(a, leader);
+            const uint64_t same = __ballot(a == want) & left;
+            const int base = at[wave][want];
+            if ((same >> lane) & 1) plan.order[base + __popcll(same & ((uint64_t(1) << lane) - 1))] = i;
+            // the wavefront's own counter: read by all lanes above, moved by one
+            __builtin_amdgcn_wave_barrier();
+            if (lane == leader) at[wave][want] = base + __popcll(same);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            left &= ~same;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Fragments.  v_mfma_f32_16x16x32: lane l holds eight values (one 16-byte register group) of row / column l % 16 at the
+// contraction indices 8 (l / 16) .. + 7 of either operand; the result's lane l holds column l % 16, rows 4 (l / 16) .. + 3.
+// ---------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ f32x4 mfma(const uint4 &a, const uint4 &b, const f32x4 &c) {
+    if constexpr (T::kDtype == KA_DTYPE_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    bf16x2 v;
+    v[0] = __bf16(lo);
+    v[1] = __bf16(hi);
+    return __builtin_bit_cast(uint32_t, v);
+}
+__device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// What rounding to bf16 left of a value; 0 behind an infinity or NaN, which the high part carries alone.
+__device__ __forceinline__ float rest(float v, float part) { return fabsf(part) < __builtin_inff() ? v - part : 0.0f; }
+
+// v = part[0] + part[1] (+ part[2]) in bf16: relative error 2^-17 with two parts, none (24 bits) with three
+template <int PARTS> __device__ __forceinline__ void split(const float (&v)[8], uint4 (&part)[PARTS]) {
+    uint32_t w[PARTS][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float a = v[2 * j], b = v[2 * j + 1];
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            w[p][j] = pack_bf16(a, b);
+            a = rest(a, low_half(w[p][j]));
+            b = rest(b, high_half(w[p][j]));
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) part[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+}
+__device__ __forceinline__ uint4 choose(bool first, const uint4 &a, const uint4 &b) {
+    return make_uint4(first ? a.x : b.x, first ? a.y : b.y, first ? a.z : b.z, first ? a.w : b.w);
+}
+// A fragment of the data's type as bf16 parts: itself, or the two that hold an fp16 exactly.
+template <typename T> struct Parts { static constexpr int kCount = T::kDtype == KA_DTYPE_BF16 ? 1 : 2; };
+template <typename T> __device__ __forceinline__ void as_bf16(const uint4 &f, uint4 (&part)[Parts<T>::kCount]) {
+    if constexpr (T::kDtype == KA_DTYPE_BF16) {
+        part[0] = f;
+    } else {
+        float v[8];
+        F16::unpack(f, v);
+        split<2>(v, part);
+    }
+}
+
+// Eight consecutive elements, zeros behind the first `n` of them.
+template <typename T, bool VEC> __device__ __forceinline__ uint4 load8(const typename T::raw_t *p, int n) {
+    if constexpr (VEC) {  // n is a multiple of 8, p 16-byte aligned
+        return n > 0 ? *reinterpret_cast<const uint4 *>(p) : make_uint4(0, 0, 0, 0);
+    } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) w[j / 2] |= uint32_t(p[j]) << (16 * (j & 1));
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+// Four consecutive elements, zeros behind the first `n`.
+template <typename T, bool VEC> __device__ __forceinline__ uint2 load4(const typename T::raw_t *p, int n) {
+    if constexpr (VEC) {
+        return n > 0 ? *reinterpret_cast<const uint2 *>(p) : make_uint2(0, 0);
+    } else {
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < n) w[j / 2] |= uint32_t(p[j]) << (16 * (j & 1));
+        return make_uint2(w[0], w[1]);
+    }
+}
+// Eight rows of four columns -> the four fragments e whose contraction index is the row: column e of each.
+__device__ __forceinline__ void transpose(const uint2 (&w)[8], uint4 (&frag)[4]) {
+    uint32_t f[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        f[0][j] = __builtin_amdgcn_perm(w[2 * j + 1].x, w[2 * j].x, 0x05040100u);
+        f[1][j] = __builtin_amdgcn_perm(w[2 * j + 1].x, w[2 * j].x, 0x07060302u);
+        f[2][j] = __builtin_amdgcn_perm(w[2 * j + 1].y, w[2 * j].y, 0x05040100u);
+        f[3][j] = __builtin_amdgcn_perm(w[2 * j + 1].y, w[2 * j].y, 0x07060302u);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) frag[e] = make_uint4(f[e][0], f[e][1], f[e][2], f[e][3]);
+}
+
+template <typename T> __device__ __forceinline__ typename T::raw_t narrow(float v) {
+    if constexpr (T::kDtype == KA_DTYPE_BF16) return __builtin_bit_cast(uint16_t, __bf16(v));
+    else return __builtin_bit_cast(uint16_t, _Float16(v));
+}
+
+// The sixteen results a lane holds for one token after four products e (row 4 m + e of the wide dimension at MFMA row m):
+// acc[e][i] belongs to column first + 4 i + e.  out = base + acc, rounded once.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_sum(const typename T::raw_t *base, typename T::raw_t *out, int first, int width,
+                                          const f32x4 (&acc)[4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int c = first + 8 * h;
+        if constexpr (VEC) {
+            if (c >= width) return;
+            float b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (base != nullptr) T::unpack(*reinterpret_cast<const uint4 *>(base + c), b);
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float v0 = b[2 * j] + acc[(2 * j) & 3][2 * h + (2 * j) / 4];
+                const float v1 = b[2 * j + 1] + acc[(2 * j + 1) & 3][2 * h + (2 * j) / 4];
+                w[j] = uint32_t(narrow<T>(v0)) | uint32_t(narrow<T>(v1)) << 16;
+            }
+            *reinterpret_cast<uint4 *>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j < width) {
+                    const float v = (base != nullptr ? T::widen(base[c + j]) : 0.0f) + acc[j & 3][2 * h + j / 4];
+                    out[c + j] = narrow<T>(v);
+                }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// lora_shrink: u = s x A^T.  H is cut into segments of 1024; inside one the wavefronts take every fourth step of 32 and are
+// added in their order, and the segments are added in theirs: by one workgroup (grid (1, tiles)), or by lora_fold_rows
+// over one partial result per segment (grid (segments, tiles)) where the tiles alone would leave CUs idle.  The bits of a
+// token's u do not depend on which of the two runs, nor on the other tokens.
+// ---------------------------------------------------------------------------
+constexpr int SEG_STEPS = 32;  // steps of 32 per segment
+struct ShrinkArgs {
+    const void *x, *a;
+    int64_t x_stride;
+    const float *scaling;
+    float scale;
+    int32_t n, h, r, segments, split;
+    float *out;  // [N, R] scaled, or with `split` [segments, N, R]
+    LoraPlan plan;
+};
+template <typename T, int RP, bool VEC>
+__global__ __launch_bounds__(THREADS) void lora_shrink(ShrinkArgs p) {
+    constexpr int RF = RP / 16;
+    __shared__ f32x4 part[WAVES][FWD_TILE][4];  // [wave][token][rank / 4] of one group of sixteen ranks
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
+    if (int(blockIdx.y) >= p.plan.head[0]) return;
+    const LoraTile tile = p.plan.tiles[blockIdx.y];
+    const int mine = tid / 4, mine_q = tid & 3;  // the thread adds up four ranks of token `mine` of the tile
+    f32x4 sum[RF];
+#pragma unroll
+    for (int f = 0; f < RF; ++f) sum[f] = f32x4{0, 0, 0, 0};
+    if (tile.adapter >= 0) {
+        const typename T::raw_t *rows[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int i = s * 16 + col;
+            rows[s] = i < tile.count ? static_cast<const typename T::raw_t *>(p.x) + int64_t(p.plan.order[tile.start + i]) * p.x_stride : nullptr;
+        }
+        const typename T::raw_t *aw = static_cast<const typename T::raw_t *>(p.a) + int64_t(tile.adapter) * p.r * p.h;
+        const int nsub = (tile.count + 15) / 16;
+        const int steps = (p.h + 31) / 32;
+        const int seg0 = p.split ? int(blockIdx.x) : 0, seg1 = p.split ? seg0 + 1 : p.segments;
+        for (int seg = seg0; seg < seg1; ++seg) {
+            f32x4 acc[RF][4];
+#pragma unroll
+            for (int f = 0; f < RF; ++f)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) acc[f][s] = f32x4{0, 0, 0, 0};
+            const int end = (seg + 1) * SEG_STEPS < steps ? (seg + 1) * SEG_STEPS : steps;
+            for (int st = seg * SEG_STEPS + wave; st < end; st += WAVES) {
+                const int k = st * 32 + 8 * quad;
+                uint4 fa[RF], fx[4];
+#pragma unroll
+                for (int f = 0; f < RF; ++f) fa[f] = load8<T, VEC>(aw + int64_t(f * 16 + col) * p.h + k, f * 16 + col < p.r ? p.h - k : 0);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) fx[s] = s < nsub ? load8<T, VEC>(rows[s] + k, rows[s] != nullptr ? p.h - k : 0) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int f = 0; f < RF; ++f)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+                        if (s < nsub) acc[f][s] = mfma<T>(fa[f], fx[s], acc[f][s]);
+            }
+#pragma unroll
+            for (int f = 0; f < RF; ++f) {
+                __syncthreads();  // the previous parts are read
+#pragma unroll
+                for (int s = 0; s < 4; ++s) part[wave][s * 16 + col][quad] = acc[f][s];
+                __syncthreads();
+                f32x4 v = part[0][mine][mine_q];
+#pragma unroll
+                for (int w = 1; w < WAVES; ++w) v += part[w][mine][mine_q];
+                sum[f] += v;
+            }
+        }
+    }
+    if (mine >= tile.count) return;
+    const float scale = tile.adapter < 0 ? 0.0f : (p.split ? 1.0f : (p.scaling != nullptr ? p.scaling[tile.adapter] : p.scale));
+    float *out = p.out + (p.split ? int64_t(blockIdx.x) * p.n * p.r : 0) + int64_t(p.plan.order[tile.start + mine]) * p.r;
+#pragma unroll
+    for (int f = 0; f < RF; ++f) {
+        const int r0 = f * 16 + mine_q * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (r0 + j < p.r) out[r0 + j] = tile.adapter < 0 ? 0.0f : sum[f][j] * scale;
+    }
+}
+
+// out[n, r] = s_a sum over the parts, in order; 0 for tokens without an adapter.
+__global__ __launch_bounds__(THREADS) void lora_fold_rows(const float *__restrict__ part, int parts, int64_t n, int r,
+                                                          const int64_t *__restrict__ ids, int s, const float *__restrict__ scaling,
+                                                          float scale, float *__restrict__ out) {
+    const int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x;
+    if (i >= n * r) return;
+    const int64_t a = ids[i / r];
+    float v = 0.0f;
+    if (a >= 0 && a < s) {
+        for (int q = 0; q < parts; ++q) v += part[int64_t(q) * n * r + i];
+        v *= scaling != nullptr ? scaling[a] : scale;
+    }
+    out[i] = v;
+}
+
+// ---------------------------------------------------------------------------
+// lora_expand: grid (blocks of O, tiles).  y = base + u B^T for the tokens of a tile.
+// ---------------------------------------------------------------------------
+struct ExpandArgs {
+    const void *base, *b;
+    void *out;
+    int64_t base_stride, out_stride;
+    const float *u;
+    int32_t o, r, groups, in_place;  // groups: of 64 outputs per wavefront
+    LoraPlan plan;
+};
+// Where R <= 16 one product of 32 holds the high parts of u in its first half and the low ones in its second.
+template <int RP> struct Steps { static constexpr int kCount = RP <= 16 ? 1 : RP / 32; };
+template <typename T, int RP, bool VEC>
+__global__ __launch_bounds__(THREADS) void lora_expand(ExpandArgs p) {
+    constexpr int KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, NP = Parts<T>::kCount;
+    __shared__ uint4 uf[4][KS][HL][kWave];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
+    if (int(blockIdx.y) >= p.plan.head[0]) return;
+    const LoraTile tile = p.plan.tiles[blockIdx.y];
+    if (tile.adapter < 0 && p.in_place) return;
+    const int nsub = (tile.count + 15) / 16;
+    const typename T::raw_t *base = static_cast<const typename T::raw_t *>(p.base);
+    typename T::raw_t *out = static_cast<typename T::raw_t *>(p.out);
+    {   // wavefront s prepares the fragments of group s: column = token
+        const int i = wave * 16 + col;
+        const float *row = i < tile.count && tile.adapter >= 0 ? p.u + int64_t(p.plan.order[tile.start + i]) * p.r : nullptr;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = row != nullptr && r0 + j < p.r ? row[r0 + j] : 0.0f;
+            uint4 hl[2];
+            split<2>(v, hl);
+            if (RP <= 16) {
+                uf[wave][0][0][lane] = choose(quad < 2, hl[0], hl[1]);
+            } else {
+                uf[wave][ks][0][lane] = hl[0];
+                uf[wave][ks][HL - 1][lane] = hl[1];
+            }
+        }
+    }
+    __syncthreads();
+    const typename T::raw_t *bw = tile.adapter < 0 ? nullptr : static_cast<const typename T::raw_t *>(p.b) + int64_t(tile.adapter) * p.o * p.r;
+    int64_t token[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) token[s] = s * 16 + col < tile.count ? p.plan.order[tile.start + s * 16 + col] : -1;
+    for (int g = 0; g < p.groups; ++g) {
+        const int o0 = ((int(blockIdx.x) * p.groups + g) * WAVES + wave) * 64;
+        if (o0 >= p.o) break;
+        uint4 fb[KS][4][NP];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int o = o0 + 4 * col + e;
+                const uint4 f = load8<T, VEC>(bw + int64_t(o) * p.r + r0, bw != nullptr && o < p.o ? p.r - r0 : 0);
+                as_bf16<T>(f, fb[ks][e]);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (s < nsub) {
+                f32x4 acc[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int hl = 0; hl < HL; ++hl) {
+                        const uint4 fu = uf[s][ks][hl][lane];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int q = 0; q < NP; ++q) acc[e] = mfma<Bf16>(fb[ks][e][q], fu, acc[e]);
+                    }
+                if (token[s] >= 0)
+                    store_sum<T, VEC>(base + token[s] * p.base_stride, out + token[s] * p.out_stride, o0 + 16 * quad, p.o, acc);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// lora_bwd_out: grid (blocks of O, tiles).  One pass over dy: the tile's part of dB, and dy B over the block's outputs.
+// A wavefront owns 64 G outputs; per 32 tokens it reads them twice (once from HBM, once from cache): transposed for dB, as
+// they are for dy B.
+// ---------------------------------------------------------------------------
+struct BwdOutArgs {
+    const void *dy, *b;
+    int64_t dy_stride;
+    const float *u;
+    int32_t n, o, r;
+    float *db, *db_part;  // [S, O, R], [slots, O, R]
+    float *du_part;       // [blocks, N, R]
+    LoraPlan plan;
+};
+// eight fp32 values of one column, contraction index = token
+__device__ __forceinline__ void load_column(const float *v, int r, int rank, const int32_t *tokens, int first, int count, float (&x)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = first + j < count && rank < r ? v[int64_t(tokens[first + j]) * r + rank] : 0.0f;
+}
+// acc += data^T v for one column group: parts of the data times parts of v, small products first
+template <typename T> __device__ __forceinline__ f32x4 outer(const uint4 (&data)[Parts<T>::kCount], const uint4 (&v)[3], f32x4 acc) {
+    if constexpr (Parts<T>::kCount == 2) {
+        acc = mfma<Bf16>(data[1], v[1], acc);
+        acc = mfma<Bf16>(data[1], v[0], acc);
+    }
+    acc = mfma<Bf16>(data[0], v[2], acc);
+    acc = mfma<Bf16>(data[0], v[1], acc);
+    return mfma<Bf16>(data[0], v[0], acc);
+}
+
+template <typename T, int RP, int G, bool VEC>
+__global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
+    constexpr int RF = RP / 16, NP = Parts<T>::kCount;
+    constexpr int RED = RF < 4 ? RF : 4;  // groups of sixteen ranks that cross the wavefronts at a time
+    __shared__ int32_t tokens[BWD_TILE_MAX];
+    __shared__ f32x4 red[WAVES][32][RED * 4];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
+    if (int(blockIdx.y) >= p.plan.head[0]) return;
+    const LoraTile tile = p.plan.tiles[blockIdx.y];
+    if (tile.adapter < 0) return;
+    for (int i = tid; i < tile.count; i += THREADS) tokens[i] = p.plan.order[tile.start + i];
+    const typename T::raw_t *dy = static_cast<const typename T::raw_t *>(p.dy);
+    const typename T::raw_t *bw = static_cast<const typename T::raw_t *>(p.b) + int64_t(tile.adapter) * p.o * p.r;
+    const int o0 = (int(blockIdx.x) * WAVES + wave) * 64 * G;
+    // B^T fragments: row = rank, contraction index = output
+    uint4 fb[G][2][RF];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int f = 0; f < RF; ++f) {
+                uint32_t w[4] = {0, 0, 0, 0};
+                const int rank = f * 16 + col, o = o0 + g * 64 + ks * 32 + 8 * quad;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (rank < p.r && o + j < p.o) w[j / 2] |= uint32_t(bw[int64_t(o + j) * p.r + rank]) << (16 * (j & 1));
+                fb[g][ks][f] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+    f32x4 acc[G][RF][4];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int f = 0; f < RF; ++f)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[g][f][e] = f32x4{0, 0, 0, 0};
+    __syncthreads();
+    for (int c = 0; c < tile.count; c += 32) {
+        f32x4 du[2][RF];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int f = 0; f < RF; ++f) du[s][f] = f32x4{0, 0, 0, 0};
+        uint4 v[RF][3];
+#pragma unroll
+        for (int f = 0; f < RF; ++f) {
+            float x[8];
+            load_column(p.u, p.r, f * 16 + col, tokens, c + 8 * quad, tile.count, x);
+            split<3>(x, v[f]);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int og = o0 + g * 64;
+            uint2 w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = c + 8 * quad + j, o = og + 4 * col;
+                w[j] = i < tile.count ? load4<T, VEC>(dy + int64_t(tokens[i]) * p.dy_stride + o, p.o - o) : make_uint2(0, 0);
+            }
+            uint4 frag[4], part[4][NP];
+            transpose(w, frag);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) as_bf16<T>(frag[e], part[e]);
+#pragma unroll
+            for (int f = 0; f < RF; ++f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[g][f][e] = outer<T>(part[e], v[f], acc[g][f][e]);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const int i = c + 16 * s + col, o = og + ks * 32 + 8 * quad;
+                    const uint4 fy = i < tile.count ? load8<T, VEC>(dy + int64_t(tokens[i]) * p.dy_stride + o, p.o - o) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int f = 0; f < RF; ++f) du[s][f] = mfma<T>(fb[g][ks][f], fy, du[s][f]);
+                }
+        }
+        // dy B of the workgroup's outputs: the wavefronts' parts in their order
+#pragma unroll
+        for (int f0 = 0; f0 < RF; f0 += RED) {
+            __syncthreads();  // the previous sums are read
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int f = 0; f < RED; ++f) red[wave][16 * s + col][f * 4 + quad] = du[s][f0 + f];
+            __syncthreads();
+            for (int q = tid; q < 32 * RED * 4; q += THREADS) {
+                const int i = q / (RED * 4), r4 = q % (RED * 4), r0 = f0 * 16 + r4 * 4;
+                if (c + i < tile.count && r0 < p.r) {
+                    f32x4 sum = red[0][i][r4];
+#pragma unroll
+                    for (int k = 1; k < WAVES; ++k) sum += red[k][i][r4];
+                    float *out = p.du_part + (int64_t(blockIdx.x) * p.n + tokens[c + i]) * p.r + r0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (r0 + j < p.r) out[j] = sum[j];
+                }
+            }
+        }
+    }
+    float *db = tile.slot < 0 ? p.db + int64_t(tile.adapter) * p.o * p.r : p.db_part + int64_t(tile.slot) * p.o * p.r;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int f = 0; f < RF; ++f)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int o = o0 + g * 64 + 16 * quad + 4 * i + e, rank = f * 16 + col;
+                    if (o < p.o && rank < p.r) db[int64_t(o) * p.r + rank] = acc[g][f][e][i];
+                }
+}
+
+// ---------------------------------------------------------------------------
+// lora_bwd_in: grid (blocks of H, tiles).  One pass over x: the tile's part of dA, and dx = dx_base + du A.
+// ---------------------------------------------------------------------------
+struct BwdInArgs {
+    const void *x, *a, *dx_base;
+    void *dx;
+    int64_t x_stride, dx_base_stride, dx_stride;
+    const float *du;
+    int32_t h, r;
+    float *da, *da_part;  // [S, R, H], [slots, R, H]
+    LoraPlan plan;
+};
+template <typename T, int RP, bool VEC>
+__global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
+    constexpr int RF = RP / 16, KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, NP = Parts<T>::kCount;
+    __shared__ int32_t tokens[BWD_TILE_MAX];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
+    if (int(blockIdx.y) >= p.plan.head[0]) return;
+    const LoraTile tile = p.plan.tiles[blockIdx.y];
+    for (int i = tid; i < tile.count; i += THREADS) tokens[i] = p.plan.order[tile.start + i];
+    __syncthreads();
+    const int h0 = (int(blockIdx.x) * WAVES + wave) * 64;
+    if (h0 >= p.h) return;  // (no barrier follows)
+    const typename T::raw_t *x = static_cast<const typename T::raw_t *>(p.x);
+    const typename T::raw_t *dx_base = static_cast<const typename T::raw_t *>(p.dx_base);
+    typename T::raw_t *dx = static_cast<typename T::raw_t *>(p.dx);
+    const bool has = tile.adapter >= 0;
+    const typename T::raw_t *aw = static_cast<const typename T::raw_t *>(p.a) + (has ? int64_t(tile.adapter) * p.r * p.h : 0);
+    // A fragments: row 4 m + e = input, contraction index = rank
+    uint4 fa[KS][4][NP];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        uint2 w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int rank = (RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad) + j, h = h0 + 4 * col;
+            w[j] = has && rank < p.r ? load4<T, VEC>(aw + int64_t(rank) * p.h + h, p.h - h) : make_uint2(0, 0);
+        }
+        uint4 frag[4];
+        transpose(w, frag);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) as_bf16<T>(frag[e], fa[ks][e]);
+    }
+    f32x4 acc[RF][4];
+#pragma unroll
+    for (int f = 0; f < RF; ++f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[f][e] = f32x4{0, 0, 0, 0};
+    for (int c = 0; c < tile.count; c += 32) {
+        if (has) {
+            uint2 w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = c + 8 * quad + j, h = h0 + 4 * col;
+                w[j] = i < tile.count ? load4<T, VEC>(x + int64_t(tokens[i]) * p.x_stride + h, p.h - h) : make_uint2(0, 0);
+            }
+            uint4 frag[4], part[4][NP];
+            transpose(w, frag);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) as_bf16<T>(frag[e], part[e]);
+#pragma unroll
+            for (int f = 0; f < RF; ++f) {
+                float col8[8];
+                uint4 v[3];
+                load_column(p.du, p.r, f * 16 + col, tokens, c + 8 * quad, tile.count, col8);
+                split<3>(col8, v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[f][e] = outer<T>(part[e], v, acc[f][e]);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int i = c + 16 * s + col;
+            const int64_t token = i < tile.count ? tokens[i] : -1;
+            f32x4 sum[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
+                float row[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) row[j] = has && token >= 0 && r0 + j < p.r ? p.du[token * p.r + r0 + j] : 0.0f;
+                uint4 hl[2];
+                split<2>(row, hl);
+                if (RP <= 16) hl[0] = choose(quad < 2, hl[0], hl[1]);
+#pragma unroll
+                for (int k = 0; k < HL; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int q = 0; q < NP; ++q) sum[e] = mfma<Bf16>(fa[ks][e][q], hl[k], sum[e]);
+            }
+            if (token >= 0)
+                store_sum<T, VEC>(dx_base != nullptr ? dx_base + token * p.dx_base_stride : nullptr, dx + token * p.dx_stride, h0 + 16 * quad, p.h, sum);
+        }
+    }
+    if (!has) return;
+    float *da = tile.slot < 0 ? p.da + int64_t(tile.adapter) * p.r * p.h : p.da_part + int64_t(tile.slot) * p.r * p.h;
+#pragma unroll
+    for (int f = 0; f < RF; ++f) {
+        const int rank = f * 16 + col;
+        if (rank >= p.r) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int h = h0 + 16 * quad + 4 * i;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (h + e < p.h) da[int64_t(rank) * p.h + h + e] = acc[f][e][i];
+        }
+    }
+}
+
+// grid (blocks of elements, adapters): adds the partial gradients of an adapter's further tiles in their order; zeros for an
+// adapter without tokens.
+__global__ __launch_bounds__(THREADS) void lora_fold_grads(float *__restrict__ grad, const float *__restrict__ part,
+                                                           int64_t elements, LoraPlan plan) {
+    const int a = blockIdx.y;
+    const int tiles = plan.per_adapter[2 * a], slot = plan.per_adapter[2 * a + 1];
+    if (tiles == 1) return;
+    float *g = grad + int64_t(a) * elements;
+    for (int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x; i < elements; i += int64_t(gridDim.x) * THREADS) {
+        float v = 0.0f;
+        if (tiles > 1) {
+            v = g[i];
+            for (int k = 0; k < tiles - 1; ++k) v += part[int64_t(slot + k) * elements + i];
+        }
+        g[i] = v;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+inline size_t align_up(size_t n) { return (n + 255) / 256 * 256; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct Shape { int64_t n, h, o, r, s; };
+
+inline int check_shape(const char *what, int dtype, const Shape &d) {
+    if (dtype != KA_DTYPE_BF16 && dtype != KA_DTYPE_F16) return fail(KA_ERR_BAD_ARG, "%s: dtype code %d is not bf16 or fp16", what, dtype);
+    if (d.n < 0 || d.h < 1 || d.o < 1 || d.r < 1 || d.s < 1)
+        return fail(KA_ERR_BAD_ARG, "%s: tokens %lld, widths %lld and %lld, rank %lld, adapters %lld must be positive", what,
+                    (long long)d.n, (long long)d.h, (long long)d.o, (long long)d.r, (long long)d.s);
+    if (d.r > MAX_RANK) return fail(KA_ERR_UNSUPPORTED, "%s: rank %lld > %d", what, (long long)d.r, MAX_RANK);
+    if (d.s > MAX_ADAPTERS) return fail(KA_ERR_UNSUPPORTED, "%s: %lld adapters > %d", what, (long long)d.s, MAX_ADAPTERS);
+    if (d.n > KA_LORA_MAX_TOKENS) return fail(KA_ERR_UNSUPPORTED, "%s: %lld tokens > %d", what, (long long)d.n, KA_LORA_MAX_TOKENS);
+    if (d.h >= (int64_t(1) << 24) || d.o >= (int64_t(1) << 24)) return fail(KA_ERR_UNSUPPORTED, "%s: a width of 2^24 or more", what);
+    return KA_OK;
+}
+
+inline int padded_rank(int64_t r) { return r <= 16 ? 16 : (r <= 32 ? 32 : (r <= 64 ? 64 : 128)); }
+
+struct PlanLayout { size_t order, tiles, per_adapter, total; int64_t max_tiles; };
+inline PlanLayout plan_layout(int64_t n, int64_t s, int64_t tile) {
+    PlanLayout l;
+    const int64_t groups = s + 1 < n ? s + 1 : n;
+    l.max_tiles = n / tile + groups;
+    l.order = 256;
+    l.tiles = l.order + align_up(size_t(n) * 4);
+    l.per_adapter = l.tiles + align_up(size_t(l.max_tiles) * sizeof(LoraTile));
+    l.total = l.per_adapter + align_up(size_t(s) * 8);
+    return l;
+}
+inline LoraPlan plan_at(unsigned char *ws, const PlanLayout &l) {
+    LoraPlan p;
+    p.head = reinterpret_cast<int32_t *>(ws);
+    p.order = reinterpret_cast<int32_t *>(ws + l.order);
+    p.tiles = reinterpret_cast<LoraTile *>(ws + l.tiles);
+    p.per_adapter = reinterpret_cast<int32_t *>(ws + l.per_adapter);
+    p.max_tiles = int32_t(l.max_tiles);
+    return p;
+}
+
+struct FwdLayout { PlanLayout plan; int64_t segments; bool split; size_t part, u, total; };
+inline FwdLayout fwd_layout(const Shape &d) {
+    FwdLayout l;
+    l.plan = plan_layout(d.n, d.s, FWD_TILE);
+    l.segments = ceil_div(d.h, SEG_STEPS * 32);
+    l.split = l.segments > 1 && l.plan.max_tiles < 256;
+    l.part = l.plan.total;
+    l.u = l.part + (l.split ? align_up(size_t(l.segments) * d.n * d.r * 4) : 0);
+    l.total = l.u + align_up(size_t(d.n) * d.r * 4);
+    return l;
+}
+
+// The backward: outputs per wavefront (64 G) and tokens per tile.
+struct BwdLayout { PlanLayout plan; int64_t tile, slots, blocks; int groups; size_t du, du_part, db_part, da_part, total; };
+inline BwdLayout bwd_layout(const Shape &d) {
+    BwdLayout l;
+    const int64_t small_blocks = ceil_div(d.o, 64 * WAVES);
+    // 1024 outputs per workgroup where that leaves work for every CU: fewer partial sums of dy B
+    l.groups = padded_rank(d.r) == 16 && ceil_div(d.n, 64) * ceil_div(small_blocks, 4) >= 512 ? 4 : 1;
+    l.blocks = ceil_div(d.o, 64 * WAVES * l.groups);
+    // about 1024 workgroups over the narrower of the two passes
+    const int64_t in_blocks = ceil_div(d.h, 64 * WAVES);
+    const int64_t narrow = l.blocks < in_blocks ? l.blocks : in_blocks;
+    int64_t tile = ceil_div(ceil_div(d.n * narrow, 1024), 32) * 32;
+    if (tile < 64) tile = 64;
+    if (tile > BWD_TILE_MAX) tile = BWD_TILE_MAX;
+    l.tile = tile;
+    l.slots = d.n / tile;
+    l.plan = plan_layout(d.n, d.s, tile);
+    l.du = l.plan.total;
+    l.du_part = l.du + align_up(size_t(d.n) * d.r * 4);
+    l.db_part = l.du_part + align_up(size_t(l.blocks) * d.n * d.r * 4);
+    l.da_part = l.db_part + align_up(size_t(l.slots) * d.o * d.r * 4);
+    l.total = l.da_part + align_up(size_t(l.slots) * d.h * d.r * 4);
+    return l;
+}
+
+inline bool aligned16(const void *p, int64_t stride) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0); }
+
+// Calls launch(type, padded rank, vector accesses), each as a compile-time value.
+template <typename F> void with_types(int dtype, int rp, bool vec, F &&launch) {
+    auto ranks = [&](auto type, auto vector) {
+        if (rp == 16) launch(type, std::integral_constant<int, 16>{}, vector);
+        else if (rp == 32) launch(type, std::integral_constant<int, 32>{}, vector);
+        else if (rp == 64) launch(type, std::integral_constant<int, 64>{}, vector);
+        else launch(type, std::integral_constant<int, 128>{}, vector);
+    };
+    auto vectors = [&](auto type) {
+        if (vec) ranks(type, std::true_type{});
+        else ranks(type, std::false_type{});
+    };
+    if (dtype == KA_DTYPE_BF16) vectors(Bf16{});
+    else vectors(F16{});
+}
+
+}  // namespace
+}  // namespace ka
+
+KA_EXPORT size_t ka_lora_workspace_bytes(int64_t n_tokens, int64_t in_dim, int64_t out_dim, int64_t rank, int64_t n_adapters,
+                                         int backward) {
+    const ka::Shape d{n_tokens, in_dim, out_dim, rank, n_adapters};
+    if (ka::check_shape("lora", KA_DTYPE_BF16, d) != KA_OK || n_tokens == 0) return 0;
+    return backward ? ka::bwd_layout(d).total : ka::fwd_layout(d).total;
+}
+
+KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, const void *hidden, int64_t hidden_stride,
+                             const void *lora_a, const void *lora_b, const int64_t *adapter_ids, const float *scaling,
+                             float scale, void *out, int64_t out_stride, float *out_shrunk, int64_t n_tokens, int64_t in_dim,
+                             int64_t out_dim, int64_t rank, int64_t n_adapters, void *workspace, size_t workspace_bytes,
+                             void *hip_stream) {
+    using namespace ka;
+    const Shape d{n_tokens, in_dim, out_dim, rank, n_adapters};
+    int rc = check_shape("lora", dtype, d);
+    if (rc != KA_OK) return rc;
+    if (n_tokens == 0) return KA_OK;
+    if (hidden == nullptr || lora_a == nullptr || adapter_ids == nullptr || (out != nullptr && (base == nullptr || lora_b == nullptr)) ||
+        (out == nullptr && out_shrunk == nullptr))
+        return fail(KA_ERR_BAD_ARG, "lora: null base / hidden / lora_a / lora_b / adapter_ids / out pointer");
+    if ((out != nullptr && (base_stride < out_dim || out_stride < out_dim)) || hidden_stride < in_dim)
+        return fail(KA_ERR_BAD_ARG, "lora: a row stride is smaller than its row");
+    const FwdLayout l = fwd_layout(d);
+    if (workspace == nullptr || workspace_bytes < l.total)
+        return fail(KA_ERR_WORKSPACE, "lora: workspace of %zu B, need %zu B", workspace == nullptr ? size_t(0) : workspace_bytes, l.total);
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(KA_ERR_BAD_ARG, "lora: workspace is not 16-byte aligned");
+    const bool vec = aligned16(base, base_stride) && aligned16(out, out_stride) && aligned16(hidden, hidden_stride) && aligned16(lora_a, 0) &&
+                     aligned16(lora_b, 0) && in_dim % 8 == 0 && out_dim % 8 == 0 && rank % 8 == 0;
+    hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    const LoraPlan plan = plan_at(ws, l.plan);
+    hipLaunchKernelGGL(lora_plan, dim3(1), dim3(PLAN_THREADS), 0, stream, adapter_ids, int(n_tokens), int(n_adapters), FWD_TILE, plan);
+    rc = check_hip(hipGetLastError(), "lora launch (plan)");
+    if (rc != KA_OK) return rc;
+    float *u = out_shrunk != nullptr ? out_shrunk : reinterpret_cast<float *>(ws + l.u);
+    ShrinkArgs sa{};
+    sa.x = hidden;
+    sa.a = lora_a;
+    sa.x_stride = hidden_stride;
+    sa.scaling = scaling;
+    sa.scale = scale;
+    sa.n = int32_t(n_tokens);
+    sa.h = int32_t(in_dim);
+    sa.r = int32_t(rank);
+    sa.segments = int32_t(l.segments);
+    sa.split = l.split ? 1 : 0;
+    sa.out = l.split ? reinterpret_cast<float *>(ws + l.part) : u;
+    sa.plan = plan;
+    const int rp = padded_rank(rank);
+    const dim3 shrink_grid{unsigned(l.split ? l.segments : 1), unsigned(l.plan.max_tiles)};
+    with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
+        using T = decltype(type);
+        constexpr int RP = decltype(rank_c)::value;
+        constexpr bool VEC = decltype(vec_c)::value;
+        hipLaunchKernelGGL((lora_shrink<T, RP, VEC>), shrink_grid, dim3(THREADS), 0, stream, sa);
+    });
+    rc = check_hip(hipGetLastError(), "lora launch (shrink)");
+    if (rc != KA_OK) return rc;
+    if (l.split) {
+        hipLaunchKernelGGL(lora_fold_rows, dim3(unsigned(ceil_div(n_tokens * rank, THREADS))), dim3(THREADS), 0, stream,
+                           reinterpret_cast<const float *>(ws + l.part), int(l.segments), n_tokens, int(rank), adapter_ids, int(n_adapters), scaling, scale, u);
+        rc = check_hip(hipGetLastError(), "lora launch (fold)");
+        if (rc != KA_OK) return rc;
+    }
+    if (out == nullptr) return KA_OK;
+    ExpandArgs ea{};
+    ea.base = base;
+    ea.b = lora_b;
+    ea.out = out;
+    ea.base_stride = base_stride;
+    ea.out_stride = out_stride;
+    ea.u = u;
+    ea.o = int32_t(out_dim);
+    ea.r = int32_t(rank);
+    ea.in_place = out == base && out_stride == base_stride ? 1 : 0;
+    ea.plan = plan;
+    // groups of 64 outputs per wavefront: as many as leave about 1024 workgroups
+    const int64_t blocks1 = ceil_div(out_dim, 64 * WAVES);
+    int64_t groups = blocks1 * l.plan.max_tiles / 1024;
+    groups = groups < 1 ? 1 : (groups > 8 ? 8 : groups);
+    ea.groups = int32_t(groups);
+    const dim3 expand_grid{unsigned(ceil_div(out_dim, 64 * WAVES * groups)), unsigned(l.plan.max_tiles)};
+    with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
+        using T = decltype(type);
+        constexpr int RP = decltype(rank_c)::value;
+        constexpr bool VEC = decltype(vec_c)::value;
+        hipLaunchKernelGGL((lora_expand<T, RP, VEC>), expand_grid, dim3(THREADS), 0, stream, ea);
+    });
+    return check_hip(hipGetLastError(), "lora launch (expand)");
+}
+
+KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t grad_stride, const void *hidden,
+                                      int64_t hidden_stride, const void *lora_a, const void *lora_b, const int64_t *adapter_ids,
+                                      const float *scaling, float scale, const float *shrunk, const void *dhidden_base,
+                                      int64_t dhidden_base_stride, void *dhidden, int64_t dhidden_stride, float *dlora_a,
+                                      float *dlora_b, int64_t n_tokens, int64_t in_dim, int64_t out_dim, int64_t rank,
+                                      int64_t n_adapters, void *workspace, size_t workspace_bytes, void *hip_stream) {
+    using namespace ka;
+    const Shape d{n_tokens, in_dim, out_dim, rank, n_adapters};
+    int rc = check_shape("lora backward", dtype, d);
+    if (rc != KA_OK) return rc;
+    if (n_tokens == 0) return fail(KA_ERR_BAD_ARG, "lora backward: no tokens (the gradients would be zero)");
+    if (grad_out == nullptr || hidden == nullptr || lora_a == nullptr || lora_b == nullptr || adapter_ids == nullptr ||
+        shrunk == nullptr || dhidden == nullptr || dlora_a == nullptr || dlora_b == nullptr)
+        return fail(KA_ERR_BAD_ARG, "lora backward: null grad_out / hidden / lora_a / lora_b / adapter_ids / shrunk / result pointer");
+    if (grad_stride < out_dim || hidden_stride < in_dim || dhidden_stride < in_dim || (dhidden_base != nullptr && dhidden_base_stride < in_dim))
+        return fail(KA_ERR_BAD_ARG, "lora backward: a row stride is smaller than its row");
+    const BwdLayout l = bwd_layout(d);
+    if (workspace == nullptr || workspace_bytes < l.total)
+        return fail(KA_ERR_WORKSPACE, "lora backward: workspace of %zu B, need %zu B", workspace == nullptr ? size_t(0) : workspace_bytes, l.total);
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(KA_ERR_BAD_ARG, "lora backward: workspace is not 16-byte aligned");
+    const bool vec = aligned16(grad_out, grad_stride) && aligned16(hidden, hidden_stride) && aligned16(dhidden_base, dhidden_base_stride) &&
+                     aligned16(dhidden, dhidden_stride) && aligned16(lora_a, 0) && aligned16(lora_b, 0) && in_dim % 8 == 0 && out_dim % 8 == 0 &&
+                     rank % 8 == 0;
+    hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    const LoraPlan plan = plan_at(ws, l.plan);
+    hipLaunchKernelGGL(lora_plan, dim3(1), dim3(PLAN_THREADS), 0, stream, adapter_ids, int(n_tokens), int(n_adapters), int(l.tile), plan);
+    rc = check_hip(hipGetLastError(), "lora backward launch (plan)");
+    if (rc != KA_OK) return rc;
+    const int rp = padded_rank(rank);
+    float *du = reinterpret_cast<float *>(ws + l.du), *du_part = reinterpret_cast<float *>(ws + l.du_part);
+    float *db_part = reinterpret_cast<float *>(ws + l.db_part), *da_part = reinterpret_cast<float *>(ws + l.da_part);
+    BwdOutArgs oa{};
+    oa.dy = grad_out;
+    oa.b = lora_b;
+    oa.dy_stride = grad_stride;
+    oa.u = shrunk;
+    oa.n = int32_t(n_tokens);
+    oa.o = int32_t(out_dim);
+    oa.r = int32_t(rank);
+    oa.db = dlora_b;
+    oa.db_part = db_part;
+    oa.du_part = du_part;
+    oa.plan = plan;
+    const dim3 out_grid{unsigned(l.blocks), unsigned(l.plan.max_tiles)};
+    with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
+        using T = decltype(type);
+        constexpr int RP = decltype(rank_c)::value;
+        constexpr bool VEC = decltype(vec_c)::value;
+        if constexpr (RP == 16) {
+            if (l.groups == 4) {
+                hipLaunchKernelGGL((lora_bwd_out<T, RP, 4, VEC>), out_grid, dim3(THREADS), 0, stream, oa);
+                return;
+            }
+        }
+        hipLaunchKernelGGL((lora_bwd_out<T, RP, 1, VEC>), out_grid, dim3(THREADS), 0, stream, oa);
+    });
+    rc = check_hip(hipGetLastError(), "lora backward launch (out)");
+    if (rc != KA_OK) return rc;
+    hipLaunchKernelGGL(lora_fold_rows, dim3(unsigned(ceil_div(n_tokens * rank, THREADS))), dim3(THREADS), 0, stream, du_part,
+                       int(l.blocks), n_tokens, int(rank), adapter_ids, int(n_adapters), scaling, scale, du);
+    rc = check_hip(hipGetLastError(), "lora backward launch (fold)");
+    if (rc != KA_OK) return rc;
+    BwdInArgs ia{};
+    ia.x = hidden;
+    ia.a = lora_a;
+    ia.dx_base = dhidden_base;
+    ia.dx = dhidden;
+    ia.x_stride = hidden_stride;
+    ia.dx_base_stride = dhidden_base_stride;
+    ia.dx_stride = dhidden_stride;
+    ia.du = du;
+    ia.h = int32_t(in_dim);
+    ia.r = int32_t(rank);
+    ia.da = dlora_a;
+    ia.da_part = da_part;
+    ia.plan = plan;
+    const dim3 in_grid{unsigned(ceil_div(in_dim, 64 * WAVES)), unsigned(l.plan.max_tiles)};
+    with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
+        using T = decltype(type);
+        constexpr int RP = decltype(rank_c)::value;
+        constexpr bool VEC = decltype(vec_c)::value;
+        hipLaunchKernelGGL((lora_bwd_in<T, RP, VEC>), in_grid, dim3(THREADS), 0, stream, ia);
+    });
+    rc = check_hip(hipGetLastError(), "lora backward launch (in)");
+    if (rc != KA_OK) return rc;
+    auto fold = [&](float *grad, const float *part, int64_t elements) {
+        int64_t blocks = ceil_div(elements, THREADS * 4);
+        if (blocks > 1024) blocks = 1024;
+        hipLaunchKernelGGL(lora_fold_grads, dim3(unsigned(blocks), unsigned(n_adapters)), dim3(THREADS), 0, stream, grad, part, elements, plan);
+        return check_hip(hipGetLastError(), "lora backward launch (gradients)");
+    };
+    rc = fold(dlora_b, db_part, out_dim * rank);
+    if (rc != KA_OK) return rc;
+    return fold(dlora_a, da_part, in_dim * rank);
+}

@@ -15,6 +15,7 @@ import torch.nn as nn
 
 from rl_engine.kernels import _hip
 from rl_engine.kernels._launch import _on_device, _raw_stream, _require_gpu
+from rl_engine.kernels.adapters import AdapterOps
 from rl_engine.kernels.pool import PoolExhausted, WorkspacePool
 from rl_engine.kernels.speculative import SpeculativeOps
 from rl_engine.platforms.constants import constants
@@ -59,7 +60,7 @@ def _rows_view(logits: torch.Tensor) -> torch.Tensor:
     return logits.contiguous().view(-1, vocab)
 
 
-class SamplerBackend(SpeculativeOps, nn.Module):
+class SamplerBackend(AdapterOps, SpeculativeOps, nn.Module):
     def __init__(self, pool_bytes: int | None = None):
         super().__init__()
         self.backend = self._detect_backend()

@@ -188,3 +188,34 @@ def test_verify_argument_checks_and_workspace_size():
         assert call(**far) == _hip.KA_ERR_UNSUPPORTED, far
     assert call(ws_bytes=ws(0, 2, 4, 100) - 1) == _hip.KA_ERR_WORKSPACE
     assert call(ws_ptr=None) == _hip.KA_ERR_WORKSPACE and b"workspace" in lib.ka_last_error()
+
+
+def test_lora_argument_checks_and_workspace_size():
+    lib = _hip.load()
+    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4104)
+    ws = lib.ka_lora_workspace_bytes
+    assert ws(0, 64, 64, 16, 1, 0) == 0 and ws(8, 64, 64, 129, 1, 0) == 0 and ws(8, 64, 64, 16, 1024, 1) == 0
+    assert ws(8, 64, 64, 16, 1, 0) > 0 and ws(8, 64, 64, 16, 1, 1) > 0
+
+    def fwd(dtype=0, base=p, bs=64, hid=p, hs=32, a=p, b=p, ids=p, out=p, os=64, u=None, n=4, h=32, o=64, r=8, s=2, w=p, wb=1 << 20):
+        return lib.ka_lora_linear(dtype, base, bs, hid, hs, a, b, ids, None, 1.0, out, os, u, n, h, o, r, s, w, wb, None)
+
+    def bwd(dtype=0, g=p, gs=64, hid=p, hs=32, a=p, b=p, ids=p, u=p, xb=None, xbs=0, dx=p, dxs=32, da=p, db=p, n=4, h=32, o=64, r=8,
+            s=2, w=p, wb=1 << 24):
+        return lib.ka_lora_linear_backward(dtype, g, gs, hid, hs, a, b, ids, None, 1.0, u, xb, xbs, dx, dxs, da, db, n, h, o, r, s,
+                                           w, wb, None)
+
+    assert fwd(n=0, base=None) == _hip.KA_OK
+    for bad in (dict(dtype=2), dict(n=-1), dict(h=0), dict(o=0), dict(r=0), dict(s=0), dict(base=None), dict(hid=None),
+                dict(a=None), dict(b=None), dict(ids=None), dict(out=None), dict(bs=63), dict(os=63), dict(hs=31), dict(w=odd)):
+        assert fwd(**bad) == _hip.KA_ERR_BAD_ARG, bad
+    for bad in (dict(dtype=2), dict(n=0), dict(n=-1), dict(g=None), dict(hid=None), dict(a=None), dict(b=None), dict(ids=None),
+                dict(u=None), dict(dx=None), dict(da=None), dict(db=None), dict(gs=63), dict(hs=31), dict(dxs=31),
+                dict(xb=p, xbs=31), dict(w=odd)):
+        assert bwd(**bad) == _hip.KA_ERR_BAD_ARG, bad
+    for call in (fwd, bwd):
+        for far in (dict(r=129), dict(s=1024), dict(n=(1 << 21) + 1), dict(h=1 << 24), dict(o=1 << 24)):
+            assert call(**far) == _hip.KA_ERR_UNSUPPORTED, far
+        assert call(w=None) == _hip.KA_ERR_WORKSPACE
+    assert fwd(wb=ws(4, 32, 64, 8, 2, 0) - 1) == _hip.KA_ERR_WORKSPACE
+    assert bwd(wb=ws(4, 32, 64, 8, 2, 1) - 1) == _hip.KA_ERR_WORKSPACE and b"workspace" in lib.ka_last_error()
