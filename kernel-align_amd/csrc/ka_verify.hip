@@ -18,7 +18,7 @@
 //                  the data: bound by HBM, 2 V (2 K + 1) bytes per request.
 //   verify_ties    (only where top-p may cut inside a group of equal logits) the index at which the cut falls, for the two rows
 //                  of the position where the request stops
-//   verify_shares  residual mass of every share of 1024 vectors of the stopping position, by as many workgroups as there are shares
+//   verify_shares  residual mass of every share of 256 vectors of the stopping position, a wavefront each
 //   verify_draw    one workgroup per request: the share, the vector and the entry that hold the draw; all outputs
 // The rows of the stopping position are read again by the last two, from L2 / MALL as a rule.
 #define KA_SAMPLING_THREADS 512
@@ -34,7 +34,7 @@ typedef unsigned __int128 u128;
 
 constexpr int VERIFY_MAX_DRAFT = KA_VERIFY_MAX_DRAFT;
 static_assert(VERIFY_MAX_DRAFT <= kWave, "one lane decides one position");
-constexpr int SHARE_VECS = 1024;   // 16-byte vectors of a row in one share; verify_draw has a thread for each
+constexpr int SHARE_VECS = 256;    // 16-byte vectors of a row in one share; verify_draw has a thread for each
 constexpr int SHARE_THREADS = 256;
 
 // What verify_rows leaves about a row.
@@ -43,7 +43,7 @@ struct RowSummary {
     uint64_t w_draft;   // of which the drafted token has this (0: filtered out, or an id outside the vocabulary)
     double lse;         // log-sum-exp of the raw row (target rows, when asked for)
     uint32_t kmax, kcut, r_cut;  // see RowCut
-    uint32_t pad;
+    uint32_t raw_cut;   // key (unscaled) below which no entry survives; 0: not known, or no filter
 };
 static_assert(sizeof(RowSummary) == 40, "the workspace query counts 40 bytes per row");
 
@@ -142,17 +142,277 @@ __device__ __forceinline__ int accepted_prefix(const VerifyParams &p, int b, int
     return first < len ? first : len;
 }
 
+// One vector of entries from `base` on; zeros behind the row.
+template <typename T>
+__device__ __forceinline__ void load_entries(const typename T::raw_t *row, bool vec, int vocab, int64_t base, typename T::raw_t (&e)[T::kPerVec]) {
+    constexpr int EPV = T::kPerVec;
+    if (vec && base + EPV <= vocab) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(row + base);
+        __builtin_memcpy(e, &v, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < EPV; ++j) e[j] = base + j < vocab ? row[base + j] : typename T::raw_t(0);
+    }
+}
+// The value below which an unscaled entry does not survive (NaN compares as surviving: its key decides).
+template <typename T> __device__ __forceinline__ float cut_value(uint32_t raw_cut) {
+    return raw_cut == 0 ? -__builtin_inff() : value_of<T>(raw_cut);
+}
+
 // ---------------------------------------------------------------------------
 // verify_rows
+//
+// A bf16 row has few distinct values, and everything a summary holds is a function of how often each occurs: one streaming
+// pass counts the values of 2^-7 <= |x| < 2^8 in 3840 bins (15 KB of LDS, so that three workgroups share a CU and one row's
+// tail runs under the reads of the others), lists the few smaller ones, and drops x <= -2^8, which has no mass next to an
+// ordinary maximum.  The masses are then evaluated once per occupied bin instead of once per entry, and a scan over the bins
+// in descending order finds the cuts.  Rows it cannot describe (values of 2^8 and above, NaN, a maximum or a cut among the
+// small values, dropped values that would count) take the radix path, as fp16 and fp32 rows do.
 // ---------------------------------------------------------------------------
+constexpr int HIST_SIDE = 15 * 128;          // values of one sign: 15 octaves of 128
+constexpr int HIST_BINS = 2 * HIST_SIDE;     // ascending: negative values first
+constexpr int HIST_POS = HIST_BINS + 1;      // positions in descending order: positive bins, the small values, negative bins
+constexpr int HIST_PER = (HIST_POS + S_THREADS - 1) / S_THREADS;
+constexpr uint32_t MAG_LOW = 0x3C00u, MAG_HIGH = 0x4380u;  // bits of 2^-7 and 2^8
+constexpr int TINY_CAP = 2048;
+static_assert(MAG_HIGH - MAG_LOW == uint32_t(HIST_SIDE), "the bins cover [2^-7, 2^8)");
+
+struct HistRow {
+    uint32_t bin[HIST_BINS];
+    uint16_t tiny[TINY_CAP];
+    uint32_t n_tiny, n_zero, give_up, dropped;
+    uint32_t first, kpos, kstar, best, kcut, n_cut, last;
+    unsigned long long before;
+    uint64_t wave_u64[S_WAVES];
+    uint32_t wave_u32[S_WAVES];
+};
 struct VerifyShared {
-    Shared sh;
+    union {
+        Shared sh;
+        HistRow hist;
+    };
     PolicyLse lse;
-    uint32_t rank_needed, ties_before;
+    uint32_t ties_before;
 };
 
+__device__ __forceinline__ uint32_t raw_of_bin(int bin) {
+    return bin >= HIST_SIDE ? MAG_LOW + uint32_t(bin - HIST_SIDE) : 0x8000u | (MAG_LOW + uint32_t(HIST_SIDE - 1 - bin));
+}
+__device__ __forceinline__ int bin_of_pos(int q) { return q < HIST_SIDE ? HIST_BINS - 1 - q : HIST_BINS - q; }
+
+// False: the row needs the radix path (nothing is decided).  Every thread gets the results; *lse only with want_lse.
+__device__ __forceinline__ bool hist_cut(HistRow &h, const uint16_t *rp, int vocab, const Filter &f, bool want_lse, RowCut &cut,
+                                         uint32_t &raw_cut, double &lse) {
+    const int tid = threadIdx.x;
+    for (int i = tid; i < HIST_BINS; i += S_THREADS) h.bin[i] = 0;
+    if (tid == 0) { h.n_tiny = h.n_zero = h.give_up = h.dropped = 0; h.best = h.last = 0; h.n_cut = 0; h.before = ~0ull; }
+    __syncthreads();
+    // ---- one pass over the row -------------------------------------------------------------
+    {
+        uint32_t zeros = 0, high = 0, low = 0;
+        auto odd = [&](uint32_t x) {  // |x| outside the bins
+            const uint32_t mag = x & 0x7fffu;
+            if (mag == 0) ++zeros;
+            else if (mag < MAG_LOW) {
+                const uint32_t at = atomicAdd(&h.n_tiny, 1u);
+                if (at < uint32_t(TINY_CAP)) h.tiny[at] = uint16_t(x);
+            } else if ((x & 0x8000u) == 0 || mag > 0x7f80u) high = 1;
+            else low = 1;
+        };
+        auto count = [&](uint32_t x) {
+            const uint32_t m = (x & 0x7fffu) - MAG_LOW, sign = uint32_t(int32_t(x << 16) >> 31);
+            if (m < uint32_t(HIST_SIDE)) atomicAdd(&h.bin[HIST_SIDE + int(m ^ sign)], 1u);
+            else odd(x & 0xffffu);
+        };
+        auto count_vector = [&](const uint4 &q) {
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                count(w[j]);
+                count(w[j] >> 16);
+            }
+        };
+        int head = int((16 - (reinterpret_cast<uintptr_t>(rp) & 15)) & 15) / 2;  // entries before the first whole vector
+        head = head < vocab ? head : vocab;
+        if (tid < head) count(rp[tid]);
+        const uint4 *vp = reinterpret_cast<const uint4 *>(rp + head);
+        const int nvec = (vocab - head) / 8;
+        constexpr int U = 8;  // loads in flight per lane
+        int v = tid;
+        for (; v + (U - 1) * S_THREADS < nvec; v += U * S_THREADS) {
+            uint4 q[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) q[u] = load_stream(vp + v + u * S_THREADS);
+#pragma unroll
+            for (int u = 0; u < U; ++u) count_vector(q[u]);
+        }
+        for (; v < nvec; v += S_THREADS) count_vector(load_stream(vp + v));
+        const int i = head + nvec * 8 + tid;
+        if (i < vocab) count(rp[i]);
+        if (zeros) atomicAdd(&h.n_zero, zeros);
+        if (high) h.give_up = 1;
+        if (low) h.dropped = 1;
+    }
+    __syncthreads();
+    const uint32_t n_tiny = h.n_tiny, n_zero = h.n_zero, dropped = h.dropped;
+    if (h.give_up != 0 || n_tiny > uint32_t(TINY_CAP)) return false;
+    const uint32_t n_mid = n_tiny + n_zero;
+    auto key_of_raw = [&](uint32_t raw) { return elem_key<Bf16>(uint16_t(raw), f.temp, f.has_t); };
+
+    // ---- the thread's positions ------------------------------------------------------------
+    uint32_t c[HIST_PER], sk[HIST_PER], mine = 0;
+#pragma unroll
+    for (int j = 0; j < HIST_PER; ++j) {
+        const int q = tid * HIST_PER + j;
+        c[j] = q >= HIST_POS ? 0u : (q == HIST_SIDE ? n_mid : h.bin[bin_of_pos(q)]);
+        mine += c[j];
+    }
+    uint32_t counted;
+    const uint32_t rank0 = block_excl_scan<uint32_t>(mine, h.wave_u32, &counted);
+    if (counted == 0) return false;
+    if (rank0 == 0 && mine > 0) {
+        int j = 0;
+        while (c[j] == 0) ++j;
+        h.first = uint32_t(tid * HIST_PER + j);
+    }
+    if (f.use_k && rank0 < uint32_t(f.top_k) && uint32_t(f.top_k) <= rank0 + mine) {
+        uint32_t run = rank0;
+        int at = 0;
+#pragma unroll
+        for (int j = 0; j < HIST_PER; ++j) {
+            if (run < uint32_t(f.top_k) && uint32_t(f.top_k) <= run + c[j]) at = j;
+            run += c[j];
+        }
+        const int q = tid * HIST_PER + at;
+        h.kpos = uint32_t(q);
+        h.kstar = q == HIST_SIDE ? 0u : key_of_raw(raw_of_bin(bin_of_pos(q)));
+    }
+    __syncthreads();
+    const int first = int(h.first);
+    if (first == HIST_SIDE || (f.use_k && (counted < uint32_t(f.top_k) || h.kpos == uint32_t(HIST_SIDE)))) return false;
+    const uint32_t raw_max = raw_of_bin(bin_of_pos(first));
+    const uint32_t kmax = key_of_raw(raw_max);
+    const float vmax = value_of<Bf16>(kmax), xmax = Bf16::widen(uint16_t(raw_max));
+    const uint32_t kstar = f.use_k ? h.kstar : 0u;
+    const uint32_t key_dropped = key_of_raw(0x8000u | MAG_HIGH), key_tiny = key_of_raw(MAG_LOW - 1), key_tiny_neg = key_of_raw(0x8000u | (MAG_LOW - 1));
+    if (dropped && (weight_fix(value_of<Bf16>(key_dropped) - vmax) != 0 || weight_fix(-256.0f - xmax) != 0)) return false;
+    // a cut that shares its scaled value with entries that are not binned (a temperature that folds values together)
+    auto shared_value = [&](uint32_t key, int q) {
+        return (dropped && key <= key_dropped) || (n_mid > 0 && (q < HIST_SIDE ? key <= key_tiny : key >= key_tiny_neg));
+    };
+    if (f.use_k && shared_value(kstar, int(h.kpos))) return false;
+    auto weight_of = [&](uint32_t key) { return weight_fix(key == kmax ? 0.0f : value_of<Bf16>(key) - vmax); };
+
+    // ---- masses ----------------------------------------------------------------------------
+    uint64_t mid = 0;
+    for (int i = tid; i < int(n_tiny); i += S_THREADS) mid += weight_of(key_of_raw(h.tiny[i]));
+    if (tid == 0 && n_zero) mid += n_zero * weight_of(key_of_raw(0));
+    uint64_t mid_mass = 0;
+    if (n_mid) block_excl_scan<uint64_t>(mid, h.wave_u64, &mid_mass);
+    uint64_t m[HIST_PER], sum = 0, sum_raw = 0;
+#pragma unroll
+    for (int j = 0; j < HIST_PER; ++j) {
+        const int q = tid * HIST_PER + j;
+        m[j] = 0;
+        sk[j] = 0;
+        if (c[j] == 0) continue;
+        if (q == HIST_SIDE) {
+            m[j] = !f.use_k || int(h.kpos) > HIST_SIDE ? mid_mass : 0ull;
+        } else {
+            const uint32_t raw = raw_of_bin(bin_of_pos(q));
+            sk[j] = key_of_raw(raw);
+            const uint64_t w = weight_of(sk[j]) * c[j];
+            if (sk[j] >= kstar) m[j] = w;
+            if (want_lse) sum_raw += f.has_t ? weight_fix(Bf16::widen(uint16_t(raw)) - xmax) * c[j] : w;
+        }
+        sum += m[j];
+    }
+    uint64_t z_topk, z_raw = 0;
+    uint64_t run = block_excl_scan<uint64_t>(sum, h.wave_u64, &z_topk);
+    if (want_lse) {
+        if (n_mid) {
+            if (f.has_t) {
+                for (int i = tid; i < int(n_tiny); i += S_THREADS) sum_raw += weight_fix(Bf16::widen(h.tiny[i]) - xmax);
+                if (tid == 0 && n_zero) sum_raw += n_zero * weight_fix(-xmax);
+            } else {
+                sum_raw += mid;
+            }
+        }
+        block_excl_scan<uint64_t>(sum_raw, h.wave_u64, &z_raw);
+        // ln(z_raw 2^-40) + max: the masses round the row's exponentials down to 2^-40 of the largest, 1.2e-7 of the sum at most
+        lse = double(xmax) + log(double(z_raw)) - FIX_BITS * 0.693147180559945309417232;
+    }
+    cut.kmax = kmax;
+    cut.kstar = cut.kcut = kstar;
+    cut.r_cut = 0xffffffffu;
+    cut.z = z_topk;
+    raw_cut = 0;
+    if (!f.use_k && !f.use_p) return true;
+    // ---- top-p -----------------------------------------------------------------------------
+    if (f.use_p) {
+        const uint64_t theta = floor_scale(f.top_p, z_topk);
+        int best = -1;
+        uint64_t upto = run;
+#pragma unroll
+        for (int j = 0; j < HIST_PER; ++j) {
+            const int q = tid * HIST_PER + j;
+            const bool in = c[j] > 0 && (q == HIST_SIDE ? (!f.use_k || int(h.kpos) > HIST_SIDE) : sk[j] >= kstar);
+            if (in && upto <= theta) best = q;
+            upto += m[j];
+        }
+        if (best >= 0) atomicMax(&h.best, uint32_t(best));
+        __syncthreads();
+        best = int(h.best);
+        if (best == HIST_SIDE) return false;
+        const uint32_t kcut = key_of_raw(raw_of_bin(bin_of_pos(best)));
+        if (shared_value(kcut, best)) return false;
+        upto = run;
+#pragma unroll
+        for (int j = 0; j < HIST_PER; ++j) {
+            if (c[j] > 0 && sk[j] == kcut) {
+                atomicAdd(&h.n_cut, c[j]);
+                atomicMin(&h.before, (unsigned long long)upto);
+            }
+            upto += m[j];
+        }
+        __syncthreads();
+        const uint32_t n_cut = h.n_cut;
+        const uint64_t before = h.before, w_cut = weight_of(kcut);
+        uint64_t r = n_cut;
+        if (w_cut > 0) {
+            const uint64_t fit = (theta - before) / w_cut + 1;  // entries t with before + t * w <= theta
+            r = fit < r ? fit : r;
+        }
+        cut.kcut = kcut;
+        cut.r_cut = r == n_cut ? 0xffffffffu : uint32_t(r);
+        cut.z = before + r * w_cut;
+    }
+#pragma unroll
+    for (int j = 0; j < HIST_PER; ++j)
+        if (c[j] > 0 && sk[j] >= cut.kcut) atomicMax(&h.last, uint32_t(tid * HIST_PER + j));
+    __syncthreads();
+    raw_cut = masked_key<Bf16>(Bf16::widen(uint16_t(raw_of_bin(bin_of_pos(int(h.last))))));
+    return true;
+}
+
+// The smallest unscaled key whose scaled value reaches kcut, by all lanes of the wavefront at once: near kcut's value times
+// the temperature.  0 where it is not found there (underflow, infinities): the later passes then scale every entry.
+template <typename T> __device__ __forceinline__ uint32_t raw_key_of_cut(uint32_t kcut, float temp, bool has_t) {
+    if (!has_t || kcut == 0) return kcut;
+    const uint32_t near = masked_key<T>(value_of<T>(kcut) * temp);
+    const int lane = int(threadIdx.x) & (kWave - 1);
+    const uint32_t mine = near + uint32_t(lane - kWave / 2) * key_step<T>();
+    const float x = value_of<T>(mine);
+    const uint64_t reach = __ballot(x == x && elem_key<T>(raw_of_key<T>(mine), temp, true) >= kcut);
+    // a run of lanes up to the last one, not all of them
+    if (reach == 0 || reach == ~uint64_t(0) || (reach >> 63) == 0) return 0;
+    const int low = __ffsll((long long)reach) - 1;
+    if ((reach >> low) != (~uint64_t(0) >> low)) return 0;
+    return near + uint32_t(low - kWave / 2) * key_step<T>();
+}
+
 template <typename T>
-__global__ __launch_bounds__(S_THREADS) void verify_rows(VerifyParams p) {
+__global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(4))) void verify_rows(VerifyParams p) {
     __shared__ VerifyShared lds;
     const int tid = threadIdx.x;
     const int64_t n_target = int64_t(p.batch) * (p.k + 1);
@@ -166,9 +426,22 @@ __global__ __launch_bounds__(S_THREADS) void verify_rows(VerifyParams p) {
     const typename T::raw_t *rp = is_target ? target_row<T>(p, b, j) : draft_row<T>(p, b, j);
     const bool vec = (is_target ? p.vec_target : p.vec_draft) != 0;
     const Filter f = filter_of(p, b);
-    const RowCut cut = radix_cut<T>(lds.sh, rp, p.vocab, vec, f.temp, f.has_t, f.use_k, f.top_k, f.use_p, f.top_p, true);
     const bool want_lse = is_target && p.out_policy != nullptr;
-    if (want_lse) row_lse_to_block<T>(rp, p.vocab, vec, lds.lse);
+    RowCut cut;
+    uint32_t raw_cut = 0;
+    double lse = 0.0;
+    bool done = false;
+    if constexpr (T::kDtype == KA_DTYPE_BF16) done = hist_cut(lds.hist, rp, p.vocab, f, want_lse, cut, raw_cut, lse);
+    if (!done) {
+        __syncthreads();
+        cut = radix_cut<T>(lds.sh, rp, p.vocab, vec, f.temp, f.has_t, f.use_k, f.top_k, f.use_p, f.top_p, true);
+        if (f.use_k || f.use_p) raw_cut = raw_key_of_cut<T>(cut.kcut, f.temp, f.has_t);
+        if (want_lse) {
+            row_lse_to_block<T>(rp, p.vocab, vec, lds.lse);
+            __syncthreads();
+            if (tid == 0) lse = lds.lse.value();
+        }
+    }
 
     // mass of the drafted token; where it sits in a tie group that survives in part, its rank in the group decides
     const int64_t d = j < len ? p.draft_ids[int64_t(b) * p.k + j] : -1;
@@ -185,65 +458,96 @@ __global__ __launch_bounds__(S_THREADS) void verify_rows(VerifyParams p) {
         __syncthreads();
         kept = lds.ties_before < cut.r_cut;
     }
-    __syncthreads();  // also: the partial log-sum-exps are in place
     if (tid == 0) {
         RowSummary s;
         s.z = cut.z;
         s.w_draft = kept ? weight_fix(key == cut.kmax ? 0.0f : value_of<T>(key) - value_of<T>(cut.kmax)) : 0ull;
-        s.lse = want_lse ? lds.lse.value() : 0.0;
+        s.lse = lse;
         s.kmax = cut.kmax;
         s.kcut = cut.kcut;
         s.r_cut = cut.r_cut;
-        s.pad = 0;
+        s.raw_cut = raw_cut;
         p.rows[r] = s;
     }
 }
 
 // ---------------------------------------------------------------------------
-// verify_ties: grid (B, 2).  Where a row's cut falls inside a tie group, the index below which the group's entries survive.
+// verify_ties: grid (B, 2).  Where a row's cut falls inside a tie group, the index below which the group's entries survive:
+// the ties of every chunk of 512 vectors are counted, and the chunk that holds the last survivor is read once more in order.
 // ---------------------------------------------------------------------------
+constexpr int MAX_CHUNKS = (1 << 22) / (4 * S_THREADS);
 template <typename T>
 __global__ __launch_bounds__(S_THREADS) void verify_ties(VerifyParams p) {
-    __shared__ uint32_t wave_ties[S_WAVES];
-    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    __shared__ uint32_t ties[MAX_CHUNKS];
+    __shared__ uint32_t wave_buf[S_WAVES];
+    __shared__ uint32_t s_chunk, s_before;
+    constexpr int EPV = T::kPerVec;
+    const int b = blockIdx.x, tid = threadIdx.x;
     const bool is_target = blockIdx.y == 0;
     const int len = draft_len(p, b);
     const int n = accepted_prefix(p, b, len);
     if (!is_target && (n == len || p.draft == nullptr)) return;
     const int64_t row = is_target ? int64_t(b) * (p.k + 1) + n : int64_t(p.batch) * (p.k + 1) + int64_t(b) * p.k + n;
     const uint32_t r_cut = p.rows[row].r_cut, kcut = p.rows[row].kcut;
+    int32_t *const limit = p.tie_limit + 2 * b + (is_target ? 0 : 1);
     if (r_cut == 0xffffffffu) {
-        if (tid == 0) p.tie_limit[2 * b + (is_target ? 0 : 1)] = 0x7fffffff;
+        if (tid == 0) *limit = 0x7fffffff;
         return;
     }
     const Filter f = filter_of(p, b);
     const typename T::raw_t *rp = is_target ? target_row<T>(p, b, n) : draft_row<T>(p, b, n);
-    // every wavefront counts the ties of a contiguous part of the row, steps of 64 entries
-    const int steps = (p.vocab + kWave - 1) / kWave, per_wave = (steps + S_WAVES - 1) / S_WAVES;
-    const int s0 = wave * per_wave, s1 = s0 + per_wave < steps ? s0 + per_wave : steps;
-    uint32_t mine = 0;
-#pragma unroll 4
-    for (int s = s0; s < s1; ++s) {
-        const int i = s * kWave + lane;
-        mine += (i < p.vocab && elem_key<T>(rp[i], f.temp, f.has_t) == kcut) ? 1u : 0u;
-    }
-    const uint32_t total = uint32_t(__builtin_amdgcn_readlane(int(wave_incl_scan_u32(mine)), kWave - 1));
-    if (lane == 0) wave_ties[wave] = total;
+    const bool vec = (is_target ? p.vec_target : p.vec_draft) != 0;
+    const float low = cut_value<T>(p.rows[row].raw_cut);
+    auto ties_of = [&](const typename T::raw_t (&e)[EPV], int base) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int j = 0; j < EPV; ++j)
+            if (!(T::widen(e[j]) < low) && base + j < p.vocab && elem_key<T>(e[j], f.temp, f.has_t) == kcut) ++c;
+        return c;
+    };
+    const int chunks = (p.vocab + EPV * S_THREADS - 1) / (EPV * S_THREADS);
+    for (int i = tid; i < chunks; i += S_THREADS) ties[i] = 0;
     __syncthreads();
-    uint32_t before = 0;
-    for (int w = 0; w < wave; ++w) before += wave_ties[w];
-    if (before < r_cut && r_cut <= before + total) {  // the last surviving tie is in this wavefront's part
-        for (int s = s0; s < s1; ++s) {
-            const int i = s * kWave + lane;
-            const uint64_t hit = __ballot(i < p.vocab && elem_key<T>(rp[i], f.temp, f.has_t) == kcut);
-            const uint32_t here = uint32_t(__popcll(hit));
-            if (before + here >= r_cut) {
-                const uint32_t rank = before + uint32_t(__popcll(hit & ((uint64_t(1) << lane) - 1)));
-                if (((hit >> lane) & 1) != 0 && rank + 1 == r_cut) p.tie_limit[2 * b + (is_target ? 0 : 1)] = i + 1;
-                break;
-            }
-            before += here;
+    constexpr int U = 8;  // vectors in flight per lane
+    for (int c0 = 0; c0 < chunks; c0 += U) {
+        typename T::raw_t e[U][EPV];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_entries<T>(rp, vec, p.vocab, ((c0 + u) * S_THREADS + tid) * int64_t(EPV), e[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t base = ((c0 + u) * S_THREADS + tid) * int64_t(EPV);
+            if (base >= p.vocab) continue;
+            const uint32_t c = ties_of(e[u], int(base));
+            if (c) atomicAdd(&ties[c0 + u], c);
         }
+    }
+    __syncthreads();
+    // chunks in order: thread t takes a run of them
+    const int per = (chunks + S_THREADS - 1) / S_THREADS;
+    uint32_t mine = 0, total;
+    for (int i = 0; i < per; ++i) mine += tid * per + i < chunks ? ties[tid * per + i] : 0u;
+    const uint32_t before = block_excl_scan<uint32_t>(mine, wave_buf, &total);
+    if (before < r_cut && r_cut <= before + mine) {
+        uint32_t at = before;
+        for (int i = 0; i < per; ++i) {
+            const uint32_t c = ties[tid * per + i];
+            if (r_cut <= at + c) { s_chunk = uint32_t(tid * per + i); s_before = at; break; }
+            at += c;
+        }
+    }
+    __syncthreads();
+    const int64_t base = (int64_t(s_chunk) * S_THREADS + tid) * EPV;
+    typename T::raw_t e[EPV];
+    load_entries<T>(rp, vec, p.vocab, base, e);
+    const uint32_t c = base < p.vocab ? ties_of(e, int(base)) : 0u;
+    const uint32_t rank = s_before + block_excl_scan<uint32_t>(c, wave_buf, &total);
+    if (rank < r_cut && r_cut <= rank + c) {
+        uint32_t at = rank;
+        int32_t found = 0;
+#pragma unroll
+        for (int j = 0; j < EPV; ++j)
+            if (base + j < p.vocab && elem_key<T>(e[j], f.temp, f.has_t) == kcut && ++at == r_cut) found = int32_t(base) + j + 1;
+        *limit = found;
     }
 }
 
@@ -266,6 +570,7 @@ template <typename T> struct Residual {
     const typename T::raw_t *rp, *rq;  // rq null: nothing is subtracted
     bool vec_p, vec_q;
     RowDist p, q;
+    float low_p, low_q;  // unscaled values below these have no mass
     uint64_t mul_p, mul_q;
     int64_t skip;  // the rejected look-up draft, or -1
     Filter f;
@@ -284,12 +589,14 @@ template <typename T> struct Residual {
         vec_q = false;
         skip = -1;
         q = p;
+        low_p = low_q = cut_value<T>(t.raw_cut);
         if (n < len) {
             if (v.draft != nullptr) {
                 const RowSummary &d = v.rows[int64_t(v.batch) * (v.k + 1) + int64_t(b) * v.k + n];
                 rq = draft_row<T>(v, b, n);
                 vec_q = v.vec_draft != 0;
                 q = RowDist{d.kmax, d.kcut, v.may_cut_ties ? v.tie_limit[2 * b + 1] : 0x7fffffff, value_of<T>(d.kmax)};
+                low_q = cut_value<T>(d.raw_cut);
                 mul_p = d.z;
                 mul_q = t.z;
             } else {
@@ -297,36 +604,43 @@ template <typename T> struct Residual {
             }
         }
     }
-    __device__ __forceinline__ void load(const typename T::raw_t *row, bool vec, int base, typename T::raw_t (&e)[T::kPerVec]) const {
-        constexpr int EPV = T::kPerVec;
-        if (vec && base + EPV <= vocab) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(row + base);
-            __builtin_memcpy(e, &v, 16);
-        } else {
-#pragma unroll
-            for (int j = 0; j < EPV; ++j) e[j] = base + j < vocab ? row[base + j] : typename T::raw_t(0);
-        }
-    }
     __device__ __forceinline__ u128 entry(typename T::raw_t x, typename T::raw_t y, int i) const {
-        if (i >= vocab || int64_t(i) == skip) return 0;
+        if (T::widen(x) < low_p || i >= vocab || int64_t(i) == skip) return 0;
         const uint64_t wp = p.template mass<T>(elem_key<T>(x, f.temp, f.has_t), i);
         if (wp == 0) return 0;
         if (rq == nullptr) return wp;
         const u128 have = u128(wp) * mul_p;
+        if (T::widen(y) < low_q) return have;
         const u128 take = u128(q.template mass<T>(elem_key<T>(y, f.temp, f.has_t), i)) * mul_q;
         return have > take ? have - take : u128(0);
     }
-    // sum over the vector of entries that starts at `base`; each(j, mass) is called for every entry in order
-    template <typename F> __device__ __forceinline__ void vector(int base, F &&each) const {
+    // residual masses of the vector that starts at `base` (0 behind the row)
+    __device__ __forceinline__ void vector(int64_t base, u128 (&m)[T::kPerVec]) const {
         constexpr int EPV = T::kPerVec;
-        if (base >= vocab) return;
         typename T::raw_t x[EPV], y[EPV];
-        load(rp, vec_p, base, x);
-        if (rq != nullptr) load(rq, vec_q, base, y);
+        load_entries<T>(rp, vec_p, vocab, base, x);
+        if (rq != nullptr) load_entries<T>(rq, vec_q, vocab, base, y);
 #pragma unroll
-        for (int j = 0; j < EPV; ++j) each(base + j, entry(x[j], rq != nullptr ? y[j] : typename T::raw_t(0), base + j));
+        for (int j = 0; j < EPV; ++j) m[j] = base + j < vocab ? entry(x[j], rq != nullptr ? y[j] : typename T::raw_t(0), int(base) + j) : u128(0);
     }
 };
+
+// The entry of a vector of masses, `before` of mass in front of it, that holds tau.
+template <int EPV> __device__ __forceinline__ int entry_at(const u128 (&m)[EPV], u128 before, u128 tau) {
+    int hit = -1;
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) {
+        before += m[j];
+        if (hit < 0 && tau < before) hit = j;
+    }
+    return hit;
+}
+template <int EPV> __device__ __forceinline__ u128 total_of(const u128 (&m)[EPV]) {
+    u128 sum = 0;
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) sum += m[j];
+    return sum;
+}
 
 __device__ __forceinline__ u128 shfl_up_u128(u128 v, int off) {
     const uint64_t lo = __shfl_up((unsigned long long)uint64_t(v), off, kWave);
@@ -360,98 +674,77 @@ template <int WAVES> __device__ __forceinline__ u128 block_excl_scan_u128(u128 v
     return base + inc - v;
 }
 
-// grid (n_shares, B)
+// grid (groups of shares, B): a wavefront per share
 template <typename T>
 __global__ __launch_bounds__(SHARE_THREADS) void verify_shares(VerifyParams p) {
-    __shared__ u128 wave_buf[SHARE_THREADS / kWave];
-    const int b = blockIdx.y, share = blockIdx.x;
+    const int b = blockIdx.y, lane = threadIdx.x & (kWave - 1);
+    const int share = int(blockIdx.x) * (SHARE_THREADS / kWave) + int(threadIdx.x) / kWave;
     const int len = draft_len(p, b);
     const int n = accepted_prefix(p, b, len);
+    if (share >= p.n_shares) return;
     Residual<T> res;
     res.setup(p, b, n, len);
     u128 sum = 0;
 #pragma unroll 1
-    for (int s = 0; s < SHARE_VECS / SHARE_THREADS; ++s) {
-        const int64_t base = (int64_t(share) * SHARE_VECS + s * SHARE_THREADS + int(threadIdx.x)) * T::kPerVec;
-        if (base < p.vocab) res.vector(int(base), [&](int, u128 m) { sum += m; });
+    for (int s = 0; s < SHARE_VECS / kWave; ++s) {
+        const int64_t base = (int64_t(share) * SHARE_VECS + s * kWave + lane) * T::kPerVec;
+        u128 m[T::kPerVec];
+        res.vector(base, m);
+        sum += total_of(m);
     }
-    u128 total;
-    block_excl_scan_u128<SHARE_THREADS / kWave>(sum, wave_buf, &total);
-    if (threadIdx.x == 0) p.shares[int64_t(b) * p.n_shares + share] = total;
+    sum = wave_incl_scan_u128(sum);
+    if (lane == kWave - 1) p.shares[int64_t(b) * p.n_shares + share] = sum;
 }
 
 // grid B; a thread per vector of the share that holds the draw
 template <typename T>
 __global__ __launch_bounds__(SHARE_VECS) void verify_draw(VerifyParams p) {
-    __shared__ u128 wave_buf[SHARE_VECS / kWave];
+    constexpr int WAVES = SHARE_VECS / kWave;
+    __shared__ u128 wave_buf[WAVES];
     __shared__ u128 s_before;
     __shared__ int s_share, s_hit;
     const int b = blockIdx.x, tid = threadIdx.x;
     const int len = draft_len(p, b);
     const int n = accepted_prefix(p, b, len);
     if (tid == 0) { s_share = -1; s_hit = -1; }
-    // the share that holds floor(u * R)
+    const float u = clean_uniform(p.uniforms[int64_t(b) * (p.k + 1) + p.k]);
+    // the share that holds floor(u * R): thread t takes a run of shares
     u128 mine = 0, r;
-    const int per = (p.n_shares + SHARE_VECS - 1) / SHARE_VECS;  // 1 up to 2^22 fp32 entries
-    for (int i = 0; i < per; ++i) {
-        const int s = tid * per + i;
-        if (s < p.n_shares) mine += p.shares[int64_t(b) * p.n_shares + s];
-    }
-    const u128 excl = block_excl_scan_u128<SHARE_VECS / kWave>(mine, wave_buf, &r);
-    const u128 tau = floor_scale_wide(clean_uniform(p.uniforms[int64_t(b) * (p.k + 1) + p.k]), r);
+    const int per = (p.n_shares + SHARE_VECS - 1) / SHARE_VECS;
+    const u128 *const shares = p.shares + int64_t(b) * p.n_shares;
+    for (int i = 0; i < per; ++i)
+        if (tid * per + i < p.n_shares) mine += shares[tid * per + i];
+    const u128 excl = block_excl_scan_u128<WAVES>(mine, wave_buf, &r);
+    u128 tau = floor_scale_wide(u, r);
     if (excl <= tau && tau < excl + mine) {
         u128 at = excl;
         for (int i = 0; i < per; ++i) {
-            const int s = tid * per + i;
-            const u128 m = s < p.n_shares ? p.shares[int64_t(b) * p.n_shares + s] : u128(0);
-            if (tau < at + m) { s_share = s; s_before = at; break; }
+            const u128 m = shares[tid * per + i];
+            if (tau < at + m) { s_share = tid * per + i; s_before = at; break; }
             at += m;
         }
     }
+    Residual<T> res;
+    res.setup(p, b, n, len);
     __syncthreads();
-    const int share = s_share;
-    if (r == 0) {
-        // no residual (see the head of the file): drawn from P, share after share
-        Residual<T> res;
-        res.setup(p, b, n, len);
+    int share = s_share, last = share;
+    u128 at = share >= 0 ? s_before : u128(0);
+    if (r == 0) {  // no residual (see the head of the file): drawn from P, share after share
         res.rq = nullptr;
         res.skip = -1;
-        const u128 target = floor_scale_wide(clean_uniform(p.uniforms[int64_t(b) * (p.k + 1) + p.k]),
-                                             p.rows[int64_t(b) * (p.k + 1) + n].z);
-        u128 at = 0;
-        for (int s = 0; s < p.n_shares; ++s) {  // block-uniform: `at` and the totals are
-            const int64_t base = (int64_t(s) * SHARE_VECS + tid) * T::kPerVec;
-            u128 sum = 0, total;
-            if (base < p.vocab) res.vector(int(base), [&](int, u128 m) { sum += m; });
-            const u128 before = at + block_excl_scan_u128<SHARE_VECS / kWave>(sum, wave_buf, &total);
-            if (before <= target && target < before + sum) {
-                u128 upto = before;
-                int hit = -1;
-                res.vector(int(base), [&](int i, u128 m) {
-                    upto += m;
-                    if (hit < 0 && target < upto) hit = i;
-                });
-                s_hit = hit;
-            }
-            at += total;
-            if (target < at) break;
-        }
-    } else if (share >= 0) {  // the same for the whole block
-        Residual<T> res;
-        res.setup(p, b, n, len);
+        tau = floor_scale_wide(u, p.rows[int64_t(b) * (p.k + 1) + n].z);
+        share = 0;
+        last = p.n_shares - 1;
+    }
+    for (; share >= 0 && share <= last; ++share) {  // block-uniform, one turn unless r is 0
         const int64_t base = (int64_t(share) * SHARE_VECS + tid) * T::kPerVec;
-        u128 sum = 0, total;
-        if (base < p.vocab) res.vector(int(base), [&](int, u128 m) { sum += m; });
-        const u128 before = s_before + block_excl_scan_u128<SHARE_VECS / kWave>(sum, wave_buf, &total);
-        if (before <= tau && tau < before + sum) {
-            u128 at = before;
-            int hit = -1;
-            res.vector(int(base), [&](int i, u128 m) {
-                at += m;
-                if (hit < 0 && tau < at) hit = i;
-            });
-            s_hit = hit;
-        }
+        u128 m[T::kPerVec], total;
+        res.vector(base, m);
+        const u128 sum = total_of(m);
+        const u128 before = at + block_excl_scan_u128<WAVES>(sum, wave_buf, &total);
+        if (before <= tau && tau < before + sum) s_hit = int(base) + entry_at(m, before, tau);
+        at += total;
+        if (tau < at) break;
     }
     __syncthreads();
     // outputs: lane j writes position j
@@ -478,7 +771,7 @@ template <typename T> int launch_verify(const VerifyParams &p, hipStream_t strea
         rc = check_hip(hipGetLastError(), "verify launch (ties)");
         if (rc != KA_OK) return rc;
     }
-    hipLaunchKernelGGL((verify_shares<T>), dim3(unsigned(p.n_shares), unsigned(p.batch)), dim3(SHARE_THREADS), 0, stream, p);
+    hipLaunchKernelGGL((verify_shares<T>), dim3(unsigned((p.n_shares * kWave + SHARE_THREADS - 1) / SHARE_THREADS), unsigned(p.batch)), dim3(SHARE_THREADS), 0, stream, p);
     rc = check_hip(hipGetLastError(), "verify launch (shares)");
     if (rc != KA_OK) return rc;
     hipLaunchKernelGGL((verify_draw<T>), dim3(unsigned(p.batch)), dim3(SHARE_VECS), 0, stream, p);
