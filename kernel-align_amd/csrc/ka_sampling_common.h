@@ -320,20 +320,29 @@ constexpr int LSE_PER_THREAD = LSE_LANES / S_THREADS;
 struct PolicyLse {  // in LDS
     float wave_ml2[LSE_WAVES];  // maximum * log2(e) of the elements of each wavefront of the 1024-lane order
     float wave_s[LSE_WAVES];    // sum of 2^(x * log2(e) - wave_ml2)
-    // the log-sum-exp (after a barrier behind to_block)
-    __device__ __forceinline__ double value() const {
-        float big = wave_ml2[0];
+    // the row's maximum times log2(e), and the sum of 2^(x log2(e) - that) (after a barrier behind to_block)
+    __device__ __forceinline__ void fold(float &big, float &total) const {
+        big = wave_ml2[0];
 #pragma unroll
         for (int w = 1; w < LSE_WAVES; ++w) big = fmaxf(big, wave_ml2[w]);
-        float total = 0.0f;
+        total = 0.0f;
 #pragma unroll
         for (int w = 0; w < LSE_WAVES; ++w) total += wave_s[w] * fast_exp2(wave_ml2[w] - big);
-        return (double(big) + log2(double(total))) * 0.693147180559945309417232;
+    }
+    // log-sum-exp = top + ln(sum)
+    __device__ __forceinline__ void parts(float &top, double &sum) const {
+        float big, total;
+        fold(big, total);
+        top = float(double(big) * 0.693147180559945309417232);
+        sum = double(total) * exp(double(big) * 0.693147180559945309417232 - double(top));
     }
     // log-probability of element `hit` of the row (thread 0, after a barrier behind to_block)
     template <typename T> __device__ __forceinline__ float finish(const typename T::raw_t *rp, int64_t hit, int vocab) const {
         if (hit < 0 || hit >= vocab) return __builtin_nanf("");
-        return float(double(T::widen(rp[hit])) - value());
+        float big, total;
+        fold(big, total);
+        const double lse = (double(big) + log2(double(total))) * 0.693147180559945309417232;
+        return float(double(T::widen(rp[hit])) - lse);
     }
 };
 

@@ -7,12 +7,17 @@
 //   position j accepts d_j  iff  u_j Q(d_j) < P(d_j);  n = the first position that does not, or the number of drafts
 //   ids[n] = inverse CDF, in index order, of max(P - Q, 0) (rejected) or of P (every draft accepted)
 //
-// Everything is decided on integers: u_j W^q Z^p < W^p Z^q (126 bits), residual masses max(W^p Z^q - W^q Z^p, 0) (102 bits
+// Everything is decided as if on integers: u_j W^q Z^p < W^p Z^q (126 bits), residual masses max(W^p Z^q - W^q Z^p, 0) (102 bits
 // each, 124 bits in sum).  A rejected draft with Q(d) > 0 always leaves a residual: P(d) <= u Q(d) < Q(d), both sum to one
 // exactly, so some other entry has P > Q.  A draft that Q cannot have drawn (filtered out, or no entry at all) may meet P = Q:
 // then the token is drawn from P.  Nothing depends on the order of a sum, on the batch or on the launch.
 //
-// Four launches, no host synchronisation:
+// The acceptance is evaluated in those integers.  The draw is first evaluated in fp64, with a bound of its error: each P_i =
+// W^p_i / Z^p is off by 3 * 2^-53 of itself, R_i by 2^-51 (P_i + Q_i), and a sum of them, added in runs and trees of fewer than
+// 2^12 terms, by 2^-41 in all (P and Q sum to one).  An entry whose prefix sums lie more than DRAW_MARGIN = 2^-38 on either side of u R is the
+// integers' answer too; otherwise (about one draw in 10^6, and u = 0) the workgroup repeats the draw in 128-bit integers.
+//
+// Three or four launches, no host synchronisation:
 //   verify_rows    one workgroup per row that counts (target rows 0 .. len, draft rows 0 .. len - 1): the cut of the row's
 //                  distribution, its total mass, the draft token's mass, the log-sum-exp of the raw row.  This is the pass over
 //                  the data: bound by HBM, 2 V (2 K + 1) bytes per request.
@@ -20,9 +25,11 @@
 //                  of the position where the request stops
 //   verify_shares  residual mass of every share of 256 vectors of the stopping position, a wavefront each
 //   verify_draw    one workgroup per request: the share, the vector and the entry that hold the draw; all outputs
-// The rows of the stopping position are read again by the last two, from L2 / MALL as a rule.
+// The rows of the stopping position are read again by the last ones, from L2 / MALL as a rule.
 #define KA_SAMPLING_THREADS 512
 #include <stddef.h>
+
+#include <mutex>
 
 #include "ka_sampling_common.h"
 #include "ka_sampling_radix.h"
@@ -41,11 +48,13 @@ constexpr int SHARE_THREADS = 256;
 struct RowSummary {
     uint64_t z;         // integer mass of the survivors
     uint64_t w_draft;   // of which the drafted token has this (0: filtered out, or an id outside the vocabulary)
-    double lse;         // log-sum-exp of the raw row (target rows, when asked for)
+    double raw_sum;     // log-sum-exp of the raw row = raw_top + ln(raw_sum) (target rows, when asked for)
+    float raw_top;
     uint32_t kmax, kcut, r_cut;  // see RowCut
     uint32_t raw_cut;   // key (unscaled) below which no entry survives; 0: not known, or no filter
+    uint32_t pad;
 };
-static_assert(sizeof(RowSummary) == 40, "the workspace query counts 40 bytes per row");
+static_assert(sizeof(RowSummary) == 48, "the workspace query counts 48 bytes per row");
 
 struct VerifyParams {
     const void *target, *draft;                          // draft may be null
@@ -61,8 +70,8 @@ struct VerifyParams {
     float *out_policy;                                   // may be null
     RowSummary *rows;                                    // [B (K + 1)] target rows, then [B K] draft rows
     int32_t *tie_limit;                                  // [B, 2]: an entry equal to kcut survives iff its index is below this
-    u128 *shares;                                        // [B, n_shares]
-    int32_t n_shares, vec_target, vec_draft, may_cut_ties;
+    double *shares;                                      // [B, n_shares]
+    int32_t n_shares, shares_per_group, vec_target, vec_draft, may_cut_ties;
 };
 
 struct Filter { float temp; bool has_t; bool use_k; int top_k; bool use_p; float top_p; };
@@ -144,15 +153,30 @@ __device__ __forceinline__ int accepted_prefix(const VerifyParams &p, int b, int
 
 // One vector of entries from `base` on; zeros behind the row.
 template <typename T>
-__device__ __forceinline__ void load_entries(const typename T::raw_t *row, bool vec, int vocab, int64_t base, typename T::raw_t (&e)[T::kPerVec]) {
+__device__ __forceinline__ uint4 load_entries(const typename T::raw_t *row, bool vec, int vocab, int64_t base) {
     constexpr int EPV = T::kPerVec;
-    if (vec && base + EPV <= vocab) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(row + base);
-        __builtin_memcpy(e, &v, 16);
-    } else {
+    if (vec && base + EPV <= vocab) return *reinterpret_cast<const uint4 *>(row + base);
+    uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < EPV; ++j) e[j] = base + j < vocab ? row[base + j] : typename T::raw_t(0);
-    }
+    for (int j = 0; j < EPV; ++j)
+        if (base + j < vocab) w[j * T::kBytes / 4] |= uint32_t(row[base + j]) << (T::kBytes == 2 ? 16 * (j & 1) : 0);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Entry j of a vector, j not known at compile time.
+template <typename T> __device__ __forceinline__ typename T::raw_t entry_of(const uint4 &v, int j) {
+    constexpr int HALF = T::kPerVec / 2;
+    const uint64_t lo = (uint64_t(v.y) << 32) | v.x, hi = (uint64_t(v.w) << 32) | v.z;
+    return typename T::raw_t((j & HALF ? hi : lo) >> (8 * T::kBytes * (j & (HALF - 1))));
+}
+// Bit j: entry base + j lies in the row and is not below `low` (NaN is not).
+template <typename T> __device__ __forceinline__ uint32_t at_least(const uint4 &v, float low, int64_t base, int vocab) {
+    float x[T::kPerVec];
+    T::unpack(v, x);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < T::kPerVec; ++j) bits |= !(x[j] < low) ? 1u << j : 0u;
+    const int64_t room = vocab - base;
+    return room >= T::kPerVec ? bits : (room <= 0 ? 0u : bits & ((1u << int(room)) - 1u));
 }
 // The value below which an unscaled entry does not survive (NaN compares as surviving: its key decides).
 template <typename T> __device__ __forceinline__ float cut_value(uint32_t raw_cut) {
@@ -163,28 +187,33 @@ template <typename T> __device__ __forceinline__ float cut_value(uint32_t raw_cu
 // verify_rows
 //
 // A bf16 row has few distinct values, and everything a summary holds is a function of how often each occurs: one streaming
-// pass counts the values of 2^-7 <= |x| < 2^8 in 3840 bins (15 KB of LDS, so that three workgroups share a CU and one row's
+// pass counts the values of 2^-11 <= |x| < 2^8 in 4864 bins (19 KB of LDS, so that three workgroups share a CU and one row's
 // tail runs under the reads of the others), lists the few smaller ones, and drops x <= -2^8, which has no mass next to an
-// ordinary maximum.  The masses are then evaluated once per occupied bin instead of once per entry, and a scan over the bins
-// in descending order finds the cuts.  Rows it cannot describe (values of 2^8 and above, NaN, a maximum or a cut among the
-// small values, dropped values that would count) take the radix path, as fp16 and fp32 rows do.
+// ordinary maximum.  Masses are then evaluated once per occupied bin instead of once per entry (by all threads where a sum
+// over the whole row is needed), and one wavefront walks the bins from the largest value down to the cuts, 64 at a time.  Rows
+// it cannot describe (values of 2^8 and above, NaN, a maximum or a cut among the small values, dropped values that would
+// count) take the radix path, as fp16 and fp32 rows do.
 // ---------------------------------------------------------------------------
-constexpr int HIST_SIDE = 15 * 128;          // values of one sign: 15 octaves of 128
-constexpr int HIST_BINS = 2 * HIST_SIDE;     // ascending: negative values first
-constexpr int HIST_POS = HIST_BINS + 1;      // positions in descending order: positive bins, the small values, negative bins
-constexpr int HIST_PER = (HIST_POS + S_THREADS - 1) / S_THREADS;
-constexpr uint32_t MAG_LOW = 0x3C00u, MAG_HIGH = 0x4380u;  // bits of 2^-7 and 2^8
-constexpr int TINY_CAP = 2048;
-static_assert(MAG_HIGH - MAG_LOW == uint32_t(HIST_SIDE), "the bins cover [2^-7, 2^8)");
+constexpr uint32_t MAG_LOW = 0x3A00u, MAG_HIGH = 0x4380u;  // bits of 2^-11 and 2^8
+constexpr int HIST_SIDE = int(MAG_HIGH - MAG_LOW);         // values of one sign: 19 octaves of 128
+constexpr int HIST_BINS = 2 * HIST_SIDE;                   // ascending: negative values first
+constexpr int HIST_POS = HIST_BINS + 1;                    // positions in descending order: positive bins, the small values, negative bins
+constexpr int TINY_CAP = 1024;
+constexpr int WINDOW = 512;                                // positions whose mass is kept: the walks to the cuts rarely leave them
+constexpr uint32_t NO_KEY = 0;                             // no value of a row has this key
 
 struct HistRow {
     uint32_t bin[HIST_BINS];
     uint16_t tiny[TINY_CAP];
-    uint32_t n_tiny, n_zero, give_up, dropped;
-    uint32_t first, kpos, kstar, best, kcut, n_cut, last;
-    unsigned long long before;
-    uint64_t wave_u64[S_WAVES];
-    uint32_t wave_u32[S_WAVES];
+    uint32_t n_tiny, n_zero, give_up, dropped, first;
+    uint64_t sums[S_WAVES][2];  // per wavefront: mass of all entries, and of the small ones
+    double raw_sums[S_WAVES];   // sum of exp(x - max) over the unscaled row
+    uint64_t win_mass[WINDOW];  // mass and scaled key of the positions from the first occupied one on
+    uint32_t win_key[WINDOW];
+    RowCut cut;
+    uint32_t raw_cut, ok;
+    double raw_sum;
+    float raw_top;
 };
 struct VerifyShared {
     union {
@@ -200,199 +229,279 @@ __device__ __forceinline__ uint32_t raw_of_bin(int bin) {
 }
 __device__ __forceinline__ int bin_of_pos(int q) { return q < HIST_SIDE ? HIST_BINS - 1 - q : HIST_BINS - q; }
 
-// False: the row needs the radix path (nothing is decided).  Every thread gets the results; *lse only with want_lse.
-__device__ __forceinline__ bool hist_cut(HistRow &h, const uint16_t *rp, int vocab, const Filter &f, bool want_lse, RowCut &cut,
-                                         uint32_t &raw_cut, double &lse) {
+__device__ __forceinline__ uint64_t wave_sum_u64_of(uint64_t v) {
+    const uint64_t inc = wave_incl_scan_u64(v);
+    return (uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(inc >> 32)), kWave - 1))) << 32) |
+           uint32_t(__builtin_amdgcn_readlane(int(uint32_t(inc)), kWave - 1));
+}
+
+// Counts the row into h.bin / h.tiny.  A barrier must follow.
+__device__ __forceinline__ void hist_count(HistRow &h, const uint16_t *rp, int vocab) {
     const int tid = threadIdx.x;
-    for (int i = tid; i < HIST_BINS; i += S_THREADS) h.bin[i] = 0;
-    if (tid == 0) { h.n_tiny = h.n_zero = h.give_up = h.dropped = 0; h.best = h.last = 0; h.n_cut = 0; h.before = ~0ull; }
-    __syncthreads();
-    // ---- one pass over the row -------------------------------------------------------------
-    {
-        uint32_t zeros = 0, high = 0, low = 0;
-        auto odd = [&](uint32_t x) {  // |x| outside the bins
-            const uint32_t mag = x & 0x7fffu;
-            if (mag == 0) ++zeros;
-            else if (mag < MAG_LOW) {
-                const uint32_t at = atomicAdd(&h.n_tiny, 1u);
-                if (at < uint32_t(TINY_CAP)) h.tiny[at] = uint16_t(x);
-            } else if ((x & 0x8000u) == 0 || mag > 0x7f80u) high = 1;
-            else low = 1;
-        };
-        auto count = [&](uint32_t x) {
-            const uint32_t m = (x & 0x7fffu) - MAG_LOW, sign = uint32_t(int32_t(x << 16) >> 31);
-            if (m < uint32_t(HIST_SIDE)) atomicAdd(&h.bin[HIST_SIDE + int(m ^ sign)], 1u);
-            else odd(x & 0xffffu);
-        };
-        auto count_vector = [&](const uint4 &q) {
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    uint32_t zeros = 0, high = 0, low = 0;
+    // m = magnitude bits - MAG_LOW (as an unsigned number: below the range wraps to the top), sign = 0 or all ones
+    auto add = [&](uint32_t m, uint32_t sign) { if (m < uint32_t(HIST_SIDE)) atomicAdd(&h.bin[HIST_SIDE + int(m ^ sign)], 1u); };
+    auto odd = [&](uint32_t x) {  // |x| outside the bins
+        const uint32_t mag = x & 0x7fffu;
+        if (mag - MAG_LOW < uint32_t(HIST_SIDE)) return;
+        if (mag == 0) ++zeros;
+        else if (mag < MAG_LOW) {
+            const uint32_t at = atomicAdd(&h.n_tiny, 1u);
+            if (at < uint32_t(TINY_CAP)) h.tiny[at] = uint16_t(x);
+        } else if ((x & 0x8000u) == 0 || mag > 0x7f80u) high = 1;
+        else low = 1;
+    };
+    auto one = [&](uint32_t x) {
+        add((x & 0x7fffu) - MAG_LOW, (x & 0x8000u) ? ~0u : 0u);
+        odd(x);
+    };
+    int head = int((16 - (reinterpret_cast<uintptr_t>(rp) & 15)) & 15) / 2;  // entries before the first whole vector
+    head = head < vocab ? head : vocab;
+    if (tid < head) one(rp[tid]);
+    const uint4 *vp = reinterpret_cast<const uint4 *>(rp + head);
+    const int nvec = (vocab - head) / 8;
+    constexpr int U = 8;  // loads in flight per lane
+    for (int v = tid; v < nvec; v += U * S_THREADS) {
+        uint4 q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = v + u * S_THREADS < nvec ? load_stream(vp + v + u * S_THREADS) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (v + u * S_THREADS >= nvec) continue;
+            const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+            uint32_t worst = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                count(w[j]);
-                count(w[j] >> 16);
+                const uint32_t m0 = (w[j] & 0x7fffu) - MAG_LOW, m1 = ((w[j] >> 16) & 0x7fffu) - MAG_LOW;
+                worst = m0 > worst ? m0 : worst;
+                worst = m1 > worst ? m1 : worst;
+                add(m0, uint32_t(int32_t(w[j] << 16) >> 31));
+                add(m1, uint32_t(int32_t(w[j]) >> 31));
             }
-        };
-        int head = int((16 - (reinterpret_cast<uintptr_t>(rp) & 15)) & 15) / 2;  // entries before the first whole vector
-        head = head < vocab ? head : vocab;
-        if (tid < head) count(rp[tid]);
-        const uint4 *vp = reinterpret_cast<const uint4 *>(rp + head);
-        const int nvec = (vocab - head) / 8;
-        constexpr int U = 8;  // loads in flight per lane
-        int v = tid;
-        for (; v + (U - 1) * S_THREADS < nvec; v += U * S_THREADS) {
-            uint4 q[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) q[u] = load_stream(vp + v + u * S_THREADS);
-#pragma unroll
-            for (int u = 0; u < U; ++u) count_vector(q[u]);
+            if (worst >= uint32_t(HIST_SIDE)) {  // rare: small values, zeros, masked entries
+                uint4 r = q[u];
+#pragma unroll 1
+                for (int j = 0; j < 4; ++j) {
+                    odd(r.x & 0xffffu);
+                    odd(r.x >> 16);
+                    r.x = r.y;
+                    r.y = r.z;
+                    r.z = r.w;
+                }
+            }
         }
-        for (; v < nvec; v += S_THREADS) count_vector(load_stream(vp + v));
-        const int i = head + nvec * 8 + tid;
-        if (i < vocab) count(rp[i]);
-        if (zeros) atomicAdd(&h.n_zero, zeros);
-        if (high) h.give_up = 1;
-        if (low) h.dropped = 1;
     }
-    __syncthreads();
-    const uint32_t n_tiny = h.n_tiny, n_zero = h.n_zero, dropped = h.dropped;
-    if (h.give_up != 0 || n_tiny > uint32_t(TINY_CAP)) return false;
-    const uint32_t n_mid = n_tiny + n_zero;
-    auto key_of_raw = [&](uint32_t raw) { return elem_key<Bf16>(uint16_t(raw), f.temp, f.has_t); };
+    const int i = head + nvec * 8 + tid;
+    if (i < vocab) one(rp[i]);
+    if (zeros) atomicAdd(&h.n_zero, zeros);
+    if (high) h.give_up = 1;
+    if (low) h.dropped = 1;
+}
 
-    // ---- the thread's positions ------------------------------------------------------------
-    uint32_t c[HIST_PER], sk[HIST_PER], mine = 0;
+// False: the row needs the radix path (nothing is decided).  h.cut, h.raw_cut and (with want_lse) h.raw_sum, h.raw_top hold the result.
+__device__ __forceinline__ bool hist_cut(HistRow &h, const uint16_t *rp, int vocab, const Filter &f, bool want_lse) {
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    for (int i = tid; i < HIST_BINS; i += S_THREADS) h.bin[i] = 0;
+    if (tid == 0) { h.n_tiny = h.n_zero = h.give_up = h.dropped = 0; h.first = HIST_POS; h.ok = 0; }
+    __syncthreads();
+    hist_count(h, rp, vocab);
+    __syncthreads();
+    const uint32_t n_tiny = h.n_tiny, n_zero = h.n_zero, n_mid = n_tiny + n_zero;
+    if (h.give_up != 0 || n_tiny > uint32_t(TINY_CAP)) return false;
+    auto key_of_raw = [&](uint32_t raw) { return elem_key<Bf16>(uint16_t(raw), f.temp, f.has_t); };
+    auto count_at = [&](int q) -> uint32_t { return q >= HIST_POS ? 0u : (q == HIST_SIDE ? n_mid : h.bin[bin_of_pos(q)]); };
+    {   // the largest value
+        int mine = HIST_POS;
+        for (int q = tid; q < HIST_POS && mine == HIST_POS; q += S_THREADS)
+            if (count_at(q) != 0) mine = q;
 #pragma unroll
-    for (int j = 0; j < HIST_PER; ++j) {
-        const int q = tid * HIST_PER + j;
-        c[j] = q >= HIST_POS ? 0u : (q == HIST_SIDE ? n_mid : h.bin[bin_of_pos(q)]);
-        mine += c[j];
-    }
-    uint32_t counted;
-    const uint32_t rank0 = block_excl_scan<uint32_t>(mine, h.wave_u32, &counted);
-    if (counted == 0) return false;
-    if (rank0 == 0 && mine > 0) {
-        int j = 0;
-        while (c[j] == 0) ++j;
-        h.first = uint32_t(tid * HIST_PER + j);
-    }
-    if (f.use_k && rank0 < uint32_t(f.top_k) && uint32_t(f.top_k) <= rank0 + mine) {
-        uint32_t run = rank0;
-        int at = 0;
-#pragma unroll
-        for (int j = 0; j < HIST_PER; ++j) {
-            if (run < uint32_t(f.top_k) && uint32_t(f.top_k) <= run + c[j]) at = j;
-            run += c[j];
+        for (int off = 32; off >= 1; off >>= 1) {
+            const int o = __shfl_xor(mine, off, kWave);
+            mine = o < mine ? o : mine;
         }
-        const int q = tid * HIST_PER + at;
-        h.kpos = uint32_t(q);
-        h.kstar = q == HIST_SIDE ? 0u : key_of_raw(raw_of_bin(bin_of_pos(q)));
+        if (lane == 0) atomicMin(&h.first, uint32_t(mine));
     }
     __syncthreads();
     const int first = int(h.first);
-    if (first == HIST_SIDE || (f.use_k && (counted < uint32_t(f.top_k) || h.kpos == uint32_t(HIST_SIDE)))) return false;
+    if (first == HIST_SIDE || first == HIST_POS) return false;
     const uint32_t raw_max = raw_of_bin(bin_of_pos(first));
     const uint32_t kmax = key_of_raw(raw_max);
     const float vmax = value_of<Bf16>(kmax), xmax = Bf16::widen(uint16_t(raw_max));
-    const uint32_t kstar = f.use_k ? h.kstar : 0u;
+    auto weight_of = [&](uint32_t key) { return weight_fix(key == kmax ? 0.0f : value_of<Bf16>(key) - vmax); };
+    // ---- masses: of all positions where a total is needed, else of the window -------------------
+    const bool total = !f.use_k;
+    {
+        uint64_t all = 0, mid = 0;
+        double raw_sum = 0.0;
+        const int end = total || want_lse ? HIST_POS : (first + WINDOW < HIST_POS ? first + WINDOW : HIST_POS);
+#pragma unroll 1
+        for (int q = first + tid; q < end; q += S_THREADS) {
+            const uint32_t c = count_at(q);
+            uint64_t w = 0;
+            uint32_t key = NO_KEY;
+            if (c != 0 && q != HIST_SIDE) {
+                const uint32_t raw = raw_of_bin(bin_of_pos(q));
+                if (total || q < first + WINDOW) {
+                    key = key_of_raw(raw);
+                    w = weight_of(key) * c;
+                    all += w;
+                }
+                // (fp32 exponentials, off by 2^-22 each: ample for a log-probability in fp32)
+                if (want_lse) raw_sum += double(float(c) * fast_exp2((Bf16::widen(uint16_t(raw)) - xmax) * kLseLog2e));
+            }
+            if (q < first + WINDOW) {
+                h.win_mass[q - first] = w;
+                h.win_key[q - first] = key;
+            }
+        }
+        if (total || want_lse) {
+#pragma unroll 1
+            for (int i = tid; i <= int(n_tiny); i += S_THREADS) {  // the small values, then zero
+                const uint32_t c = i < int(n_tiny) ? 1u : n_zero;
+                const uint32_t raw = i < int(n_tiny) ? uint32_t(h.tiny[i]) : 0u;
+                if (total) mid += weight_of(key_of_raw(raw)) * c;
+                if (want_lse) raw_sum += double(float(c) * fast_exp2((Bf16::widen(uint16_t(raw)) - xmax) * kLseLog2e));
+            }
+            all = wave_sum_u64_of(all);
+            mid = wave_sum_u64_of(mid);
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) raw_sum += __shfl_xor(raw_sum, off, kWave);
+            if (lane == 0) {
+                h.sums[wave][0] = all;
+                h.sums[wave][1] = mid;
+                h.raw_sums[wave] = raw_sum;
+            }
+        }
+        __syncthreads();
+    }
+    if (wave != 0) {
+        __syncthreads();  // the first wavefront's result
+        return h.ok != 0;
+    }
+    // ---- the first wavefront finishes the row --------------------------------------------------
+    uint64_t z_all = 0, z_mid = 0;
+    double raw_sum = 0.0;
+    if (total || want_lse)
+        for (int w = 0; w < S_WAVES; ++w) {
+            z_all += h.sums[w][0];
+            z_mid += h.sums[w][1];
+            raw_sum += h.raw_sums[w];
+        }
+    z_all += z_mid;
     const uint32_t key_dropped = key_of_raw(0x8000u | MAG_HIGH), key_tiny = key_of_raw(MAG_LOW - 1), key_tiny_neg = key_of_raw(0x8000u | (MAG_LOW - 1));
-    if (dropped && (weight_fix(value_of<Bf16>(key_dropped) - vmax) != 0 || weight_fix(-256.0f - xmax) != 0)) return false;
+    const bool dropped = h.dropped != 0;
+    bool ok = !dropped || (weight_fix(value_of<Bf16>(key_dropped) - vmax) == 0 && weight_fix(-256.0f - xmax) == 0);
     // a cut that shares its scaled value with entries that are not binned (a temperature that folds values together)
     auto shared_value = [&](uint32_t key, int q) {
         return (dropped && key <= key_dropped) || (n_mid > 0 && (q < HIST_SIDE ? key <= key_tiny : key >= key_tiny_neg));
     };
-    if (f.use_k && shared_value(kstar, int(h.kpos))) return false;
-    auto weight_of = [&](uint32_t key) { return weight_fix(key == kmax ? 0.0f : value_of<Bf16>(key) - vmax); };
-
-    // ---- masses ----------------------------------------------------------------------------
-    uint64_t mid = 0;
-    for (int i = tid; i < int(n_tiny); i += S_THREADS) mid += weight_of(key_of_raw(h.tiny[i]));
-    if (tid == 0 && n_zero) mid += n_zero * weight_of(key_of_raw(0));
-    uint64_t mid_mass = 0;
-    if (n_mid) block_excl_scan<uint64_t>(mid, h.wave_u64, &mid_mass);
-    uint64_t m[HIST_PER], sum = 0, sum_raw = 0;
-#pragma unroll
-    for (int j = 0; j < HIST_PER; ++j) {
-        const int q = tid * HIST_PER + j;
-        m[j] = 0;
-        sk[j] = 0;
-        if (c[j] == 0) continue;
-        if (q == HIST_SIDE) {
-            m[j] = !f.use_k || int(h.kpos) > HIST_SIDE ? mid_mass : 0ull;
-        } else {
-            const uint32_t raw = raw_of_bin(bin_of_pos(q));
-            sk[j] = key_of_raw(raw);
-            const uint64_t w = weight_of(sk[j]) * c[j];
-            if (sk[j] >= kstar) m[j] = w;
-            if (want_lse) sum_raw += f.has_t ? weight_fix(Bf16::widen(uint16_t(raw)) - xmax) * c[j] : w;
+    RowCut cut{kmax, 0u, 0u, 0xffffffffu, z_all};
+    uint32_t raw_cut = 0;
+    auto last_u64 = [&](uint64_t v) {
+        return (uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), kWave - 1))) << 32) |
+               uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), kWave - 1));
+    };
+    if (ok && f.use_k) {  // the position that holds the top_k-th largest entry
+        uint32_t upto = 0;
+        int kpos = -1;
+        for (int q0 = first; q0 < HIST_POS && kpos < 0; q0 += kWave) {
+            const uint32_t inc = upto + wave_incl_scan_u32(count_at(q0 + lane));
+            const uint64_t reached = __ballot(inc >= uint32_t(f.top_k));
+            if (reached != 0) kpos = q0 + __ffsll((long long)reached) - 1;
+            upto = uint32_t(__builtin_amdgcn_readlane(int(inc), kWave - 1));
         }
-        sum += m[j];
-    }
-    uint64_t z_topk, z_raw = 0;
-    uint64_t run = block_excl_scan<uint64_t>(sum, h.wave_u64, &z_topk);
-    if (want_lse) {
-        if (n_mid) {
-            if (f.has_t) {
-                for (int i = tid; i < int(n_tiny); i += S_THREADS) sum_raw += weight_fix(Bf16::widen(h.tiny[i]) - xmax);
-                if (tid == 0 && n_zero) sum_raw += n_zero * weight_fix(-xmax);
-            } else {
-                sum_raw += mid;
-            }
+        if (kpos < 0 || kpos == HIST_SIDE) ok = false;
+        else {
+            cut.kstar = cut.kcut = key_of_raw(raw_of_bin(bin_of_pos(kpos)));
+            ok = !shared_value(cut.kstar, kpos);
+            if (kpos > HIST_SIDE && n_mid > 0) ok = false;  // the small values would be among the survivors without a total
         }
-        block_excl_scan<uint64_t>(sum_raw, h.wave_u64, &z_raw);
-        // ln(z_raw 2^-40) + max: the masses round the row's exponentials down to 2^-40 of the largest, 1.2e-7 of the sum at most
-        lse = double(xmax) + log(double(z_raw)) - FIX_BITS * 0.693147180559945309417232;
     }
-    cut.kmax = kmax;
-    cut.kstar = cut.kcut = kstar;
-    cut.r_cut = 0xffffffffu;
-    cut.z = z_topk;
-    raw_cut = 0;
-    if (!f.use_k && !f.use_p) return true;
-    // ---- top-p -----------------------------------------------------------------------------
-    if (f.use_p) {
-        const uint64_t theta = floor_scale(f.top_p, z_topk);
+    // Key (NO_KEY: empty, the small values or below the top-k cut), count and mass of one position.
+    auto position = [&](int q, uint32_t &key, uint32_t &c, uint64_t &m) {
+        c = count_at(q);
+        key = NO_KEY;
+        m = 0;
+        if (c == 0) return;
+        if (q == HIST_SIDE) { m = z_mid; return; }
+        key = q < first + WINDOW ? h.win_key[q - first] : key_of_raw(raw_of_bin(bin_of_pos(q)));
+        if (key < cut.kstar) { key = NO_KEY; c = 0; return; }
+        m = q < first + WINDOW ? h.win_mass[q - first] : weight_of(key) * c;
+    };
+    if (ok && f.use_k) {  // mass of the survivors of top-k: up to the first step with an entry below the cut
+        uint64_t z = 0;
+        for (int q0 = first; q0 < HIST_POS; q0 += kWave) {
+            uint32_t key, c;
+            uint64_t m;
+            position(q0 + lane, key, c, m);
+            z += wave_sum_u64_of(m);
+            const bool below = q0 + lane < HIST_POS && count_at(q0 + lane) != 0 && key == NO_KEY;
+            const uint64_t alive = __ballot(key != NO_KEY);
+            if (alive != 0) raw_cut = raw_of_bin(bin_of_pos(q0 + 63 - __builtin_clzll(alive)));
+            if (__ballot(below) != 0) break;
+        }
+        cut.z = z;
+    }
+    if (ok && f.use_p) {
+        const uint64_t theta = floor_scale(f.top_p, cut.z);
         int best = -1;
-        uint64_t upto = run;
-#pragma unroll
-        for (int j = 0; j < HIST_PER; ++j) {
-            const int q = tid * HIST_PER + j;
-            const bool in = c[j] > 0 && (q == HIST_SIDE ? (!f.use_k || int(h.kpos) > HIST_SIDE) : sk[j] >= kstar);
-            if (in && upto <= theta) best = q;
-            upto += m[j];
+        uint64_t run = 0;
+        for (int q0 = first; q0 < HIST_POS && run <= theta; q0 += kWave) {
+            uint32_t key, c;
+            uint64_t m;
+            position(q0 + lane, key, c, m);
+            const uint64_t inc = wave_incl_scan_u64(m);
+            const uint64_t in = __ballot(c != 0 && run + inc - m <= theta);
+            if (in != 0) best = q0 + 63 - __builtin_clzll(in);
+            run += last_u64(inc);
         }
-        if (best >= 0) atomicMax(&h.best, uint32_t(best));
-        __syncthreads();
-        best = int(h.best);
-        if (best == HIST_SIDE) return false;
-        const uint32_t kcut = key_of_raw(raw_of_bin(bin_of_pos(best)));
-        if (shared_value(kcut, best)) return false;
-        upto = run;
-#pragma unroll
-        for (int j = 0; j < HIST_PER; ++j) {
-            if (c[j] > 0 && sk[j] == kcut) {
-                atomicAdd(&h.n_cut, c[j]);
-                atomicMin(&h.before, (unsigned long long)upto);
+        ok = best != HIST_SIDE;
+        if (ok) {
+            cut.kcut = key_of_raw(raw_of_bin(bin_of_pos(best)));
+            ok = !shared_value(cut.kcut, best);
+        }
+        if (ok) {
+            uint64_t before = 0;
+            uint32_t n_cut = 0;
+            run = 0;
+            for (int q0 = first; q0 < HIST_POS; q0 += kWave) {
+                uint32_t key, c;
+                uint64_t m;
+                position(q0 + lane, key, c, m);
+                const uint64_t inc = wave_incl_scan_u64(m);
+                const uint64_t group = __ballot(key == cut.kcut);
+                if (group != 0) {
+                    const uint64_t excl = run + inc - m;
+                    if (n_cut == 0) {
+                        const int l = __ffsll((long long)group) - 1;
+                        before = (uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(excl >> 32)), l))) << 32) |
+                                 uint32_t(__builtin_amdgcn_readlane(int(uint32_t(excl)), l));
+                    }
+                    n_cut += uint32_t(__builtin_amdgcn_readlane(int(wave_incl_scan_u32(key == cut.kcut ? c : 0u)), kWave - 1));
+                    raw_cut = raw_of_bin(bin_of_pos(q0 + 63 - __builtin_clzll(group)));
+                }
+                if (__ballot(q0 + lane > best && count_at(q0 + lane) != 0 && key != cut.kcut) != 0) break;  // behind the group
+                run += last_u64(inc);
             }
-            upto += m[j];
+            const uint64_t w_cut = weight_of(cut.kcut);
+            uint64_t r = n_cut;
+            if (w_cut > 0) {
+                const uint64_t fit = (theta - before) / w_cut + 1;  // entries t with before + t * w <= theta
+                r = fit < r ? fit : r;
+            }
+            cut.r_cut = r == n_cut ? 0xffffffffu : uint32_t(r);
+            cut.z = before + r * w_cut;
         }
-        __syncthreads();
-        const uint32_t n_cut = h.n_cut;
-        const uint64_t before = h.before, w_cut = weight_of(kcut);
-        uint64_t r = n_cut;
-        if (w_cut > 0) {
-            const uint64_t fit = (theta - before) / w_cut + 1;  // entries t with before + t * w <= theta
-            r = fit < r ? fit : r;
-        }
-        cut.kcut = kcut;
-        cut.r_cut = r == n_cut ? 0xffffffffu : uint32_t(r);
-        cut.z = before + r * w_cut;
     }
-#pragma unroll
-    for (int j = 0; j < HIST_PER; ++j)
-        if (c[j] > 0 && sk[j] >= cut.kcut) atomicMax(&h.last, uint32_t(tid * HIST_PER + j));
+    if (lane == 0) {
+        h.cut = cut;
+        h.raw_cut = f.use_k || f.use_p ? masked_key<Bf16>(Bf16::widen(uint16_t(raw_cut))) : 0u;
+        h.raw_sum = raw_sum;
+        h.raw_top = xmax;
+        h.ok = ok ? 1u : 0u;
+    }
     __syncthreads();
-    raw_cut = masked_key<Bf16>(Bf16::widen(uint16_t(raw_of_bin(bin_of_pos(int(h.last))))));
-    return true;
+    return ok;
 }
 
 // The smallest unscaled key whose scaled value reaches kcut, by all lanes of the wavefront at once: near kcut's value times
@@ -412,7 +521,7 @@ template <typename T> __device__ __forceinline__ uint32_t raw_key_of_cut(uint32_
 }
 
 template <typename T>
-__global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(4))) void verify_rows(VerifyParams p) {
+__global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(6, 6))) void verify_rows(VerifyParams p) {
     __shared__ VerifyShared lds;
     const int tid = threadIdx.x;
     const int64_t n_target = int64_t(p.batch) * (p.k + 1);
@@ -426,12 +535,24 @@ __global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(4))) 
     const typename T::raw_t *rp = is_target ? target_row<T>(p, b, j) : draft_row<T>(p, b, j);
     const bool vec = (is_target ? p.vec_target : p.vec_draft) != 0;
     const Filter f = filter_of(p, b);
+    const int64_t d = j < len ? p.draft_ids[int64_t(b) * p.k + j] : -1;
+    const bool in_vocab = d >= 0 && d < p.vocab;
+    const typename T::raw_t drafted = in_vocab ? rp[d] : typename T::raw_t(0);  // (long before it is needed)
     const bool want_lse = is_target && p.out_policy != nullptr;
     RowCut cut;
     uint32_t raw_cut = 0;
-    double lse = 0.0;
+    double raw_sum = 1.0;
+    float raw_top = 0.0f;
     bool done = false;
-    if constexpr (T::kDtype == KA_DTYPE_BF16) done = hist_cut(lds.hist, rp, p.vocab, f, want_lse, cut, raw_cut, lse);
+    if constexpr (T::kDtype == KA_DTYPE_BF16) {
+        done = hist_cut(lds.hist, rp, p.vocab, f, want_lse);
+        if (done) {
+            cut = lds.hist.cut;
+            raw_cut = lds.hist.raw_cut;
+            raw_sum = lds.hist.raw_sum;
+            raw_top = lds.hist.raw_top;
+        }
+    }
     if (!done) {
         __syncthreads();
         cut = radix_cut<T>(lds.sh, rp, p.vocab, vec, f.temp, f.has_t, f.use_k, f.top_k, f.use_p, f.top_p, true);
@@ -439,14 +560,12 @@ __global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(4))) 
         if (want_lse) {
             row_lse_to_block<T>(rp, p.vocab, vec, lds.lse);
             __syncthreads();
-            if (tid == 0) lse = lds.lse.value();
+            if (tid == 0) lds.lse.parts(raw_top, raw_sum);
         }
     }
 
     // mass of the drafted token; where it sits in a tie group that survives in part, its rank in the group decides
-    const int64_t d = j < len ? p.draft_ids[int64_t(b) * p.k + j] : -1;
-    const bool in_vocab = d >= 0 && d < p.vocab;
-    const uint32_t key = in_vocab ? elem_key<T>(rp[d], f.temp, f.has_t) : 0u;
+    const uint32_t key = in_vocab ? elem_key<T>(drafted, f.temp, f.has_t) : 0u;
     bool kept = in_vocab && (key > cut.kcut || (key == cut.kcut && key >= cut.kstar));
     if (kept && key == cut.kcut && cut.r_cut != 0xffffffffu) {  // the same for the whole block
         __syncthreads();
@@ -462,7 +581,9 @@ __global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(4))) 
         RowSummary s;
         s.z = cut.z;
         s.w_draft = kept ? weight_fix(key == cut.kmax ? 0.0f : value_of<T>(key) - value_of<T>(cut.kmax)) : 0ull;
-        s.lse = lse;
+        s.raw_sum = raw_sum;
+        s.raw_top = raw_top;
+        s.pad = 0;
         s.kmax = cut.kmax;
         s.kcut = cut.kcut;
         s.r_cut = cut.r_cut;
@@ -498,26 +619,26 @@ __global__ __launch_bounds__(S_THREADS) void verify_ties(VerifyParams p) {
     const typename T::raw_t *rp = is_target ? target_row<T>(p, b, n) : draft_row<T>(p, b, n);
     const bool vec = (is_target ? p.vec_target : p.vec_draft) != 0;
     const float low = cut_value<T>(p.rows[row].raw_cut);
-    auto ties_of = [&](const typename T::raw_t (&e)[EPV], int base) {
-        uint32_t c = 0;
-#pragma unroll
-        for (int j = 0; j < EPV; ++j)
-            if (!(T::widen(e[j]) < low) && base + j < p.vocab && elem_key<T>(e[j], f.temp, f.has_t) == kcut) ++c;
-        return c;
+    // bit j: entry j belongs to the group
+    auto ties_of = [&](const uint4 &v, int64_t base) {
+        uint32_t ties = 0;
+        for (uint32_t left = at_least<T>(v, low, base, p.vocab); left != 0; left &= left - 1) {
+            const int j = __ffs(left) - 1;
+            if (elem_key<T>(entry_of<T>(v, j), f.temp, f.has_t) == kcut) ties |= 1u << j;
+        }
+        return ties;
     };
     const int chunks = (p.vocab + EPV * S_THREADS - 1) / (EPV * S_THREADS);
     for (int i = tid; i < chunks; i += S_THREADS) ties[i] = 0;
     __syncthreads();
     constexpr int U = 8;  // vectors in flight per lane
     for (int c0 = 0; c0 < chunks; c0 += U) {
-        typename T::raw_t e[U][EPV];
+        uint4 v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) load_entries<T>(rp, vec, p.vocab, ((c0 + u) * S_THREADS + tid) * int64_t(EPV), e[u]);
+        for (int u = 0; u < U; ++u) v[u] = load_entries<T>(rp, vec, p.vocab, ((c0 + u) * S_THREADS + tid) * int64_t(EPV));
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t base = ((c0 + u) * S_THREADS + tid) * int64_t(EPV);
-            if (base >= p.vocab) continue;
-            const uint32_t c = ties_of(e[u], int(base));
+            const uint32_t c = uint32_t(__popc(ties_of(v[u], ((c0 + u) * S_THREADS + tid) * int64_t(EPV))));
             if (c) atomicAdd(&ties[c0 + u], c);
         }
     }
@@ -537,41 +658,48 @@ __global__ __launch_bounds__(S_THREADS) void verify_ties(VerifyParams p) {
     }
     __syncthreads();
     const int64_t base = (int64_t(s_chunk) * S_THREADS + tid) * EPV;
-    typename T::raw_t e[EPV];
-    load_entries<T>(rp, vec, p.vocab, base, e);
-    const uint32_t c = base < p.vocab ? ties_of(e, int(base)) : 0u;
+    uint32_t group = ties_of(load_entries<T>(rp, vec, p.vocab, base), base);
+    const uint32_t c = uint32_t(__popc(group));
     const uint32_t rank = s_before + block_excl_scan<uint32_t>(c, wave_buf, &total);
     if (rank < r_cut && r_cut <= rank + c) {
-        uint32_t at = rank;
-        int32_t found = 0;
-#pragma unroll
-        for (int j = 0; j < EPV; ++j)
-            if (base + j < p.vocab && elem_key<T>(e[j], f.temp, f.has_t) == kcut && ++at == r_cut) found = int32_t(base) + j + 1;
-        *limit = found;
+        for (uint32_t skip = r_cut - rank - 1; skip != 0; --skip) group &= group - 1;
+        *limit = int32_t(base) + __ffs(group);  // the last survivor's index + 1
     }
 }
 
 // ---------------------------------------------------------------------------
 // Residual masses of the stopping position
 // ---------------------------------------------------------------------------
-// A row's distribution as the last two kernels evaluate it, entry by entry.
+constexpr double DRAW_MARGIN = 0x1p-38;
+
+// A row's distribution, entry by entry.
 struct RowDist {
     uint32_t kmax, kcut;
     int limit;
-    float vmax;
-    template <typename T> __device__ __forceinline__ uint64_t mass(uint32_t key, int i) const {
+    float vmax, low;  // unscaled values below `low` have no mass
+    uint64_t z;
+    template <typename T> __device__ __forceinline__ uint64_t mass(typename T::raw_t x, int i, const Filter &f) const {
+        if (T::widen(x) < low) return 0ull;
+        const uint32_t key = elem_key<T>(x, f.temp, f.has_t);
         if (key < kcut || (key == kcut && i >= limit)) return 0ull;
         return weight_fix(key == kmax ? 0.0f : value_of<T>(key) - vmax);
     }
+    template <typename T> __device__ __forceinline__ void from(const RowSummary &s, int tie_limit) {
+        kmax = s.kmax;
+        kcut = s.kcut;
+        limit = tie_limit;
+        vmax = value_of<T>(s.kmax);
+        low = cut_value<T>(s.raw_cut);
+        z = s.z;
+    }
 };
 
-// Residual mass of entry i: max(W^p mul_p - W^q mul_q, 0), 0 for a looked-up draft that was rejected.
+// Residual of entry i: max(P - Q, 0); P alone where nothing was rejected, 0 for a looked-up draft that was.
 template <typename T> struct Residual {
     const typename T::raw_t *rp, *rq;  // rq null: nothing is subtracted
     bool vec_p, vec_q;
     RowDist p, q;
-    float low_p, low_q;  // unscaled values below these have no mass
-    uint64_t mul_p, mul_q;
+    double inv_p, inv_q;
     int64_t skip;  // the rejected look-up draft, or -1
     Filter f;
     int vocab;
@@ -582,91 +710,86 @@ template <typename T> struct Residual {
         vocab = v.vocab;
         rp = target_row<T>(v, b, n);
         vec_p = v.vec_target != 0;
-        p = RowDist{t.kmax, t.kcut, v.may_cut_ties ? v.tie_limit[2 * b] : 0x7fffffff, value_of<T>(t.kmax)};
-        mul_p = 1;
-        mul_q = 0;
+        p.template from<T>(t, v.may_cut_ties ? v.tie_limit[2 * b] : 0x7fffffff);
+        inv_p = 1.0 / double(p.z);
+        inv_q = 0.0;
         rq = nullptr;
         vec_q = false;
         skip = -1;
         q = p;
-        low_p = low_q = cut_value<T>(t.raw_cut);
         if (n < len) {
             if (v.draft != nullptr) {
-                const RowSummary &d = v.rows[int64_t(v.batch) * (v.k + 1) + int64_t(b) * v.k + n];
                 rq = draft_row<T>(v, b, n);
                 vec_q = v.vec_draft != 0;
-                q = RowDist{d.kmax, d.kcut, v.may_cut_ties ? v.tie_limit[2 * b + 1] : 0x7fffffff, value_of<T>(d.kmax)};
-                low_q = cut_value<T>(d.raw_cut);
-                mul_p = d.z;
-                mul_q = t.z;
+                q.template from<T>(v.rows[int64_t(v.batch) * (v.k + 1) + int64_t(b) * v.k + n], v.may_cut_ties ? v.tie_limit[2 * b + 1] : 0x7fffffff);
+                inv_q = 1.0 / double(q.z);
             } else {
                 skip = v.draft_ids[int64_t(b) * v.k + n];
             }
         }
     }
-    __device__ __forceinline__ u128 entry(typename T::raw_t x, typename T::raw_t y, int i) const {
-        if (T::widen(x) < low_p || i >= vocab || int64_t(i) == skip) return 0;
-        const uint64_t wp = p.template mass<T>(elem_key<T>(x, f.temp, f.has_t), i);
-        if (wp == 0) return 0;
-        if (rq == nullptr) return wp;
-        const u128 have = u128(wp) * mul_p;
-        if (T::widen(y) < low_q) return have;
-        const u128 take = u128(q.template mass<T>(elem_key<T>(y, f.temp, f.has_t), i)) * mul_q;
-        return have > take ? have - take : u128(0);
+    __device__ __forceinline__ double entry(typename T::raw_t x, typename T::raw_t y, int i) const {
+        if (int64_t(i) == skip) return 0.0;
+        const uint64_t wp = p.template mass<T>(x, i, f);
+        if (wp == 0) return 0.0;
+        double r = double(wp) * inv_p;
+        if (rq != nullptr) r -= double(q.template mass<T>(y, i, f)) * inv_q;
+        return r > 0.0 ? r : 0.0;
     }
-    // residual masses of the vector that starts at `base` (0 behind the row)
-    __device__ __forceinline__ void vector(int64_t base, u128 (&m)[T::kPerVec]) const {
-        constexpr int EPV = T::kPerVec;
-        typename T::raw_t x[EPV], y[EPV];
-        load_entries<T>(rp, vec_p, vocab, base, x);
-        if (rq != nullptr) load_entries<T>(rq, vec_q, vocab, base, y);
-#pragma unroll
-        for (int j = 0; j < EPV; ++j) m[j] = base + j < vocab ? entry(x[j], rq != nullptr ? y[j] : typename T::raw_t(0), int(base) + j) : u128(0);
+    // each(j, residual) for the entries of the vector at `base` that may have one, in order
+    template <typename F> __device__ __forceinline__ void vector(int64_t base, F &&each) const {
+        const uint4 x = load_entries<T>(rp, vec_p, vocab, base);
+        const uint4 y = rq != nullptr ? load_entries<T>(rq, vec_q, vocab, base) : make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+        for (uint32_t left = at_least<T>(x, p.low, base, vocab); left != 0; left &= left - 1) {
+            const int j = __ffs(left) - 1;
+            each(j, entry(entry_of<T>(x, j), entry_of<T>(y, j), int(base) + j));
+        }
+    }
+    // the same in integers, times Z^p Z^q (times Z^p where nothing is subtracted)
+    template <typename F> __device__ __forceinline__ void exact_vector(int64_t base, F &&each) const {
+        const uint4 x = load_entries<T>(rp, vec_p, vocab, base);
+        const uint4 y = rq != nullptr ? load_entries<T>(rq, vec_q, vocab, base) : make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+        for (uint32_t left = at_least<T>(x, p.low, base, vocab); left != 0; left &= left - 1) {
+            const int j = __ffs(left) - 1, i = int(base) + j;
+            if (int64_t(i) == skip) continue;
+            u128 have = p.template mass<T>(entry_of<T>(x, j), i, f), take = 0;
+            if (rq != nullptr) {
+                have *= q.z;
+                take = u128(q.template mass<T>(entry_of<T>(y, j), i, f)) * p.z;
+            }
+            each(j, have > take ? have - take : u128(0));
+        }
     }
 };
 
-// The entry of a vector of masses, `before` of mass in front of it, that holds tau.
-template <int EPV> __device__ __forceinline__ int entry_at(const u128 (&m)[EPV], u128 before, u128 tau) {
-    int hit = -1;
-#pragma unroll
-    for (int j = 0; j < EPV; ++j) {
-        before += m[j];
-        if (hit < 0 && tau < before) hit = j;
-    }
-    return hit;
-}
-template <int EPV> __device__ __forceinline__ u128 total_of(const u128 (&m)[EPV]) {
-    u128 sum = 0;
-#pragma unroll
-    for (int j = 0; j < EPV; ++j) sum += m[j];
-    return sum;
-}
-
-__device__ __forceinline__ u128 shfl_up_u128(u128 v, int off) {
+__device__ __forceinline__ u128 shfl_up_of(u128 v, int off) {
     const uint64_t lo = __shfl_up((unsigned long long)uint64_t(v), off, kWave);
     const uint64_t hi = __shfl_up((unsigned long long)uint64_t(v >> 64), off, kWave);
     return (u128(hi) << 64) | lo;
 }
-__device__ __forceinline__ u128 wave_incl_scan_u128(u128 v) {
+__device__ __forceinline__ double shfl_up_of(double v, int off) { return __shfl_up(v, off, kWave); }
+template <typename V> __device__ __forceinline__ V wave_incl_scan_of(V v) {
     const int lane = threadIdx.x & (kWave - 1);
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) {
-        const u128 o = shfl_up_u128(v, off);
+        const V o = shfl_up_of(v, off);
         if (lane >= off) v += o;
     }
     return v;
 }
 // Exclusive prefix sum over the block in thread order; `*total` = sum over the block.  Every thread calls it.
-template <int WAVES> __device__ __forceinline__ u128 block_excl_scan_u128(u128 v, u128 *wave_buf, u128 *total) {
+template <int WAVES, typename V> __device__ __forceinline__ V block_excl_scan_of(V v, V *wave_buf, V *total) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const u128 inc = wave_incl_scan_u128(v);
+    const V inc = wave_incl_scan_of(v);
     __syncthreads();  // wave_buf may still be read from a previous call
     if (lane == kWave - 1) wave_buf[wave] = inc;
     __syncthreads();
-    u128 base = 0, sum = 0;
+    V base = 0, sum = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-        const u128 x = wave_buf[w];
+        const V x = wave_buf[w];
         if (w < wave) base += x;
         sum += x;
     }
@@ -684,81 +807,227 @@ __global__ __launch_bounds__(SHARE_THREADS) void verify_shares(VerifyParams p) {
     if (share >= p.n_shares) return;
     Residual<T> res;
     res.setup(p, b, n, len);
-    u128 sum = 0;
+    double sum = 0.0;
 #pragma unroll 1
-    for (int s = 0; s < SHARE_VECS / kWave; ++s) {
-        const int64_t base = (int64_t(share) * SHARE_VECS + s * kWave + lane) * T::kPerVec;
-        u128 m[T::kPerVec];
-        res.vector(base, m);
-        sum += total_of(m);
-    }
-    sum = wave_incl_scan_u128(sum);
+    for (int s = 0; s < SHARE_VECS / kWave; ++s)
+        res.vector((int64_t(share) * SHARE_VECS + s * kWave + lane) * T::kPerVec, [&](int, double r) { sum += r; });
+    sum = wave_incl_scan_of(sum);
     if (lane == kWave - 1) p.shares[int64_t(b) * p.n_shares + share] = sum;
+}
+
+// The same for bf16 rows of which many entries survive (no top-k, or a large one): the masses come from two tables in LDS, one
+// value per bin of verify_rows, so that an entry costs two reads of LDS instead of two evaluations of the mass polynomial.
+// Entries outside the bins (about one in 10^4) are evaluated.  A workgroup builds the tables (9728 evaluations) for
+// shares_per_group shares.  grid (groups, B)
+constexpr int TABLE_THREADS = 512;
+constexpr size_t TABLE_LDS_BYTES = size_t(2) * HIST_BINS * sizeof(double);
+__global__ __launch_bounds__(TABLE_THREADS) void verify_shares_table(VerifyParams p) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char dyn_lds[];
+    double *const tab_p = reinterpret_cast<double *>(dyn_lds), *const tab_q = tab_p + HIST_BINS;
+    using T = Bf16;
+    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    const int len = draft_len(p, b);
+    const int n = accepted_prefix(p, b, len);
+    Residual<T> res;
+    res.setup(p, b, n, len);
+    const bool two = res.rq != nullptr, looked_up = res.skip >= 0;
+    // a value of the group that survives in part is marked by its sign
+    const bool part_p = res.p.limit != 0x7fffffff, part_q = res.q.limit != 0x7fffffff;
+    auto probability = [&](const RowDist &d, double inv, bool part, uint32_t raw) {
+        const uint32_t key = elem_key<T>(uint16_t(raw), res.f.temp, res.f.has_t);
+        if (key < d.kcut) return 0.0;
+        const double v = double(weight_fix(key == d.kmax ? 0.0f : value_of<T>(key) - d.vmax)) * inv;
+        return part && key == d.kcut ? -v : v;
+    };
+#pragma unroll 1
+    for (int i = tid; i < HIST_BINS; i += TABLE_THREADS) {
+        const uint32_t raw = raw_of_bin(i);
+        tab_p[i] = probability(res.p, res.inv_p, part_p, raw);
+        if (two) tab_q[i] = probability(res.q, res.inv_q, part_q, raw);
+    }
+    __syncthreads();
+    // magnitude bits above the bins' lowest, and the entry's probability where that is below HIST_SIDE
+    auto above = [](uint32_t x) { return (x & 0x7fffu) - MAG_LOW; };
+    auto value = [](const double *tab, uint32_t m, uint32_t x) { return tab[HIST_SIDE + int(m ^ uint32_t(int32_t(x << 16) >> 31))]; };
+    auto kept = [](double v, int i, int limit) { return v < 0.0 ? (i < limit ? -v : 0.0) : v; };
+    const int first = int(blockIdx.x) * p.shares_per_group;
+    const int end = first + p.shares_per_group < p.n_shares ? first + p.shares_per_group : p.n_shares;
+    for (int share = first + wave; share < end; share += TABLE_THREADS / kWave) {
+        double sum = 0.0;
+        uint4 x[SHARE_VECS / kWave], y[SHARE_VECS / kWave];
+#pragma unroll
+        for (int s = 0; s < SHARE_VECS / kWave; ++s) {
+            const int64_t base = (int64_t(share) * SHARE_VECS + s * kWave + lane) * T::kPerVec;
+            x[s] = load_entries<T>(res.rp, res.vec_p, res.vocab, base);
+            y[s] = two ? load_entries<T>(res.rq, res.vec_q, res.vocab, base) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int s = 0; s < SHARE_VECS / kWave; ++s) {
+            const int64_t base = (int64_t(share) * SHARE_VECS + s * kWave + lane) * T::kPerVec;
+            const uint32_t xw[4] = {x[s].x, x[s].y, x[s].z, x[s].w}, yw[4] = {y[s].x, y[s].y, y[s].z, y[s].w};
+            if (base >= res.vocab) continue;
+            // entries evaluated one by one: outside the bins, and all of the row's last vector if it is cut short
+            const bool whole = base + 8 <= res.vocab;
+            uint32_t odd = whole ? 0u : (1u << int(res.vocab - base)) - 1u;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t xe = xw[j / 2] >> (16 * (j & 1)), ye = yw[j / 2] >> (16 * (j & 1));
+                const uint32_t mx = above(xe), my = above(ye);
+                if (mx >= uint32_t(HIST_SIDE) || (two && my >= uint32_t(HIST_SIDE))) {
+                    odd |= whole ? 1u << j : 0u;
+                } else if (whole) {
+                    double r = value(tab_p, mx, xe);
+                    if (part_p) r = kept(r, int(base) + j, res.p.limit);
+                    if (two) {
+                        double t = value(tab_q, my, ye);
+                        if (part_q) t = kept(t, int(base) + j, res.q.limit);
+                        r -= t;
+                    }
+                    if (looked_up && int64_t(base) + j == res.skip) r = 0.0;
+                    sum += fmax(r, 0.0);
+                }
+            }
+#pragma unroll 1
+            for (; odd != 0; odd &= odd - 1) {
+                const int j = __ffs(odd) - 1;
+                sum += res.entry(entry_of<T>(x[s], j), entry_of<T>(y[s], j), int(base) + j);
+            }
+        }
+        sum = wave_incl_scan_of(sum);
+        if (lane == kWave - 1) p.shares[int64_t(b) * p.n_shares + share] = sum;
+    }
+}
+
+// The draw in integers, by the whole block (blocks of SHARE_VECS threads): the total, then the entry.
+template <typename T> __device__ __forceinline__ int exact_draw(Residual<T> res, float u, int n_shares, u128 *wave_buf, int *hit) {
+    constexpr int WAVES = SHARE_VECS / kWave;
+    const int tid = threadIdx.x;
+    u128 tau = 0;
+    for (int turn = 0; turn < 2; ++turn) {
+        u128 at = 0;
+        for (int share = 0; share < n_shares; ++share) {  // block-uniform: `at` and the totals are
+            const int64_t base = (int64_t(share) * SHARE_VECS + tid) * T::kPerVec;
+            u128 sum = 0, total;
+            res.exact_vector(base, [&](int, u128 m) { sum += m; });
+            u128 before = at + block_excl_scan_of<WAVES, u128>(sum, wave_buf, &total);
+            at += total;
+            if (turn == 0) continue;
+            if (before <= tau && tau < before + sum) {
+                int found = -1;
+                res.exact_vector(base, [&](int j, u128 m) {
+                    before += m;
+                    if (found < 0 && tau < before) found = int(base) + j;
+                });
+                *hit = found;
+            }
+            if (tau < at) break;
+        }
+        if (turn == 0) {
+            if (at == 0) {  // no residual (see the head of the file): drawn from P
+                res.rq = nullptr;
+                res.skip = -1;
+                at = res.p.z;
+            }
+            tau = floor_scale_wide(u, at);
+        }
+    }
+    __syncthreads();
+    return *hit;
 }
 
 // grid B; a thread per vector of the share that holds the draw
 template <typename T>
 __global__ __launch_bounds__(SHARE_VECS) void verify_draw(VerifyParams p) {
-    constexpr int WAVES = SHARE_VECS / kWave;
-    __shared__ u128 wave_buf[WAVES];
-    __shared__ u128 s_before;
+    constexpr int WAVES = SHARE_VECS / kWave, EPV = T::kPerVec;
+    __shared__ union { double d[WAVES]; u128 w[WAVES]; } wave_buf;
+    __shared__ double s_before;
     __shared__ int s_share, s_hit;
     const int b = blockIdx.x, tid = threadIdx.x;
     const int len = draft_len(p, b);
     const int n = accepted_prefix(p, b, len);
     if (tid == 0) { s_share = -1; s_hit = -1; }
     const float u = clean_uniform(p.uniforms[int64_t(b) * (p.k + 1) + p.k]);
-    // the share that holds floor(u * R): thread t takes a run of shares
-    u128 mine = 0, r;
+    // the share that holds u R: thread t takes a run of shares
+    double mine = 0.0, r;
     const int per = (p.n_shares + SHARE_VECS - 1) / SHARE_VECS;
-    const u128 *const shares = p.shares + int64_t(b) * p.n_shares;
+    const double *const shares = p.shares + int64_t(b) * p.n_shares;
     for (int i = 0; i < per; ++i)
         if (tid * per + i < p.n_shares) mine += shares[tid * per + i];
-    const u128 excl = block_excl_scan_u128<WAVES>(mine, wave_buf, &r);
-    u128 tau = floor_scale_wide(u, r);
+    Residual<T> res;
+    res.setup(p, b, n, len);
+    const double excl = block_excl_scan_of<WAVES, double>(mine, wave_buf.d, &r);
+    const double tau = double(u) * r;
     if (excl <= tau && tau < excl + mine) {
-        u128 at = excl;
-        for (int i = 0; i < per; ++i) {
-            const u128 m = shares[tid * per + i];
-            if (tau < at + m) { s_share = tid * per + i; s_before = at; break; }
+        double at = excl;
+        for (int i = 0; i < per && tid * per + i < p.n_shares; ++i) {
+            const double m = shares[tid * per + i];
+            // (near a border two threads can take tau for theirs: neither keeps the margin then)
+            if (tau - at >= DRAW_MARGIN && at + m - tau >= DRAW_MARGIN) { s_share = tid * per + i; s_before = at; break; }
             at += m;
         }
     }
-    Residual<T> res;
-    res.setup(p, b, n, len);
     __syncthreads();
-    int share = s_share, last = share;
-    u128 at = share >= 0 ? s_before : u128(0);
-    if (r == 0) {  // no residual (see the head of the file): drawn from P, share after share
-        res.rq = nullptr;
-        res.skip = -1;
-        tau = floor_scale_wide(u, p.rows[int64_t(b) * (p.k + 1) + n].z);
-        share = 0;
-        last = p.n_shares - 1;
-    }
-    for (; share >= 0 && share <= last; ++share) {  // block-uniform, one turn unless r is 0
-        const int64_t base = (int64_t(share) * SHARE_VECS + tid) * T::kPerVec;
-        u128 m[T::kPerVec], total;
-        res.vector(base, m);
-        const u128 sum = total_of(m);
-        const u128 before = at + block_excl_scan_u128<WAVES>(sum, wave_buf, &total);
-        if (before <= tau && tau < before + sum) s_hit = int(base) + entry_at(m, before, tau);
-        at += total;
-        if (tau < at) break;
+    if (s_share >= 0) {  // the same for the whole block
+        const int64_t base = (int64_t(s_share) * SHARE_VECS + tid) * EPV;
+        double m[EPV], sum = 0.0, total;
+#pragma unroll
+        for (int j = 0; j < EPV; ++j) m[j] = 0.0;
+        res.vector(base, [&](int j, double v) {
+#pragma unroll
+            for (int k = 0; k < EPV; ++k) m[k] = j == k ? v : m[k];
+            sum += v;
+        });
+        double before = s_before + block_excl_scan_of<WAVES, double>(sum, wave_buf.d, &total);
+        if (before <= tau && tau < before + sum) {
+            bool found = false;
+#pragma unroll
+            for (int j = 0; j < EPV; ++j) {
+                if (!found && tau < before + m[j]) {
+                    found = true;
+                    if (tau - before >= DRAW_MARGIN && before + m[j] - tau >= DRAW_MARGIN) s_hit = int(base) + j;
+                }
+                before += m[j];
+            }
+        }
     }
     __syncthreads();
-    // outputs: lane j writes position j
+    int hit = s_hit;
+    if (hit < 0) {  // block-uniform
+        __syncthreads();
+        hit = exact_draw<T>(res, u, p.n_shares, wave_buf.w, &s_hit);
+    }
+    // outputs: thread j writes position j
     for (int j = tid; j <= p.k; j += SHARE_VECS) {
         const int64_t at = int64_t(b) * (p.k + 1) + j;
-        const int64_t id = j < n ? p.draft_ids[int64_t(b) * p.k + j] : (j == n ? int64_t(s_hit) : int64_t(-1));
+        const int64_t id = j < n ? p.draft_ids[int64_t(b) * p.k + j] : (j == n ? int64_t(hit) : int64_t(-1));
         p.out_ids[at] = id;
         if (p.out_policy != nullptr) {
             float lp = 0.0f;
-            if (j <= n) lp = id >= 0 ? float(double(T::widen(target_row<T>(p, b, j)[id])) - p.rows[at].lse) : __builtin_nanf("");
+            if (j <= n) {
+                const double lse = double(p.rows[at].raw_top) + log(p.rows[at].raw_sum);
+                lp = id >= 0 ? float(double(T::widen(target_row<T>(p, b, j)[id])) - lse) : __builtin_nanf("");
+            }
             p.out_policy[at] = lp;
         }
     }
     if (tid == 0) p.out_accepted[b] = n;
+}
+
+// verify_shares_table uses 78 KB of LDS: the attribute belongs to the device, set once for each.
+inline int reserve_table_lds() {
+    static std::mutex mutex;
+    static bool done[64] = {};
+    int device = 0;
+    hipError_t rc = hipGetDevice(&device);
+    if (rc != hipSuccess) return check_hip(rc, "verify: hipGetDevice");
+    if (device < 0 || device >= 64) return fail(KA_ERR_UNSUPPORTED, "verify: device index %d", device);
+    std::lock_guard<std::mutex> lock(mutex);
+    if (!done[device]) {
+        rc = hipFuncSetAttribute(reinterpret_cast<const void *>(verify_shares_table), hipFuncAttributeMaxDynamicSharedMemorySize, int(TABLE_LDS_BYTES));
+        if (rc != hipSuccess) return check_hip(rc, "verify: reserving LDS for the tables");
+        done[device] = true;
+    }
+    return KA_OK;
 }
 
 template <typename T> int launch_verify(const VerifyParams &p, hipStream_t stream) {
@@ -771,7 +1040,14 @@ template <typename T> int launch_verify(const VerifyParams &p, hipStream_t strea
         rc = check_hip(hipGetLastError(), "verify launch (ties)");
         if (rc != KA_OK) return rc;
     }
-    hipLaunchKernelGGL((verify_shares<T>), dim3(unsigned((p.n_shares * kWave + SHARE_THREADS - 1) / SHARE_THREADS), unsigned(p.batch)), dim3(SHARE_THREADS), 0, stream, p);
+    if (T::kDtype == KA_DTYPE_BF16 && p.shares_per_group > 0) {
+        rc = reserve_table_lds();
+        if (rc != KA_OK) return rc;
+        hipLaunchKernelGGL(verify_shares_table, dim3(unsigned((p.n_shares + p.shares_per_group - 1) / p.shares_per_group), unsigned(p.batch)),
+                           dim3(TABLE_THREADS), TABLE_LDS_BYTES, stream, p);
+    } else {
+        hipLaunchKernelGGL((verify_shares<T>), dim3(unsigned((p.n_shares * kWave + SHARE_THREADS - 1) / SHARE_THREADS), unsigned(p.batch)), dim3(SHARE_THREADS), 0, stream, p);
+    }
     rc = check_hip(hipGetLastError(), "verify launch (shares)");
     if (rc != KA_OK) return rc;
     hipLaunchKernelGGL((verify_draw<T>), dim3(unsigned(p.batch)), dim3(SHARE_VECS), 0, stream, p);
@@ -791,7 +1067,7 @@ inline VerifyLayout verify_layout(int dtype, int64_t batch, int64_t k, int64_t v
     l.rows = 0;
     l.ties = align_up(size_t(batch) * size_t(2 * k + 1) * sizeof(RowSummary), 256);
     l.shares = l.ties + align_up(size_t(batch) * 8, 256);
-    l.total = l.shares + size_t(batch) * size_t(l.n_shares) * sizeof(u128);
+    l.total = l.shares + size_t(batch) * size_t(l.n_shares) * sizeof(double);
     return l;
 }
 
@@ -867,8 +1143,16 @@ KA_EXPORT int ka_verify_draft(int dtype, const void *target_logits, int64_t targ
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     p.rows = reinterpret_cast<RowSummary *>(ws + l.rows);
     p.tie_limit = reinterpret_cast<int32_t *>(ws + l.ties);
-    p.shares = reinterpret_cast<u128 *>(ws + l.shares);
+    p.shares = reinterpret_cast<double *>(ws + l.shares);
     p.n_shares = int32_t(l.n_shares);
+    // Tables pay where most entries may have mass: two of them cost 9728 evaluations, a share of 2048 entries 4096 without.
+    // Enough groups to fill the device twice, of at least eight shares (one per wavefront).
+    const bool many = top_k_rows != nullptr || top_k == 0 || top_k > 1024;
+    if (dtype == KA_DTYPE_BF16 && many && l.n_shares >= 16) {
+        int64_t groups = (512 + batch - 1) / batch;
+        if (groups > (l.n_shares + 7) / 8) groups = (l.n_shares + 7) / 8;
+        p.shares_per_group = int32_t(((l.n_shares + groups - 1) / groups + 7) / 8 * 8);
+    }
     auto aligned = [&](const void *base, int64_t batch_stride, int64_t pos_stride, int64_t positions) {
         return reinterpret_cast<uintptr_t>(base) % 16 == 0 && (batch == 1 || (batch_stride * esize) % 16 == 0) &&
                (positions <= 1 || (pos_stride * esize) % 16 == 0);

@@ -130,6 +130,40 @@ def test_special_rows(sampler, dtype, kw):
         assert torch.equal(got[1].cpu(), want[1]) and torch.equal(got[0].cpu(), want[0])
 
 
+@pytest.mark.parametrize("kw", [{}, {"temperature": 0.6}, {"top_p": 0.5}, {"top_p": 0.97, "temperature": 1.3}, {"top_k": 2000}])
+def test_special_rows_of_a_large_vocabulary(sampler, kw):
+    """bf16 rows long enough for the tables of the last pass, with values outside their bins: tiny ones of both signs, zeros,
+    masked entries, values far from zero - and the same as drafts."""
+    rows = _special_rows(torch.bfloat16, vocab=40004)
+    del rows["one left"]
+    g = torch.Generator().manual_seed(15)
+    rows["tiny and not"] = torch.where(torch.rand(40004, generator=g) < 0.02, torch.randn(40004, generator=g) * 3e-4,
+                                       torch.randn(40004, generator=g)).bfloat16()
+    names = sorted(rows)
+    target = torch.stack([torch.stack([rows[n], rows["masked"]]) for n in names for _ in range(2)])
+    draft = torch.stack([rows[names[(i + s) % len(names)]].unsqueeze(0) for i in range(len(names)) for s in (0, 5)])
+    batch, vocab = target.shape[0], target.shape[2]
+    ids = torch.randint(0, vocab, (batch, 1), generator=g)
+    u = torch.rand(batch, 2, generator=g)
+    for q in (draft, None):
+        got = sampler.verify_draft(target.cuda(), ids.cuda(), u.cuda(), draft_logits=_gpu(q), **kw)
+        want = verify_ref.verify(target, ids, u, q, **kw)
+        assert torch.equal(got[1].cpu(), want[1]) and torch.equal(got[0].cpu(), want[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_draws_on_a_border(sampler, dtype):
+    """Rows of equal masses whose uniform falls exactly on the border between two entries: decided in integers."""
+    t = torch.zeros(8, 2, 4096, dtype=dtype)
+    q = t[:, :1].clone()
+    u = torch.zeros(8, 2)
+    u[:, 1] = torch.arange(8) / 8.0
+    ids = torch.arange(8).unsqueeze(1)
+    got = _check(sampler, t, ids, u, q, None)
+    assert got[1].tolist() == [1] * 8 and got[0][:, 1].tolist() == [512 * i for i in range(8)]
+    _check(sampler, t[:, :1], ids[:, :0], u[:, 1:], None, None)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_ties_at_the_cut(sampler, dtype):
     """Rows of a handful of values: top-p cuts inside a group of equal logits, and the drafts sit in that group on both sides
