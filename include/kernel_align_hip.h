@@ -213,7 +213,7 @@ int ka_sample_mass_fixed(const float *d, int64_t n, uint64_t *out, void *hip_str
  * out_policy_logprob (optional, fp32 [batch, max_draft + 1]): log-probability of every emitted token under the unfiltered
  * softmax of its target row (to 1e-5 what ka_logprob_* returns), 0 behind the last.
  * Limits: max_draft <= KA_VERIFY_MAX_DRAFT, vocab < 2^22, batch <= 65535.  The workspace is 16-byte aligned, of
- * ka_verify_workspace_bytes (0 for arguments the call refuses): 48 bytes per row and 8 per request and share of 256
+ * ka_verify_workspace_bytes (0 for arguments the call refuses): 48 bytes per row and 40 per request and share of 256
  * 16-byte vectors.  Any alignment of the rows is taken.  No counterpart in the reference, whose sampler draws one token per
  * forward pass (rl_engine/kernels/sampling.py:39-88).
  */

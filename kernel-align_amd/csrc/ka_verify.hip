@@ -17,14 +17,15 @@
 // 2^12 terms, by 2^-41 in all (P and Q sum to one).  An entry whose prefix sums lie more than DRAW_MARGIN = 2^-38 on either side of u R is the
 // integers' answer too; otherwise (about one draw in 10^6, and u = 0) the workgroup repeats the draw in 128-bit integers.
 //
-// Three or four launches, no host synchronisation:
+// Three launches, no host synchronisation:
 //   verify_rows    one workgroup per row that counts (target rows 0 .. len, draft rows 0 .. len - 1): the cut of the row's
 //                  distribution, its total mass, the draft token's mass, the log-sum-exp of the raw row.  This is the pass over
 //                  the data: bound by HBM, 2 V (2 K + 1) bytes per request.
-//   verify_ties    (only where top-p may cut inside a group of equal logits) the index at which the cut falls, for the two rows
-//                  of the position where the request stops
 //   verify_shares  residual mass of every share of 256 vectors of the stopping position, a wavefront each
 //   verify_draw    one workgroup per request: the share, the vector and the entry that hold the draw; all outputs
+// Where top-p cuts inside a group of equal logits, the first r of the group survive, in index order.  verify_shares cannot know
+// which those are: it counts the group's entries in its share and leaves the share's sum for either case, with the group or
+// without it, and verify_draw, which sees all counts, picks one and evaluates the share again in which the r-th lies.
 // The rows of the stopping position are read again by the last ones, from L2 / MALL as a rule.
 #define KA_SAMPLING_THREADS 512
 #include <stddef.h>
@@ -56,6 +57,16 @@ struct RowSummary {
 };
 static_assert(sizeof(RowSummary) == 48, "the workspace query counts 48 bytes per row");
 
+// Residual mass of a share of the stopping position, by what becomes of the two rows' tie groups at their cuts.
+struct ShareSums {
+    double all;       // both groups survive
+    double without_p; // the target's group does not
+    double without_q; // the draft's group does not
+    double neither;
+    uint32_t ties_p, ties_q;  // entries of the groups; 0 where a group survives whole
+};
+static_assert(sizeof(ShareSums) == 40, "the workspace query counts 40 bytes per share");
+
 struct VerifyParams {
     const void *target, *draft;                          // draft may be null
     int64_t t_batch, t_pos, d_batch, d_pos;              // strides in elements
@@ -69,9 +80,8 @@ struct VerifyParams {
     int64_t *out_ids, *out_accepted;
     float *out_policy;                                   // may be null
     RowSummary *rows;                                    // [B (K + 1)] target rows, then [B K] draft rows
-    int32_t *tie_limit;                                  // [B, 2]: an entry equal to kcut survives iff its index is below this
-    double *shares;                                      // [B, n_shares]
-    int32_t n_shares, shares_per_group, vec_target, vec_draft, may_cut_ties;
+    ShareSums *shares;                                   // [B, n_shares]
+    int32_t n_shares, shares_per_group, vec_target, vec_draft;
 };
 
 struct Filter { float temp; bool has_t; bool use_k; int top_k; bool use_p; float top_p; };
@@ -177,6 +187,16 @@ template <typename T> __device__ __forceinline__ uint32_t at_least(const uint4 &
     for (int j = 0; j < T::kPerVec; ++j) bits |= !(x[j] < low) ? 1u << j : 0u;
     const int64_t room = vocab - base;
     return room >= T::kPerVec ? bits : (room <= 0 ? 0u : bits & ((1u << int(room)) - 1u));
+}
+// Bit j: entry base + j lies in the row and its scaled key is `key` (no entry below `low` has it).
+template <typename T> __device__ __forceinline__ uint32_t ties_of(const uint4 &v, float low, int64_t base, int vocab, uint32_t key, const Filter &f) {
+    uint32_t ties = 0;
+#pragma unroll 1
+    for (uint32_t left = at_least<T>(v, low, base, vocab); left != 0; left &= left - 1) {
+        const int j = __ffs(left) - 1;
+        if (elem_key<T>(entry_of<T>(v, j), f.temp, f.has_t) == key) ties |= 1u << j;
+    }
+    return ties;
 }
 // The value below which an unscaled entry does not survive (NaN compares as surviving: its key decides).
 template <typename T> __device__ __forceinline__ float cut_value(uint32_t raw_cut) {
@@ -333,26 +353,23 @@ __device__ __forceinline__ bool hist_cut(HistRow &h, const uint16_t *rp, int voc
     {
         uint64_t all = 0, mid = 0;
         double raw_sum = 0.0;
-        const int end = total || want_lse ? HIST_POS : (first + WINDOW < HIST_POS ? first + WINDOW : HIST_POS);
-#pragma unroll 1
+        // (without branches on empty bins, two at a time: the chain of fused multiply-adds is what takes the time)
+        const int end = total ? HIST_POS : (first + WINDOW < HIST_POS ? first + WINDOW : HIST_POS);
+#pragma unroll 2
         for (int q = first + tid; q < end; q += S_THREADS) {
-            const uint32_t c = count_at(q);
-            uint64_t w = 0;
-            uint32_t key = NO_KEY;
-            if (c != 0 && q != HIST_SIDE) {
-                const uint32_t raw = raw_of_bin(bin_of_pos(q));
-                if (total || q < first + WINDOW) {
-                    key = key_of_raw(raw);
-                    w = weight_of(key) * c;
-                    all += w;
-                }
-                // (fp32 exponentials, off by 2^-22 each: ample for a log-probability in fp32)
-                if (want_lse) raw_sum += double(float(c) * fast_exp2((Bf16::widen(uint16_t(raw)) - xmax) * kLseLog2e));
-            }
+            const uint32_t c = q == HIST_SIDE ? 0u : count_at(q);
+            const uint32_t key = key_of_raw(raw_of_bin(bin_of_pos(q == HIST_SIDE ? first : q)));
+            const uint64_t w = weight_of(key) * c;
+            all += w;
             if (q < first + WINDOW) {
                 h.win_mass[q - first] = w;
-                h.win_key[q - first] = key;
+                h.win_key[q - first] = c != 0 ? key : NO_KEY;
             }
+        }
+        if (want_lse) {  // (fp32 exponentials, off by 2^-22 each: ample for a log-probability in fp32)
+#pragma unroll 2
+            for (int q = first + tid; q < HIST_POS; q += S_THREADS)
+                if (q != HIST_SIDE) raw_sum += double(float(count_at(q)) * fast_exp2((Bf16::widen(uint16_t(raw_of_bin(bin_of_pos(q)))) - xmax) * kLseLog2e));
         }
         if (total || want_lse) {
 #pragma unroll 1
@@ -388,9 +405,17 @@ __device__ __forceinline__ bool hist_cut(HistRow &h, const uint16_t *rp, int voc
             raw_sum += h.raw_sums[w];
         }
     z_all += z_mid;
-    const uint32_t key_dropped = key_of_raw(0x8000u | MAG_HIGH), key_tiny = key_of_raw(MAG_LOW - 1), key_tiny_neg = key_of_raw(0x8000u | (MAG_LOW - 1));
     const bool dropped = h.dropped != 0;
-    bool ok = !dropped || (weight_fix(value_of<Bf16>(key_dropped) - vmax) == 0 && weight_fix(-256.0f - xmax) == 0);
+    uint32_t key_dropped = 0, key_tiny = 0, key_tiny_neg = 0;
+    bool ok = true;
+    if (dropped) {
+        key_dropped = key_of_raw(0x8000u | MAG_HIGH);
+        ok = weight_fix(value_of<Bf16>(key_dropped) - vmax) == 0 && weight_fix(-256.0f - xmax) == 0;
+    }
+    if (f.use_k || f.use_p) {
+        key_tiny = key_of_raw(MAG_LOW - 1);
+        key_tiny_neg = key_of_raw(0x8000u | (MAG_LOW - 1));
+    }
     // a cut that shares its scaled value with entries that are not binned (a temperature that folds values together)
     auto shared_value = [&](uint32_t key, int q) {
         return (dropped && key <= key_dropped) || (n_mid > 0 && (q < HIST_SIDE ? key <= key_tiny : key >= key_tiny_neg));
@@ -571,8 +596,17 @@ __global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(6, 6)
         __syncthreads();
         if (tid == 0) lds.ties_before = 0;
         __syncthreads();
+        const float low = cut_value<T>(raw_cut);
         uint32_t mine = 0;
-        for_each_key<T>(rp, int(d), vec, f.temp, f.has_t, [&](int, uint32_t k) { mine += k == cut.kcut ? 1u : 0u; });
+        constexpr int U = 8, EPV = T::kPerVec;  // vectors in flight per lane
+        for (int64_t base = int64_t(tid) * EPV; base < d; base += U * S_THREADS * EPV) {
+            uint4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = load_entries<T>(rp, vec, int(d), base + u * S_THREADS * EPV);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                mine += uint32_t(__popc(ties_of<T>(v[u], low, base + u * S_THREADS * EPV, int(d), cut.kcut, f)));
+        }
         if (mine) atomicAdd(&lds.ties_before, mine);
         __syncthreads();
         kept = lds.ties_before < cut.r_cut;
@@ -593,171 +627,127 @@ __global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(6, 6)
 }
 
 // ---------------------------------------------------------------------------
-// verify_ties: grid (B, 2).  Where a row's cut falls inside a tie group, the index below which the group's entries survive:
-// the ties of every chunk of 512 vectors are counted, and the chunk that holds the last survivor is read once more in order.
-// ---------------------------------------------------------------------------
-constexpr int MAX_CHUNKS = (1 << 22) / (4 * S_THREADS);
-template <typename T>
-__global__ __launch_bounds__(S_THREADS) void verify_ties(VerifyParams p) {
-    __shared__ uint32_t ties[MAX_CHUNKS];
-    __shared__ uint32_t wave_buf[S_WAVES];
-    __shared__ uint32_t s_chunk, s_before;
-    constexpr int EPV = T::kPerVec;
-    const int b = blockIdx.x, tid = threadIdx.x;
-    const bool is_target = blockIdx.y == 0;
-    const int len = draft_len(p, b);
-    const int n = accepted_prefix(p, b, len);
-    if (!is_target && (n == len || p.draft == nullptr)) return;
-    const int64_t row = is_target ? int64_t(b) * (p.k + 1) + n : int64_t(p.batch) * (p.k + 1) + int64_t(b) * p.k + n;
-    const uint32_t r_cut = p.rows[row].r_cut, kcut = p.rows[row].kcut;
-    int32_t *const limit = p.tie_limit + 2 * b + (is_target ? 0 : 1);
-    if (r_cut == 0xffffffffu) {
-        if (tid == 0) *limit = 0x7fffffff;
-        return;
-    }
-    const Filter f = filter_of(p, b);
-    const typename T::raw_t *rp = is_target ? target_row<T>(p, b, n) : draft_row<T>(p, b, n);
-    const bool vec = (is_target ? p.vec_target : p.vec_draft) != 0;
-    const float low = cut_value<T>(p.rows[row].raw_cut);
-    // bit j: entry j belongs to the group
-    auto ties_of = [&](const uint4 &v, int64_t base) {
-        uint32_t ties = 0;
-        for (uint32_t left = at_least<T>(v, low, base, p.vocab); left != 0; left &= left - 1) {
-            const int j = __ffs(left) - 1;
-            if (elem_key<T>(entry_of<T>(v, j), f.temp, f.has_t) == kcut) ties |= 1u << j;
-        }
-        return ties;
-    };
-    const int chunks = (p.vocab + EPV * S_THREADS - 1) / (EPV * S_THREADS);
-    for (int i = tid; i < chunks; i += S_THREADS) ties[i] = 0;
-    __syncthreads();
-    constexpr int U = 8;  // vectors in flight per lane
-    for (int c0 = 0; c0 < chunks; c0 += U) {
-        uint4 v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = load_entries<T>(rp, vec, p.vocab, ((c0 + u) * S_THREADS + tid) * int64_t(EPV));
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t c = uint32_t(__popc(ties_of(v[u], ((c0 + u) * S_THREADS + tid) * int64_t(EPV))));
-            if (c) atomicAdd(&ties[c0 + u], c);
-        }
-    }
-    __syncthreads();
-    // chunks in order: thread t takes a run of them
-    const int per = (chunks + S_THREADS - 1) / S_THREADS;
-    uint32_t mine = 0, total;
-    for (int i = 0; i < per; ++i) mine += tid * per + i < chunks ? ties[tid * per + i] : 0u;
-    const uint32_t before = block_excl_scan<uint32_t>(mine, wave_buf, &total);
-    if (before < r_cut && r_cut <= before + mine) {
-        uint32_t at = before;
-        for (int i = 0; i < per; ++i) {
-            const uint32_t c = ties[tid * per + i];
-            if (r_cut <= at + c) { s_chunk = uint32_t(tid * per + i); s_before = at; break; }
-            at += c;
-        }
-    }
-    __syncthreads();
-    const int64_t base = (int64_t(s_chunk) * S_THREADS + tid) * EPV;
-    uint32_t group = ties_of(load_entries<T>(rp, vec, p.vocab, base), base);
-    const uint32_t c = uint32_t(__popc(group));
-    const uint32_t rank = s_before + block_excl_scan<uint32_t>(c, wave_buf, &total);
-    if (rank < r_cut && r_cut <= rank + c) {
-        for (uint32_t skip = r_cut - rank - 1; skip != 0; --skip) group &= group - 1;
-        *limit = int32_t(base) + __ffs(group);  // the last survivor's index + 1
-    }
-}
-
-// ---------------------------------------------------------------------------
 // Residual masses of the stopping position
 // ---------------------------------------------------------------------------
 constexpr double DRAW_MARGIN = 0x1p-38;
 
 // A row's distribution, entry by entry.
 struct RowDist {
-    uint32_t kmax, kcut;
-    int limit;
+    uint32_t kmax, kcut, r_cut;
+    int limit;        // entries equal to kcut survive below this index
     float vmax, low;  // unscaled values below `low` have no mass
     uint64_t z;
-    template <typename T> __device__ __forceinline__ uint64_t mass(typename T::raw_t x, int i, const Filter &f) const {
+    double inv;       // 1 / z
+    __device__ __forceinline__ bool partial() const { return r_cut != 0xffffffffu; }
+    // mass of an entry if the tie group survives; `tie`: it belongs to one that survives in part
+    template <typename T> __device__ __forceinline__ uint64_t mass(typename T::raw_t x, const Filter &f, bool &tie) const {
+        tie = false;
         if (T::widen(x) < low) return 0ull;
         const uint32_t key = elem_key<T>(x, f.temp, f.has_t);
-        if (key < kcut || (key == kcut && i >= limit)) return 0ull;
+        if (key < kcut) return 0ull;
+        tie = key == kcut && partial();
         return weight_fix(key == kmax ? 0.0f : value_of<T>(key) - vmax);
     }
-    template <typename T> __device__ __forceinline__ void from(const RowSummary &s, int tie_limit) {
+    template <typename T> __device__ __forceinline__ uint64_t mass_at(typename T::raw_t x, int i, const Filter &f) const {
+        bool tie;
+        const uint64_t w = mass<T>(x, f, tie);
+        return tie && i >= limit ? 0ull : w;
+    }
+    template <typename T> __device__ __forceinline__ void from(const RowSummary &s) {
         kmax = s.kmax;
         kcut = s.kcut;
-        limit = tie_limit;
+        r_cut = s.r_cut;
+        limit = 0x7fffffff;
         vmax = value_of<T>(s.kmax);
         low = cut_value<T>(s.raw_cut);
         z = s.z;
+        inv = 1.0 / double(s.z);
     }
 };
+
+__device__ __forceinline__ double positive(double r) { return r > 0.0 ? r : 0.0; }
+
+// Adds one entry to a share's sums: p and q are its probabilities if the groups survive.
+__device__ __forceinline__ void add_entry(ShareSums &s, double p, double q, bool tie_p, bool tie_q) {
+    const double r = positive(p - q);
+    s.all += r;
+    s.without_p += tie_p ? 0.0 : r;
+    const double alone = tie_q ? p : r;
+    s.without_q += alone;
+    s.neither += tie_p ? 0.0 : alone;
+    s.ties_p += tie_p ? 1u : 0u;
+    s.ties_q += tie_q ? 1u : 0u;
+}
 
 // Residual of entry i: max(P - Q, 0); P alone where nothing was rejected, 0 for a looked-up draft that was.
 template <typename T> struct Residual {
     const typename T::raw_t *rp, *rq;  // rq null: nothing is subtracted
     bool vec_p, vec_q;
     RowDist p, q;
-    double inv_p, inv_q;
     int64_t skip;  // the rejected look-up draft, or -1
     Filter f;
     int vocab;
 
     __device__ __forceinline__ void setup(const VerifyParams &v, int b, int n, int len) {
-        const RowSummary &t = v.rows[int64_t(b) * (v.k + 1) + n];
         f = filter_of(v, b);
         vocab = v.vocab;
         rp = target_row<T>(v, b, n);
         vec_p = v.vec_target != 0;
-        p.template from<T>(t, v.may_cut_ties ? v.tie_limit[2 * b] : 0x7fffffff);
-        inv_p = 1.0 / double(p.z);
-        inv_q = 0.0;
+        p.template from<T>(v.rows[int64_t(b) * (v.k + 1) + n]);
         rq = nullptr;
         vec_q = false;
         skip = -1;
         q = p;
+        q.r_cut = 0xffffffffu;
         if (n < len) {
             if (v.draft != nullptr) {
                 rq = draft_row<T>(v, b, n);
                 vec_q = v.vec_draft != 0;
-                q.template from<T>(v.rows[int64_t(v.batch) * (v.k + 1) + int64_t(b) * v.k + n], v.may_cut_ties ? v.tie_limit[2 * b + 1] : 0x7fffffff);
-                inv_q = 1.0 / double(q.z);
+                q.template from<T>(v.rows[int64_t(v.batch) * (v.k + 1) + int64_t(b) * v.k + n]);
             } else {
                 skip = v.draft_ids[int64_t(b) * v.k + n];
             }
         }
     }
-    __device__ __forceinline__ double entry(typename T::raw_t x, typename T::raw_t y, int i) const {
-        if (int64_t(i) == skip) return 0.0;
-        const uint64_t wp = p.template mass<T>(x, i, f);
-        if (wp == 0) return 0.0;
-        double r = double(wp) * inv_p;
-        if (rq != nullptr) r -= double(q.template mass<T>(y, i, f)) * inv_q;
-        return r > 0.0 ? r : 0.0;
+    __device__ __forceinline__ uint4 load_p(int64_t base) const { return load_entries<T>(rp, vec_p, vocab, base); }
+    __device__ __forceinline__ uint4 load_q(int64_t base) const {
+        return rq != nullptr ? load_entries<T>(rq, vec_q, vocab, base) : make_uint4(0, 0, 0, 0);
     }
-    // each(j, residual) for the entries of the vector at `base` that may have one, in order
-    template <typename F> __device__ __forceinline__ void vector(int64_t base, F &&each) const {
-        const uint4 x = load_entries<T>(rp, vec_p, vocab, base);
-        const uint4 y = rq != nullptr ? load_entries<T>(rq, vec_q, vocab, base) : make_uint4(0, 0, 0, 0);
+    // the entries `left` of the vector at `base` into a share's sums
+    __device__ __forceinline__ void add_entries(const uint4 &x, const uint4 &y, int64_t base, uint32_t left, ShareSums &s) const {
 #pragma unroll 1
-        for (uint32_t left = at_least<T>(x, p.low, base, vocab); left != 0; left &= left - 1) {
+        for (; left != 0; left &= left - 1) {
             const int j = __ffs(left) - 1;
-            each(j, entry(entry_of<T>(x, j), entry_of<T>(y, j), int(base) + j));
+            bool tie_p, tie_q = false;
+            double pv = double(p.template mass<T>(entry_of<T>(x, j), f, tie_p)) * p.inv;
+            if (base + j == skip) pv = 0.0;  // (it still has its place in a tie group)
+            const double qv = rq != nullptr ? double(q.template mass<T>(entry_of<T>(y, j), f, tie_q)) * q.inv : 0.0;
+            add_entry(s, pv, qv, tie_p, tie_q);
         }
     }
-    // the same in integers, times Z^p Z^q (times Z^p where nothing is subtracted)
-    template <typename F> __device__ __forceinline__ void exact_vector(int64_t base, F &&each) const {
-        const uint4 x = load_entries<T>(rp, vec_p, vocab, base);
-        const uint4 y = rq != nullptr ? load_entries<T>(rq, vec_q, vocab, base) : make_uint4(0, 0, 0, 0);
+    // each(j, residual) for the entries of the vector at `base` that may have one, in order; the limits are known
+    template <typename F> __device__ __forceinline__ void vector(int64_t base, F &&each) const {
+        const uint4 x = load_p(base), y = load_q(base);
 #pragma unroll 1
         for (uint32_t left = at_least<T>(x, p.low, base, vocab); left != 0; left &= left - 1) {
             const int j = __ffs(left) - 1, i = int(base) + j;
             if (int64_t(i) == skip) continue;
-            u128 have = p.template mass<T>(entry_of<T>(x, j), i, f), take = 0;
+            double r = double(p.template mass_at<T>(entry_of<T>(x, j), i, f)) * p.inv;
+            if (rq != nullptr) r -= double(q.template mass_at<T>(entry_of<T>(y, j), i, f)) * q.inv;
+            each(j, positive(r));
+        }
+    }
+    // the same in integers, times Z^p Z^q (times Z^p where nothing is subtracted)
+    template <typename F> __device__ __forceinline__ void exact_vector(int64_t base, F &&each) const {
+        const uint4 x = load_p(base), y = load_q(base);
+#pragma unroll 1
+        for (uint32_t left = at_least<T>(x, p.low, base, vocab); left != 0; left &= left - 1) {
+            const int j = __ffs(left) - 1, i = int(base) + j;
+            if (int64_t(i) == skip) continue;
+            u128 have = p.template mass_at<T>(entry_of<T>(x, j), i, f), take = 0;
             if (rq != nullptr) {
                 have *= q.z;
-                take = u128(q.template mass<T>(entry_of<T>(y, j), i, f)) * p.z;
+                take = u128(q.template mass_at<T>(entry_of<T>(y, j), i, f)) * p.z;
             }
             each(j, have > take ? have - take : u128(0));
         }
@@ -769,6 +759,7 @@ __device__ __forceinline__ u128 shfl_up_of(u128 v, int off) {
     const uint64_t hi = __shfl_up((unsigned long long)uint64_t(v >> 64), off, kWave);
     return (u128(hi) << 64) | lo;
 }
+__device__ __forceinline__ uint64_t shfl_up_of(uint64_t v, int off) { return __shfl_up((unsigned long long)v, off, kWave); }
 __device__ __forceinline__ double shfl_up_of(double v, int off) { return __shfl_up(v, off, kWave); }
 template <typename V> __device__ __forceinline__ V wave_incl_scan_of(V v) {
     const int lane = threadIdx.x & (kWave - 1);
@@ -797,9 +788,23 @@ template <int WAVES, typename V> __device__ __forceinline__ V block_excl_scan_of
     return base + inc - v;
 }
 
+// The wavefront's sums over its lanes, in a fixed order; the last lane writes them.  `parts`: some tie group survives in part.
+__device__ __forceinline__ void store_share(ShareSums s, bool parts, ShareSums *out) {
+    s.all = wave_incl_scan_of(s.all);
+    if (parts) {
+        s.without_p = wave_incl_scan_of(s.without_p);
+        s.without_q = wave_incl_scan_of(s.without_q);
+        s.neither = wave_incl_scan_of(s.neither);
+        s.ties_p = wave_incl_scan_u32(s.ties_p);
+        s.ties_q = wave_incl_scan_u32(s.ties_q);
+    }
+    if ((threadIdx.x & (kWave - 1)) == kWave - 1) *out = s;
+}
+
 // grid (groups of shares, B): a wavefront per share
 template <typename T>
 __global__ __launch_bounds__(SHARE_THREADS) void verify_shares(VerifyParams p) {
+    constexpr int STEPS = SHARE_VECS / kWave;
     const int b = blockIdx.y, lane = threadIdx.x & (kWave - 1);
     const int share = int(blockIdx.x) * (SHARE_THREADS / kWave) + int(threadIdx.x) / kWave;
     const int len = draft_len(p, b);
@@ -807,12 +812,20 @@ __global__ __launch_bounds__(SHARE_THREADS) void verify_shares(VerifyParams p) {
     if (share >= p.n_shares) return;
     Residual<T> res;
     res.setup(p, b, n, len);
-    double sum = 0.0;
-#pragma unroll 1
-    for (int s = 0; s < SHARE_VECS / kWave; ++s)
-        res.vector((int64_t(share) * SHARE_VECS + s * kWave + lane) * T::kPerVec, [&](int, double r) { sum += r; });
-    sum = wave_incl_scan_of(sum);
-    if (lane == kWave - 1) p.shares[int64_t(b) * p.n_shares + share] = sum;
+    ShareSums sums{};
+    uint4 x[STEPS], y[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const int64_t base = (int64_t(share) * SHARE_VECS + s * kWave + lane) * T::kPerVec;
+        x[s] = res.load_p(base);
+        y[s] = res.load_q(base);
+    }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const int64_t base = (int64_t(share) * SHARE_VECS + s * kWave + lane) * T::kPerVec;
+        res.add_entries(x[s], y[s], base, at_least<T>(x[s], res.p.low, base, res.vocab) | (res.q.partial() ? at_least<T>(y[s], res.q.low, base, res.vocab) : 0u), sums);
+    }
+    store_share(sums, res.p.partial() || res.q.partial(), p.shares + int64_t(b) * p.n_shares + share);
 }
 
 // The same for bf16 rows of which many entries survive (no top-k, or a large one): the masses come from two tables in LDS, one
@@ -830,39 +843,38 @@ __global__ __launch_bounds__(TABLE_THREADS) void verify_shares_table(VerifyParam
     const int n = accepted_prefix(p, b, len);
     Residual<T> res;
     res.setup(p, b, n, len);
-    const bool two = res.rq != nullptr, looked_up = res.skip >= 0;
-    // a value of the group that survives in part is marked by its sign
-    const bool part_p = res.p.limit != 0x7fffffff, part_q = res.q.limit != 0x7fffffff;
-    auto probability = [&](const RowDist &d, double inv, bool part, uint32_t raw) {
+    const bool two = res.rq != nullptr, looked_up = res.skip >= 0, parts = res.p.partial() || res.q.partial();
+    // a value of a group that survives in part is marked by its sign
+    auto probability = [&](const RowDist &d, uint32_t raw) {
         const uint32_t key = elem_key<T>(uint16_t(raw), res.f.temp, res.f.has_t);
         if (key < d.kcut) return 0.0;
-        const double v = double(weight_fix(key == d.kmax ? 0.0f : value_of<T>(key) - d.vmax)) * inv;
-        return part && key == d.kcut ? -v : v;
+        const double v = double(weight_fix(key == d.kmax ? 0.0f : value_of<T>(key) - d.vmax)) * d.inv;
+        return d.partial() && key == d.kcut ? -v : v;
     };
-#pragma unroll 1
+#pragma unroll 2
     for (int i = tid; i < HIST_BINS; i += TABLE_THREADS) {
         const uint32_t raw = raw_of_bin(i);
-        tab_p[i] = probability(res.p, res.inv_p, part_p, raw);
-        if (two) tab_q[i] = probability(res.q, res.inv_q, part_q, raw);
+        tab_p[i] = probability(res.p, raw);
+        if (two) tab_q[i] = probability(res.q, raw);
     }
     __syncthreads();
     // magnitude bits above the bins' lowest, and the entry's probability where that is below HIST_SIDE
     auto above = [](uint32_t x) { return (x & 0x7fffu) - MAG_LOW; };
     auto value = [](const double *tab, uint32_t m, uint32_t x) { return tab[HIST_SIDE + int(m ^ uint32_t(int32_t(x << 16) >> 31))]; };
-    auto kept = [](double v, int i, int limit) { return v < 0.0 ? (i < limit ? -v : 0.0) : v; };
     const int first = int(blockIdx.x) * p.shares_per_group;
     const int end = first + p.shares_per_group < p.n_shares ? first + p.shares_per_group : p.n_shares;
+    constexpr int STEPS = SHARE_VECS / kWave;
     for (int share = first + wave; share < end; share += TABLE_THREADS / kWave) {
-        double sum = 0.0;
-        uint4 x[SHARE_VECS / kWave], y[SHARE_VECS / kWave];
+        ShareSums sums{};
+        uint4 x[STEPS], y[STEPS];
 #pragma unroll
-        for (int s = 0; s < SHARE_VECS / kWave; ++s) {
+        for (int s = 0; s < STEPS; ++s) {
             const int64_t base = (int64_t(share) * SHARE_VECS + s * kWave + lane) * T::kPerVec;
-            x[s] = load_entries<T>(res.rp, res.vec_p, res.vocab, base);
-            y[s] = two ? load_entries<T>(res.rq, res.vec_q, res.vocab, base) : make_uint4(0, 0, 0, 0);
+            x[s] = res.load_p(base);
+            y[s] = res.load_q(base);
         }
 #pragma unroll
-        for (int s = 0; s < SHARE_VECS / kWave; ++s) {
+        for (int s = 0; s < STEPS; ++s) {
             const int64_t base = (int64_t(share) * SHARE_VECS + s * kWave + lane) * T::kPerVec;
             const uint32_t xw[4] = {x[s].x, x[s].y, x[s].z, x[s].w}, yw[4] = {y[s].x, y[s].y, y[s].z, y[s].w};
             if (base >= res.vocab) continue;
@@ -876,25 +888,15 @@ __global__ __launch_bounds__(TABLE_THREADS) void verify_shares_table(VerifyParam
                 if (mx >= uint32_t(HIST_SIDE) || (two && my >= uint32_t(HIST_SIDE))) {
                     odd |= whole ? 1u << j : 0u;
                 } else if (whole) {
-                    double r = value(tab_p, mx, xe);
-                    if (part_p) r = kept(r, int(base) + j, res.p.limit);
-                    if (two) {
-                        double t = value(tab_q, my, ye);
-                        if (part_q) t = kept(t, int(base) + j, res.q.limit);
-                        r -= t;
-                    }
-                    if (looked_up && int64_t(base) + j == res.skip) r = 0.0;
-                    sum += fmax(r, 0.0);
+                    const double pv = value(tab_p, mx, xe), qv = two ? value(tab_q, my, ye) : 0.0;
+                    const bool skipped = looked_up && base + j == res.skip;
+                    if (!parts) sums.all += skipped ? 0.0 : positive(pv - qv);
+                    else add_entry(sums, skipped ? 0.0 : fabs(pv), fabs(qv), pv < 0.0, qv < 0.0);
                 }
             }
-#pragma unroll 1
-            for (; odd != 0; odd &= odd - 1) {
-                const int j = __ffs(odd) - 1;
-                sum += res.entry(entry_of<T>(x[s], j), entry_of<T>(y[s], j), int(base) + j);
-            }
+            res.add_entries(x[s], y[s], base, odd, sums);
         }
-        sum = wave_incl_scan_of(sum);
-        if (lane == kWave - 1) p.shares[int64_t(b) * p.n_shares + share] = sum;
+        store_share(sums, parts, p.shares + int64_t(b) * p.n_shares + share);
     }
 }
 
@@ -939,30 +941,92 @@ template <typename T> __device__ __forceinline__ int exact_draw(Residual<T> res,
 template <typename T>
 __global__ __launch_bounds__(SHARE_VECS) void verify_draw(VerifyParams p) {
     constexpr int WAVES = SHARE_VECS / kWave, EPV = T::kPerVec;
-    __shared__ union { double d[WAVES]; u128 w[WAVES]; } wave_buf;
-    __shared__ double s_before;
-    __shared__ int s_share, s_hit;
+    __shared__ union { double d[WAVES]; uint64_t u[WAVES]; u128 w[WAVES]; } wave_buf;
+    __shared__ double s_before, s_value[2];
+    __shared__ int s_share, s_hit, s_cut[2], s_limit[2];
+    __shared__ uint32_t s_rank[2];
     const int b = blockIdx.x, tid = threadIdx.x;
     const int len = draft_len(p, b);
     const int n = accepted_prefix(p, b, len);
-    if (tid == 0) { s_share = -1; s_hit = -1; }
+    if (tid == 0) { s_share = s_hit = -1; s_cut[0] = s_cut[1] = -1; s_limit[0] = s_limit[1] = 0x7fffffff; }
     const float u = clean_uniform(p.uniforms[int64_t(b) * (p.k + 1) + p.k]);
-    // the share that holds u R: thread t takes a run of shares
-    double mine = 0.0, r;
-    const int per = (p.n_shares + SHARE_VECS - 1) / SHARE_VECS;
-    const double *const shares = p.shares + int64_t(b) * p.n_shares;
-    for (int i = 0; i < per; ++i)
-        if (tid * per + i < p.n_shares) mine += shares[tid * per + i];
     Residual<T> res;
     res.setup(p, b, n, len);
+    const ShareSums *const shares = p.shares + int64_t(b) * p.n_shares;
+    const bool parts = res.p.partial() || res.q.partial();
+    const int per = (p.n_shares + SHARE_VECS - 1) / SHARE_VECS;  // thread t takes a run of shares
+    const int s0 = tid * per, s1 = s0 + per < p.n_shares ? s0 + per : p.n_shares;
+    uint32_t before_p = 0, before_q = 0;  // ties in front of the thread's shares
+    if (parts) {
+        // ---- the shares and the indices at which the groups are cut ----
+        uint32_t cp = 0, cq = 0;
+        for (int s = s0; s < s1; ++s) { cp += shares[s].ties_p; cq += shares[s].ties_q; }
+        uint64_t total;
+        const uint64_t both = block_excl_scan_of<WAVES, uint64_t>((uint64_t(cq) << 32) | cp, wave_buf.u, &total);
+        before_p = uint32_t(both);
+        before_q = uint32_t(both >> 32);
+        uint32_t rp = before_p, rq = before_q;
+        for (int s = s0; s < s1; ++s) {
+            // the share that holds the last survivor, and how many of its entries survive
+            if (res.p.partial() && rp < res.p.r_cut && res.p.r_cut <= rp + shares[s].ties_p) { s_cut[0] = s; s_rank[0] = res.p.r_cut - rp; }
+            if (res.q.partial() && rq < res.q.r_cut && res.q.r_cut <= rq + shares[s].ties_q) { s_cut[1] = s; s_rank[1] = res.q.r_cut - rq; }
+            rp += shares[s].ties_p;
+            rq += shares[s].ties_q;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int side = 0; side < 2; ++side) {
+            const RowDist &d = side == 0 ? res.p : res.q;
+            if (!d.partial() || s_cut[side] < 0) continue;  // block-uniform
+            const int64_t base = (int64_t(s_cut[side]) * SHARE_VECS + tid) * EPV;
+            uint32_t group = ties_of<T>(side == 0 ? res.load_p(base) : res.load_q(base), d.low, base, p.vocab, d.kcut, res.f);
+            uint64_t all;
+            const uint32_t rank = uint32_t(block_excl_scan_of<WAVES, uint64_t>(uint64_t(__popc(group)), wave_buf.u, &all));
+            if (rank < s_rank[side] && s_rank[side] <= rank + uint32_t(__popc(group))) {
+                for (uint32_t skip = s_rank[side] - rank - 1; skip != 0; --skip) group &= group - 1;
+                s_limit[side] = int(base) + __ffs(group);  // the last survivor's index + 1
+            }
+        }
+        __syncthreads();
+        res.p.limit = s_limit[0];
+        res.q.limit = s_limit[1];
+        // ---- the one or two shares that are cut, with the limits known ----
+#pragma unroll 1
+        for (int side = 0; side < 2; ++side) {
+            if (s_cut[side] < 0 || (side == 1 && s_cut[1] == s_cut[0])) continue;
+            double sum = 0.0, total_here;
+            res.vector((int64_t(s_cut[side]) * SHARE_VECS + tid) * EPV, [&](int, double r) { sum += r; });
+            block_excl_scan_of<WAVES, double>(sum, wave_buf.d, &total_here);
+            if (tid == 0) s_value[side] = total_here;
+        }
+        __syncthreads();
+    }
+    // a share's sum, given the ties in front of it
+    auto share_sum = [&](int s, uint32_t &rp, uint32_t &rq) {
+        const ShareSums &x = shares[s];
+        if (!parts) return x.all;
+        const bool out_p = res.p.partial() && rp >= res.p.r_cut, out_q = res.q.partial() && rq >= res.q.r_cut;
+        rp += x.ties_p;
+        rq += x.ties_q;
+        if (s == s_cut[0]) return s_value[0];
+        if (s == s_cut[1]) return s_value[1];
+        return out_p ? (out_q ? x.neither : x.without_p) : (out_q ? x.without_q : x.all);
+    };
+    // the share that holds u R
+    double mine = 0.0, r;
+    {
+        uint32_t rp = before_p, rq = before_q;
+        for (int s = s0; s < s1; ++s) mine += share_sum(s, rp, rq);
+    }
     const double excl = block_excl_scan_of<WAVES, double>(mine, wave_buf.d, &r);
     const double tau = double(u) * r;
     if (excl <= tau && tau < excl + mine) {
         double at = excl;
-        for (int i = 0; i < per && tid * per + i < p.n_shares; ++i) {
-            const double m = shares[tid * per + i];
+        uint32_t rp = before_p, rq = before_q;
+        for (int s = s0; s < s1; ++s) {
+            const double m = share_sum(s, rp, rq);
             // (near a border two threads can take tau for theirs: neither keeps the margin then)
-            if (tau - at >= DRAW_MARGIN && at + m - tau >= DRAW_MARGIN) { s_share = tid * per + i; s_before = at; break; }
+            if (tau - at >= DRAW_MARGIN && at + m - tau >= DRAW_MARGIN) { s_share = s; s_before = at; break; }
             at += m;
         }
     }
@@ -1035,11 +1099,6 @@ template <typename T> int launch_verify(const VerifyParams &p, hipStream_t strea
     hipLaunchKernelGGL((verify_rows<T>), dim3(unsigned(rows)), dim3(S_THREADS), 0, stream, p);
     int rc = check_hip(hipGetLastError(), "verify launch (rows)");
     if (rc != KA_OK) return rc;
-    if (p.may_cut_ties) {
-        hipLaunchKernelGGL((verify_ties<T>), dim3(unsigned(p.batch), 2), dim3(S_THREADS), 0, stream, p);
-        rc = check_hip(hipGetLastError(), "verify launch (ties)");
-        if (rc != KA_OK) return rc;
-    }
     if (T::kDtype == KA_DTYPE_BF16 && p.shares_per_group > 0) {
         rc = reserve_table_lds();
         if (rc != KA_OK) return rc;
@@ -1058,16 +1117,15 @@ inline size_t align_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
 struct VerifyLayout {
     int64_t n_shares;
-    size_t rows, ties, shares, total;
+    size_t rows, shares, total;
 };
 inline VerifyLayout verify_layout(int dtype, int64_t batch, int64_t k, int64_t vocab) {
     VerifyLayout l;
     const int64_t epv = dtype == KA_DTYPE_F32 ? 4 : 8;
     l.n_shares = (vocab + SHARE_VECS * epv - 1) / (SHARE_VECS * epv);
     l.rows = 0;
-    l.ties = align_up(size_t(batch) * size_t(2 * k + 1) * sizeof(RowSummary), 256);
-    l.shares = l.ties + align_up(size_t(batch) * 8, 256);
-    l.total = l.shares + size_t(batch) * size_t(l.n_shares) * sizeof(double);
+    l.shares = align_up(size_t(batch) * size_t(2 * k + 1) * sizeof(RowSummary), 256);
+    l.total = l.shares + size_t(batch) * size_t(l.n_shares) * sizeof(ShareSums);
     return l;
 }
 
@@ -1142,8 +1200,7 @@ KA_EXPORT int ka_verify_draft(int dtype, const void *target_logits, int64_t targ
     p.out_policy = out_policy_logprob;
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     p.rows = reinterpret_cast<RowSummary *>(ws + l.rows);
-    p.tie_limit = reinterpret_cast<int32_t *>(ws + l.ties);
-    p.shares = reinterpret_cast<double *>(ws + l.shares);
+    p.shares = reinterpret_cast<ShareSums *>(ws + l.shares);
     p.n_shares = int32_t(l.n_shares);
     // Tables pay where most entries may have mass: two of them cost 9728 evaluations, a share of 2048 entries 4096 without.
     // Enough groups to fill the device twice, of at least eight shares (one per wavefront).
@@ -1159,7 +1216,6 @@ KA_EXPORT int ka_verify_draft(int dtype, const void *target_logits, int64_t targ
     };
     p.vec_target = aligned(target_logits, target_batch_stride, target_pos_stride, max_draft + 1) ? 1 : 0;
     p.vec_draft = p.draft != nullptr && aligned(draft_logits, draft_batch_stride, draft_pos_stride, max_draft) ? 1 : 0;
-    p.may_cut_ties = (top_p_rows != nullptr || top_p < 1.0f) ? 1 : 0;
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     if (dtype == KA_DTYPE_BF16) return launch_verify<Bf16>(p, stream);
     if (dtype == KA_DTYPE_F16) return launch_verify<F16>(p, stream);

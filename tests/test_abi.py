@@ -169,8 +169,8 @@ def test_verify_argument_checks_and_workspace_size():
     p = ctypes.c_void_p(4096)
     ws = lib.ka_verify_workspace_bytes
     up = lambda n: (n + 255) // 256 * 256  # noqa: E731
-    assert ws(0, 64, 4, 128256) == up(64 * 9 * 48) + up(64 * 8) + 64 * 63 * 8
-    assert ws(2, 3, 0, 4097) == up(3 * 48) + up(24) + 3 * 5 * 8
+    assert ws(0, 64, 4, 128256) == up(64 * 9 * 48) + 64 * 63 * 40
+    assert ws(2, 3, 0, 4097) == up(3 * 48) + 3 * 5 * 40
     assert ws(0, 0, 4, 128256) == 0 and ws(0, 4, 65, 100) == 0 and ws(0, 4, 4, 1 << 22) == 0
 
     def call(dtype=0, target=p, tb=500, tp=100, draft=p, db=400, dp=100, ids=p, lens=None, u=p, batch=2, k=4, vocab=100,
