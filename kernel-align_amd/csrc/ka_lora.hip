@@ -37,54 +37,73 @@ struct LoraTile {
     int32_t start, count;  // in `order`
     int32_t slot;          // backward: -1 writes the adapter's gradient, others this partial one
 };
-struct LoraPlan {          // device pointers into the workspace
-    int32_t *head;         // [0] = number of tiles
-    int32_t *order;        // [N] tokens sorted by adapter, those without one last
+struct TileList {
+    int32_t *count;        // [1]
     LoraTile *tiles;
     int32_t *per_adapter;  // [2 S]: tiles of the adapter, its first partial slot
-    int32_t max_tiles;
+    int32_t tokens;        // per tile
+};
+struct LoraPlan {          // device pointers into the workspace
+    int32_t *order;        // [N] tokens sorted by adapter, those without one last
+    TileList list[2];      // of the forward, or of the backward's two passes
 };
 
 // ---------------------------------------------------------------------------
 // lora_plan: one workgroup sorts the tokens.  Every wavefront takes a contiguous share of them: counts, a prefix over
-// (adapter, wavefront), then the ranks inside a step of 64 tokens from ballots.
+// (adapter, wavefront), then the ranks inside a step of 64 tokens from ballots.  The ids of eight steps are requested together.
 // ---------------------------------------------------------------------------
 constexpr int PLAN_THREADS = 512;
 constexpr int PLAN_WAVES = PLAN_THREADS / kWave;
 
-__global__ __launch_bounds__(PLAN_THREADS) void lora_plan(const int64_t *__restrict__ ids, int n, int s, int tile, LoraPlan plan) {
+__global__ __launch_bounds__(PLAN_THREADS) void lora_plan(const int64_t *__restrict__ ids, int n, int s, int lists, LoraPlan plan) {
     __shared__ int32_t at[PLAN_WAVES][MAX_ADAPTERS + 1];  // counts, then the next position of the wavefront's tokens
-    __shared__ int32_t wave_sum[PLAN_WAVES][3];
+    __shared__ int32_t wave_sum[PLAN_WAVES][5];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    for (int i = tid; i < PLAN_WAVES * (MAX_ADAPTERS + 1); i += PLAN_THREADS) (&at[0][0])[i] = 0;
-    __syncthreads();
+    constexpr int U = 8;
     const int steps = (n + kWave - 1) / kWave, per = (steps + PLAN_WAVES - 1) / PLAN_WAVES;
     const int s0 = wave * per, s1 = s0 + per < steps ? s0 + per : steps;
-    auto adapter_of = [&](int i) {
-        const int64_t a = ids[i];
-        return a >= 0 && a < s ? int(a) : s;
+    int a[U];  // adapters of eight steps of this wavefront; s: none, -1: behind the end
+    auto load = [&](int st) {
+        int64_t id[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (st + u) * kWave + lane;
+            id[u] = st + u < s1 && i < n ? ids[i] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (st + u) * kWave + lane;
+            a[u] = st + u < s1 && i < n ? (id[u] >= 0 && id[u] < s ? int(id[u]) : s) : -1;
+        }
     };
-    for (int st = s0; st < s1; ++st) {
-        const int i = st * kWave + lane;
-        if (i < n) atomicAdd(&at[wave][adapter_of(i)], 1);
+    load(s0);
+    for (int i = tid; i < PLAN_WAVES * (s + 1); i += PLAN_THREADS) at[i / (s + 1)][i % (s + 1)] = 0;
+    __syncthreads();
+    for (int st = s0; st < s1; st += U) {
+        if (st != s0) load(st);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (a[u] >= 0) atomicAdd(&at[wave][a[u]], 1);
     }
     __syncthreads();
-    // thread t owns the adapters t * own .. : tokens, tiles and partial slots before its first
+    // thread t owns the adapters t * own .. : tokens, and per list tiles and partial slots, before its first
     const int own = (s + 1 + PLAN_THREADS - 1) / PLAN_THREADS;
-    int mine[3] = {0, 0, 0};
+    int mine[5] = {0, 0, 0, 0, 0};
     for (int j = 0; j < own; ++j) {
-        const int a = tid * own + j;
-        if (a > s) break;
+        const int ad = tid * own + j;
+        if (ad > s) break;
         int c = 0;
-        for (int w = 0; w < PLAN_WAVES; ++w) c += at[w][a];
-        const int t = (c + tile - 1) / tile;
+        for (int w = 0; w < PLAN_WAVES; ++w) c += at[w][ad];
         mine[0] += c;
-        mine[1] += t;
-        if (a < s && t > 1) mine[2] += t - 1;
+        for (int l = 0; l < lists; ++l) {
+            const int t = (c + plan.list[l].tokens - 1) / plan.list[l].tokens;
+            mine[1 + 2 * l] += t;
+            if (ad < s && t > 1) mine[2 + 2 * l] += t - 1;
+        }
     }
-    int before[3];
+    int before[5];
 #pragma unroll
-    for (int q = 0; q < 3; ++q) {
+    for (int q = 0; q < 5; ++q) {
         int inc = mine[q];
 #pragma unroll
         for (int off = 1; off < kWave; off <<= 1) {
@@ -95,58 +114,66 @@ __global__ __launch_bounds__(PLAN_THREADS) void lora_plan(const int64_t *__restr
         before[q] = inc - mine[q];
     }
     __syncthreads();
-    int total_tiles = 0;
+    int total[2] = {0, 0};
     for (int w = 0; w < PLAN_WAVES; ++w) {
         if (w < wave) {
 #pragma unroll
-            for (int q = 0; q < 3; ++q) before[q] += wave_sum[w][q];
+            for (int q = 0; q < 5; ++q) before[q] += wave_sum[w][q];
         }
-        total_tiles += wave_sum[w][1];
+        total[0] += wave_sum[w][1];
+        total[1] += wave_sum[w][3];
     }
     for (int j = 0; j < own; ++j) {
-        const int a = tid * own + j;
-        if (a > s) break;
+        const int ad = tid * own + j;
+        if (ad > s) break;
         int c = 0;
         for (int w = 0; w < PLAN_WAVES; ++w) {
-            const int x = at[w][a];
-            at[w][a] = before[0] + c;
+            const int x = at[w][ad];
+            at[w][ad] = before[0] + c;
             c += x;
         }
-        const int t = (c + tile - 1) / tile;
-        for (int k = 0; k < t; ++k) {
-            LoraTile lt;
-            lt.adapter = a < s ? a : -1;
-            lt.start = before[0] + k * tile;
-            lt.count = c - k * tile < tile ? c - k * tile : tile;
-            lt.slot = k == 0 ? -1 : before[2] + k - 1;
-            plan.tiles[before[1] + k] = lt;
-        }
-        if (a < s) {
-            plan.per_adapter[2 * a] = t;
-            plan.per_adapter[2 * a + 1] = before[2];
+#pragma unroll
+        for (int l = 0; l < 2; ++l) {
+            if (l >= lists) break;
+            const TileList &list = plan.list[l];
+            const int t = (c + list.tokens - 1) / list.tokens;
+            for (int k = 0; k < t; ++k) {
+                LoraTile lt;
+                lt.adapter = ad < s ? ad : -1;
+                lt.start = before[0] + k * list.tokens;
+                lt.count = c - k * list.tokens < list.tokens ? c - k * list.tokens : list.tokens;
+                lt.slot = k == 0 ? -1 : before[2 + 2 * l] + k - 1;
+                list.tiles[before[1 + 2 * l] + k] = lt;
+            }
+            if (ad < s) {
+                list.per_adapter[2 * ad] = t;
+                list.per_adapter[2 * ad + 1] = before[2 + 2 * l];
+            }
+            before[1 + 2 * l] += t;
+            if (ad < s && t > 1) before[2 + 2 * l] += t - 1;
         }
         before[0] += c;
-        before[1] += t;
-        if (a < s && t > 1) before[2] += t - 1;
     }
-    if (tid == 0) plan.head[0] = total_tiles;
+    if (tid < lists) *plan.list[tid].count = total[tid];
     __syncthreads();
-    for (int st = s0; st < s1; ++st) {
-        const int i = st * kWave + lane;
-        const int a = i < n ? adapter_of(i) : -1;
-        uint64_t left = __ballot(a >= 0);
-        while (left != 0) {  // one turn per adapter that occurs in the step
-            const int leader = __ffsll((long long)left) - 1;
-            const int want = __builtin_amdgcn_readlane(a, leader);
-            const uint64_t same = __ballot(a == want) & left;
-            const int base = at[wave][want];
-            if ((same >> lane) & 1) plan.order[base + __popcll(same & ((uint64_t(1) << lane) - 1))] = i;
-            // the wavefront's own counter: read by all lanes above, moved by one
-            __builtin_amdgcn_wave_barrier();
-            if (lane == leader) at[wave][want] = base + __popcll(same);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            left &= ~same;
+    for (int st = s0; st < s1; st += U) {
+        if (per > U) load(st);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            uint64_t left = __ballot(a[u] >= 0);
+            while (left != 0) {  // one turn per adapter that occurs in the step
+                const int leader = __ffsll((long long)left) - 1;
+                const int want = __builtin_amdgcn_readlane(a[u], leader);
+                const uint64_t same = __ballot(a[u] == want);
+                const int base = at[wave][want];
+                if (a[u] == want) plan.order[base + __popcll(same & ((uint64_t(1) << lane) - 1))] = (st + u) * kWave + lane;
+                // the wavefront's own counter: read by all lanes above, moved by one
+                __builtin_amdgcn_wave_barrier();
+                if (lane == leader) at[wave][want] = base + __popcll(same);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                left &= ~same;
+            }
         }
     }
 }
@@ -299,8 +326,8 @@ __global__ __launch_bounds__(THREADS) void lora_shrink(ShrinkArgs p) {
     constexpr int RF = RP / 16;
     __shared__ f32x4 part[WAVES][FWD_TILE][4];  // [wave][token][rank / 4] of one group of sixteen ranks
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
-    if (int(blockIdx.y) >= p.plan.head[0]) return;
-    const LoraTile tile = p.plan.tiles[blockIdx.y];
+    if (int(blockIdx.y) >= *p.plan.list[0].count) return;
+    const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];
     const int mine = tid / 4, mine_q = tid & 3;  // the thread adds up four ranks of token `mine` of the tile
     f32x4 sum[RF];
 #pragma unroll
@@ -361,6 +388,20 @@ __global__ __launch_bounds__(THREADS) void lora_shrink(ShrinkArgs p) {
     }
 }
 
+// first + part[0] + part[1] + ..., added in that order, eight of them requested together; the parts are `step` elements apart.
+__device__ __forceinline__ float add_parts(float first, const float *__restrict__ part, int parts, int64_t step) {
+    float sum = first;
+    for (int q = 0; q < parts; q += 8) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = q + u < parts ? part[int64_t(q + u) * step] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (q + u < parts) sum += v[u];
+    }
+    return sum;
+}
+
 // out[n, r] = s_a sum over the parts, in order; 0 for tokens without an adapter.
 __global__ __launch_bounds__(THREADS) void lora_fold_rows(const float *__restrict__ part, int parts, int64_t n, int r,
                                                           const int64_t *__restrict__ ids, int s, const float *__restrict__ scaling,
@@ -369,10 +410,7 @@ __global__ __launch_bounds__(THREADS) void lora_fold_rows(const float *__restric
     if (i >= n * r) return;
     const int64_t a = ids[i / r];
     float v = 0.0f;
-    if (a >= 0 && a < s) {
-        for (int q = 0; q < parts; ++q) v += part[int64_t(q) * n * r + i];
-        v *= scaling != nullptr ? scaling[a] : scale;
-    }
+    if (a >= 0 && a < s) v = add_parts(0.0f, part + i, parts, n * r) * (scaling != nullptr ? scaling[a] : scale);
     out[i] = v;
 }
 
@@ -394,8 +432,8 @@ __global__ __launch_bounds__(THREADS) void lora_expand(ExpandArgs p) {
     constexpr int KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, NP = Parts<T>::kCount;
     __shared__ uint4 uf[4][KS][HL][kWave];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
-    if (int(blockIdx.y) >= p.plan.head[0]) return;
-    const LoraTile tile = p.plan.tiles[blockIdx.y];
+    if (int(blockIdx.y) >= *p.plan.list[0].count) return;
+    const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];
     if (tile.adapter < 0 && p.in_place) return;
     const int nsub = (tile.count + 15) / 16;
     const typename T::raw_t *base = static_cast<const typename T::raw_t *>(p.base);
@@ -498,8 +536,8 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
     __shared__ int32_t tokens[BWD_TILE_MAX];
     __shared__ f32x4 red[WAVES][32][RED * 4];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
-    if (int(blockIdx.y) >= p.plan.head[0]) return;
-    const LoraTile tile = p.plan.tiles[blockIdx.y];
+    if (int(blockIdx.y) >= *p.plan.list[0].count) return;
+    const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];
     if (tile.adapter < 0) return;
     for (int i = tid; i < tile.count; i += THREADS) tokens[i] = p.plan.order[tile.start + i];
     const typename T::raw_t *dy = static_cast<const typename T::raw_t *>(p.dy);
@@ -622,8 +660,8 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
     constexpr int RF = RP / 16, KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, NP = Parts<T>::kCount;
     __shared__ int32_t tokens[BWD_TILE_MAX];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
-    if (int(blockIdx.y) >= p.plan.head[0]) return;
-    const LoraTile tile = p.plan.tiles[blockIdx.y];
+    if (int(blockIdx.y) >= *p.plan.list[1].count) return;
+    const LoraTile tile = p.plan.list[1].tiles[blockIdx.y];
     for (int i = tid; i < tile.count; i += THREADS) tokens[i] = p.plan.order[tile.start + i];
     __syncthreads();
     const int h0 = (int(blockIdx.x) * WAVES + wave) * 64;
@@ -718,22 +756,23 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
     }
 }
 
-// grid (blocks of elements, adapters): adds the partial gradients of an adapter's further tiles in their order; zeros for an
-// adapter without tokens.
-__global__ __launch_bounds__(THREADS) void lora_fold_grads(float *__restrict__ grad, const float *__restrict__ part,
-                                                           int64_t elements, LoraPlan plan) {
-    const int a = blockIdx.y;
-    const int tiles = plan.per_adapter[2 * a], slot = plan.per_adapter[2 * a + 1];
+// grid (blocks of elements of dB, then of dA; adapters): adds the partial gradients of an adapter's further tiles in their
+// order; zeros for an adapter without tokens.
+struct FoldArgs {
+    float *grad[2];
+    const float *part[2];
+    int64_t elements[2];
+    int32_t blocks[2];
+    LoraPlan plan;
+};
+__global__ __launch_bounds__(THREADS) void lora_fold_grads(FoldArgs p) {
+    const int which = int(blockIdx.x) < p.blocks[0] ? 0 : 1, a = blockIdx.y;
+    const int tiles = p.plan.list[which].per_adapter[2 * a], slot = p.plan.list[which].per_adapter[2 * a + 1];
     if (tiles == 1) return;
-    float *g = grad + int64_t(a) * elements;
-    for (int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x; i < elements; i += int64_t(gridDim.x) * THREADS) {
-        float v = 0.0f;
-        if (tiles > 1) {
-            v = g[i];
-            for (int k = 0; k < tiles - 1; ++k) v += part[int64_t(slot + k) * elements + i];
-        }
-        g[i] = v;
-    }
+    const int64_t elements = p.elements[which], step = int64_t(p.blocks[which]) * THREADS;
+    float *g = p.grad[which] + int64_t(a) * elements;
+    for (int64_t i = int64_t(int(blockIdx.x) - (which ? p.blocks[0] : 0)) * THREADS + threadIdx.x; i < elements; i += step)
+        g[i] = tiles == 0 ? 0.0f : add_parts(g[i], p.part[which] + int64_t(slot) * elements + i, tiles - 1, elements);
 }
 
 // ---------------------------------------------------------------------------
@@ -758,61 +797,71 @@ inline int check_shape(const char *what, int dtype, const Shape &d) {
 
 inline int padded_rank(int64_t r) { return r <= 16 ? 16 : (r <= 32 ? 32 : (r <= 64 ? 64 : 128)); }
 
-struct PlanLayout { size_t order, tiles, per_adapter, total; int64_t max_tiles; };
-inline PlanLayout plan_layout(int64_t n, int64_t s, int64_t tile) {
-    PlanLayout l;
+struct PlanLayout { size_t order, tiles[2], per_adapter[2], total; int64_t tokens[2], max_tiles[2]; };
+inline PlanLayout plan_layout(int64_t n, int64_t s, int64_t tile0, int64_t tile1) {  // tile1 0: one list
+    PlanLayout l{};
     const int64_t groups = s + 1 < n ? s + 1 : n;
-    l.max_tiles = n / tile + groups;
-    l.order = 256;
-    l.tiles = l.order + align_up(size_t(n) * 4);
-    l.per_adapter = l.tiles + align_up(size_t(l.max_tiles) * sizeof(LoraTile));
-    l.total = l.per_adapter + align_up(size_t(s) * 8);
+    l.order = 256;  // behind the counts
+    size_t at = l.order + align_up(size_t(n) * 4);
+    for (int i = 0; i < 2; ++i) {
+        l.tokens[i] = i == 0 ? tile0 : tile1;
+        if (l.tokens[i] == 0) continue;
+        l.max_tiles[i] = n / l.tokens[i] + groups;
+        l.tiles[i] = at;
+        l.per_adapter[i] = at + align_up(size_t(l.max_tiles[i]) * sizeof(LoraTile));
+        at = l.per_adapter[i] + align_up(size_t(s) * 8);
+    }
+    l.total = at;
     return l;
 }
 inline LoraPlan plan_at(unsigned char *ws, const PlanLayout &l) {
-    LoraPlan p;
-    p.head = reinterpret_cast<int32_t *>(ws);
+    LoraPlan p{};
     p.order = reinterpret_cast<int32_t *>(ws + l.order);
-    p.tiles = reinterpret_cast<LoraTile *>(ws + l.tiles);
-    p.per_adapter = reinterpret_cast<int32_t *>(ws + l.per_adapter);
-    p.max_tiles = int32_t(l.max_tiles);
+    for (int i = 0; i < 2; ++i) {
+        p.list[i].count = reinterpret_cast<int32_t *>(ws) + i;
+        p.list[i].tiles = reinterpret_cast<LoraTile *>(ws + l.tiles[i]);
+        p.list[i].per_adapter = reinterpret_cast<int32_t *>(ws + l.per_adapter[i]);
+        p.list[i].tokens = int32_t(l.tokens[i]);
+    }
     return p;
 }
 
 struct FwdLayout { PlanLayout plan; int64_t segments; bool split; size_t part, u, total; };
 inline FwdLayout fwd_layout(const Shape &d) {
     FwdLayout l;
-    l.plan = plan_layout(d.n, d.s, FWD_TILE);
+    l.plan = plan_layout(d.n, d.s, FWD_TILE, 0);
     l.segments = ceil_div(d.h, SEG_STEPS * 32);
-    l.split = l.segments > 1 && l.plan.max_tiles < 256;
+    l.split = l.segments > 1 && l.plan.max_tiles[0] < 256;
     l.part = l.plan.total;
     l.u = l.part + (l.split ? align_up(size_t(l.segments) * d.n * d.r * 4) : 0);
     l.total = l.u + align_up(size_t(d.n) * d.r * 4);
     return l;
 }
 
-// The backward: outputs per wavefront (64 G) and tokens per tile.
-struct BwdLayout { PlanLayout plan; int64_t tile, slots, blocks; int groups; size_t du, du_part, db_part, da_part, total; };
+// The backward: outputs per wavefront (64 G) of the first pass, tokens per tile of both.
+struct BwdLayout { PlanLayout plan; int64_t slots[2], blocks[2]; int groups; size_t du, du_part, db_part, da_part, total; };
+// Tokens per tile such that `blocks` times the tiles make about `want` workgroups.
+inline int64_t bwd_tile(int64_t n, int64_t blocks, int64_t want) {
+    const int64_t tiles = ceil_div(want, blocks);
+    int64_t tile = ceil_div(ceil_div(n, tiles), 32) * 32;
+    return tile < 64 ? 64 : (tile > BWD_TILE_MAX ? BWD_TILE_MAX : tile);
+}
 inline BwdLayout bwd_layout(const Shape &d) {
     BwdLayout l;
     const int64_t small_blocks = ceil_div(d.o, 64 * WAVES);
     // 1024 outputs per workgroup where that leaves work for every CU: fewer partial sums of dy B
     l.groups = padded_rank(d.r) == 16 && ceil_div(d.n, 64) * ceil_div(small_blocks, 4) >= 512 ? 4 : 1;
-    l.blocks = ceil_div(d.o, 64 * WAVES * l.groups);
-    // about 1024 workgroups over the narrower of the two passes
-    const int64_t in_blocks = ceil_div(d.h, 64 * WAVES);
-    const int64_t narrow = l.blocks < in_blocks ? l.blocks : in_blocks;
-    int64_t tile = ceil_div(ceil_div(d.n * narrow, 1024), 32) * 32;
-    if (tile < 64) tile = 64;
-    if (tile > BWD_TILE_MAX) tile = BWD_TILE_MAX;
-    l.tile = tile;
-    l.slots = d.n / tile;
-    l.plan = plan_layout(d.n, d.s, tile);
+    l.blocks[0] = ceil_div(d.o, 64 * WAVES * l.groups);
+    l.blocks[1] = ceil_div(d.h, 64 * WAVES);
+    const int64_t tile0 = bwd_tile(d.n, l.blocks[0], 1024), tile1 = bwd_tile(d.n, l.blocks[1], 512);
+    l.slots[0] = d.n / tile0;
+    l.slots[1] = d.n / tile1;
+    l.plan = plan_layout(d.n, d.s, tile0, tile1);
     l.du = l.plan.total;
     l.du_part = l.du + align_up(size_t(d.n) * d.r * 4);
-    l.db_part = l.du_part + align_up(size_t(l.blocks) * d.n * d.r * 4);
-    l.da_part = l.db_part + align_up(size_t(l.slots) * d.o * d.r * 4);
-    l.total = l.da_part + align_up(size_t(l.slots) * d.h * d.r * 4);
+    l.db_part = l.du_part + align_up(size_t(l.blocks[0]) * d.n * d.r * 4);
+    l.da_part = l.db_part + align_up(size_t(l.slots[0]) * d.o * d.r * 4);
+    l.total = l.da_part + align_up(size_t(l.slots[1]) * d.h * d.r * 4);
     return l;
 }
 
@@ -868,7 +917,7 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     const LoraPlan plan = plan_at(ws, l.plan);
-    hipLaunchKernelGGL(lora_plan, dim3(1), dim3(PLAN_THREADS), 0, stream, adapter_ids, int(n_tokens), int(n_adapters), FWD_TILE, plan);
+    hipLaunchKernelGGL(lora_plan, dim3(1), dim3(PLAN_THREADS), 0, stream, adapter_ids, int(n_tokens), int(n_adapters), 1, plan);
     rc = check_hip(hipGetLastError(), "lora launch (plan)");
     if (rc != KA_OK) return rc;
     float *u = out_shrunk != nullptr ? out_shrunk : reinterpret_cast<float *>(ws + l.u);
@@ -886,7 +935,7 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     sa.out = l.split ? reinterpret_cast<float *>(ws + l.part) : u;
     sa.plan = plan;
     const int rp = padded_rank(rank);
-    const dim3 shrink_grid{unsigned(l.split ? l.segments : 1), unsigned(l.plan.max_tiles)};
+    const dim3 shrink_grid{unsigned(l.split ? l.segments : 1), unsigned(l.plan.max_tiles[0])};
     with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
         using T = decltype(type);
         constexpr int RP = decltype(rank_c)::value;
@@ -915,10 +964,10 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     ea.plan = plan;
     // groups of 64 outputs per wavefront: as many as leave about 1024 workgroups
     const int64_t blocks1 = ceil_div(out_dim, 64 * WAVES);
-    int64_t groups = blocks1 * l.plan.max_tiles / 1024;
+    int64_t groups = blocks1 * l.plan.max_tiles[0] / 1024;
     groups = groups < 1 ? 1 : (groups > 8 ? 8 : groups);
     ea.groups = int32_t(groups);
-    const dim3 expand_grid{unsigned(ceil_div(out_dim, 64 * WAVES * groups)), unsigned(l.plan.max_tiles)};
+    const dim3 expand_grid{unsigned(ceil_div(out_dim, 64 * WAVES * groups)), unsigned(l.plan.max_tiles[0])};
     with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
         using T = decltype(type);
         constexpr int RP = decltype(rank_c)::value;
@@ -954,7 +1003,7 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     const LoraPlan plan = plan_at(ws, l.plan);
-    hipLaunchKernelGGL(lora_plan, dim3(1), dim3(PLAN_THREADS), 0, stream, adapter_ids, int(n_tokens), int(n_adapters), int(l.tile), plan);
+    hipLaunchKernelGGL(lora_plan, dim3(1), dim3(PLAN_THREADS), 0, stream, adapter_ids, int(n_tokens), int(n_adapters), 2, plan);
     rc = check_hip(hipGetLastError(), "lora backward launch (plan)");
     if (rc != KA_OK) return rc;
     const int rp = padded_rank(rank);
@@ -972,7 +1021,7 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     oa.db_part = db_part;
     oa.du_part = du_part;
     oa.plan = plan;
-    const dim3 out_grid{unsigned(l.blocks), unsigned(l.plan.max_tiles)};
+    const dim3 out_grid{unsigned(l.blocks[0]), unsigned(l.plan.max_tiles[0])};
     with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
         using T = decltype(type);
         constexpr int RP = decltype(rank_c)::value;
@@ -988,7 +1037,7 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     rc = check_hip(hipGetLastError(), "lora backward launch (out)");
     if (rc != KA_OK) return rc;
     hipLaunchKernelGGL(lora_fold_rows, dim3(unsigned(ceil_div(n_tokens * rank, THREADS))), dim3(THREADS), 0, stream, du_part,
-                       int(l.blocks), n_tokens, int(rank), adapter_ids, int(n_adapters), scaling, scale, du);
+                       int(l.blocks[0]), n_tokens, int(rank), adapter_ids, int(n_adapters), scaling, scale, du);
     rc = check_hip(hipGetLastError(), "lora backward launch (fold)");
     if (rc != KA_OK) return rc;
     BwdInArgs ia{};
@@ -1005,7 +1054,7 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     ia.da = dlora_a;
     ia.da_part = da_part;
     ia.plan = plan;
-    const dim3 in_grid{unsigned(ceil_div(in_dim, 64 * WAVES)), unsigned(l.plan.max_tiles)};
+    const dim3 in_grid{unsigned(l.blocks[1]), unsigned(l.plan.max_tiles[1])};
     with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
         using T = decltype(type);
         constexpr int RP = decltype(rank_c)::value;
@@ -1014,13 +1063,17 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     });
     rc = check_hip(hipGetLastError(), "lora backward launch (in)");
     if (rc != KA_OK) return rc;
-    auto fold = [&](float *grad, const float *part, int64_t elements) {
-        int64_t blocks = ceil_div(elements, THREADS * 4);
-        if (blocks > 1024) blocks = 1024;
-        hipLaunchKernelGGL(lora_fold_grads, dim3(unsigned(blocks), unsigned(n_adapters)), dim3(THREADS), 0, stream, grad, part, elements, plan);
-        return check_hip(hipGetLastError(), "lora backward launch (gradients)");
-    };
-    rc = fold(dlora_b, db_part, out_dim * rank);
-    if (rc != KA_OK) return rc;
-    return fold(dlora_a, da_part, in_dim * rank);
+    FoldArgs fa{};
+    fa.plan = plan;
+    fa.grad[0] = dlora_b;
+    fa.grad[1] = dlora_a;
+    fa.part[0] = db_part;
+    fa.part[1] = da_part;
+    for (int i = 0; i < 2; ++i) {
+        fa.elements[i] = (i == 0 ? out_dim : in_dim) * rank;
+        const int64_t blocks = ceil_div(fa.elements[i], THREADS);
+        fa.blocks[i] = int32_t(blocks < 2048 ? blocks : 2048);
+    }
+    hipLaunchKernelGGL(lora_fold_grads, dim3(unsigned(fa.blocks[0] + fa.blocks[1]), unsigned(n_adapters)), dim3(THREADS), 0, stream, fa);
+    return check_hip(hipGetLastError(), "lora backward launch (gradients)");
 }
