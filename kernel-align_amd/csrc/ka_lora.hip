@@ -231,28 +231,40 @@ template <typename T> __device__ __forceinline__ void as_bf16(const uint4 &f, ui
     }
 }
 
-// Eight consecutive elements, zeros behind the first `n` of them.
-template <typename T, bool VEC> __device__ __forceinline__ uint4 load8(const typename T::raw_t *p, int n) {
-    if constexpr (VEC) {  // n is a multiple of 8, p 16-byte aligned
-        return n > 0 ? *reinterpret_cast<const uint4 *>(p) : make_uint4(0, 0, 0, 0);
+// Loads are never conditional: a lane without work of its own reads a place that exists (another row of the tile, the
+// start of a row), so that all loads of a step are in flight together, and what it read meets a zero in the other operand or a
+// result that is not stored.  (An infinity read that way belongs to the same token or adapter.)
+//
+// Columns col .. col + 7 of a row of `width`; where they do not exist, its first columns.
+template <typename T, bool VEC> __device__ __forceinline__ uint4 load8(const typename T::raw_t *row, int col, int width) {
+    if constexpr (VEC) {  // width is a multiple of 8, the row 16-byte aligned
+        return *reinterpret_cast<const uint4 *>(row + (col < width ? col : 0));
     } else {
-        uint32_t w[4] = {0, 0, 0, 0};
+        uint32_t e[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < n) w[j / 2] |= uint32_t(p[j]) << (16 * (j & 1));
-        return make_uint4(w[0], w[1], w[2], w[3]);
+        for (int j = 0; j < 8; ++j) e[j] = row[col + j < width ? col + j : 0];
+        return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
     }
 }
-// Four consecutive elements, zeros behind the first `n`.
-template <typename T, bool VEC> __device__ __forceinline__ uint2 load4(const typename T::raw_t *p, int n) {
-    if constexpr (VEC) {
-        return n > 0 ? *reinterpret_cast<const uint2 *>(p) : make_uint2(0, 0);
-    } else {
-        uint32_t w[2] = {0, 0};
+// The same with zeros behind the row.
+template <typename T, bool VEC> __device__ __forceinline__ uint4 load8_zero(const typename T::raw_t *row, int col, int width) {
+    const uint4 v = load8<T, VEC>(row, col, width);
+    const int n = width - col;
+    if constexpr (VEC) return n > 0 ? v : make_uint4(0, 0, 0, 0);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t k[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < n) w[j / 2] |= uint32_t(p[j]) << (16 * (j & 1));
-        return make_uint2(w[0], w[1]);
+    for (int j = 0; j < 4; ++j) k[j] = w[j] & ((2 * j < n ? 0xffffu : 0u) | (2 * j + 1 < n ? 0xffff0000u : 0u));
+    return make_uint4(k[0], k[1], k[2], k[3]);
+}
+template <typename T, bool VEC> __device__ __forceinline__ uint2 load4(const typename T::raw_t *row, int col, int width) {
+    if constexpr (VEC) {
+        return *reinterpret_cast<const uint2 *>(row + (col < width ? col : 0));
+    } else {
+        uint32_t e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[j] = row[col + j < width ? col + j : 0];
+        return make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
     }
 }
 // Eight rows of four columns -> the four fragments e whose contraction index is the row: column e of each.
@@ -306,8 +318,8 @@ __device__ __forceinline__ void store_sum(const typename T::raw_t *base, typenam
 }
 
 // ---------------------------------------------------------------------------
-// lora_shrink: u = s x A^T.  H is cut into segments of 1024; inside one the wavefronts take every fourth step of 32 and are
-// added in their order, and the segments are added in theirs: by one workgroup (grid (1, tiles)), or by lora_fold_rows
+// lora_shrink: u = s x A^T.  H is cut into segments of 1024; inside one the wavefronts take two of every eight steps of 32 and
+// are added in their order, and the segments are added in theirs: by one workgroup (grid (1, tiles)), or by lora_fold_rows
 // over one partial result per segment (grid (segments, tiles)) where the tiles alone would leave CUs idle.  The bits of a
 // token's u do not depend on which of the two runs, nor on the other tokens.
 // ---------------------------------------------------------------------------
@@ -337,7 +349,7 @@ __global__ __launch_bounds__(THREADS) void lora_shrink(ShrinkArgs p) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const int i = s * 16 + col;
-            rows[s] = i < tile.count ? static_cast<const typename T::raw_t *>(p.x) + int64_t(p.plan.order[tile.start + i]) * p.x_stride : nullptr;
+            rows[s] = static_cast<const typename T::raw_t *>(p.x) + int64_t(p.plan.order[tile.start + (i < tile.count ? i : 0)]) * p.x_stride;
         }
         const typename T::raw_t *aw = static_cast<const typename T::raw_t *>(p.a) + int64_t(tile.adapter) * p.r * p.h;
         const int nsub = (tile.count + 15) / 16;
@@ -350,18 +362,25 @@ __global__ __launch_bounds__(THREADS) void lora_shrink(ShrinkArgs p) {
 #pragma unroll
                 for (int s = 0; s < 4; ++s) acc[f][s] = f32x4{0, 0, 0, 0};
             const int end = (seg + 1) * SEG_STEPS < steps ? (seg + 1) * SEG_STEPS : steps;
-            for (int st = seg * SEG_STEPS + wave; st < end; st += WAVES) {
-                const int k = st * 32 + 8 * quad;
-                uint4 fa[RF], fx[4];
+            // a wavefront takes two neighbouring steps of every eight: whole 128-byte lines of the rows
+            for (int st = seg * SEG_STEPS + 2 * wave; st < end; st += 2 * WAVES) {
+                uint4 fa[2][RF], fx[2][4];
 #pragma unroll
-                for (int f = 0; f < RF; ++f) fa[f] = load8<T, VEC>(aw + int64_t(f * 16 + col) * p.h + k, f * 16 + col < p.r ? p.h - k : 0);
+                for (int t = 0; t < 2; ++t) {
+                    const int k = (st + t) * 32 + 8 * quad;
 #pragma unroll
-                for (int s = 0; s < 4; ++s) fx[s] = s < nsub ? load8<T, VEC>(rows[s] + k, rows[s] != nullptr ? p.h - k : 0) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int f = 0; f < RF; ++f)
+                    for (int f = 0; f < RF; ++f) fa[t][f] = load8_zero<T, VEC>(aw + int64_t(f * 16 + col < p.r ? f * 16 + col : 0) * p.h, k, p.h);
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
-                        if (s < nsub) acc[f][s] = mfma<T>(fa[f], fx[s], acc[f][s]);
+                        if (s < nsub) fx[t][s] = load8<T, VEC>(rows[s], k, p.h);
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int f = 0; f < RF; ++f)
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+                            if (s < nsub) acc[f][s] = mfma<T>(fa[t][f], fx[t][s], acc[f][s]);
             }
 #pragma unroll
             for (int f = 0; f < RF; ++f) {
@@ -440,13 +459,16 @@ __global__ __launch_bounds__(THREADS) void lora_expand(ExpandArgs p) {
     typename T::raw_t *out = static_cast<typename T::raw_t *>(p.out);
     {   // wavefront s prepares the fragments of group s: column = token
         const int i = wave * 16 + col;
-        const float *row = i < tile.count && tile.adapter >= 0 ? p.u + int64_t(p.plan.order[tile.start + i]) * p.r : nullptr;
+        const bool live = i < tile.count && tile.adapter >= 0;
+        const float *row = p.u + int64_t(p.plan.order[tile.start + (i < tile.count ? i : 0)]) * p.r;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = row != nullptr && r0 + j < p.r ? row[r0 + j] : 0.0f;
+            for (int j = 0; j < 8; ++j) v[j] = row[r0 + j < p.r ? r0 + j : 0];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = live && r0 + j < p.r ? v[j] : 0.0f;
             uint4 hl[2];
             split<2>(v, hl);
             if (RP <= 16) {
@@ -458,7 +480,7 @@ __global__ __launch_bounds__(THREADS) void lora_expand(ExpandArgs p) {
         }
     }
     __syncthreads();
-    const typename T::raw_t *bw = tile.adapter < 0 ? nullptr : static_cast<const typename T::raw_t *>(p.b) + int64_t(tile.adapter) * p.o * p.r;
+    const typename T::raw_t *bw = static_cast<const typename T::raw_t *>(p.b) + int64_t(tile.adapter < 0 ? 0 : tile.adapter) * p.o * p.r;
     int64_t token[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) token[s] = s * 16 + col < tile.count ? p.plan.order[tile.start + s * 16 + col] : -1;
@@ -472,7 +494,7 @@ __global__ __launch_bounds__(THREADS) void lora_expand(ExpandArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int o = o0 + 4 * col + e;
-                const uint4 f = load8<T, VEC>(bw + int64_t(o) * p.r + r0, bw != nullptr && o < p.o ? p.r - r0 : 0);
+                const uint4 f = load8<T, VEC>(bw + int64_t(o < p.o ? o : 0) * p.r, r0, p.r);
                 as_bf16<T>(f, fb[ks][e]);
             }
         }
@@ -513,10 +535,22 @@ struct BwdOutArgs {
     float *du_part;       // [blocks, N, R]
     LoraPlan plan;
 };
-// eight fp32 values of one column, contraction index = token
-__device__ __forceinline__ void load_column(const float *v, int r, int rank, const int32_t *tokens, int first, int count, float (&x)[8]) {
+// Eight tokens' values of one column, contraction index = token; zeros behind the `live` first of them.
+__device__ __forceinline__ void load_column(const float *v, int r, int rank, const int32_t (&tokens)[8], int live, float (&x)[8]) {
+    const float *col = v + (rank < r ? rank : 0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = first + j < count && rank < r ? v[int64_t(tokens[first + j]) * r + rank] : 0.0f;
+    for (int j = 0; j < 8; ++j) x[j] = col[int64_t(tokens[j]) * r];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < live ? x[j] : 0.0f;
+}
+// The tile's tokens into LDS, the last one repeated up to a multiple of 32.
+__device__ __forceinline__ void load_tokens(const int32_t *order, const LoraTile &tile, int32_t *tokens) {
+    for (int i = threadIdx.x; i < (tile.count + 31) / 32 * 32; i += THREADS) tokens[i] = order[tile.start + (i < tile.count ? i : tile.count - 1)];
+}
+__device__ __forceinline__ void eight_tokens(const int32_t *tokens, int32_t (&t)[8]) {
+    const int4 a = *reinterpret_cast<const int4 *>(tokens), b = *reinterpret_cast<const int4 *>(tokens + 4);
+    t[0] = a.x; t[1] = a.y; t[2] = a.z; t[3] = a.w;
+    t[4] = b.x; t[5] = b.y; t[6] = b.z; t[7] = b.w;
 }
 // acc += data^T v for one column group: parts of the data times parts of v, small products first
 template <typename T> __device__ __forceinline__ f32x4 outer(const uint4 (&data)[Parts<T>::kCount], const uint4 (&v)[3], f32x4 acc) {
@@ -533,13 +567,13 @@ template <typename T, int RP, int G, bool VEC>
 __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
     constexpr int RF = RP / 16, NP = Parts<T>::kCount;
     constexpr int RED = RF < 4 ? RF : 4;  // groups of sixteen ranks that cross the wavefronts at a time
-    __shared__ int32_t tokens[BWD_TILE_MAX];
+    __shared__ __attribute__((aligned(16))) int32_t tokens[BWD_TILE_MAX];
     __shared__ f32x4 red[WAVES][32][RED * 4];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
     if (int(blockIdx.y) >= *p.plan.list[0].count) return;
     const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];
     if (tile.adapter < 0) return;
-    for (int i = tid; i < tile.count; i += THREADS) tokens[i] = p.plan.order[tile.start + i];
+    load_tokens(p.plan.order, tile, tokens);
     const typename T::raw_t *dy = static_cast<const typename T::raw_t *>(p.dy);
     const typename T::raw_t *bw = static_cast<const typename T::raw_t *>(p.b) + int64_t(tile.adapter) * p.o * p.r;
     const int o0 = (int(blockIdx.x) * WAVES + wave) * 64 * G;
@@ -551,11 +585,13 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int f = 0; f < RF; ++f) {
-                uint32_t w[4] = {0, 0, 0, 0};
-                const int rank = f * 16 + col, o = o0 + g * 64 + ks * 32 + 8 * quad;
+                uint32_t w[4];
+                const int rank = f * 16 + col < p.r ? f * 16 + col : 0, o = o0 + g * 64 + ks * 32 + 8 * quad;
+                uint32_t e[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (rank < p.r && o + j < p.o) w[j / 2] |= uint32_t(bw[int64_t(o + j) * p.r + rank]) << (16 * (j & 1));
+                for (int j = 0; j < 8; ++j) e[j] = bw[int64_t(o + j < p.o ? o + j : 0) * p.r + rank];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (o + 2 * j < p.o ? e[2 * j] : 0u) | (o + 2 * j + 1 < p.o ? e[2 * j + 1] << 16 : 0u);
                 fb[g][ks][f] = make_uint4(w[0], w[1], w[2], w[3]);
             }
     f32x4 acc[G][RF][4];
@@ -572,22 +608,23 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int f = 0; f < RF; ++f) du[s][f] = f32x4{0, 0, 0, 0};
+        int32_t tk[8];
+        eight_tokens(tokens + c + 8 * quad, tk);
+        const typename T::raw_t *row[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) row[s] = dy + int64_t(tokens[c + 16 * s + col]) * p.dy_stride;
+        float x[RF][8];
+#pragma unroll
+        for (int f = 0; f < RF; ++f) load_column(p.u, p.r, f * 16 + col, tk, tile.count - c - 8 * quad, x[f]);
         uint4 v[RF][3];
 #pragma unroll
-        for (int f = 0; f < RF; ++f) {
-            float x[8];
-            load_column(p.u, p.r, f * 16 + col, tokens, c + 8 * quad, tile.count, x);
-            split<3>(x, v[f]);
-        }
+        for (int f = 0; f < RF; ++f) split<3>(x[f], v[f]);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const int og = o0 + g * 64;
             uint2 w[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int i = c + 8 * quad + j, o = og + 4 * col;
-                w[j] = i < tile.count ? load4<T, VEC>(dy + int64_t(tokens[i]) * p.dy_stride + o, p.o - o) : make_uint2(0, 0);
-            }
+            for (int j = 0; j < 8; ++j) w[j] = load4<T, VEC>(dy + int64_t(tk[j]) * p.dy_stride, og + 4 * col, p.o);
             uint4 frag[4], part[4][NP];
             transpose(w, frag);
 #pragma unroll
@@ -600,8 +637,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const int i = c + 16 * s + col, o = og + ks * 32 + 8 * quad;
-                    const uint4 fy = i < tile.count ? load8<T, VEC>(dy + int64_t(tokens[i]) * p.dy_stride + o, p.o - o) : make_uint4(0, 0, 0, 0);
+                    const uint4 fy = load8<T, VEC>(row[s], og + ks * 32 + 8 * quad, p.o);
 #pragma unroll
                     for (int f = 0; f < RF; ++f) du[s][f] = mfma<T>(fb[g][ks][f], fy, du[s][f]);
                 }
@@ -658,11 +694,11 @@ struct BwdInArgs {
 template <typename T, int RP, bool VEC>
 __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
     constexpr int RF = RP / 16, KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, NP = Parts<T>::kCount;
-    __shared__ int32_t tokens[BWD_TILE_MAX];
+    __shared__ __attribute__((aligned(16))) int32_t tokens[BWD_TILE_MAX];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
     if (int(blockIdx.y) >= *p.plan.list[1].count) return;
     const LoraTile tile = p.plan.list[1].tiles[blockIdx.y];
-    for (int i = tid; i < tile.count; i += THREADS) tokens[i] = p.plan.order[tile.start + i];
+    load_tokens(p.plan.order, tile, tokens);
     __syncthreads();
     const int h0 = (int(blockIdx.x) * WAVES + wave) * 64;
     if (h0 >= p.h) return;  // (no barrier follows)
@@ -678,8 +714,8 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
         uint2 w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int rank = (RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad) + j, h = h0 + 4 * col;
-            w[j] = has && rank < p.r ? load4<T, VEC>(aw + int64_t(rank) * p.h + h, p.h - h) : make_uint2(0, 0);
+            const int rank = (RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad) + j;
+            w[j] = load4<T, VEC>(aw + int64_t(rank < p.r ? rank : 0) * p.h, h0 + 4 * col, p.h);
         }
         uint4 frag[4];
         transpose(w, frag);
@@ -693,12 +729,11 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
         for (int e = 0; e < 4; ++e) acc[f][e] = f32x4{0, 0, 0, 0};
     for (int c = 0; c < tile.count; c += 32) {
         if (has) {
+            int32_t tk[8];
+            eight_tokens(tokens + c + 8 * quad, tk);
             uint2 w[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int i = c + 8 * quad + j, h = h0 + 4 * col;
-                w[j] = i < tile.count ? load4<T, VEC>(x + int64_t(tokens[i]) * p.x_stride + h, p.h - h) : make_uint2(0, 0);
-            }
+            for (int j = 0; j < 8; ++j) w[j] = load4<T, VEC>(x + int64_t(tk[j]) * p.x_stride, h0 + 4 * col, p.h);
             uint4 frag[4], part[4][NP];
             transpose(w, frag);
 #pragma unroll
@@ -707,7 +742,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
             for (int f = 0; f < RF; ++f) {
                 float col8[8];
                 uint4 v[3];
-                load_column(p.du, p.r, f * 16 + col, tokens, c + 8 * quad, tile.count, col8);
+                load_column(p.du, p.r, f * 16 + col, tk, tile.count - c - 8 * quad, col8);
                 split<3>(col8, v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[f][e] = outer<T>(part[e], v, acc[f][e]);
@@ -716,7 +751,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int i = c + 16 * s + col;
-            const int64_t token = i < tile.count ? tokens[i] : -1;
+            const int64_t token = tokens[i];
             f32x4 sum[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum[e] = f32x4{0, 0, 0, 0};
@@ -725,7 +760,9 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
                 const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
                 float row[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) row[j] = has && token >= 0 && r0 + j < p.r ? p.du[token * p.r + r0 + j] : 0.0f;
+                for (int j = 0; j < 8; ++j) row[j] = p.du[token * p.r + (r0 + j < p.r ? r0 + j : 0)];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) row[j] = has && r0 + j < p.r ? row[j] : 0.0f;
                 uint4 hl[2];
                 split<2>(row, hl);
                 if (RP <= 16) hl[0] = choose(quad < 2, hl[0], hl[1]);
@@ -736,7 +773,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
 #pragma unroll
                         for (int q = 0; q < NP; ++q) sum[e] = mfma<Bf16>(fa[ks][e][q], hl[k], sum[e]);
             }
-            if (token >= 0)
+            if (i < tile.count)
                 store_sum<T, VEC>(dx_base != nullptr ? dx_base + token * p.dx_base_stride : nullptr, dx + token * p.dx_stride, h0 + 16 * quad, p.h, sum);
         }
     }
