@@ -267,6 +267,29 @@ template <typename T, bool VEC> __device__ __forceinline__ uint2 load4(const typ
         return make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
     }
 }
+
+// How the backward's kernels reach the rows of a matrix: element by element, or in vectors from a byte offset of 32 bits
+// (matrices below 4 GiB: one addition per load) or 64.
+enum RowMode { ROWS_SCALAR = 0, ROWS_NARROW = 1, ROWS_WIDE = 2 };
+template <int MODE> struct RowOffset { using type = int64_t; };
+template <> struct RowOffset<ROWS_NARROW> { using type = uint32_t; };
+template <int MODE> using row_offset_t = typename RowOffset<MODE>::type;
+template <int MODE> __device__ __forceinline__ row_offset_t<MODE> row_offset(int token, int64_t stride) {
+    return row_offset_t<MODE>(token) * row_offset_t<MODE>(stride * 2);
+}
+template <typename T, int MODE> __device__ __forceinline__ const typename T::raw_t *row_at(const void *base, row_offset_t<MODE> at) {
+    return reinterpret_cast<const typename T::raw_t *>(static_cast<const char *>(base) + at);
+}
+// Columns of a lane that stay the same for every row of a kernel: clamped to the row once where vectors are used.
+template <int MODE> __device__ __forceinline__ int lane_column(int col, int width) { return MODE == ROWS_SCALAR || col < width ? col : 0; }
+template <typename T, int MODE> __device__ __forceinline__ uint2 row_load4(const void *base, row_offset_t<MODE> at, int col, int width) {
+    if constexpr (MODE != ROWS_SCALAR) return *reinterpret_cast<const uint2 *>(row_at<T, MODE>(base, at + row_offset_t<MODE>(col * 2)));
+    else return load4<T, false>(row_at<T, MODE>(base, at), col, width);
+}
+template <typename T, int MODE> __device__ __forceinline__ uint4 row_load8(const void *base, row_offset_t<MODE> at, int col, int width) {
+    if constexpr (MODE != ROWS_SCALAR) return *reinterpret_cast<const uint4 *>(row_at<T, MODE>(base, at + row_offset_t<MODE>(col * 2)));
+    else return load8<T, false>(row_at<T, MODE>(base, at), col, width);
+}
 // Eight rows of four columns -> the four fragments e whose contraction index is the row: column e of each.
 __device__ __forceinline__ void transpose(const uint2 (&w)[8], uint4 (&frag)[4]) {
     uint32_t f[4][4];
@@ -287,17 +310,20 @@ template <typename T> __device__ __forceinline__ typename T::raw_t narrow(float 
 }
 
 // The sixteen results a lane holds for one token after four products e (row 4 m + e of the wide dimension at MFMA row m):
-// acc[e][i] belongs to column first + 4 i + e.  out = base + acc, rounded once.
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_sum(const typename T::raw_t *base, typename T::raw_t *out, int first, int width,
-                                          const f32x4 (&acc)[4]) {
+// acc[e][i] belongs to column first + 4 i + e.  out = base + acc, rounded once; the base is loaded ahead of the products.
+template <typename T, bool VEC> struct BaseRow {
+    uint4 v[2];
+    __device__ __forceinline__ void load(const void *base, int64_t row, int first, int width) {
+        const typename T::raw_t *p = static_cast<const typename T::raw_t *>(base) + row;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int c = first + 8 * h;
-        if constexpr (VEC) {
-            if (c >= width) return;
-            float b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (base != nullptr) T::unpack(*reinterpret_cast<const uint4 *>(base + c), b);
+        for (int h = 0; h < 2; ++h) v[h] = base != nullptr ? load8<T, VEC>(p, first + 8 * h, width) : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void store(typename T::raw_t *out, int first, int width, const f32x4 (&acc)[4]) const {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = first + 8 * h;
+            float b[8];
+            T::unpack(v[h], b);
             uint32_t w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -305,16 +331,32 @@ __device__ __forceinline__ void store_sum(const typename T::raw_t *base, typenam
                 const float v1 = b[2 * j + 1] + acc[(2 * j + 1) & 3][2 * h + (2 * j) / 4];
                 w[j] = uint32_t(narrow<T>(v0)) | uint32_t(narrow<T>(v1)) << 16;
             }
-            *reinterpret_cast<uint4 *>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
+            if constexpr (VEC) {
+                if (c < width) *reinterpret_cast<uint4 *>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c + j < width) {
-                    const float v = (base != nullptr ? T::widen(base[c + j]) : 0.0f) + acc[j & 3][2 * h + j / 4];
-                    out[c + j] = narrow<T>(v);
-                }
+                for (int j = 0; j < 8; ++j)
+                    if (c + j < width) out[c + j] = typename T::raw_t(w[j / 2] >> (16 * (j & 1)));
+            }
         }
     }
+};
+
+// Where R <= 16 one product of 32 holds the high parts of u in its first half and the low ones in its second.
+template <int RP> struct Steps { static constexpr int kCount = RP <= 16 ? 1 : RP / 32; };
+
+// first + part[0] + part[step] + ..., added in that order, eight of them requested together.
+__device__ __forceinline__ float add_parts(float first, const float *__restrict__ part, int parts, int64_t step) {
+    float sum = first;
+    for (int q = 0; q < parts; q += 8) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = part[int64_t(q + u < parts ? q + u : q) * step];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (q + u < parts) sum += v[u];
+    }
+    return sum;
 }
 
 // ---------------------------------------------------------------------------
@@ -407,20 +449,6 @@ __global__ __launch_bounds__(THREADS) void lora_shrink(ShrinkArgs p) {
     }
 }
 
-// first + part[0] + part[1] + ..., added in that order, eight of them requested together; the parts are `step` elements apart.
-__device__ __forceinline__ float add_parts(float first, const float *__restrict__ part, int parts, int64_t step) {
-    float sum = first;
-    for (int q = 0; q < parts; q += 8) {
-        float v[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = q + u < parts ? part[int64_t(q + u) * step] : 0.0f;
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (q + u < parts) sum += v[u];
-    }
-    return sum;
-}
-
 // out[n, r] = s_a sum over the parts, in order; 0 for tokens without an adapter.
 __global__ __launch_bounds__(THREADS) void lora_fold_rows(const float *__restrict__ part, int parts, int64_t n, int r,
                                                           const int64_t *__restrict__ ids, int s, const float *__restrict__ scaling,
@@ -444,8 +472,6 @@ struct ExpandArgs {
     int32_t o, r, groups, in_place;  // groups: of 64 outputs per wavefront
     LoraPlan plan;
 };
-// Where R <= 16 one product of 32 holds the high parts of u in its first half and the low ones in its second.
-template <int RP> struct Steps { static constexpr int kCount = RP <= 16 ? 1 : RP / 32; };
 template <typename T, int RP, bool VEC>
 __global__ __launch_bounds__(THREADS) void lora_expand(ExpandArgs p) {
     constexpr int KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, NP = Parts<T>::kCount;
@@ -484,9 +510,14 @@ __global__ __launch_bounds__(THREADS) void lora_expand(ExpandArgs p) {
     int64_t token[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) token[s] = s * 16 + col < tile.count ? p.plan.order[tile.start + s * 16 + col] : -1;
+    const int64_t any = p.plan.order[tile.start];
     for (int g = 0; g < p.groups; ++g) {
         const int o0 = ((int(blockIdx.x) * p.groups + g) * WAVES + wave) * 64;
         if (o0 >= p.o) break;
+        BaseRow<T, VEC> row[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            if (s < nsub) row[s].load(base, (token[s] < 0 ? any : token[s]) * p.base_stride, o0 + 16 * quad, p.o);
         uint4 fb[KS][4][NP];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -514,9 +545,79 @@ __global__ __launch_bounds__(THREADS) void lora_expand(ExpandArgs p) {
 #pragma unroll
                             for (int q = 0; q < NP; ++q) acc[e] = mfma<Bf16>(fb[ks][e][q], fu, acc[e]);
                     }
-                if (token[s] >= 0)
-                    store_sum<T, VEC>(base + token[s] * p.base_stride, out + token[s] * p.out_stride, o0 + 16 * quad, p.o, acc);
+                if (token[s] >= 0) row[s].store(out + token[s] * p.out_stride, o0 + 16 * quad, p.o, acc);
             }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// lora_pack: grid (tiles of the first list).  u, or the sum of the partial results of dy B times s_a, for every 32 tokens of an
+// adapter in the layout and precision the matrix cores take it in, so that the workgroups of the two passes over the data load
+// fragments and split nothing:
+//   columns  [rank group][part 0 .. 2][lane]   contraction index = token, three bf16 parts (24 bits)
+//   rows     [group of 16 tokens][step][high, low][lane]   contraction index = rank (only for dy B)
+// The chunk of 32 tokens that starts at position i of `order`, in adapter a, is chunk i / 32 + a.
+// ---------------------------------------------------------------------------
+template <int RP> struct Packed {
+    static constexpr int kColumns = RP / 16 * 3 * kWave;                               // in uint4
+    static constexpr int kRows = 2 * Steps<RP>::kCount * (RP <= 16 ? 1 : 2) * kWave;
+};
+struct PackArgs {
+    const float *part;  // [parts, N, R]
+    int32_t parts, r, rows;
+    int64_t n;
+    const float *scaling;  // null: scale
+    float scale;
+    int32_t scaled;
+    uint4 *out;
+    LoraPlan plan;
+};
+template <int RP>
+__global__ __launch_bounds__(THREADS) void lora_pack(PackArgs p) {
+    constexpr int RF = RP / 16, KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, LD = RP + 1;
+    __shared__ float v[32 * LD];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
+    if (int(blockIdx.y) >= *p.plan.list[0].count) return;
+    const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];
+    const int c = int(blockIdx.x) * 32;
+    if (tile.adapter < 0 || c >= tile.count) return;
+    const float scale = !p.scaled ? 1.0f : (p.scaling != nullptr ? p.scaling[tile.adapter] : p.scale);
+    for (int i = tid; i < 32 * RP; i += THREADS) {
+        const int t = i / RP, rank = i % RP;
+        float x = 0.0f;
+        if (c + t < tile.count && rank < p.r) {
+            const float *at = p.part + int64_t(p.plan.order[tile.start + c + t]) * p.r + rank;
+            x = add_parts(0.0f, at, p.parts, p.n * p.r) * scale;
+        }
+        v[t * LD + rank] = x;
+    }
+    __syncthreads();
+    uint4 *out = p.out + int64_t((tile.start + c) / 32 + tile.adapter) * (Packed<RP>::kColumns + (p.rows ? Packed<RP>::kRows : 0));
+    for (int f = wave; f < RF; f += WAVES) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = v[(8 * quad + j) * LD + f * 16 + col];
+        uint4 part[3];
+        split<3>(x, part);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) out[(f * 3 + k) * kWave + lane] = part[k];
+    }
+    if (!p.rows) return;
+    out += Packed<RP>::kColumns;
+    for (int q = wave; q < 2 * KS; q += WAVES) {
+        const int s = q / KS, ks = q % KS;
+        const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = v[(16 * s + col) * LD + r0 + j];
+        uint4 hl[2];
+        split<2>(x, hl);
+        if (RP <= 16) {
+            out[q * kWave + lane] = choose(quad < 2, hl[0], hl[1]);
+        } else {
+            out[(q * HL) * kWave + lane] = hl[0];
+            out[(q * HL + HL - 1) * kWave + lane] = hl[1];
         }
     }
 }
@@ -524,25 +625,17 @@ __global__ __launch_bounds__(THREADS) void lora_expand(ExpandArgs p) {
 // ---------------------------------------------------------------------------
 // lora_bwd_out: grid (blocks of O, tiles).  One pass over dy: the tile's part of dB, and dy B over the block's outputs.
 // A wavefront owns 64 G outputs; per 32 tokens it reads them twice (once from HBM, once from cache): transposed for dB, as
-// they are for dy B.
+// they are for dy B.  What a step needs from HBM is requested a step ahead.
 // ---------------------------------------------------------------------------
 struct BwdOutArgs {
     const void *dy, *b;
     int64_t dy_stride;
-    const float *u;
+    const uint4 *u;       // packed columns
     int32_t n, o, r;
     float *db, *db_part;  // [S, O, R], [slots, O, R]
     float *du_part;       // [blocks, N, R]
     LoraPlan plan;
 };
-// Eight tokens' values of one column, contraction index = token; zeros behind the `live` first of them.
-__device__ __forceinline__ void load_column(const float *v, int r, int rank, const int32_t (&tokens)[8], int live, float (&x)[8]) {
-    const float *col = v + (rank < r ? rank : 0);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = col[int64_t(tokens[j]) * r];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = j < live ? x[j] : 0.0f;
-}
 // The tile's tokens into LDS, the last one repeated up to a multiple of 32.
 __device__ __forceinline__ void load_tokens(const int32_t *order, const LoraTile &tile, int32_t *tokens) {
     for (int i = threadIdx.x; i < (tile.count + 31) / 32 * 32; i += THREADS) tokens[i] = order[tile.start + (i < tile.count ? i : tile.count - 1)];
@@ -562,8 +655,14 @@ template <typename T> __device__ __forceinline__ f32x4 outer(const uint4 (&data)
     acc = mfma<Bf16>(data[0], v[1], acc);
     return mfma<Bf16>(data[0], v[0], acc);
 }
+// A barrier that orders LDS only: loads in flight stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 
-template <typename T, int RP, int G, bool VEC>
+template <typename T, int RP, int G, int MODE>
 __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
     constexpr int RF = RP / 16, NP = Parts<T>::kCount;
     constexpr int RED = RF < 4 ? RF : 4;  // groups of sixteen ranks that cross the wavefronts at a time
@@ -574,7 +673,6 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
     const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];
     if (tile.adapter < 0) return;
     load_tokens(p.plan.order, tile, tokens);
-    const typename T::raw_t *dy = static_cast<const typename T::raw_t *>(p.dy);
     const typename T::raw_t *bw = static_cast<const typename T::raw_t *>(p.b) + int64_t(tile.adapter) * p.o * p.r;
     const int o0 = (int(blockIdx.x) * WAVES + wave) * 64 * G;
     // B^T fragments: row = rank, contraction index = output
@@ -602,31 +700,50 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[g][f][e] = f32x4{0, 0, 0, 0};
     __syncthreads();
-    for (int c = 0; c < tile.count; c += 32) {
+    int col4[G], col8[G][2];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        col4[g] = lane_column<MODE>(o0 + g * 64 + 4 * col, p.o);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) col8[g][ks] = lane_column<MODE>(o0 + g * 64 + ks * 32 + 8 * quad, p.o);
+    }
+    const uint4 *const packed = p.u + int64_t(tile.start / 32 + tile.adapter) * Packed<RP>::kColumns + lane;
+    auto request = [&](int c, uint2 (&w)[G][8]) {
+        int32_t tk[8];
+        eight_tokens(tokens + c + 8 * quad, tk);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const row_offset_t<MODE> at = row_offset<MODE>(tk[j], p.dy_stride);
+#pragma unroll
+            for (int g = 0; g < G; ++g) w[g][j] = row_load4<T, MODE>(p.dy, at, col4[g], p.o);
+        }
+    };
+    auto step = [&](int c, const uint2 (&w)[G][8], uint2 (&next)[G][8]) {
+        // the step's own remaining loads first (they come from cache), then the next step's
+        uint4 fy[G][2][2], v[RF][3];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const row_offset_t<MODE> at = row_offset<MODE>(tokens[c + 16 * s + col], p.dy_stride);
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) fy[g][ks][s] = row_load8<T, MODE>(p.dy, at, col8[g][ks], p.o);
+        }
+        const uint4 *pu = packed + int64_t(c / 32) * Packed<RP>::kColumns;
+#pragma unroll
+        for (int f = 0; f < RF; ++f)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) v[f][k] = pu[(f * 3 + k) * kWave];
+        request(c + 32 < tile.count ? c + 32 : c, next);
         f32x4 du[2][RF];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int f = 0; f < RF; ++f) du[s][f] = f32x4{0, 0, 0, 0};
-        int32_t tk[8];
-        eight_tokens(tokens + c + 8 * quad, tk);
-        const typename T::raw_t *row[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) row[s] = dy + int64_t(tokens[c + 16 * s + col]) * p.dy_stride;
-        float x[RF][8];
-#pragma unroll
-        for (int f = 0; f < RF; ++f) load_column(p.u, p.r, f * 16 + col, tk, tile.count - c - 8 * quad, x[f]);
-        uint4 v[RF][3];
-#pragma unroll
-        for (int f = 0; f < RF; ++f) split<3>(x[f], v[f]);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            const int og = o0 + g * 64;
-            uint2 w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = load4<T, VEC>(dy + int64_t(tk[j]) * p.dy_stride, og + 4 * col, p.o);
             uint4 frag[4], part[4][NP];
-            transpose(w, frag);
+            transpose(w[g], frag);
 #pragma unroll
             for (int e = 0; e < 4; ++e) as_bf16<T>(frag[e], part[e]);
 #pragma unroll
@@ -636,21 +753,19 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const uint4 fy = load8<T, VEC>(row[s], og + ks * 32 + 8 * quad, p.o);
+                for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int f = 0; f < RF; ++f) du[s][f] = mfma<T>(fb[g][ks][f], fy, du[s][f]);
-                }
+                    for (int f = 0; f < RF; ++f) du[s][f] = mfma<T>(fb[g][ks][f], fy[g][ks][s], du[s][f]);
         }
         // dy B of the workgroup's outputs: the wavefronts' parts in their order
 #pragma unroll
         for (int f0 = 0; f0 < RF; f0 += RED) {
-            __syncthreads();  // the previous sums are read
+            lds_barrier();  // the previous sums are read
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int f = 0; f < RED; ++f) red[wave][16 * s + col][f * 4 + quad] = du[s][f0 + f];
-            __syncthreads();
+            lds_barrier();
             for (int q = tid; q < 32 * RED * 4; q += THREADS) {
                 const int i = q / (RED * 4), r4 = q % (RED * 4), r0 = f0 * 16 + r4 * 4;
                 if (c + i < tile.count && r0 < p.r) {
@@ -664,6 +779,13 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
                 }
             }
         }
+    };
+    uint2 even[G][8], odd[G][8];
+    request(0, even);
+    for (int c = 0; c < tile.count; c += 64) {
+        step(c, even, odd);
+        if (c + 32 >= tile.count) break;
+        step(c + 32, odd, even);
     }
     float *db = tile.slot < 0 ? p.db + int64_t(tile.adapter) * p.o * p.r : p.db_part + int64_t(tile.slot) * p.o * p.r;
 #pragma unroll
@@ -686,13 +808,14 @@ struct BwdInArgs {
     const void *x, *a, *dx_base;
     void *dx;
     int64_t x_stride, dx_base_stride, dx_stride;
-    const float *du;
+    const uint4 *du;      // packed columns and rows
     int32_t h, r;
     float *da, *da_part;  // [S, R, H], [slots, R, H]
     LoraPlan plan;
 };
-template <typename T, int RP, bool VEC>
+template <typename T, int RP, int MODE>
 __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
+    constexpr bool VEC = MODE != ROWS_SCALAR;
     constexpr int RF = RP / 16, KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, NP = Parts<T>::kCount;
     __shared__ __attribute__((aligned(16))) int32_t tokens[BWD_TILE_MAX];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
@@ -702,11 +825,10 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
     __syncthreads();
     const int h0 = (int(blockIdx.x) * WAVES + wave) * 64;
     if (h0 >= p.h) return;  // (no barrier follows)
-    const typename T::raw_t *x = static_cast<const typename T::raw_t *>(p.x);
-    const typename T::raw_t *dx_base = static_cast<const typename T::raw_t *>(p.dx_base);
-    typename T::raw_t *dx = static_cast<typename T::raw_t *>(p.dx);
     const bool has = tile.adapter >= 0;
     const typename T::raw_t *aw = static_cast<const typename T::raw_t *>(p.a) + (has ? int64_t(tile.adapter) * p.r * p.h : 0);
+    const int col4 = lane_column<MODE>(h0 + 4 * col, p.h), out_col = h0 + 16 * quad;
+    const uint4 *const packed = p.du + int64_t(tile.start / 32 + (has ? tile.adapter : 0)) * (Packed<RP>::kColumns + Packed<RP>::kRows) + lane;
     // A fragments: row 4 m + e = input, contraction index = rank
     uint4 fa[KS][4][NP];
 #pragma unroll
@@ -727,55 +849,63 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
     for (int f = 0; f < RF; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[f][e] = f32x4{0, 0, 0, 0};
-    for (int c = 0; c < tile.count; c += 32) {
-        if (has) {
-            int32_t tk[8];
-            eight_tokens(tokens + c + 8 * quad, tk);
-            uint2 w[8];
+    auto request = [&](int c, uint2 (&w)[8]) {
+        int32_t tk[8];
+        eight_tokens(tokens + c + 8 * quad, tk);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = load4<T, VEC>(x + int64_t(tk[j]) * p.x_stride, h0 + 4 * col, p.h);
+        for (int j = 0; j < 8; ++j) w[j] = row_load4<T, MODE>(p.x, row_offset<MODE>(tk[j], p.x_stride), col4, p.h);
+    };
+    auto step = [&](int c, const uint2 (&w)[8], uint2 (&next)[8]) {
+        const uint4 *pu = packed + int64_t(c / 32) * (Packed<RP>::kColumns + Packed<RP>::kRows);
+        BaseRow<T, VEC> base[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            base[s].load(p.dx_base, p.dx_base == nullptr ? 0 : int64_t(tokens[c + 16 * s + col]) * p.dx_base_stride, out_col, p.h);
+        uint4 rows[2][KS][HL];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int k = 0; k < HL; ++k) rows[s][ks][k] = has ? pu[Packed<RP>::kColumns + ((s * KS + ks) * HL + k) * kWave] : make_uint4(0, 0, 0, 0);
+        request(c + 32 < tile.count ? c + 32 : c, next);
+        if (has) {
             uint4 frag[4], part[4][NP];
             transpose(w, frag);
 #pragma unroll
             for (int e = 0; e < 4; ++e) as_bf16<T>(frag[e], part[e]);
 #pragma unroll
             for (int f = 0; f < RF; ++f) {
-                float col8[8];
                 uint4 v[3];
-                load_column(p.du, p.r, f * 16 + col, tk, tile.count - c - 8 * quad, col8);
-                split<3>(col8, v);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) v[k] = pu[(f * 3 + k) * kWave];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[f][e] = outer<T>(part[e], v, acc[f][e]);
             }
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int i = c + 16 * s + col;
-            const int64_t token = tokens[i];
             f32x4 sum[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum[e] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
-                float row[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) row[j] = p.du[token * p.r + (r0 + j < p.r ? r0 + j : 0)];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) row[j] = has && r0 + j < p.r ? row[j] : 0.0f;
-                uint4 hl[2];
-                split<2>(row, hl);
-                if (RP <= 16) hl[0] = choose(quad < 2, hl[0], hl[1]);
+            for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int k = 0; k < HL; ++k)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int q = 0; q < NP; ++q) sum[e] = mfma<Bf16>(fa[ks][e][q], hl[k], sum[e]);
-            }
-            if (i < tile.count)
-                store_sum<T, VEC>(dx_base != nullptr ? dx_base + token * p.dx_base_stride : nullptr, dx + token * p.dx_stride, h0 + 16 * quad, p.h, sum);
+                        for (int q = 0; q < NP; ++q) sum[e] = mfma<Bf16>(fa[ks][e][q], rows[s][ks][k], sum[e]);
+            if (c + 16 * s + col < tile.count)
+                base[s].store(static_cast<typename T::raw_t *>(p.dx) + int64_t(tokens[c + 16 * s + col]) * p.dx_stride, out_col, p.h, sum);
         }
+    };
+    uint2 even[8], odd[8];
+    request(0, even);
+    for (int c = 0; c < tile.count; c += 64) {
+        step(c, even, odd);
+        if (c + 32 >= tile.count) break;
+        step(c + 32, odd, even);
     }
     if (!has) return;
     float *da = tile.slot < 0 ? p.da + int64_t(tile.adapter) * p.r * p.h : p.da_part + int64_t(tile.slot) * p.r * p.h;
@@ -876,7 +1006,7 @@ inline FwdLayout fwd_layout(const Shape &d) {
 }
 
 // The backward: outputs per wavefront (64 G) of the first pass, tokens per tile of both.
-struct BwdLayout { PlanLayout plan; int64_t slots[2], blocks[2]; int groups; size_t du, du_part, db_part, da_part, total; };
+struct BwdLayout { PlanLayout plan; int64_t slots[2], blocks[2]; int groups; size_t packed, du_part, db_part, da_part, total; };
 // Tokens per tile such that `blocks` times the tiles make about `want` workgroups.
 inline int64_t bwd_tile(int64_t n, int64_t blocks, int64_t want) {
     const int64_t tiles = ceil_div(want, blocks);
@@ -894,8 +1024,11 @@ inline BwdLayout bwd_layout(const Shape &d) {
     l.slots[0] = d.n / tile0;
     l.slots[1] = d.n / tile1;
     l.plan = plan_layout(d.n, d.s, tile0, tile1);
-    l.du = l.plan.total;
-    l.du_part = l.du + align_up(size_t(d.n) * d.r * 4);
+    // fragments of u, then of dy B in the same place: 3 + 2 (or 4) KB per 32 tokens and 16 (or 32) ranks
+    const int64_t rp = padded_rank(d.r);
+    const size_t chunk = size_t(rp) / 16 * 3 * 1024 + (rp == 16 ? 2048 : size_t(rp) / 32 * 4 * 1024);
+    l.packed = l.plan.total;
+    l.du_part = l.packed + align_up(size_t(d.n / 32 + d.s + 1) * chunk);
     l.db_part = l.du_part + align_up(size_t(l.blocks[0]) * d.n * d.r * 4);
     l.da_part = l.db_part + align_up(size_t(l.slots[0]) * d.o * d.r * 4);
     l.total = l.da_part + align_up(size_t(l.slots[1]) * d.h * d.r * 4);
@@ -918,6 +1051,15 @@ template <typename F> void with_types(int dtype, int rp, bool vec, F &&launch) {
     };
     if (dtype == KA_DTYPE_BF16) vectors(Bf16{});
     else vectors(F16{});
+}
+
+// The backward's kernels, by the layout of the matrix they stream (of `bytes`).
+template <typename F> void with_modes(int dtype, int rp, bool vec, int64_t bytes, F &&launch) {
+    with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
+        if constexpr (!decltype(vec_c)::value) launch(type, rank_c, std::integral_constant<int, ROWS_SCALAR>{});
+        else if (bytes < (int64_t(1) << 32)) launch(type, rank_c, std::integral_constant<int, ROWS_NARROW>{});
+        else launch(type, rank_c, std::integral_constant<int, ROWS_WIDE>{});
+    });
 }
 
 }  // namespace
@@ -1044,13 +1186,35 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     rc = check_hip(hipGetLastError(), "lora backward launch (plan)");
     if (rc != KA_OK) return rc;
     const int rp = padded_rank(rank);
-    float *du = reinterpret_cast<float *>(ws + l.du), *du_part = reinterpret_cast<float *>(ws + l.du_part);
+    uint4 *packed = reinterpret_cast<uint4 *>(ws + l.packed);
+    float *du_part = reinterpret_cast<float *>(ws + l.du_part);
     float *db_part = reinterpret_cast<float *>(ws + l.db_part), *da_part = reinterpret_cast<float *>(ws + l.da_part);
+    auto pack = [&](const float *part, int64_t parts, bool scaled) {
+        PackArgs pa{};
+        pa.part = part;
+        pa.parts = int32_t(parts);
+        pa.r = int32_t(rank);
+        pa.rows = scaled ? 1 : 0;
+        pa.n = n_tokens;
+        pa.scaling = scaling;
+        pa.scale = scale;
+        pa.scaled = scaled ? 1 : 0;
+        pa.out = packed;
+        pa.plan = plan;
+        const dim3 grid{unsigned(l.plan.tokens[0] / 32), unsigned(l.plan.max_tiles[0])};
+        with_types(dtype, rp, vec, [&](auto, auto rank_c, auto) {
+            constexpr int RP = decltype(rank_c)::value;
+            hipLaunchKernelGGL((lora_pack<RP>), grid, dim3(THREADS), 0, stream, pa);
+        });
+        return check_hip(hipGetLastError(), "lora backward launch (pack)");
+    };
+    rc = pack(shrunk, 1, false);
+    if (rc != KA_OK) return rc;
     BwdOutArgs oa{};
     oa.dy = grad_out;
     oa.b = lora_b;
     oa.dy_stride = grad_stride;
-    oa.u = shrunk;
+    oa.u = packed;
     oa.n = int32_t(n_tokens);
     oa.o = int32_t(out_dim);
     oa.r = int32_t(rank);
@@ -1059,23 +1223,20 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     oa.du_part = du_part;
     oa.plan = plan;
     const dim3 out_grid{unsigned(l.blocks[0]), unsigned(l.plan.max_tiles[0])};
-    with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
+    with_modes(dtype, rp, vec, n_tokens * grad_stride * 2, [&](auto type, auto rank_c, auto mode_c) {
         using T = decltype(type);
-        constexpr int RP = decltype(rank_c)::value;
-        constexpr bool VEC = decltype(vec_c)::value;
+        constexpr int RP = decltype(rank_c)::value, MODE = decltype(mode_c)::value;
         if constexpr (RP == 16) {
             if (l.groups == 4) {
-                hipLaunchKernelGGL((lora_bwd_out<T, RP, 4, VEC>), out_grid, dim3(THREADS), 0, stream, oa);
+                hipLaunchKernelGGL((lora_bwd_out<T, RP, 4, MODE>), out_grid, dim3(THREADS), 0, stream, oa);
                 return;
             }
         }
-        hipLaunchKernelGGL((lora_bwd_out<T, RP, 1, VEC>), out_grid, dim3(THREADS), 0, stream, oa);
+        hipLaunchKernelGGL((lora_bwd_out<T, RP, 1, MODE>), out_grid, dim3(THREADS), 0, stream, oa);
     });
     rc = check_hip(hipGetLastError(), "lora backward launch (out)");
     if (rc != KA_OK) return rc;
-    hipLaunchKernelGGL(lora_fold_rows, dim3(unsigned(ceil_div(n_tokens * rank, THREADS))), dim3(THREADS), 0, stream, du_part,
-                       int(l.blocks[0]), n_tokens, int(rank), adapter_ids, int(n_adapters), scaling, scale, du);
-    rc = check_hip(hipGetLastError(), "lora backward launch (fold)");
+    rc = pack(du_part, l.blocks[0], true);
     if (rc != KA_OK) return rc;
     BwdInArgs ia{};
     ia.x = hidden;
@@ -1085,18 +1246,17 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     ia.x_stride = hidden_stride;
     ia.dx_base_stride = dhidden_base_stride;
     ia.dx_stride = dhidden_stride;
-    ia.du = du;
+    ia.du = packed;
     ia.h = int32_t(in_dim);
     ia.r = int32_t(rank);
     ia.da = dlora_a;
     ia.da_part = da_part;
     ia.plan = plan;
     const dim3 in_grid{unsigned(l.blocks[1]), unsigned(l.plan.max_tiles[1])};
-    with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
+    with_modes(dtype, rp, vec, n_tokens * hidden_stride * 2, [&](auto type, auto rank_c, auto mode_c) {
         using T = decltype(type);
-        constexpr int RP = decltype(rank_c)::value;
-        constexpr bool VEC = decltype(vec_c)::value;
-        hipLaunchKernelGGL((lora_bwd_in<T, RP, VEC>), in_grid, dim3(THREADS), 0, stream, ia);
+        constexpr int RP = decltype(rank_c)::value, MODE = decltype(mode_c)::value;
+        hipLaunchKernelGGL((lora_bwd_in<T, RP, MODE>), in_grid, dim3(THREADS), 0, stream, ia);
     });
     rc = check_hip(hipGetLastError(), "lora backward launch (in)");
     if (rc != KA_OK) return rc;

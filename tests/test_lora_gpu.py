@@ -156,6 +156,26 @@ def test_layouts_and_in_place(sampler):
                             c["ids"].view(12, 5), inplace=True)
 
 
+def test_rows_that_lie_more_than_4_gib_apart(sampler):
+    n, h, o, r, s = 70, 64, 72, 16, 2
+    c = {k: v.cuda() for k, v in _inputs(n, h, o, r, s, torch.bfloat16, seed=12).items()}
+    step = 1 << 25                                            # 64 MiB per row: 4.4 GiB in all
+    store = torch.empty(n * step, dtype=torch.bfloat16, device="cuda")
+
+    def far(t, at):
+        v = store.as_strided(t.shape, (step, 1), at)
+        v.copy_(t)
+        return v
+
+    base, hidden, dy, dx = far(c["base"], 0), far(c["hidden"], 1024), far(c["dy"], 2048), far(c["dx"], 4096)
+    out, u = sampler.lora_linear(base, hidden, c["a"], c["b"], c["ids"], c["scaling"], return_shrunk=True)
+    want, want_u = sampler.lora_linear(c["base"], c["hidden"], c["a"], c["b"], c["ids"], c["scaling"], return_shrunk=True)
+    assert torch.equal(out, want) and torch.equal(u, want_u)
+    got = sampler.lora_linear_backward(dy, hidden, c["a"], c["b"], c["ids"], c["scaling"], u, dx)
+    ref = sampler.lora_linear_backward(c["dy"], c["hidden"], c["a"], c["b"], c["ids"], c["scaling"], u, c["dx"])
+    assert all(torch.equal(x, y) for x, y in zip(got, ref))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_infinities_stay_with_their_token(sampler, dtype):
     c = {k: v.cuda() for k, v in _inputs(40, 64, 72, 16, 2, dtype, seed=9, ids=torch.arange(40) % 2).items()}
