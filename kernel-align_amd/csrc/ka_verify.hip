@@ -31,6 +31,7 @@
 #include <stddef.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "ka_sampling_common.h"
 #include "ka_sampling_radix.h"
@@ -212,7 +213,7 @@ template <typename T> __device__ __forceinline__ float cut_value(uint32_t raw_cu
 // ordinary maximum.  Masses are then evaluated once per occupied bin instead of once per entry (by all threads where a sum
 // over the whole row is needed), and one wavefront walks the bins from the largest value down to the cuts, 64 at a time.  Rows
 // it cannot describe (values of 2^8 and above, NaN, a maximum or a cut among the small values, dropped values that would
-// count) take the radix path, as fp16 and fp32 rows do.
+// count) take the radix path.
 // ---------------------------------------------------------------------------
 constexpr uint32_t MAG_LOW = 0x3A00u, MAG_HIGH = 0x4380u;  // bits of 2^-11 and 2^8
 constexpr int HIST_SIDE = int(MAG_HIGH - MAG_LOW);         // values of one sign: 19 octaves of 128
@@ -235,10 +236,28 @@ struct HistRow {
     double raw_sum;
     float raw_top;
 };
-struct VerifyShared {
+// fp16 and fp32 rows: see coarse_cut
+constexpr int LIST_CAP = 2048;
+struct CoarseRow {
+    union {
+        uint32_t count[HIST_BINS];
+        uint64_t mass[HIST_BINS];
+    };
+    alignas(16) uint32_t key[LIST_CAP];
+    uint32_t sorted[LIST_CAP];
+    uint32_t n_list, give_up, max_key, ok;
+    uint64_t sums[S_WAVES];  // per wavefront: mass of all entries
+    double raw_sums[S_WAVES];
+    float edge_low, edge_high;  // the list takes entries of [edge_low, edge_high)
+    uint64_t before;            // mass above edge_high
+    RowCut cut;
+    double raw_sum;
+    float raw_top;
+};
+template <typename T> struct VerifyShared {
     union {
         Shared sh;
-        HistRow hist;
+        std::conditional_t<T::kDtype == KA_DTYPE_BF16, HistRow, CoarseRow> row;
     };
     PolicyLse lse;
     uint32_t ties_before;
@@ -545,9 +564,307 @@ template <typename T> __device__ __forceinline__ uint32_t raw_key_of_cut(uint32_
     return near + uint32_t(low - kWave / 2) * key_step<T>();
 }
 
+// ---------------------------------------------------------------------------
+// fp16 and fp32 rows have too many values for a bin each.  The same bins, of the values cut to bf16, locate the cut; the
+// entries of the bins around it (about top_k of them, or a few hundred) then go to a list, are sorted, and decide as in the
+// definition.  No filter: the maximum, then the masses (two passes over the row).  Top-k: counts, then the list (two).  Top-p
+// alone: the maximum, the mass of every bin, the list (three).  What does not fit (values of 2^8 and above, NaN, a cut among
+// values below 2^-11 or at the edge of the list, more than 2048 entries in it) takes the radix path.
+// ---------------------------------------------------------------------------
+// f(entry) for every entry of the row by the whole block, in any order; eight vectors in flight per lane, any alignment.
+// UNROLL: f is short enough to be written out for each of the eight.
+template <typename T, bool UNROLL, typename F> __device__ __forceinline__ void each_entry(const typename T::raw_t *rp, int vocab, F &&f) {
+    constexpr int EPV = T::kPerVec, U = 8;
+    const int tid = threadIdx.x;
+    int head = int((16 - (reinterpret_cast<uintptr_t>(rp) & 15)) & 15) / T::kBytes;
+    head = head < vocab ? head : vocab;
+    const int nvec = (vocab - head) / EPV, tail = head + nvec * EPV + tid;
+    if (tid < head) f(rp[tid]);
+    if (tail < vocab) f(rp[tail]);
+    const uint4 *vp = reinterpret_cast<const uint4 *>(rp + head);
+    for (int v = tid; v < nvec; v += U * S_THREADS) {
+        uint4 q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = vp[v + u * S_THREADS < nvec ? v + u * S_THREADS : v];
+        if constexpr (UNROLL) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (v + u * S_THREADS >= nvec) continue;
+#pragma unroll
+                for (int j = 0; j < EPV; ++j) f(entry_of<T>(q[u], j));
+            }
+        } else {
+#pragma unroll 1
+            for (int u = 0; u < U; ++u) {
+                if (v + u * S_THREADS >= nvec) break;
+#pragma unroll
+                for (int j = 0; j < EPV; ++j) f(entry_of<T>(q[0], j));
+#pragma unroll
+                for (int t = 0; t + 1 < U; ++t) q[t] = q[t + 1];
+            }
+        }
+    }
+}
+
+// Bin of a value, or HIST_BINS (small, zero), HIST_BINS + 1 (-2^8 and below), HIST_BINS + 2 (2^8 and above, NaN).
+__device__ __forceinline__ int coarse_bin(float x) {
+    const uint32_t b = __float_as_uint(x), mag = (b >> 16) & 0x7fffu, m = mag - MAG_LOW;
+    if (m < uint32_t(HIST_SIDE)) return HIST_SIDE + int(m ^ uint32_t(int32_t(b) >> 31));
+    if (mag < MAG_LOW) return HIST_BINS;
+    return int32_t(b) < 0 && x == x ? HIST_BINS + 1 : HIST_BINS + 2;
+}
+// Largest value, in magnitude order of its sign, that a bin begins with (the bins are of values cut towards zero).
+__device__ __forceinline__ float bin_value(int bin) { return __uint_as_float(raw_of_bin(bin) << 16); }
+// Bins b .. hold the values from lower_edge(b) on.
+__device__ __forceinline__ float lower_edge(int bin) {
+    if (bin <= 0) return -256.0f;
+    if (bin > HIST_BINS - 1) return 256.0f;
+    // a negative bin holds (next bin down's value, its own value]: its lower edge is just above the value of the bin below
+    return bin >= HIST_SIDE ? bin_value(bin) : __uint_as_float(__float_as_uint(bin_value(bin - 1)) - 1u);
+}
+
+template <typename T>
+__device__ __forceinline__ bool coarse_cut(CoarseRow &h, const typename T::raw_t *rp, int vocab, const Filter &f, bool want_lse) {
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    for (int i = tid; i < HIST_BINS; i += S_THREADS) h.mass[i] = 0;
+    if (tid == 0) { h.n_list = h.give_up = h.max_key = h.ok = 0; }
+    __syncthreads();
+    auto last_u64 = [&](uint64_t v) {
+        return (uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), kWave - 1))) << 32) |
+               uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), kWave - 1));
+    };
+    // ---- first pass: the maximum, and with top-k the counts ----------------------------------
+    {
+        uint32_t top = 0, bad = 0;
+        each_entry<T, true>(rp, vocab, [&](typename T::raw_t raw) {
+            const float x = T::widen(raw);
+            const uint32_t key = masked_key<T>(x);
+            top = key > top && x == x ? key : top;
+            bad |= !(x < 256.0f) ? 1u : 0u;
+            if (f.use_k) {
+                const int bin = coarse_bin(x);
+                if (bin < HIST_BINS) atomicAdd(&h.count[bin], 1u);
+            }
+        });
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) {
+            const uint32_t o = __shfl_xor(top, off, kWave);
+            top = o > top ? o : top;
+        }
+        if (lane == 0) atomicMax(&h.max_key, top);
+        if (bad) h.give_up = 1;
+    }
+    __syncthreads();
+    const float xmax = value_of<T>(h.max_key);
+    if (h.give_up != 0 || h.max_key == 0 || !(xmax >= 0x1p-11f || xmax <= -0x1p-11f) || !(xmax > -256.0f)) return false;
+    const uint32_t kmax = elem_key<T>(raw_of_key<T>(h.max_key), f.temp, f.has_t);
+    const float vmax = value_of<T>(kmax);
+    auto weight_of = [&](uint32_t key) { return weight_fix(key == kmax ? 0.0f : value_of<T>(key) - vmax); };
+    const int top_bin = coarse_bin(xmax);
+    if (f.use_k) {
+        // ---- the bin of the top_k-th largest entry; the list reaches one bin further ----------
+        if (wave == 0) {
+            uint32_t upto = 0;
+            int found = -1;
+            for (int b0 = top_bin; b0 >= 0 && found < 0; b0 -= kWave) {
+                const int b = b0 - lane;
+                const uint32_t inc = upto + wave_incl_scan_u32(b >= 0 ? h.count[b] : 0u);
+                const uint64_t reached = __ballot(inc >= uint32_t(f.top_k));
+                if (reached != 0) found = b0 - (__ffsll((long long)reached) - 1);
+                upto = uint32_t(__builtin_amdgcn_readlane(int(inc), kWave - 1));
+                // (past the smallest positive values lie entries that are not counted)
+                if (found < HIST_SIDE && top_bin >= HIST_SIDE && b0 - kWave < HIST_SIDE) break;
+            }
+            if (lane == 0) {
+                const bool side = found >= 0 && (found > HIST_SIDE || (found < HIST_SIDE && top_bin < HIST_SIDE && found > 0));
+                h.ok = side ? 1u : 0u;
+                h.edge_low = side ? lower_edge(found - 1) : 0.0f;
+                h.edge_high = 256.0f;
+                h.before = 0;
+            }
+        }
+        __syncthreads();
+        if (h.ok == 0) return false;
+    }
+    // ---- second pass: the list (top-k), or the masses -----------------------------------------
+    uint64_t z_all = 0;
+    double raw_sum = 0.0;
+    {
+        uint64_t all = 0;
+        const float low = f.use_k ? h.edge_low : 0.0f;
+        if (f.use_k) {
+            each_entry<T, true>(rp, vocab, [&](typename T::raw_t raw) {
+                const float x = T::widen(raw);
+                if (want_lse) raw_sum += double(fast_exp2((x - xmax) * kLseLog2e));
+                if (x >= low) {
+                    const uint32_t at = atomicAdd(&h.n_list, 1u);
+                    if (at < uint32_t(LIST_CAP)) h.key[at] = elem_key<T>(raw, f.temp, f.has_t);
+                }
+            });
+        } else {
+            each_entry<T, false>(rp, vocab, [&](typename T::raw_t raw) {
+                const float x = T::widen(raw);
+                if (want_lse) raw_sum += double(fast_exp2((x - xmax) * kLseLog2e));
+                const uint64_t w = weight_of(elem_key<T>(raw, f.temp, f.has_t));
+                all += w;
+                if (f.use_p && w != 0) {
+                    const int bin = coarse_bin(x);
+                    if (bin < HIST_BINS) atomicAdd(reinterpret_cast<unsigned long long *>(&h.mass[bin]), (unsigned long long)w);
+                }
+            });
+        }
+        all = wave_sum_u64_of(all);
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) raw_sum += __shfl_xor(raw_sum, off, kWave);
+        if (lane == 0) {
+            h.sums[wave] = all;
+            h.raw_sums[wave] = raw_sum;
+        }
+        __syncthreads();
+        raw_sum = 0.0;
+        for (int w = 0; w < S_WAVES; ++w) {
+            z_all += h.sums[w];
+            raw_sum += h.raw_sums[w];
+        }
+        if (f.use_p && !f.use_k) {
+            // ---- the bin where the mass before an entry passes theta; the list: it and its two neighbours ----
+            if (wave == 0) {
+                const uint64_t theta = floor_scale(f.top_p, z_all);
+                uint64_t run = 0, before = 0;
+                int found = -1;
+                for (int b0 = top_bin; b0 >= 0 && found < 0; b0 -= kWave) {
+                    const int b = b0 - lane;
+                    const uint64_t m = b >= 0 ? h.mass[b] : 0ull;
+                    const uint64_t inc = run + wave_incl_scan_u64(m);
+                    const uint64_t passed = __ballot(inc > theta);  // the last entry kept lies in the first of these
+                    if (passed != 0) {
+                        const int l = __ffsll((long long)passed) - 1;
+                        found = b0 - l;
+                        const uint64_t at = inc - m;
+                        before = (uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(at >> 32)), l))) << 32) |
+                                 uint32_t(__builtin_amdgcn_readlane(int(uint32_t(at)), l));
+                    }
+                    run = last_u64(inc);
+                    if (found < HIST_SIDE && top_bin >= HIST_SIDE && b0 - kWave < HIST_SIDE) break;
+                }
+                if (lane == 0) {
+                    const bool side = found >= 0 && (found > HIST_SIDE || (found < HIST_SIDE && top_bin < HIST_SIDE && found > 0));
+                    // (one bin up, unless that is another sign's)
+                    const bool up = side && found + 1 < HIST_BINS && found + 1 != HIST_SIDE;
+                    h.ok = side ? 1u : 0u;
+                    h.edge_low = side ? lower_edge(found - 1) : 0.0f;
+                    h.edge_high = side ? lower_edge(up ? found + 2 : found + 1) : 0.0f;
+                    if (side && found + 1 == HIST_SIDE) h.edge_high = 0.0f;
+                    h.before = before - (up ? h.mass[found + 1] : 0ull);
+                }
+            }
+            __syncthreads();
+            if (h.ok == 0) return false;
+            const float lo = h.edge_low, hi = h.edge_high;
+            each_entry<T, true>(rp, vocab, [&](typename T::raw_t raw) {
+                const float x = T::widen(raw);
+                if (x >= lo && x < hi) {
+                    const uint32_t at = atomicAdd(&h.n_list, 1u);
+                    if (at < uint32_t(LIST_CAP)) h.key[at] = elem_key<T>(raw, f.temp, f.has_t);
+                }
+            });
+            __syncthreads();
+        }
+    }
+    RowCut cut{kmax, 0u, 0u, 0xffffffffu, z_all};
+    bool ok = true;
+    if (f.use_k || f.use_p) {
+        const uint32_t n = h.n_list;
+        if (n > uint32_t(LIST_CAP) || n == 0 || (f.use_k && n < uint32_t(f.top_k))) return false;
+        // ---- sorted by key, descending (equal keys in any order: they have equal masses) ---------
+        if (tid < 4 && n + uint32_t(tid) < uint32_t(LIST_CAP)) h.key[n + uint32_t(tid)] = NO_KEY;  // up to a multiple of four
+        __syncthreads();
+        for (uint32_t i = uint32_t(tid); i < n; i += S_THREADS) {
+            const uint32_t k = h.key[i];
+            uint32_t rank = 0;
+            for (uint32_t j = 0; j < n; j += 4) {
+                const uint4 o = *reinterpret_cast<const uint4 *>(h.key + j);
+                rank += (o.x > k || (o.x == k && j < i) ? 1u : 0u) + (o.y > k || (o.y == k && j + 1 < i) ? 1u : 0u) +
+                        (o.z > k || (o.z == k && j + 2 < i) ? 1u : 0u) + (o.w > k || (o.w == k && j + 3 < i) ? 1u : 0u);
+            }
+            h.sorted[rank] = k;
+        }
+        __syncthreads();
+        if (wave != 0) {
+            __syncthreads();  // the first wavefront's result
+            return h.ok != 0;
+        }
+        // a group at the list's lower end may go on behind it
+        const uint32_t key_edge = masked_key<T>(h.edge_low) <= key_step<T>() ? 0u : elem_key<T>(raw_of_key<T>(masked_key<T>(h.edge_low)), f.temp, f.has_t);
+        const uint32_t key_high = h.edge_high < 256.0f ? elem_key<T>(raw_of_key<T>(masked_key<T>(h.edge_high)), f.temp, f.has_t) : 0xffffffffu;
+        uint64_t z = z_all;
+        uint32_t na = n;  // entries of the list that survive top-k
+        if (f.use_k) {
+            cut.kstar = cut.kcut = h.sorted[f.top_k - 1];
+            ok = cut.kstar > key_edge;
+            z = 0;
+            na = 0;
+            for (uint32_t i0 = 0; i0 < n; i0 += kWave) {
+                const uint32_t i = i0 + uint32_t(lane);
+                const bool in = i < n && h.sorted[i] >= cut.kstar;
+                z += wave_sum_u64_of(in ? weight_of(h.sorted[i]) : 0ull);
+                const uint32_t here = uint32_t(__popcll(__ballot(in)));
+                na += here;
+                if (here < uint32_t(kWave)) break;
+            }
+            cut.z = z;
+        }
+        if (f.use_p && ok) {
+            const uint64_t theta = floor_scale(f.top_p, z);
+            uint64_t run = h.before;
+            int best = -1;
+            for (uint32_t i0 = 0; i0 < na && run <= theta; i0 += kWave) {
+                const uint32_t i = i0 + uint32_t(lane);
+                const uint64_t m = i < na ? weight_of(h.sorted[i]) : 0ull;
+                const uint64_t inc = run + wave_incl_scan_u64(m);
+                const uint64_t in = __ballot(i < na && inc - m <= theta);
+                if (in != 0) best = int(i0) + 63 - __builtin_clzll(in);
+                run = last_u64(inc);
+            }
+            ok = best >= 0;
+            if (ok) {
+                cut.kcut = h.sorted[best];
+                ok = cut.kcut > key_edge && cut.kcut < key_high;
+            }
+            if (ok) {
+                uint64_t before = h.before;
+                uint32_t n_cut = 0;
+                for (uint32_t i0 = 0; i0 < na; i0 += kWave) {
+                    const uint32_t i = i0 + uint32_t(lane);
+                    const uint32_t key = i < na ? h.sorted[i] : 0u;
+                    before += wave_sum_u64_of(key > cut.kcut ? weight_of(key) : 0ull);
+                    n_cut += uint32_t(__popcll(__ballot(i < na && key == cut.kcut)));
+                    if (__ballot(key < cut.kcut) != 0) break;
+                }
+                const uint64_t w_cut = weight_of(cut.kcut);
+                uint64_t r = n_cut;
+                if (w_cut > 0) {
+                    const uint64_t fit = (theta - before) / w_cut + 1;  // entries t with before + t * w <= theta
+                    r = fit < r ? fit : r;
+                }
+                cut.r_cut = r == n_cut ? 0xffffffffu : uint32_t(r);
+                cut.z = before + r * w_cut;
+            }
+        }
+    }
+    if (tid == 0) {
+        h.cut = cut;
+        h.raw_sum = raw_sum;
+        h.raw_top = xmax;
+        h.ok = ok ? 1u : 0u;
+    }
+    __syncthreads();
+    return (f.use_k || f.use_p) ? ok : true;
+}
+
 template <typename T>
 __global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(6, 6))) void verify_rows(VerifyParams p) {
-    __shared__ VerifyShared lds;
+    __shared__ VerifyShared<T> lds;
     const int tid = threadIdx.x;
     const int64_t n_target = int64_t(p.batch) * (p.k + 1);
     const int64_t r = blockIdx.x;
@@ -569,14 +886,14 @@ __global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(6, 6)
     double raw_sum = 1.0;
     float raw_top = 0.0f;
     bool done = false;
-    if constexpr (T::kDtype == KA_DTYPE_BF16) {
-        done = hist_cut(lds.hist, rp, p.vocab, f, want_lse);
-        if (done) {
-            cut = lds.hist.cut;
-            raw_cut = lds.hist.raw_cut;
-            raw_sum = lds.hist.raw_sum;
-            raw_top = lds.hist.raw_top;
-        }
+    if constexpr (T::kDtype == KA_DTYPE_BF16) done = hist_cut(lds.row, rp, p.vocab, f, want_lse);
+    else done = coarse_cut<T>(lds.row, rp, p.vocab, f, want_lse);
+    if (done) {
+        cut = lds.row.cut;
+        raw_sum = lds.row.raw_sum;
+        raw_top = lds.row.raw_top;
+        if constexpr (T::kDtype == KA_DTYPE_BF16) raw_cut = lds.row.raw_cut;
+        else if (f.use_k || f.use_p) raw_cut = raw_key_of_cut<T>(cut.kcut, f.temp, f.has_t);
     }
     if (!done) {
         __syncthreads();
