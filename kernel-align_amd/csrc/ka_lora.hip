@@ -29,7 +29,8 @@ constexpr int MAX_RANK = KA_LORA_MAX_RANK;
 constexpr int MAX_ADAPTERS = KA_LORA_MAX_ADAPTERS;
 constexpr int THREADS = 256;
 constexpr int WAVES = THREADS / kWave;
-constexpr int FWD_TILE = 64;    // tokens per tile of the forward: four groups of sixteen
+constexpr int FWD_TILE = 32;    // tokens per tile of the forward: two groups of sixteen
+constexpr int FWD_SUBS = FWD_TILE / 16;
 constexpr int BWD_TILE_MAX = 1024;  // ... of the backward at most (a multiple of 32)
 
 struct LoraTile {
@@ -52,12 +53,15 @@ struct LoraPlan {          // device pointers into the workspace
 // lora_plan: one workgroup sorts the tokens.  Every wavefront takes a contiguous share of them: counts, a prefix over
 // (adapter, wavefront), then the ranks inside a step of 64 tokens from ballots.  The ids of eight steps are requested together.
 // ---------------------------------------------------------------------------
-constexpr int PLAN_THREADS = 512;
-constexpr int PLAN_WAVES = PLAN_THREADS / kWave;
-
-__global__ __launch_bounds__(PLAN_THREADS) void lora_plan(const int64_t *__restrict__ ids, int n, int s, int lists, LoraPlan plan) {
-    __shared__ int32_t at[PLAN_WAVES][MAX_ADAPTERS + 1];  // counts, then the next position of the wavefront's tokens
-    __shared__ int32_t wave_sum[PLAN_WAVES][5];
+template <int PLAN_THREADS> struct PlanShared {
+    int32_t at[PLAN_THREADS / kWave][MAX_ADAPTERS + 1];  // counts, then the next position of the wavefront's tokens
+    int32_t wave_sum[PLAN_THREADS / kWave][5];
+};
+template <int PLAN_THREADS>
+__device__ __forceinline__ void make_plan(PlanShared<PLAN_THREADS> &sh, const int64_t *__restrict__ ids, int n, int s, int lists, const LoraPlan &plan) {
+    constexpr int PLAN_WAVES = PLAN_THREADS / kWave;
+    auto &at = sh.at;
+    auto &wave_sum = sh.wave_sum;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
     constexpr int U = 8;
     const int steps = (n + kWave - 1) / kWave, per = (steps + PLAN_WAVES - 1) / PLAN_WAVES;
@@ -177,6 +181,11 @@ __global__ __launch_bounds__(PLAN_THREADS) void lora_plan(const int64_t *__restr
         }
     }
 }
+constexpr int PLAN_THREADS = 512;
+__global__ __launch_bounds__(PLAN_THREADS) void lora_plan(const int64_t *__restrict__ ids, int n, int s, int lists, LoraPlan plan) {
+    __shared__ PlanShared<PLAN_THREADS> sh;
+    make_plan(sh, ids, n, s, lists, plan);
+}
 
 // ---------------------------------------------------------------------------
 // Fragments.  v_mfma_f32_16x16x32: lane l holds eight values (one 16-byte register group) of row / column l % 16 at the
@@ -215,6 +224,20 @@ template <int PARTS> __device__ __forceinline__ void split(const float (&v)[8], 
     }
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) part[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+}
+// v * down = part[0] + part[1] in fp16, |v * down| < 2: to 2^-22 of it, or 2^-25
+__device__ __forceinline__ void split_f16(const float (&v)[8], float down, uint4 (&part)[2]) {
+    uint32_t w[2][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float x = v[j] * down;
+        const _Float16 hi = _Float16(x), lo = _Float16(rest(x, float(hi)));
+        const uint32_t h = __builtin_bit_cast(uint16_t, hi), l = __builtin_bit_cast(uint16_t, lo);
+        w[0][j / 2] = j & 1 ? w[0][j / 2] | h << 16 : h;
+        w[1][j / 2] = j & 1 ? w[1][j / 2] | l << 16 : l;
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) part[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
 }
 __device__ __forceinline__ uint4 choose(bool first, const uint4 &a, const uint4 &b) {
     return make_uint4(first ? a.x : b.x, first ? a.y : b.y, first ? a.z : b.z, first ? a.w : b.w);
@@ -309,26 +332,34 @@ template <typename T> __device__ __forceinline__ typename T::raw_t narrow(float 
     else return __builtin_bit_cast(uint16_t, _Float16(v));
 }
 
-// The sixteen results a lane holds for one token after four products e (row 4 m + e of the wide dimension at MFMA row m):
-// acc[e][i] belongs to column first + 4 i + e.  out = base + acc, rounded once; the base is loaded ahead of the products.
-template <typename T, bool VEC> struct BaseRow {
+// The sixteen results a lane holds for one token after four products e: columns first .. + 7 and first + 32 .. + 7, so that the
+// four quads of a wavefront reach 64 contiguous bytes of a row with every access.  Which product and row they come from:
+//   BY_HALF   MFMA row m of product e is column 32 (e / 2) + 8 (m / 4) + 4 (e % 2) + m % 4   (sixteen rows of B per load: four runs
+//             of four)
+//   BY_ROW    MFMA row m of product e is column permuted(m) + e                              (four columns of A per load)
+// out = base + acc, rounded once; the base is loaded ahead of the products.
+enum ColumnMap { BY_HALF, BY_ROW };
+__device__ __forceinline__ int permuted(int m) { return (m & 2) * 16 + (m >> 2) * 8 + (m & 1) * 4; }
+template <typename T, bool VEC, int MAP> struct BaseRow {
     uint4 v[2];
     __device__ __forceinline__ void load(const void *base, int64_t row, int first, int width) {
         const typename T::raw_t *p = static_cast<const typename T::raw_t *>(base) + row;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) v[h] = base != nullptr ? load8<T, VEC>(p, first + 8 * h, width) : make_uint4(0, 0, 0, 0);
+        for (int h = 0; h < 2; ++h) v[h] = base != nullptr ? load8<T, VEC>(p, first + 32 * h, width) : make_uint4(0, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float result(const f32x4 (&acc)[4], int h, int j) {
+        return MAP == BY_HALF ? acc[2 * h + j / 4][j & 3] : acc[j & 3][2 * h + j / 4];
     }
     __device__ __forceinline__ void store(typename T::raw_t *out, int first, int width, const f32x4 (&acc)[4]) const {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int c = first + 8 * h;
+            const int c = first + 32 * h;
             float b[8];
             T::unpack(v[h], b);
             uint32_t w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float v0 = b[2 * j] + acc[(2 * j) & 3][2 * h + (2 * j) / 4];
-                const float v1 = b[2 * j + 1] + acc[(2 * j + 1) & 3][2 * h + (2 * j) / 4];
+                const float v0 = b[2 * j] + result(acc, h, 2 * j), v1 = b[2 * j + 1] + result(acc, h, 2 * j + 1);
                 w[j] = uint32_t(narrow<T>(v0)) | uint32_t(narrow<T>(v1)) << 16;
             }
             if constexpr (VEC) {
@@ -341,6 +372,13 @@ template <typename T, bool VEC> struct BaseRow {
         }
     }
 };
+
+// A barrier that orders LDS only: loads in flight stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 
 // Where R <= 16 one product of 32 holds the high parts of u in its first half and the low ones in its second.
 template <int RP> struct Steps { static constexpr int kCount = RP <= 16 ? 1 : RP / 32; };
@@ -361,85 +399,99 @@ __device__ __forceinline__ float add_parts(float first, const float *__restrict_
 
 // ---------------------------------------------------------------------------
 // lora_shrink: u = s x A^T.  H is cut into segments of 1024; inside one the wavefronts take two of every eight steps of 32 and
-// are added in their order, and the segments are added in theirs: by one workgroup (grid (1, tiles)), or by lora_fold_rows
-// over one partial result per segment (grid (segments, tiles)) where the tiles alone would leave CUs idle.  The bits of a
-// token's u do not depend on which of the two runs, nor on the other tokens.
+// are added in their order, and the segments are added in theirs: by one workgroup (grid (1, tiles)), or by the reader of one
+// partial result per segment (grid (segments, tiles)) where the tiles alone would leave CUs idle.  The bits of a token's u
+// do not depend on which of the two runs, nor on the other tokens.
+// ONE: a call of few tokens, one per workgroup, which need no plan; one more workgroup makes it for the kernel behind.
 // ---------------------------------------------------------------------------
 constexpr int SEG_STEPS = 32;  // steps of 32 per segment
 struct ShrinkArgs {
     const void *x, *a;
     int64_t x_stride;
+    const int64_t *ids;
     const float *scaling;
     float scale;
-    int32_t n, h, r, segments, split;
+    int32_t n, h, r, s, segments, split;
     float *out;  // [N, R] scaled, or with `split` [segments, N, R]
     LoraPlan plan;
 };
-template <typename T, int RP, bool VEC>
+template <typename T, int RP, bool VEC, bool ONE>
 __global__ __launch_bounds__(THREADS) void lora_shrink(ShrinkArgs p) {
-    constexpr int RF = RP / 16;
-    __shared__ f32x4 part[WAVES][FWD_TILE][4];  // [wave][token][rank / 4] of one group of sixteen ranks
+    constexpr int RF = RP / 16, SUBS = ONE ? 1 : FWD_SUBS;
+    __shared__ union {
+        f32x4 part[WAVES][SUBS * 16][4];  // [wave][token][rank / 4] of one group of sixteen ranks
+        std::conditional_t<ONE, PlanShared<THREADS>, int> plan;
+    } sh;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
-    if (int(blockIdx.y) >= *p.plan.list[0].count) return;
-    const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];
+    LoraTile tile;
+    if constexpr (ONE) {
+        if (int(blockIdx.y) == p.n) {
+            if (blockIdx.x == 0) make_plan(sh.plan, p.ids, p.n, p.s, 1, p.plan);
+            return;
+        }
+        const int64_t id = p.ids[blockIdx.y];
+        tile.adapter = id >= 0 && id < p.s ? int(id) : -1;
+        tile.count = 1;
+    } else {
+        if (int(blockIdx.y) >= *p.plan.list[0].count) return;
+        tile = p.plan.list[0].tiles[blockIdx.y];
+    }
+    auto token_of = [&](int i) { return ONE ? int(blockIdx.y) : p.plan.order[tile.start + (i < tile.count ? i : 0)]; };
     const int mine = tid / 4, mine_q = tid & 3;  // the thread adds up four ranks of token `mine` of the tile
     f32x4 sum[RF];
 #pragma unroll
     for (int f = 0; f < RF; ++f) sum[f] = f32x4{0, 0, 0, 0};
     if (tile.adapter >= 0) {
-        const typename T::raw_t *rows[4];
+        const typename T::raw_t *rows[SUBS];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int i = s * 16 + col;
-            rows[s] = static_cast<const typename T::raw_t *>(p.x) + int64_t(p.plan.order[tile.start + (i < tile.count ? i : 0)]) * p.x_stride;
-        }
+        for (int s = 0; s < SUBS; ++s) rows[s] = static_cast<const typename T::raw_t *>(p.x) + int64_t(token_of(s * 16 + col)) * p.x_stride;
         const typename T::raw_t *aw = static_cast<const typename T::raw_t *>(p.a) + int64_t(tile.adapter) * p.r * p.h;
-        const int nsub = (tile.count + 15) / 16;
         const int steps = (p.h + 31) / 32;
         const int seg0 = p.split ? int(blockIdx.x) : 0, seg1 = p.split ? seg0 + 1 : p.segments;
         for (int seg = seg0; seg < seg1; ++seg) {
-            f32x4 acc[RF][4];
+            f32x4 acc[RF][SUBS];
 #pragma unroll
             for (int f = 0; f < RF; ++f)
 #pragma unroll
-                for (int s = 0; s < 4; ++s) acc[f][s] = f32x4{0, 0, 0, 0};
+                for (int s = 0; s < SUBS; ++s) acc[f][s] = f32x4{0, 0, 0, 0};
             const int end = (seg + 1) * SEG_STEPS < steps ? (seg + 1) * SEG_STEPS : steps;
             // a wavefront takes two neighbouring steps of every eight: whole 128-byte lines of the rows
+#pragma unroll(RP <= 32 ? 2 : 1)
             for (int st = seg * SEG_STEPS + 2 * wave; st < end; st += 2 * WAVES) {
-                uint4 fa[2][RF], fx[2][4];
+                uint4 fa[2][RF], fx[2][SUBS];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     const int k = (st + t) * 32 + 8 * quad;
 #pragma unroll
                     for (int f = 0; f < RF; ++f) fa[t][f] = load8_zero<T, VEC>(aw + int64_t(f * 16 + col < p.r ? f * 16 + col : 0) * p.h, k, p.h);
 #pragma unroll
-                    for (int s = 0; s < 4; ++s)
-                        if (s < nsub) fx[t][s] = load8<T, VEC>(rows[s], k, p.h);
+                    for (int s = 0; s < SUBS; ++s) fx[t][s] = load8<T, VEC>(rows[s], k, p.h);
                 }
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int f = 0; f < RF; ++f)
 #pragma unroll
-                        for (int s = 0; s < 4; ++s)
-                            if (s < nsub) acc[f][s] = mfma<T>(fa[t][f], fx[t][s], acc[f][s]);
+                        for (int s = 0; s < SUBS; ++s) acc[f][s] = mfma<T>(fa[t][f], fx[t][s], acc[f][s]);
             }
 #pragma unroll
             for (int f = 0; f < RF; ++f) {
                 __syncthreads();  // the previous parts are read
 #pragma unroll
-                for (int s = 0; s < 4; ++s) part[wave][s * 16 + col][quad] = acc[f][s];
+                for (int s = 0; s < SUBS; ++s) sh.part[wave][s * 16 + col][quad] = acc[f][s];
                 __syncthreads();
-                f32x4 v = part[0][mine][mine_q];
+                if (mine < SUBS * 16) {
+                    f32x4 v = sh.part[0][mine][mine_q];
 #pragma unroll
-                for (int w = 1; w < WAVES; ++w) v += part[w][mine][mine_q];
-                sum[f] += v;
+                    for (int w = 1; w < WAVES; ++w) v += sh.part[w][mine][mine_q];
+                    sum[f] += v;
+                }
             }
         }
     }
     if (mine >= tile.count) return;
     const float scale = tile.adapter < 0 ? 0.0f : (p.split ? 1.0f : (p.scaling != nullptr ? p.scaling[tile.adapter] : p.scale));
-    float *out = p.out + (p.split ? int64_t(blockIdx.x) * p.n * p.r : 0) + int64_t(p.plan.order[tile.start + mine]) * p.r;
+    float *out = p.out + (p.split ? int64_t(blockIdx.x) * p.n * p.r : 0) + int64_t(token_of(mine)) * p.r;
 #pragma unroll
     for (int f = 0; f < RF; ++f) {
         const int r0 = f * 16 + mine_q * 4;
@@ -462,92 +514,162 @@ __global__ __launch_bounds__(THREADS) void lora_fold_rows(const float *__restric
 }
 
 // ---------------------------------------------------------------------------
-// lora_expand: grid (blocks of O, tiles).  y = base + u B^T for the tokens of a tile.
+// lora_expand: grid (blocks of O, tiles).  y = base + u B^T for the tokens of a tile; what the next 64 outputs of a wavefront
+// need is requested before the products of the present ones.
 // ---------------------------------------------------------------------------
 struct ExpandArgs {
     const void *base, *b;
     void *out;
     int64_t base_stride, out_stride;
-    const float *u;
-    int32_t o, r, groups, in_place;  // groups: of 64 outputs per wavefront
+    const float *u;     // [N, R], or with PARTS [parts, N, R]: its segments before the scaling
+    float *out_shrunk;  // u, written by the first block of outputs of every tile (null: not wanted, or already there)
+    const float *scaling;
+    float scale;
+    int64_t n;
+    int32_t parts, o, r, groups, in_place;  // groups: of 64 outputs per wavefront
     LoraPlan plan;
 };
-template <typename T, int RP, bool VEC>
-__global__ __launch_bounds__(THREADS) void lora_expand(ExpandArgs p) {
-    constexpr int KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, NP = Parts<T>::kCount;
-    __shared__ uint4 uf[4][KS][HL][kWave];
+template <typename T, int RP, bool VEC, bool PARTS>
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 64 ? 4 : 2))) void lora_expand(ExpandArgs p) {
+    constexpr int KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2;
+    __shared__ uint4 uf[FWD_SUBS][KS][HL][kWave];
+    __shared__ float back[FWD_SUBS][16];  // fp16: the power of two that a token's u was divided by
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
+    const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];  // (in the list's memory also where there is no such tile)
     if (int(blockIdx.y) >= *p.plan.list[0].count) return;
-    const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];
-    if (tile.adapter < 0 && p.in_place) return;
-    const int nsub = (tile.count + 15) / 16;
-    const typename T::raw_t *base = static_cast<const typename T::raw_t *>(p.base);
-    typename T::raw_t *out = static_cast<typename T::raw_t *>(p.out);
-    {   // wavefront s prepares the fragments of group s: column = token
-        const int i = wave * 16 + col;
-        const bool live = i < tile.count && tile.adapter >= 0;
-        const float *row = p.u + int64_t(p.plan.order[tile.start + (i < tile.count ? i : 0)]) * p.r;
+    const bool shrunk_out = p.out_shrunk != nullptr && blockIdx.x == 0;
+    if (tile.adapter < 0 && p.in_place && !shrunk_out) return;
+    const bool two = tile.count > 16;
+    int token[FWD_SUBS];  // (a column without a token: the tile's first)
+    bool live[FWD_SUBS];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = row[r0 + j < p.r ? r0 + j : 0];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = live && r0 + j < p.r ? v[j] : 0.0f;
-            uint4 hl[2];
-            split<2>(v, hl);
-            if (RP <= 16) {
-                uf[wave][0][0][lane] = choose(quad < 2, hl[0], hl[1]);
-            } else {
-                uf[wave][ks][0][lane] = hl[0];
-                uf[wave][ks][HL - 1][lane] = hl[1];
-            }
-        }
+    for (int s = 0; s < FWD_SUBS; ++s) {
+        live[s] = s * 16 + col < tile.count;
+        token[s] = p.plan.order[tile.start + (live[s] ? s * 16 + col : 0)];
     }
-    __syncthreads();
     const typename T::raw_t *bw = static_cast<const typename T::raw_t *>(p.b) + int64_t(tile.adapter < 0 ? 0 : tile.adapter) * p.o * p.r;
-    int64_t token[4];
+    struct Stage {
+        BaseRow<T, VEC, BY_HALF> row[FWD_SUBS];
+        uint4 b[KS][4];
+    };
+    auto first_of = [&](int g) { return ((int(blockIdx.x) * p.groups + g) * WAVES + wave) * 64; };
+    auto request = [&](int g, Stage &st) {
+        const int o0 = first_of(g) < p.o ? first_of(g) : 0;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) token[s] = s * 16 + col < tile.count ? p.plan.order[tile.start + s * 16 + col] : -1;
-    const int64_t any = p.plan.order[tile.start];
-    for (int g = 0; g < p.groups; ++g) {
-        const int o0 = ((int(blockIdx.x) * p.groups + g) * WAVES + wave) * 64;
-        if (o0 >= p.o) break;
-        BaseRow<T, VEC> row[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-            if (s < nsub) row[s].load(base, (token[s] < 0 ? any : token[s]) * p.base_stride, o0 + 16 * quad, p.o);
-        uint4 fb[KS][4][NP];
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int o = o0 + 4 * col + e;
-                const uint4 f = load8<T, VEC>(bw + int64_t(o < p.o ? o : 0) * p.r, r0, p.r);
-                as_bf16<T>(f, fb[ks][e]);
+                const int o = o0 + 32 * (e / 2) + 8 * (col / 4) + 4 * (e & 1) + (col & 3);
+                st.b[ks][e] = load8<T, VEC>(bw + int64_t(o < p.o ? o : 0) * p.r, RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad, p.r);
             }
-        }
+        st.row[0].load(p.base, token[0] * p.base_stride, o0 + 8 * quad, p.o);
+        if (two) st.row[1].load(p.base, token[1] * p.base_stride, o0 + 8 * quad, p.o);
+    };
+    Stage even, odd;
+    request(0, even);
+    // u of the tile's tokens as fragments: column = token, contraction index = rank.  In B's own type: bf16 has fp32's range, for
+    // fp16 a token's u is brought to [1, 2) by a power of two, and its products back by it.  High + low then hold 17 (bf16)
+    // or 22 (fp16) bits.
+    const float scale = tile.adapter < 0 ? 0.0f : (p.scaling != nullptr ? p.scaling[tile.adapter] : p.scale);
+    for (int q = wave; q < FWD_SUBS * KS; q += WAVES) {
+        const int s = q % FWD_SUBS, ks = q / FWD_SUBS;
+        const bool mine = (s == 0 ? live[0] : live[1]) && tile.adapter >= 0;
+        const int64_t row = int64_t(s == 0 ? token[0] : token[1]) * p.r;
+        auto load_u = [&](int r0, float (&v)[8]) {
+            if constexpr (!PARTS) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if (s < nsub) {
-                f32x4 acc[4];
+                for (int j = 0; j < 8; ++j) v[j] = p.u[row + (r0 + j < p.r ? r0 + j : 0)];
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[e] = f32x4{0, 0, 0, 0};
+                for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+                for (int part = 0; part < p.parts; part += 4) {
+                    float x[4][8];
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
+                    for (int t = 0; t < 4; ++t) {
+                        const float *at = p.u + (part + t < p.parts ? part + t : part) * p.n * p.r + row;
 #pragma unroll
-                    for (int hl = 0; hl < HL; ++hl) {
-                        const uint4 fu = uf[s][ks][hl][lane];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int q = 0; q < NP; ++q) acc[e] = mfma<Bf16>(fb[ks][e][q], fu, acc[e]);
+                        for (int j = 0; j < 8; ++j) x[t][j] = at[r0 + j < p.r ? r0 + j : 0];
                     }
-                if (token[s] >= 0) row[s].store(out + token[s] * p.out_stride, o0 + 16 * quad, p.o, acc);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        if (part + t < p.parts) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[j] += x[t][j];
+                        }
+                }
             }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = mine && r0 + j < p.r ? (PARTS ? v[j] * scale : v[j]) : 0.0f;
+        };
+        const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
+        float own[8];
+        load_u(r0, own);
+        if (shrunk_out && (s == 0 ? live[0] : live[1]) && (RP > 16 || quad < 2)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (r0 + j < p.r) p.out_shrunk[row + r0 + j] = own[j];
         }
+        uint4 hl[2];
+        if constexpr (T::kDtype == KA_DTYPE_F16) {
+            float big = 0.0f;  // the largest of the token's whole row
+#pragma unroll 1
+            for (int k = 0; k < KS; ++k) {
+                float v[8];
+                load_u(RP <= 16 ? r0 : 32 * k + 8 * quad, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(v[j]));
+            }
+            big = fmaxf(big, __shfl_xor(big, 16, kWave));
+            big = fmaxf(big, __shfl_xor(big, 32, kWave));
+            const uint32_t exponent = __float_as_uint(big) & 0x7f800000u;
+            const bool plain = exponent == 0u || exponent >= 0x7e000000u;  // nothing to bring to range, or infinite
+            const float up = plain ? 1.0f : __uint_as_float(exponent), down = plain ? 1.0f : __uint_as_float(0x7f000000u - exponent);
+            split_f16(own, down, hl);
+            if (ks == 0 && quad == 0) back[s][col] = up;
+        } else {
+            split<2>(own, hl);
+        }
+        if (RP <= 16) {
+            uf[s][0][0][lane] = choose(quad < 2, hl[0], hl[1]);
+        } else {
+            uf[s][ks][0][lane] = hl[0];
+            uf[s][ks][HL - 1][lane] = hl[1];
+        }
+    }
+    lds_barrier();
+    if (tile.adapter < 0 && p.in_place) return;
+    typename T::raw_t *out = static_cast<typename T::raw_t *>(p.out);
+    float up[FWD_SUBS];
+#pragma unroll
+    for (int s = 0; s < FWD_SUBS; ++s) up[s] = T::kDtype == KA_DTYPE_F16 ? back[s][col] : 1.0f;
+    auto step = [&](int g, const Stage &st, Stage &next) {
+        if (g + 1 < p.groups) request(g + 1, next);
+        const int o0 = first_of(g);
+        if (o0 >= p.o) return;
+#pragma unroll
+        for (int s = 0; s < FWD_SUBS; ++s) {
+            if (s == 1 && !two) continue;
+            f32x4 acc[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int hl = 0; hl < HL; ++hl) {
+                    const uint4 fu = uf[s][ks][hl][lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[e] = mfma<T>(st.b[ks][e], fu, acc[e]);
+                }
+            if constexpr (T::kDtype == KA_DTYPE_F16) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] *= up[s];
+            }
+            if (live[s]) st.row[s].store(out + token[s] * p.out_stride, o0 + 8 * quad, p.o, acc);
+        }
+    };
+    for (int g = 0; g < p.groups; g += 2) {
+        step(g, even, odd);
+        if (g + 1 < p.groups) step(g + 1, odd, even);
     }
 }
 
@@ -655,13 +777,6 @@ template <typename T> __device__ __forceinline__ f32x4 outer(const uint4 (&data)
     acc = mfma<Bf16>(data[0], v[1], acc);
     return mfma<Bf16>(data[0], v[0], acc);
 }
-// A barrier that orders LDS only: loads in flight stay in flight.
-__device__ __forceinline__ void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 template <typename T, int RP, int G, int MODE>
 __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
     constexpr int RF = RP / 16, NP = Parts<T>::kCount;
@@ -827,9 +942,9 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
     if (h0 >= p.h) return;  // (no barrier follows)
     const bool has = tile.adapter >= 0;
     const typename T::raw_t *aw = static_cast<const typename T::raw_t *>(p.a) + (has ? int64_t(tile.adapter) * p.r * p.h : 0);
-    const int col4 = lane_column<MODE>(h0 + 4 * col, p.h), out_col = h0 + 16 * quad;
+    const int col4 = lane_column<MODE>(h0 + permuted(col), p.h), out_col = h0 + 8 * quad;
     const uint4 *const packed = p.du + int64_t(tile.start / 32 + (has ? tile.adapter : 0)) * (Packed<RP>::kColumns + Packed<RP>::kRows) + lane;
-    // A fragments: row 4 m + e = input, contraction index = rank
+    // A fragments: row permuted(m) + e = input, contraction index = rank
     uint4 fa[KS][4][NP];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -837,7 +952,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int rank = (RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad) + j;
-            w[j] = load4<T, VEC>(aw + int64_t(rank < p.r ? rank : 0) * p.h, h0 + 4 * col, p.h);
+            w[j] = load4<T, VEC>(aw + int64_t(rank < p.r ? rank : 0) * p.h, h0 + permuted(col), p.h);
         }
         uint4 frag[4];
         transpose(w, frag);
@@ -857,7 +972,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
     };
     auto step = [&](int c, const uint2 (&w)[8], uint2 (&next)[8]) {
         const uint4 *pu = packed + int64_t(c / 32) * (Packed<RP>::kColumns + Packed<RP>::kRows);
-        BaseRow<T, VEC> base[2];
+        BaseRow<T, VEC, BY_ROW> base[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
             base[s].load(p.dx_base, p.dx_base == nullptr ? 0 : int64_t(tokens[c + 16 * s + col]) * p.dx_base_stride, out_col, p.h);
@@ -915,7 +1030,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
         if (rank >= p.r) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int h = h0 + 16 * quad + 4 * i;
+            const int h = h0 + permuted(4 * quad + i);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (h + e < p.h) da[int64_t(rank) * p.h + h + e] = acc[f][e][i];
@@ -1096,36 +1211,47 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     const LoraPlan plan = plan_at(ws, l.plan);
-    hipLaunchKernelGGL(lora_plan, dim3(1), dim3(PLAN_THREADS), 0, stream, adapter_ids, int(n_tokens), int(n_adapters), 1, plan);
-    rc = check_hip(hipGetLastError(), "lora launch (plan)");
-    if (rc != KA_OK) return rc;
+    // one workgroup per token and segment, and the plan made by one more: up to 2 MB of A per 16 KB of x, all from L2
+    const bool one = n_tokens * rank <= 2048 && n_tokens <= 256;
+    if (!one) {
+        hipLaunchKernelGGL(lora_plan, dim3(1), dim3(PLAN_THREADS), 0, stream, adapter_ids, int(n_tokens), int(n_adapters), 1, plan);
+        rc = check_hip(hipGetLastError(), "lora launch (plan)");
+        if (rc != KA_OK) return rc;
+    }
+    // u whole, or its segments for lora_expand to add
     float *u = out_shrunk != nullptr ? out_shrunk : reinterpret_cast<float *>(ws + l.u);
+    float *parts = reinterpret_cast<float *>(ws + l.part);
     ShrinkArgs sa{};
     sa.x = hidden;
     sa.a = lora_a;
     sa.x_stride = hidden_stride;
+    sa.ids = adapter_ids;
     sa.scaling = scaling;
     sa.scale = scale;
     sa.n = int32_t(n_tokens);
     sa.h = int32_t(in_dim);
     sa.r = int32_t(rank);
+    sa.s = int32_t(n_adapters);
     sa.segments = int32_t(l.segments);
     sa.split = l.split ? 1 : 0;
-    sa.out = l.split ? reinterpret_cast<float *>(ws + l.part) : u;
+    sa.out = l.split ? parts : u;
     sa.plan = plan;
     const int rp = padded_rank(rank);
-    const dim3 shrink_grid{unsigned(l.split ? l.segments : 1), unsigned(l.plan.max_tiles[0])};
+    const dim3 shrink_grid{unsigned(l.split ? l.segments : 1), unsigned(one ? n_tokens + 1 : l.plan.max_tiles[0])};
     with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
         using T = decltype(type);
         constexpr int RP = decltype(rank_c)::value;
         constexpr bool VEC = decltype(vec_c)::value;
-        hipLaunchKernelGGL((lora_shrink<T, RP, VEC>), shrink_grid, dim3(THREADS), 0, stream, sa);
+        if (one) hipLaunchKernelGGL((lora_shrink<T, RP, VEC, true>), shrink_grid, dim3(THREADS), 0, stream, sa);
+        else hipLaunchKernelGGL((lora_shrink<T, RP, VEC, false>), shrink_grid, dim3(THREADS), 0, stream, sa);
     });
     rc = check_hip(hipGetLastError(), "lora launch (shrink)");
     if (rc != KA_OK) return rc;
-    if (l.split) {
+    // (a call of few tokens saves the launch: its segments are added by the few workgroups that read them)
+    const bool parted = l.split && one && out != nullptr;
+    if (l.split && !parted) {
         hipLaunchKernelGGL(lora_fold_rows, dim3(unsigned(ceil_div(n_tokens * rank, THREADS))), dim3(THREADS), 0, stream,
-                           reinterpret_cast<const float *>(ws + l.part), int(l.segments), n_tokens, int(rank), adapter_ids, int(n_adapters), scaling, scale, u);
+                           parts, int(l.segments), n_tokens, int(rank), adapter_ids, int(n_adapters), scaling, scale, u);
         rc = check_hip(hipGetLastError(), "lora launch (fold)");
         if (rc != KA_OK) return rc;
     }
@@ -1136,7 +1262,12 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     ea.out = out;
     ea.base_stride = base_stride;
     ea.out_stride = out_stride;
-    ea.u = u;
+    ea.u = parted ? parts : u;
+    ea.out_shrunk = parted ? out_shrunk : nullptr;
+    ea.scaling = scaling;
+    ea.scale = scale;
+    ea.n = n_tokens;
+    ea.parts = int32_t(l.segments);
     ea.o = int32_t(out_dim);
     ea.r = int32_t(rank);
     ea.in_place = out == base && out_stride == base_stride ? 1 : 0;
@@ -1151,7 +1282,8 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
         using T = decltype(type);
         constexpr int RP = decltype(rank_c)::value;
         constexpr bool VEC = decltype(vec_c)::value;
-        hipLaunchKernelGGL((lora_expand<T, RP, VEC>), expand_grid, dim3(THREADS), 0, stream, ea);
+        if (parted) hipLaunchKernelGGL((lora_expand<T, RP, VEC, true>), expand_grid, dim3(THREADS), 0, stream, ea);
+        else hipLaunchKernelGGL((lora_expand<T, RP, VEC, false>), expand_grid, dim3(THREADS), 0, stream, ea);
     });
     return check_hip(hipGetLastError(), "lora launch (expand)");
 }
