@@ -160,8 +160,26 @@ __device__ __forceinline__ void make_plan(PlanShared<PLAN_THREADS> &sh, const in
     }
     if (tid < lists) *plan.list[tid].count = total[tid];
     __syncthreads();
+    // up to 64 groups: lane l keeps the next position of group l in a register
+    const bool in_lanes = s + 1 <= kWave;
+    int next = in_lanes && lane <= s ? at[wave][lane] : 0;
     for (int st = s0; st < s1; st += U) {
         if (per > U) load(st);
+        if (in_lanes) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                uint64_t left = __ballot(a[u] >= 0);
+                while (left != 0) {  // one turn per adapter that occurs in the step
+                    const int want = __builtin_amdgcn_readlane(a[u], __ffsll((long long)left) - 1);
+                    const uint64_t same = __ballot(a[u] == want);
+                    const int base = __builtin_amdgcn_readlane(next, want);
+                    if (a[u] == want) plan.order[base + __popcll(same & ((uint64_t(1) << lane) - 1))] = (st + u) * kWave + lane;
+                    next += lane == want ? __popcll(same) : 0;
+                    left &= ~same;
+                }
+            }
+            continue;
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             uint64_t left = __ballot(a[u] >= 0);
@@ -514,15 +532,95 @@ __global__ __launch_bounds__(THREADS) void lora_fold_rows(const float *__restric
 }
 
 // ---------------------------------------------------------------------------
-// lora_expand: grid (blocks of O, tiles).  y = base + u B^T for the tokens of a tile; what the next 64 outputs of a wavefront
-// need is requested before the products of the present ones.
+// lora_expand: grid (blocks of O, tiles).  y = base + u B^T for the tokens of a tile.
+//
+// u enters as fragments (column = token, contraction index = rank) in B's own type: bf16 has fp32's range, for fp16 a token's u is
+// brought to [1, 2) by a power of two, and its products back by it.  High + low parts then hold 17 (bf16) or 22 (fp16)
+// bits.  They come packed from lora_pack_rows, or in calls of few tokens (PARTS) from the segments of lora_shrink.
 // ---------------------------------------------------------------------------
+template <int RP> struct RowFragments {  // of 32 tokens, in uint4: [group of 16][step][high, low][lane], then 32 powers of two
+    static constexpr int kSteps = Steps<RP>::kCount, kParts = RP <= 16 ? 1 : 2;
+    static constexpr int kFragments = FWD_SUBS * kSteps * kParts * kWave;
+    static constexpr int kTotal = kFragments + 8;
+};
+// The fragment of group s, step ks (both parts) from eight values of u a lane, and the token's power of two (1 for bf16).
+// `big`: the largest |u| of the token.
+template <typename T, int RP>
+__device__ __forceinline__ float row_fragment(const float (&v)[8], float big, uint4 *out, int lane) {
+    uint4 hl[2];
+    float up = 1.0f;
+    if constexpr (T::kDtype == KA_DTYPE_F16) {
+        const uint32_t exponent = __float_as_uint(big) & 0x7f800000u;
+        const bool plain = exponent == 0u || exponent >= 0x7e000000u;  // nothing to bring to range, or infinite
+        up = plain ? 1.0f : __uint_as_float(exponent);
+        split_f16(v, plain ? 1.0f : __uint_as_float(0x7f000000u - exponent), hl);
+    } else {
+        split<2>(v, hl);
+    }
+    if (RP <= 16) {
+        out[lane] = choose((lane >> 4) < 2, hl[0], hl[1]);
+    } else {
+        out[lane] = hl[0];
+        out[kWave + lane] = hl[1];
+    }
+    return up;
+}
+
+// grid (tiles): u of a tile's tokens from `parts` segments, added in order and scaled; also to out_shrunk.
+struct PackRowsArgs {
+    const float *part;
+    float *out_shrunk;  // may be null
+    const float *scaling;
+    float scale;
+    int32_t parts, scaled, r;
+    int64_t n;
+    uint4 *out;
+    LoraPlan plan;
+};
+template <typename T, int RP>
+__global__ __launch_bounds__(THREADS) void lora_pack_rows(PackRowsArgs p) {
+    constexpr int KS = Steps<RP>::kCount, LD = RP + 1;
+    __shared__ float v[FWD_TILE * LD];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
+    const LoraTile tile = p.plan.list[0].tiles[blockIdx.x];
+    if (int(blockIdx.x) >= *p.plan.list[0].count) return;
+    const float scale = tile.adapter < 0 ? 0.0f : (p.scaling != nullptr ? p.scaling[tile.adapter] : p.scale);
+    for (int i = tid; i < FWD_TILE * RP; i += THREADS) {
+        const int t = i / RP, rank = i % RP;
+        float x = 0.0f;
+        if (t < tile.count && rank < p.r) {
+            const int64_t at = int64_t(p.plan.order[tile.start + t]) * p.r + rank;
+            if (tile.adapter >= 0) {
+                x = add_parts(0.0f, p.part + at, p.parts, p.n * p.r);
+                if (p.scaled) x *= scale;
+            }
+            if (p.out_shrunk != nullptr) p.out_shrunk[at] = x;
+        }
+        v[t * LD + rank] = x;
+    }
+    __syncthreads();
+    uint4 *out = p.out + int64_t(blockIdx.x) * RowFragments<RP>::kTotal;
+    for (int q = wave; q < FWD_SUBS * KS; q += WAVES) {
+        const int s = q / KS, ks = q % KS;
+        const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
+        const float *row = v + (16 * s + col) * LD;
+        float x[8], big = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = row[r0 + j];
+        if (T::kDtype == KA_DTYPE_F16)
+            for (int j = 0; j < RP; ++j) big = fmaxf(big, fabsf(row[j]));
+        const float up = row_fragment<T, RP>(x, big, out + q * RowFragments<RP>::kParts * kWave, lane);
+        if (ks == 0 && quad == 0) reinterpret_cast<float *>(out + RowFragments<RP>::kFragments)[s * 16 + col] = up;
+    }
+}
+
 struct ExpandArgs {
     const void *base, *b;
     void *out;
     int64_t base_stride, out_stride;
-    const float *u;     // [N, R], or with PARTS [parts, N, R]: its segments before the scaling
-    float *out_shrunk;  // u, written by the first block of outputs of every tile (null: not wanted, or already there)
+    const uint4 *packed;  // RowFragments per tile
+    const float *u;       // PARTS: [parts, N, R], the segments before the scaling
+    float *out_shrunk;    // PARTS: u, written by the first block of outputs of every tile; may be null
     const float *scaling;
     float scale;
     int64_t n;
@@ -530,14 +628,14 @@ struct ExpandArgs {
     LoraPlan plan;
 };
 template <typename T, int RP, bool VEC, bool PARTS>
-__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 64 ? 4 : 2))) void lora_expand(ExpandArgs p) {
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 32 ? 4 : 2))) void lora_expand(ExpandArgs p) {
     constexpr int KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2;
-    __shared__ uint4 uf[FWD_SUBS][KS][HL][kWave];
-    __shared__ float back[FWD_SUBS][16];  // fp16: the power of two that a token's u was divided by
+    __shared__ uint4 uf[PARTS ? FWD_SUBS * KS * HL * kWave : 1];
+    __shared__ float back[FWD_SUBS][16];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
     const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];  // (in the list's memory also where there is no such tile)
     if (int(blockIdx.y) >= *p.plan.list[0].count) return;
-    const bool shrunk_out = p.out_shrunk != nullptr && blockIdx.x == 0;
+    const bool shrunk_out = PARTS && p.out_shrunk != nullptr && blockIdx.x == 0;
     if (tile.adapter < 0 && p.in_place && !shrunk_out) return;
     const bool two = tile.count > 16;
     int token[FWD_SUBS];  // (a column without a token: the tile's first)
@@ -565,21 +663,27 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 6
         st.row[0].load(p.base, token[0] * p.base_stride, o0 + 8 * quad, p.o);
         if (two) st.row[1].load(p.base, token[1] * p.base_stride, o0 + 8 * quad, p.o);
     };
-    Stage even, odd;
+    Stage even;
     request(0, even);
-    // u of the tile's tokens as fragments: column = token, contraction index = rank.  In B's own type: bf16 has fp32's range, for
-    // fp16 a token's u is brought to [1, 2) by a power of two, and its products back by it.  High + low then hold 17 (bf16)
-    // or 22 (fp16) bits.
-    const float scale = tile.adapter < 0 ? 0.0f : (p.scaling != nullptr ? p.scaling[tile.adapter] : p.scale);
-    for (int q = wave; q < FWD_SUBS * KS; q += WAVES) {
-        const int s = q % FWD_SUBS, ks = q / FWD_SUBS;
-        const bool mine = (s == 0 ? live[0] : live[1]) && tile.adapter >= 0;
-        const int64_t row = int64_t(s == 0 ? token[0] : token[1]) * p.r;
-        auto load_u = [&](int r0, float (&v)[8]) {
-            if constexpr (!PARTS) {
+    uint4 fu[PARTS ? 1 : FWD_SUBS][KS][HL];
+    float up[FWD_SUBS];
+    if constexpr (!PARTS) {
+        const uint4 *packed = p.packed + int64_t(blockIdx.y) * RowFragments<RP>::kTotal;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = p.u[row + (r0 + j < p.r ? r0 + j : 0)];
-            } else {
+        for (int s = 0; s < FWD_SUBS; ++s) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int k = 0; k < HL; ++k) fu[s][ks][k] = packed[((s * KS + ks) * HL + k) * kWave + lane];
+            up[s] = T::kDtype == KA_DTYPE_F16 ? reinterpret_cast<const float *>(packed + RowFragments<RP>::kFragments)[s * 16 + col] : 1.0f;
+        }
+    } else {
+        const float scale = tile.adapter < 0 ? 0.0f : (p.scaling != nullptr ? p.scaling[tile.adapter] : p.scale);
+        for (int q = wave; q < FWD_SUBS * KS; q += WAVES) {
+            const int s = q % FWD_SUBS, ks = q / FWD_SUBS;
+            const bool mine = (s == 0 ? live[0] : live[1]) && tile.adapter >= 0;
+            const int64_t row = int64_t(s == 0 ? token[0] : token[1]) * p.r;
+            auto load_u = [&](int r0, float (&v)[8]) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = 0.0f;
                 for (int part = 0; part < p.parts; part += 4) {
@@ -597,53 +701,37 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 6
                             for (int j = 0; j < 8; ++j) v[j] += x[t][j];
                         }
                 }
-            }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = mine && r0 + j < p.r ? (PARTS ? v[j] * scale : v[j]) : 0.0f;
-        };
-        const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
-        float own[8];
-        load_u(r0, own);
-        if (shrunk_out && (s == 0 ? live[0] : live[1]) && (RP > 16 || quad < 2)) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (r0 + j < p.r) p.out_shrunk[row + r0 + j] = own[j];
-        }
-        uint4 hl[2];
-        if constexpr (T::kDtype == KA_DTYPE_F16) {
-            float big = 0.0f;  // the largest of the token's whole row
+                for (int j = 0; j < 8; ++j) v[j] = mine && r0 + j < p.r ? v[j] * scale : 0.0f;
+            };
+            const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
+            float own[8], big = 0.0f;
+            if constexpr (T::kDtype == KA_DTYPE_F16) {  // the largest of the token's whole row
 #pragma unroll 1
-            for (int k = 0; k < KS; ++k) {
-                float v[8];
-                load_u(RP <= 16 ? r0 : 32 * k + 8 * quad, v);
+                for (int k = 0; k < KS; ++k) {
+                    load_u(RP <= 16 ? r0 : 32 * k + 8 * quad, own);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(v[j]));
+                    for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(own[j]));
+                }
+                big = fmaxf(big, __shfl_xor(big, 16, kWave));
+                big = fmaxf(big, __shfl_xor(big, 32, kWave));
             }
-            big = fmaxf(big, __shfl_xor(big, 16, kWave));
-            big = fmaxf(big, __shfl_xor(big, 32, kWave));
-            const uint32_t exponent = __float_as_uint(big) & 0x7f800000u;
-            const bool plain = exponent == 0u || exponent >= 0x7e000000u;  // nothing to bring to range, or infinite
-            const float up = plain ? 1.0f : __uint_as_float(exponent), down = plain ? 1.0f : __uint_as_float(0x7f000000u - exponent);
-            split_f16(own, down, hl);
-            if (ks == 0 && quad == 0) back[s][col] = up;
-        } else {
-            split<2>(own, hl);
+            load_u(r0, own);
+            if (shrunk_out && (s == 0 ? live[0] : live[1]) && (RP > 16 || quad < 2)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (r0 + j < p.r) p.out_shrunk[row + r0 + j] = own[j];
+            }
+            const float power = row_fragment<T, RP>(own, big, uf + (s * KS + ks) * HL * kWave, lane);
+            if (ks == 0 && quad == 0) back[s][col] = power;
         }
-        if (RP <= 16) {
-            uf[s][0][0][lane] = choose(quad < 2, hl[0], hl[1]);
-        } else {
-            uf[s][ks][0][lane] = hl[0];
-            uf[s][ks][HL - 1][lane] = hl[1];
-        }
+        lds_barrier();
+#pragma unroll
+        for (int s = 0; s < FWD_SUBS; ++s) up[s] = T::kDtype == KA_DTYPE_F16 ? back[s][col] : 1.0f;
     }
-    lds_barrier();
     if (tile.adapter < 0 && p.in_place) return;
     typename T::raw_t *out = static_cast<typename T::raw_t *>(p.out);
-    float up[FWD_SUBS];
-#pragma unroll
-    for (int s = 0; s < FWD_SUBS; ++s) up[s] = T::kDtype == KA_DTYPE_F16 ? back[s][col] : 1.0f;
-    auto step = [&](int g, const Stage &st, Stage &next) {
-        if (g + 1 < p.groups) request(g + 1, next);
+    auto finish = [&](int g, const Stage &st) {
         const int o0 = first_of(g);
         if (o0 >= p.o) return;
 #pragma unroll
@@ -655,10 +743,12 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 6
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int hl = 0; hl < HL; ++hl) {
-                    const uint4 fu = uf[s][ks][hl][lane];
+                for (int k = 0; k < HL; ++k) {
+                    uint4 f;
+                    if constexpr (PARTS) f = uf[((s * KS + ks) * HL + k) * kWave + lane];
+                    else f = fu[s][ks][k];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[e] = mfma<T>(st.b[ks][e], fu, acc[e]);
+                    for (int e = 0; e < 4; ++e) acc[e] = mfma<T>(st.b[ks][e], f, acc[e]);
                 }
             if constexpr (T::kDtype == KA_DTYPE_F16) {
 #pragma unroll
@@ -667,9 +757,22 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 6
             if (live[s]) st.row[s].store(out + token[s] * p.out_stride, o0 + 8 * quad, p.o, acc);
         }
     };
-    for (int g = 0; g < p.groups; g += 2) {
-        step(g, even, odd);
-        if (g + 1 < p.groups) step(g + 1, odd, even);
+    if constexpr (RP <= 32) {
+        // what the next 64 outputs need is requested before the products of the present ones
+        Stage odd;
+        for (int g = 0; g < p.groups; g += 2) {
+            if (g + 1 < p.groups) request(g + 1, odd);
+            finish(g, even);
+            if (g + 1 < p.groups) {
+                if (g + 2 < p.groups) request(g + 2, even);
+                finish(g + 1, odd);
+            }
+        }
+    } else {  // (two stages of B would take the registers of half the wavefronts)
+        for (int g = 0; g < p.groups; ++g) {
+            if (g > 0) request(g, even);
+            finish(g, even);
+        }
     }
 }
 
@@ -1108,7 +1211,7 @@ inline LoraPlan plan_at(unsigned char *ws, const PlanLayout &l) {
     return p;
 }
 
-struct FwdLayout { PlanLayout plan; int64_t segments; bool split; size_t part, u, total; };
+struct FwdLayout { PlanLayout plan; int64_t segments; bool split; size_t part, u, packed, total; };
 inline FwdLayout fwd_layout(const Shape &d) {
     FwdLayout l;
     l.plan = plan_layout(d.n, d.s, FWD_TILE, 0);
@@ -1116,7 +1219,10 @@ inline FwdLayout fwd_layout(const Shape &d) {
     l.split = l.segments > 1 && l.plan.max_tiles[0] < 256;
     l.part = l.plan.total;
     l.u = l.part + (l.split ? align_up(size_t(l.segments) * d.n * d.r * 4) : 0);
-    l.total = l.u + align_up(size_t(d.n) * d.r * 4);
+    l.packed = l.u + align_up(size_t(d.n) * d.r * 4);
+    const int64_t rp = padded_rank(d.r);
+    l.total = l.packed + size_t(l.plan.max_tiles[0]) * (rp == 16 ? RowFragments<16>::kTotal : rp == 32 ? RowFragments<32>::kTotal
+                                                        : rp == 64 ? RowFragments<64>::kTotal : RowFragments<128>::kTotal) * sizeof(uint4);
     return l;
 }
 
@@ -1247,12 +1353,33 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     });
     rc = check_hip(hipGetLastError(), "lora launch (shrink)");
     if (rc != KA_OK) return rc;
-    // (a call of few tokens saves the launch: its segments are added by the few workgroups that read them)
+    // (a call of few tokens saves a launch: its segments are added by the few workgroups that read them)
     const bool parted = l.split && one && out != nullptr;
-    if (l.split && !parted) {
+    if (l.split && out == nullptr) {
         hipLaunchKernelGGL(lora_fold_rows, dim3(unsigned(ceil_div(n_tokens * rank, THREADS))), dim3(THREADS), 0, stream,
                            parts, int(l.segments), n_tokens, int(rank), adapter_ids, int(n_adapters), scaling, scale, u);
         rc = check_hip(hipGetLastError(), "lora launch (fold)");
+        if (rc != KA_OK) return rc;
+    }
+    uint4 *packed = reinterpret_cast<uint4 *>(ws + l.packed);
+    if (out != nullptr && !parted) {
+        PackRowsArgs pa{};
+        pa.part = l.split ? parts : u;
+        pa.out_shrunk = l.split ? out_shrunk : nullptr;
+        pa.scaling = scaling;
+        pa.scale = scale;
+        pa.parts = l.split ? int32_t(l.segments) : 1;
+        pa.scaled = l.split ? 1 : 0;
+        pa.r = int32_t(rank);
+        pa.n = n_tokens;
+        pa.out = packed;
+        pa.plan = plan;
+        with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto) {
+            using T = decltype(type);
+            constexpr int RP = decltype(rank_c)::value;
+            hipLaunchKernelGGL((lora_pack_rows<T, RP>), dim3(unsigned(l.plan.max_tiles[0])), dim3(THREADS), 0, stream, pa);
+        });
+        rc = check_hip(hipGetLastError(), "lora launch (pack)");
         if (rc != KA_OK) return rc;
     }
     if (out == nullptr) return KA_OK;
@@ -1262,8 +1389,9 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     ea.out = out;
     ea.base_stride = base_stride;
     ea.out_stride = out_stride;
-    ea.u = parted ? parts : u;
-    ea.out_shrunk = parted ? out_shrunk : nullptr;
+    ea.packed = packed;
+    ea.u = parts;
+    ea.out_shrunk = out_shrunk;
     ea.scaling = scaling;
     ea.scale = scale;
     ea.n = n_tokens;
