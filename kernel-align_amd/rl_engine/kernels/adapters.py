@@ -39,7 +39,8 @@ class AdapterOps:
             with self._workspace(nbytes, device) as ptr:
                 yield ptr
             return
-        yield torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr()
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)  # held until the launches are enqueued
+        yield scratch.data_ptr()
 
     def _check_adapters(self, hidden, lora_a, lora_b, adapter_ids, scaling):
         """Shapes of one call: (hidden rows, A, B, ids, scaling tensor or None, scaling number)."""

@@ -28,6 +28,8 @@ class OpBackend(Enum, metaclass=_OpEnumMeta):
     HIP_LOGPROB = "rl_engine.kernels.sampling.SamplerBackend.compute_logp"
     HIP_FUSED_LMHEAD_LOGPROB = "rl_engine.kernels.sampling.SamplerBackend.fused_linear_logp"
     HIP_SAMPLING = "rl_engine.kernels.sampling.SamplerBackend.sample"
+    HIP_VERIFY_DRAFT = "rl_engine.kernels.sampling.SamplerBackend.verify_draft"
+    HIP_LORA_LINEAR = "rl_engine.kernels.sampling.SamplerBackend.lora_linear"
     # Operators the reference's callers ask for by name (e.g. "attention", rollout.py:23) that lie outside the
     # HIP hot path: dispatch() still answers with a name, as registry.py:41-55 always does; resolve() refuses.
     NOT_ON_HIP_PATH = "rl_engine.kernels.registry.not_on_hip_path"
@@ -41,12 +43,16 @@ class KernelRegistry:
 
     def dispatch(self, op_type: str) -> str:
         """Name of the backend serving `op_type` (substring match, as in registry.py:41-55)."""
+        if "lora" in op_type or "adapter" in op_type:
+            return OpBackend.HIP_LORA_LINEAR.name
         if "lm_head" in op_type or "linear" in op_type:
             return OpBackend.HIP_FUSED_LMHEAD_LOGPROB.name
         if "logp" in op_type:
             return OpBackend.HIP_LOGPROB.name
         if "sampl" in op_type:
             return OpBackend.HIP_SAMPLING.name
+        if "verif" in op_type or "draft" in op_type:
+            return OpBackend.HIP_VERIFY_DRAFT.name
         return OpBackend.NOT_ON_HIP_PATH.name
 
     def get_op_path(self, backend: OpBackend) -> str:
@@ -56,7 +62,8 @@ class KernelRegistry:
         """The bound method that implements `op_type`, on a lazily built shared SamplerBackend."""
         backend = OpBackend[self.dispatch(op_type)]
         if backend is OpBackend.NOT_ON_HIP_PATH:
-            raise ValueError(f"no HIP operator serves '{op_type}' (known: logp, lm_head/linear, sampling)")
+            raise ValueError(f"no HIP operator serves '{op_type}' (known: logp, lm_head/linear, sampling, "
+                             "verify/draft, lora/adapter)")
         if self._sampler is None:
             from rl_engine.kernels.sampling import SamplerBackend
 
@@ -66,7 +73,8 @@ class KernelRegistry:
 
 def not_on_hip_path(*_args, **_kwargs):
     """Target of OpBackend.NOT_ON_HIP_PATH: there is no kernel behind the name."""
-    raise NotImplementedError("this operator is not part of the HIP hot path (logprob, lm_head logprob, sampling)")
+    raise NotImplementedError("this operator is not part of the HIP hot path (logprob, lm_head logprob, sampling, "
+                              "verification of drafts, adapters)")
 
 
 kernel_registry = KernelRegistry()
