@@ -276,10 +276,30 @@ template <typename T> __device__ __forceinline__ void as_bf16(const uint4 &f, ui
 // start of a row), so that all loads of a step are in flight together, and what it read meets a zero in the other operand or a
 // result that is not stored.  (An infinity read that way belongs to the same token or adapter.)
 //
-// Columns col .. col + 7 of a row of `width`; where they do not exist, its first columns.
-template <typename T, bool VEC> __device__ __forceinline__ uint4 load8(const typename T::raw_t *row, int col, int width) {
-    if constexpr (VEC) {  // width is a multiple of 8, the row 16-byte aligned
+// How a kernel reaches the rows of its matrices:
+//   ROWS_ALIGNED  16-byte vectors at 16-byte addresses, widths multiples of 8; the backward's kernels then step through the matrix they
+//                 stream with byte offsets of 32 bits (matrices below 4 GiB: one addition per load)
+//   ROWS_LOOSE    the same vectors at any address, the last one of a row moved back into it and shifted: odd widths, strides and
+//                 starting points (511 tokens, H 1327, O 32,000, rank 32: 147 us a call entry by entry, 48 us so)
+//   ROWS_SCALAR   entry by entry: rows of fewer than 8 entries
+enum RowMode { ROWS_SCALAR = 0, ROWS_LOOSE = 1, ROWS_ALIGNED = 2 };
+struct __attribute__((packed, aligned(2))) Loose16 { uint32_t w[4]; };
+struct __attribute__((packed, aligned(2))) Loose8 { uint32_t w[2]; };
+// The vector without its first d entries, 0 <= d < 8; zeros come in behind.
+__device__ __forceinline__ uint4 drop_entries(const Loose16 &v, int d) {
+    const uint64_t first = (uint64_t(v.w[1]) << 32) | v.w[0], second = (uint64_t(v.w[3]) << 32) | v.w[2];
+    const uint64_t lo = d & 4 ? second : first, hi = d & 4 ? 0 : second;
+    const int s = 16 * (d & 3);
+    const uint64_t l = (lo >> s) | ((hi << 1) << (63 - s)), h = hi >> s;
+    return make_uint4(uint32_t(l), uint32_t(l >> 32), uint32_t(h), uint32_t(h >> 32));
+}
+// Columns col .. col + 7 of a row of `width`; where they do not exist, other entries of the row, or zeros.
+template <typename T, int MODE> __device__ __forceinline__ uint4 load8(const typename T::raw_t *row, int col, int width) {
+    if constexpr (MODE == ROWS_ALIGNED) {
         return *reinterpret_cast<const uint4 *>(row + (col < width ? col : 0));
+    } else if constexpr (MODE == ROWS_LOOSE) {
+        const int c = col < width - 8 ? col : width - 8;
+        return drop_entries(*reinterpret_cast<const Loose16 *>(row + c), (col - c) & 7);
     } else {
         uint32_t e[8];
 #pragma unroll
@@ -287,20 +307,40 @@ template <typename T, bool VEC> __device__ __forceinline__ uint4 load8(const typ
         return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
     }
 }
-// The same with zeros behind the row.
-template <typename T, bool VEC> __device__ __forceinline__ uint4 load8_zero(const typename T::raw_t *row, int col, int width) {
-    const uint4 v = load8<T, VEC>(row, col, width);
-    const int n = width - col;
-    if constexpr (VEC) return n > 0 ? v : make_uint4(0, 0, 0, 0);
+// The first n entries of a vector, zeros behind them.
+__device__ __forceinline__ uint4 first_entries(const uint4 &v, int n) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t k[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) k[j] = w[j] & ((2 * j < n ? 0xffffu : 0u) | (2 * j + 1 < n ? 0xffff0000u : 0u));
     return make_uint4(k[0], k[1], k[2], k[3]);
 }
-template <typename T, bool VEC> __device__ __forceinline__ uint2 load4(const typename T::raw_t *row, int col, int width) {
-    if constexpr (VEC) {
+// load8 with zeros behind the row.
+template <typename T, int MODE> __device__ __forceinline__ uint4 load8_zero(const typename T::raw_t *row, int col, int width) {
+    const uint4 v = load8<T, MODE>(row, col, width);
+    if constexpr (MODE == ROWS_ALIGNED) return col < width ? v : make_uint4(0, 0, 0, 0);
+    else return first_entries(v, width - col);
+}
+// Columns col .. col + 7 of row `row` of a dense matrix [rows, width] of at least 8 entries, whose rows may be shorter than that;
+// what lies behind the row is zero, or the row's own.
+template <typename T, int MODE>
+__device__ __forceinline__ uint4 dense_load8(const typename T::raw_t *matrix, int row, int rows, int col, int width) {
+    if constexpr (MODE == ROWS_LOOSE) {
+        const int64_t at = int64_t(row) * width + col, last = int64_t(rows) * width - 8;
+        const int64_t from = at < last ? at : last;
+        return first_entries(drop_entries(*reinterpret_cast<const Loose16 *>(matrix + from), int(at - from) & 7), width - col);
+    } else {
+        return load8<T, MODE>(matrix + int64_t(row) * width, col, width);
+    }
+}
+template <typename T, int MODE> __device__ __forceinline__ uint2 load4(const typename T::raw_t *row, int col, int width) {
+    if constexpr (MODE == ROWS_ALIGNED) {
         return *reinterpret_cast<const uint2 *>(row + (col < width ? col : 0));
+    } else if constexpr (MODE == ROWS_LOOSE) {
+        const int c = col < width - 4 ? col : width - 4;
+        const Loose8 v = *reinterpret_cast<const Loose8 *>(row + c);
+        const uint64_t l = ((uint64_t(v.w[1]) << 32) | v.w[0]) >> (16 * ((col - c) & 3));
+        return make_uint2(uint32_t(l), uint32_t(l >> 32));
     } else {
         uint32_t e[4];
 #pragma unroll
@@ -309,27 +349,23 @@ template <typename T, bool VEC> __device__ __forceinline__ uint2 load4(const typ
     }
 }
 
-// How the backward's kernels reach the rows of a matrix: element by element, or in vectors from a byte offset of 32 bits
-// (matrices below 4 GiB: one addition per load) or 64.
-enum RowMode { ROWS_SCALAR = 0, ROWS_NARROW = 1, ROWS_WIDE = 2 };
-template <int MODE> struct RowOffset { using type = int64_t; };
-template <> struct RowOffset<ROWS_NARROW> { using type = uint32_t; };
-template <int MODE> using row_offset_t = typename RowOffset<MODE>::type;
+// Rows of a streamed matrix, by byte offset.
+template <int MODE> using row_offset_t = std::conditional_t<MODE == ROWS_ALIGNED, uint32_t, int64_t>;
 template <int MODE> __device__ __forceinline__ row_offset_t<MODE> row_offset(int token, int64_t stride) {
     return row_offset_t<MODE>(token) * row_offset_t<MODE>(stride * 2);
 }
 template <typename T, int MODE> __device__ __forceinline__ const typename T::raw_t *row_at(const void *base, row_offset_t<MODE> at) {
     return reinterpret_cast<const typename T::raw_t *>(static_cast<const char *>(base) + at);
 }
-// Columns of a lane that stay the same for every row of a kernel: clamped to the row once where vectors are used.
-template <int MODE> __device__ __forceinline__ int lane_column(int col, int width) { return MODE == ROWS_SCALAR || col < width ? col : 0; }
+// Columns of a lane that stay the same for every row of a kernel: clamped to the row once where vectors are aligned.
+template <int MODE> __device__ __forceinline__ int lane_column(int col, int width) { return MODE != ROWS_ALIGNED || col < width ? col : 0; }
 template <typename T, int MODE> __device__ __forceinline__ uint2 row_load4(const void *base, row_offset_t<MODE> at, int col, int width) {
-    if constexpr (MODE != ROWS_SCALAR) return *reinterpret_cast<const uint2 *>(row_at<T, MODE>(base, at + row_offset_t<MODE>(col * 2)));
-    else return load4<T, false>(row_at<T, MODE>(base, at), col, width);
+    if constexpr (MODE == ROWS_ALIGNED) return *reinterpret_cast<const uint2 *>(row_at<T, MODE>(base, at + row_offset_t<MODE>(col * 2)));
+    else return load4<T, MODE>(row_at<T, MODE>(base, at), col, width);
 }
 template <typename T, int MODE> __device__ __forceinline__ uint4 row_load8(const void *base, row_offset_t<MODE> at, int col, int width) {
-    if constexpr (MODE != ROWS_SCALAR) return *reinterpret_cast<const uint4 *>(row_at<T, MODE>(base, at + row_offset_t<MODE>(col * 2)));
-    else return load8<T, false>(row_at<T, MODE>(base, at), col, width);
+    if constexpr (MODE == ROWS_ALIGNED) return *reinterpret_cast<const uint4 *>(row_at<T, MODE>(base, at + row_offset_t<MODE>(col * 2)));
+    else return load8<T, MODE>(row_at<T, MODE>(base, at), col, width);
 }
 // Eight rows of four columns -> the four fragments e whose contraction index is the row: column e of each.
 __device__ __forceinline__ void transpose(const uint2 (&w)[8], uint4 (&frag)[4]) {
@@ -358,12 +394,12 @@ template <typename T> __device__ __forceinline__ typename T::raw_t narrow(float 
 // out = base + acc, rounded once; the base is loaded ahead of the products.
 enum ColumnMap { BY_HALF, BY_ROW };
 __device__ __forceinline__ int permuted(int m) { return (m & 2) * 16 + (m >> 2) * 8 + (m & 1) * 4; }
-template <typename T, bool VEC, int MAP> struct BaseRow {
+template <typename T, int MODE, int MAP> struct BaseRow {
     uint4 v[2];
     __device__ __forceinline__ void load(const void *base, int64_t row, int first, int width) {
         const typename T::raw_t *p = static_cast<const typename T::raw_t *>(base) + row;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) v[h] = base != nullptr ? load8<T, VEC>(p, first + 32 * h, width) : make_uint4(0, 0, 0, 0);
+        for (int h = 0; h < 2; ++h) v[h] = base != nullptr ? load8<T, MODE>(p, first + 32 * h, width) : make_uint4(0, 0, 0, 0);
     }
     static __device__ __forceinline__ float result(const f32x4 (&acc)[4], int h, int j) {
         return MAP == BY_HALF ? acc[2 * h + j / 4][j & 3] : acc[j & 3][2 * h + j / 4];
@@ -380,8 +416,10 @@ template <typename T, bool VEC, int MAP> struct BaseRow {
                 const float v0 = b[2 * j] + result(acc, h, 2 * j), v1 = b[2 * j + 1] + result(acc, h, 2 * j + 1);
                 w[j] = uint32_t(narrow<T>(v0)) | uint32_t(narrow<T>(v1)) << 16;
             }
-            if constexpr (VEC) {
+            if constexpr (MODE == ROWS_ALIGNED) {
                 if (c < width) *reinterpret_cast<uint4 *>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else if (MODE == ROWS_LOOSE && c + 8 <= width) {
+                *reinterpret_cast<Loose16 *>(out + c) = Loose16{{w[0], w[1], w[2], w[3]}};
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -433,7 +471,7 @@ struct ShrinkArgs {
     float *out;  // [N, R] scaled, or with `split` [segments, N, R]
     LoraPlan plan;
 };
-template <typename T, int RP, bool VEC, bool ONE>
+template <typename T, int RP, int MODE, bool ONE>
 __global__ __launch_bounds__(THREADS) void lora_shrink(ShrinkArgs p) {
     constexpr int RF = RP / 16, SUBS = ONE ? 1 : FWD_SUBS;
     __shared__ union {
@@ -481,9 +519,9 @@ __global__ __launch_bounds__(THREADS) void lora_shrink(ShrinkArgs p) {
                 for (int t = 0; t < 2; ++t) {
                     const int k = (st + t) * 32 + 8 * quad;
 #pragma unroll
-                    for (int f = 0; f < RF; ++f) fa[t][f] = load8_zero<T, VEC>(aw + int64_t(f * 16 + col < p.r ? f * 16 + col : 0) * p.h, k, p.h);
+                    for (int f = 0; f < RF; ++f) fa[t][f] = load8_zero<T, MODE>(aw + int64_t(f * 16 + col < p.r ? f * 16 + col : 0) * p.h, k, p.h);
 #pragma unroll
-                    for (int s = 0; s < SUBS; ++s) fx[t][s] = load8<T, VEC>(rows[s], k, p.h);
+                    for (int s = 0; s < SUBS; ++s) fx[t][s] = load8<T, MODE>(rows[s], k, p.h);
                 }
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -627,7 +665,7 @@ struct ExpandArgs {
     int32_t parts, o, r, groups, in_place;  // groups: of 64 outputs per wavefront
     LoraPlan plan;
 };
-template <typename T, int RP, bool VEC, bool PARTS>
+template <typename T, int RP, int MODE, bool PARTS>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 32 ? 4 : 2))) void lora_expand(ExpandArgs p) {
     constexpr int KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2;
     __shared__ uint4 uf[PARTS ? FWD_SUBS * KS * HL * kWave : 1];
@@ -647,7 +685,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
     }
     const typename T::raw_t *bw = static_cast<const typename T::raw_t *>(p.b) + int64_t(tile.adapter < 0 ? 0 : tile.adapter) * p.o * p.r;
     struct Stage {
-        BaseRow<T, VEC, BY_HALF> row[FWD_SUBS];
+        BaseRow<T, MODE, BY_HALF> row[FWD_SUBS];
         uint4 b[KS][4];
     };
     auto first_of = [&](int g) { return ((int(blockIdx.x) * p.groups + g) * WAVES + wave) * 64; };
@@ -658,7 +696,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int o = o0 + 32 * (e / 2) + 8 * (col / 4) + 4 * (e & 1) + (col & 3);
-                st.b[ks][e] = load8<T, VEC>(bw + int64_t(o < p.o ? o : 0) * p.r, RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad, p.r);
+                st.b[ks][e] = dense_load8<T, MODE>(bw, o < p.o ? o : 0, p.o, RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad, p.r);
             }
         st.row[0].load(p.base, token[0] * p.base_stride, o0 + 8 * quad, p.o);
         if (two) st.row[1].load(p.base, token[1] * p.base_stride, o0 + 8 * quad, p.o);
@@ -1033,7 +1071,6 @@ struct BwdInArgs {
 };
 template <typename T, int RP, int MODE>
 __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
-    constexpr bool VEC = MODE != ROWS_SCALAR;
     constexpr int RF = RP / 16, KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, NP = Parts<T>::kCount;
     __shared__ __attribute__((aligned(16))) int32_t tokens[BWD_TILE_MAX];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
@@ -1055,7 +1092,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int rank = (RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad) + j;
-            w[j] = load4<T, VEC>(aw + int64_t(rank < p.r ? rank : 0) * p.h, h0 + permuted(col), p.h);
+            w[j] = load4<T, MODE>(aw + int64_t(rank < p.r ? rank : 0) * p.h, h0 + permuted(col), p.h);
         }
         uint4 frag[4];
         transpose(w, frag);
@@ -1075,7 +1112,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
     };
     auto step = [&](int c, const uint2 (&w)[8], uint2 (&next)[8]) {
         const uint4 *pu = packed + int64_t(c / 32) * (Packed<RP>::kColumns + Packed<RP>::kRows);
-        BaseRow<T, VEC, BY_ROW> base[2];
+        BaseRow<T, MODE, BY_ROW> base[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
             base[s].load(p.dx_base, p.dx_base == nullptr ? 0 : int64_t(tokens[c + 16 * s + col]) * p.dx_base_stride, out_col, p.h);
@@ -1259,28 +1296,25 @@ inline BwdLayout bwd_layout(const Shape &d) {
 inline bool aligned16(const void *p, int64_t stride) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0); }
 
 // Calls launch(type, padded rank, vector accesses), each as a compile-time value.
-template <typename F> void with_types(int dtype, int rp, bool vec, F &&launch) {
-    auto ranks = [&](auto type, auto vector) {
-        if (rp == 16) launch(type, std::integral_constant<int, 16>{}, vector);
-        else if (rp == 32) launch(type, std::integral_constant<int, 32>{}, vector);
-        else if (rp == 64) launch(type, std::integral_constant<int, 64>{}, vector);
-        else launch(type, std::integral_constant<int, 128>{}, vector);
+template <typename F> void with_types(int dtype, int rp, F &&launch) {
+    auto ranks = [&](auto type) {
+        if (rp == 16) launch(type, std::integral_constant<int, 16>{});
+        else if (rp == 32) launch(type, std::integral_constant<int, 32>{});
+        else if (rp == 64) launch(type, std::integral_constant<int, 64>{});
+        else launch(type, std::integral_constant<int, 128>{});
     };
-    auto vectors = [&](auto type) {
-        if (vec) ranks(type, std::true_type{});
-        else ranks(type, std::false_type{});
-    };
-    if (dtype == KA_DTYPE_BF16) vectors(Bf16{});
-    else vectors(F16{});
+    if (dtype == KA_DTYPE_BF16) ranks(Bf16{});
+    else ranks(F16{});
 }
-
-// The backward's kernels, by the layout of the matrix they stream (of `bytes`).
-template <typename F> void with_modes(int dtype, int rp, bool vec, int64_t bytes, F &&launch) {
-    with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
-        if constexpr (!decltype(vec_c)::value) launch(type, rank_c, std::integral_constant<int, ROWS_SCALAR>{});
-        else if (bytes < (int64_t(1) << 32)) launch(type, rank_c, std::integral_constant<int, ROWS_NARROW>{});
-        else launch(type, rank_c, std::integral_constant<int, ROWS_WIDE>{});
+template <typename F> void with_modes(int dtype, int rp, RowMode mode, F &&launch) {
+    with_types(dtype, rp, [&](auto type, auto rank_c) {
+        if (mode == ROWS_ALIGNED) launch(type, rank_c, std::integral_constant<int, ROWS_ALIGNED>{});
+        else if (mode == ROWS_LOOSE) launch(type, rank_c, std::integral_constant<int, ROWS_LOOSE>{});
+        else launch(type, rank_c, std::integral_constant<int, ROWS_SCALAR>{});
     });
+}
+inline RowMode row_mode(bool aligned, int64_t width) {
+    return aligned && width % 8 == 0 ? ROWS_ALIGNED : (width >= 8 ? ROWS_LOOSE : ROWS_SCALAR);
 }
 
 }  // namespace
@@ -1312,8 +1346,8 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     if (workspace == nullptr || workspace_bytes < l.total)
         return fail(KA_ERR_WORKSPACE, "lora: workspace of %zu B, need %zu B", workspace == nullptr ? size_t(0) : workspace_bytes, l.total);
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(KA_ERR_BAD_ARG, "lora: workspace is not 16-byte aligned");
-    const bool vec = aligned16(base, base_stride) && aligned16(out, out_stride) && aligned16(hidden, hidden_stride) && aligned16(lora_a, 0) &&
-                     aligned16(lora_b, 0) && in_dim % 8 == 0 && out_dim % 8 == 0 && rank % 8 == 0;
+    const RowMode shrink_mode = row_mode(aligned16(hidden, hidden_stride) && aligned16(lora_a, 0), in_dim);
+    const RowMode expand_mode = row_mode(aligned16(base, base_stride) && aligned16(out, out_stride) && aligned16(lora_b, 0) && rank % 8 == 0, out_dim);
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     const LoraPlan plan = plan_at(ws, l.plan);
@@ -1344,12 +1378,11 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     sa.plan = plan;
     const int rp = padded_rank(rank);
     const dim3 shrink_grid{unsigned(l.split ? l.segments : 1), unsigned(one ? n_tokens + 1 : l.plan.max_tiles[0])};
-    with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
+    with_modes(dtype, rp, shrink_mode, [&](auto type, auto rank_c, auto mode_c) {
         using T = decltype(type);
-        constexpr int RP = decltype(rank_c)::value;
-        constexpr bool VEC = decltype(vec_c)::value;
-        if (one) hipLaunchKernelGGL((lora_shrink<T, RP, VEC, true>), shrink_grid, dim3(THREADS), 0, stream, sa);
-        else hipLaunchKernelGGL((lora_shrink<T, RP, VEC, false>), shrink_grid, dim3(THREADS), 0, stream, sa);
+        constexpr int RP = decltype(rank_c)::value, MODE = decltype(mode_c)::value;
+        if (one) hipLaunchKernelGGL((lora_shrink<T, RP, MODE, true>), shrink_grid, dim3(THREADS), 0, stream, sa);
+        else hipLaunchKernelGGL((lora_shrink<T, RP, MODE, false>), shrink_grid, dim3(THREADS), 0, stream, sa);
     });
     rc = check_hip(hipGetLastError(), "lora launch (shrink)");
     if (rc != KA_OK) return rc;
@@ -1374,7 +1407,7 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
         pa.n = n_tokens;
         pa.out = packed;
         pa.plan = plan;
-        with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto) {
+        with_types(dtype, rp, [&](auto type, auto rank_c) {
             using T = decltype(type);
             constexpr int RP = decltype(rank_c)::value;
             hipLaunchKernelGGL((lora_pack_rows<T, RP>), dim3(unsigned(l.plan.max_tiles[0])), dim3(THREADS), 0, stream, pa);
@@ -1406,12 +1439,11 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     groups = groups < 1 ? 1 : (groups > 8 ? 8 : groups);
     ea.groups = int32_t(groups);
     const dim3 expand_grid{unsigned(ceil_div(out_dim, 64 * WAVES * groups)), unsigned(l.plan.max_tiles[0])};
-    with_types(dtype, rp, vec, [&](auto type, auto rank_c, auto vec_c) {
+    with_modes(dtype, rp, expand_mode, [&](auto type, auto rank_c, auto mode_c) {
         using T = decltype(type);
-        constexpr int RP = decltype(rank_c)::value;
-        constexpr bool VEC = decltype(vec_c)::value;
-        if (parted) hipLaunchKernelGGL((lora_expand<T, RP, VEC, true>), expand_grid, dim3(THREADS), 0, stream, ea);
-        else hipLaunchKernelGGL((lora_expand<T, RP, VEC, false>), expand_grid, dim3(THREADS), 0, stream, ea);
+        constexpr int RP = decltype(rank_c)::value, MODE = decltype(mode_c)::value;
+        if (parted) hipLaunchKernelGGL((lora_expand<T, RP, MODE, true>), expand_grid, dim3(THREADS), 0, stream, ea);
+        else hipLaunchKernelGGL((lora_expand<T, RP, MODE, false>), expand_grid, dim3(THREADS), 0, stream, ea);
     });
     return check_hip(hipGetLastError(), "lora launch (expand)");
 }
@@ -1436,9 +1468,10 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     if (workspace == nullptr || workspace_bytes < l.total)
         return fail(KA_ERR_WORKSPACE, "lora backward: workspace of %zu B, need %zu B", workspace == nullptr ? size_t(0) : workspace_bytes, l.total);
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return fail(KA_ERR_BAD_ARG, "lora backward: workspace is not 16-byte aligned");
-    const bool vec = aligned16(grad_out, grad_stride) && aligned16(hidden, hidden_stride) && aligned16(dhidden_base, dhidden_base_stride) &&
-                     aligned16(dhidden, dhidden_stride) && aligned16(lora_a, 0) && aligned16(lora_b, 0) && in_dim % 8 == 0 && out_dim % 8 == 0 &&
-                     rank % 8 == 0;
+    constexpr int64_t NARROW = int64_t(1) << 32;  // bytes of a matrix that offsets of 32 bits reach
+    const RowMode out_mode = row_mode(aligned16(grad_out, grad_stride) && n_tokens * grad_stride * 2 < NARROW, out_dim);
+    const RowMode in_mode = row_mode(aligned16(hidden, hidden_stride) && aligned16(dhidden_base, dhidden_base_stride) &&
+                                     aligned16(dhidden, dhidden_stride) && aligned16(lora_a, 0) && n_tokens * hidden_stride * 2 < NARROW, in_dim);
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     const LoraPlan plan = plan_at(ws, l.plan);
@@ -1462,7 +1495,7 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
         pa.out = packed;
         pa.plan = plan;
         const dim3 grid{unsigned(l.plan.tokens[0] / 32), unsigned(l.plan.max_tiles[0])};
-        with_types(dtype, rp, vec, [&](auto, auto rank_c, auto) {
+        with_types(dtype, rp, [&](auto, auto rank_c) {
             constexpr int RP = decltype(rank_c)::value;
             hipLaunchKernelGGL((lora_pack<RP>), grid, dim3(THREADS), 0, stream, pa);
         });
@@ -1483,7 +1516,7 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     oa.du_part = du_part;
     oa.plan = plan;
     const dim3 out_grid{unsigned(l.blocks[0]), unsigned(l.plan.max_tiles[0])};
-    with_modes(dtype, rp, vec, n_tokens * grad_stride * 2, [&](auto type, auto rank_c, auto mode_c) {
+    with_modes(dtype, rp, out_mode, [&](auto type, auto rank_c, auto mode_c) {
         using T = decltype(type);
         constexpr int RP = decltype(rank_c)::value, MODE = decltype(mode_c)::value;
         if constexpr (RP == 16) {
@@ -1513,7 +1546,7 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     ia.da_part = da_part;
     ia.plan = plan;
     const dim3 in_grid{unsigned(l.blocks[1]), unsigned(l.plan.max_tiles[1])};
-    with_modes(dtype, rp, vec, n_tokens * hidden_stride * 2, [&](auto type, auto rank_c, auto mode_c) {
+    with_modes(dtype, rp, in_mode, [&](auto type, auto rank_c, auto mode_c) {
         using T = decltype(type);
         constexpr int RP = decltype(rank_c)::value, MODE = decltype(mode_c)::value;
         hipLaunchKernelGGL((lora_bwd_in<T, RP, MODE>), in_grid, dim3(THREADS), 0, stream, ia);
