@@ -5,8 +5,6 @@ token adds its own adapter's product.  The reference has no counterpart.  ``Samp
 """
 from __future__ import annotations
 
-from contextlib import contextmanager
-
 import torch
 
 from rl_engine.kernels import _hip
@@ -30,17 +28,27 @@ def _stride(rows):
     return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
 
 
+class _OwnScratch:
+    """Scratch from torch's stream-ordered allocator, held until the launches on the current stream are enqueued."""
+
+    __slots__ = ("_memory",)
+
+    def __init__(self, nbytes, device):
+        self._memory = torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+    def __enter__(self):
+        return self._memory.data_ptr()
+
+    def __exit__(self, *exc):
+        self._memory = None
+        return False
+
+
 class AdapterOps:
-    @contextmanager
     def _scratch(self, nbytes, device):
-        """Device pointer of scratch for launches on the current stream: the pool where it is large enough, torch's
-        (stream-ordered) allocator where the partial sums of a large call are not."""
-        if nbytes <= self.pool.capacity:
-            with self._workspace(nbytes, device) as ptr:
-                yield ptr
-            return
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)  # held until the launches are enqueued
-        yield scratch.data_ptr()
+        """Device pointer of scratch for launches on the current stream: the pool where it is large enough, memory of its own
+        where the partial sums of a large call are not."""
+        return self._workspace(nbytes, device) if nbytes <= self.pool.capacity else _OwnScratch(nbytes, device)
 
     def _check_adapters(self, hidden, lora_a, lora_b, adapter_ids, scaling):
         """Shapes of one call: (hidden rows, A, B, ids, scaling tensor or None, scaling number)."""
@@ -68,18 +76,22 @@ class AdapterOps:
             raise ValueError(f"adapter_ids shape {tuple(adapter_ids.shape)} != hidden.shape[:-1] {tuple(hidden.shape[:-1])}")
         if adapter_ids.is_floating_point() or adapter_ids.is_complex() or adapter_ids.dtype == torch.bool:
             raise TypeError(f"adapter_ids must be integers (got {adapter_ids.dtype})")
-        ids = adapter_ids.to(device=hidden.device, dtype=torch.int64).contiguous().view(-1)
+        ids = adapter_ids
+        if ids.dtype != torch.int64 or ids.device != hidden.device or not ids.is_contiguous():
+            ids = ids.to(device=hidden.device, dtype=torch.int64).contiguous()
         if ids.numel() > MAX_TOKENS:
             raise ValueError(f"{ids.numel()} tokens > {MAX_TOKENS}")
         if isinstance(scaling, torch.Tensor):
             if tuple(scaling.shape) != (s,):
                 raise ValueError(f"scaling tensor must have shape ({s},)")
-            scaling, scale = scaling.to(device=hidden.device, dtype=torch.float32).contiguous(), 1.0
+            if scaling.dtype != torch.float32 or scaling.device != hidden.device or not scaling.is_contiguous():
+                scaling = scaling.to(device=hidden.device, dtype=torch.float32).contiguous()
+            scale = 1.0
         else:
             scaling, scale = None, float(scaling)
         return _flat_rows(hidden), lora_a.contiguous(), lora_b.contiguous(), ids, scaling, scale
 
-    def _launch_lora(self, base, hidden, a, b, ids, scaling, scale, out, shrunk):
+    def _launch_lora(self, base, hidden, a, b, ids, scaling, scale, out, out_stride, shrunk):
         """ka_lora_linear on checked [N, ..] rows; without `out` only the product with lora_a, into `shrunk`."""
         n, (s, r, h), o = hidden.shape[0], a.shape, b.shape[1]
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
@@ -88,8 +100,8 @@ class AdapterOps:
             with self._scratch(ws_bytes, hidden.device) as ws_ptr:
                 status = self._lib.ka_lora_linear(
                     _DTYPE_CODE[hidden.dtype], ptr(base), 0 if base is None else _stride(base), hidden.data_ptr(),
-                    _stride(hidden), a.data_ptr(), b.data_ptr(), ids.data_ptr(), ptr(scaling), scale, ptr(out),
-                    0 if out is None else _stride(out), ptr(shrunk), n, h, o, r, s, ws_ptr, ws_bytes, _raw_stream())
+                    _stride(hidden), a.data_ptr(), b.data_ptr(), ids.data_ptr(), ptr(scaling), scale, ptr(out), out_stride,
+                    ptr(shrunk), n, h, o, r, s, ws_ptr, ws_bytes, _raw_stream())
         _hip.check(status, "ka_lora_linear")
 
     @torch.inference_mode()
@@ -122,12 +134,11 @@ class AdapterOps:
         if inplace and base_rows.data_ptr() != base.data_ptr():
             raise ValueError("inplace=True needs base as rows of one [N, O] layout")
         n = rows.shape[0]
-        out = base_rows if inplace else torch.empty(n, o, dtype=base.dtype, device=base.device)
-        shrunk = torch.empty(n, r, dtype=torch.float32, device=base.device) if return_shrunk else None
+        out = base if inplace else torch.empty(lead + (o,), dtype=base.dtype, device=base.device)
+        shrunk = torch.empty(lead + (r,), dtype=torch.float32, device=base.device) if return_shrunk else None
         if n > 0:
-            self._launch_lora(base_rows, rows, a, b, ids, scaling, scale, out, shrunk)
-        result = base if inplace else out.view(lead + (o,))
-        return (result, shrunk.view(lead + (r,))) if return_shrunk else result
+            self._launch_lora(base_rows, rows, a, b, ids, scaling, scale, out, _stride(base_rows) if inplace else o, shrunk)
+        return (out, shrunk) if return_shrunk else out
 
     @torch.inference_mode()
     def lora_linear_backward(self, grad_out, hidden, lora_a, lora_b, adapter_ids, scaling=1.0, shrunk=None,
@@ -165,16 +176,16 @@ class AdapterOps:
                 raise ValueError(f"shrunk shape {tuple(shrunk.shape)} != {lead + (r,)}")
             if shrunk.dtype != torch.float32 or shrunk.device != dev:
                 raise TypeError(f"shrunk must be fp32 on {dev}")
-            u = shrunk.contiguous().view(-1, r)
+            u = shrunk.contiguous()
         if n == 0:
             return (torch.zeros(lead + (h,), dtype=hidden.dtype, device=dev), torch.zeros_like(a, dtype=torch.float32),
                     torch.zeros_like(b, dtype=torch.float32))
         dy = _flat_rows(grad_out)
         if shrunk is None:
             u = torch.empty(n, r, dtype=torch.float32, device=dev)
-            self._launch_lora(None, rows, a, b, ids, scaling, scale, None, u)
+            self._launch_lora(None, rows, a, b, ids, scaling, scale, None, 0, u)
         dx_base = None if dhidden_base is None else _flat_rows(dhidden_base)
-        dx = torch.empty(n, h, dtype=hidden.dtype, device=dev)
+        dx = torch.empty(lead + (h,), dtype=hidden.dtype, device=dev)
         da = torch.empty(s, r, h, dtype=torch.float32, device=dev)
         db = torch.empty(s, o, r, dtype=torch.float32, device=dev)
         with _on_device(dev):
@@ -186,4 +197,4 @@ class AdapterOps:
                     None if dx_base is None else dx_base.data_ptr(), 0 if dx_base is None else _stride(dx_base),
                     dx.data_ptr(), h, da.data_ptr(), db.data_ptr(), n, h, o, r, s, ws_ptr, ws_bytes, _raw_stream())
         _hip.check(status, "ka_lora_linear_backward")
-        return dx.view(lead + (h,)), da, db
+        return dx, da, db

@@ -8,7 +8,7 @@ nothing falls back to torch ops.
 """
 from __future__ import annotations
 
-from contextlib import contextmanager
+from contextlib import nullcontext
 
 import torch
 import torch.nn as nn
@@ -76,15 +76,10 @@ class SamplerBackend(AdapterOps, SpeculativeOps, nn.Module):
         self.pool = WorkspacePool(pool_bytes)
         logger.info_once(f"Loaded {self._lib.ka_version().decode()}")
 
-    @contextmanager
     def _workspace(self, nbytes: int, device):
         """Device pointer of `nbytes` of scratch for launches on the current stream (None for no bytes).  The
         pool orders users of different streams and threads, so one SamplerBackend may be shared by them."""
-        if nbytes == 0:
-            yield None
-            return
-        with self.pool.lease(nbytes, device) as view:
-            yield view.data_ptr()
+        return nullcontext() if nbytes == 0 else self.pool.lease_pointer(nbytes, device)
 
     # ------------------------------------------------------------------ logprob
     @torch.inference_mode()

@@ -57,7 +57,7 @@ class SpeculativeOps:
                 raise ValueError(f"{name} shape {tuple(t.shape)} != {shape}")
             if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
                 raise TypeError(f"{name} must be integers (got {t.dtype})")
-            return t.to(device=dev, dtype=torch.int64).contiguous()
+            return t if t.dtype == torch.int64 and t.device == dev and t.is_contiguous() else t.to(device=dev, dtype=torch.int64).contiguous()
 
         ids = whole(draft_ids, "draft_ids", (batch, k))
         lens = None if draft_lens is None else whole(draft_lens, "draft_lens", (batch,))
