@@ -439,17 +439,21 @@ __device__ __forceinline__ void lds_barrier() {
 // Where R <= 16 one product of 32 holds the high parts of u in its first half and the low ones in its second.
 template <int RP> struct Steps { static constexpr int kCount = RP <= 16 ? 1 : RP / 32; };
 
-// first + part[0] + part[step] + ..., added in that order, eight of them requested together.
+// first + part[0] + part[step] + ..., added in that order; U of them requested together (those that exist: the rest read the first).
+template <int U> __device__ __forceinline__ float add_some(float sum, const float *__restrict__ part, int count, int64_t step) {
+    float v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = part[int64_t(u < count ? u : 0) * step];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (u < count) sum += v[u];
+    return sum;
+}
 __device__ __forceinline__ float add_parts(float first, const float *__restrict__ part, int parts, int64_t step) {
     float sum = first;
-    for (int q = 0; q < parts; q += 8) {
-        float v[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = part[int64_t(q + u < parts ? q + u : q) * step];
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (q + u < parts) sum += v[u];
-    }
+    int q = 0;
+    for (; q + 32 <= parts; q += 32) sum = add_some<32>(sum, part + int64_t(q) * step, 32, step);
+    for (; q < parts; q += 8) sum = add_some<8>(sum, part + int64_t(q) * step, parts - q, step);
     return sum;
 }
 

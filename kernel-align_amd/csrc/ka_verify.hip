@@ -17,7 +17,8 @@
 // 2^12 terms, by 2^-41 in all (P and Q sum to one).  An entry whose prefix sums lie more than DRAW_MARGIN = 2^-38 on either side of u R is the
 // integers' answer too; otherwise (about one draw in 10^6, and u = 0) the workgroup repeats the draw in 128-bit integers.
 //
-// Three launches, no host synchronisation:
+// Three launches, five where rows are split, no host synchronisation:
+//   verify_split_top, verify_split_mass   few fp16 / fp32 rows without top-k only: maxima and masses by several workgroups per row
 //   verify_rows    one workgroup per row that counts (target rows 0 .. len, draft rows 0 .. len - 1): the cut of the row's
 //                  distribution, its total mass, the draft token's mass, the log-sum-exp of the raw row.  This is the pass over
 //                  the data: bound by HBM, 2 V (2 K + 1) bytes per request.
@@ -68,6 +69,13 @@ struct ShareSums {
 };
 static_assert(sizeof(ShareSums) == 40, "the workspace query counts 40 bytes per share");
 
+// Of one part of a row that several workgroups work on (see verify_split_top).
+struct SplitPart {
+    uint64_t mass, raw;  // masses; exp(x - maximum) of the unscaled row in 2^-40
+    uint32_t top, bad;   // largest key; an entry of 2^8 or more, or NaN
+};
+static_assert(sizeof(SplitPart) == 24, "the workspace query counts 24 bytes per part");
+
 struct VerifyParams {
     const void *target, *draft;                          // draft may be null
     int64_t t_batch, t_pos, d_batch, d_pos;              // strides in elements
@@ -83,6 +91,9 @@ struct VerifyParams {
     RowSummary *rows;                                    // [B (K + 1)] target rows, then [B K] draft rows
     ShareSums *shares;                                   // [B, n_shares]
     int32_t n_shares, shares_per_group, vec_target, vec_draft;
+    int32_t n_rows, split_parts, split_entries;          // rows; parts of a row that was worked on ahead (0: none), entries in each
+    SplitPart *split;                                    // [rows, split_parts]
+    uint64_t *split_bins;                                // [rows, HIST_BINS]
 };
 
 struct Filter { float temp; bool has_t; bool use_k; int top_k; bool use_p; float top_p; };
@@ -246,8 +257,7 @@ struct CoarseRow {
     alignas(16) uint32_t key[LIST_CAP];
     uint32_t sorted[LIST_CAP];
     uint32_t n_list, give_up, max_key, ok;
-    uint64_t sums[S_WAVES];  // per wavefront: mass of all entries
-    double raw_sums[S_WAVES];
+    uint64_t sums[S_WAVES][2];  // per wavefront: mass of all entries, and raw_fix of them
     float edge_low, edge_high;  // the list takes entries of [edge_low, edge_high)
     uint64_t before;            // mass above edge_high
     RowCut cut;
@@ -623,10 +633,52 @@ __device__ __forceinline__ float lower_edge(int bin) {
     return bin >= HIST_SIDE ? bin_value(bin) : __uint_as_float(__float_as_uint(bin_value(bin - 1)) - 1u);
 }
 
+// exp(x - xmax) in 2^-40, rounded: sums of it do not depend on their order, and are off by V 2^-41 + 2^-22 of themselves.
+__device__ __forceinline__ uint64_t raw_fix(float x, float xmax) {
+    const double e = double(fast_exp2((x - xmax) * kLseLog2e)) + 4096.0;  // (its last bit is 2^-40)
+    return uint64_t(__double_as_longlong(e)) & 0x000fffffffffffffull;
+}
+// The maxima at which the bins describe a row.
+__device__ __forceinline__ bool coarse_top(float xmax) { return (xmax >= 0x1p-11f || xmax <= -0x1p-11f) && xmax > -256.0f && xmax < 256.0f; }
+// Mass and raw_fix of entries of a row, and the bins' masses (added to `bins` where `use_p`).
 template <typename T>
-__device__ __forceinline__ bool coarse_cut(CoarseRow &h, const typename T::raw_t *rp, int vocab, const Filter &f, bool want_lse) {
+__device__ __forceinline__ void coarse_masses(const typename T::raw_t *rp, int count, const Filter &f, bool want_lse, float xmax, uint32_t kmax,
+                                              uint64_t *bins, uint64_t &all, uint64_t &raw) {
+    const float vmax = value_of<T>(kmax);
+    each_entry<T, false>(rp, count, [&](typename T::raw_t r) {
+        const float x = T::widen(r);
+        if (want_lse) raw += raw_fix(x, xmax);
+        const uint32_t key = elem_key<T>(r, f.temp, f.has_t);
+        const uint64_t w = weight_fix(key == kmax ? 0.0f : value_of<T>(key) - vmax);
+        all += w;
+        if (f.use_p && w != 0) {
+            const int bin = coarse_bin(x);
+            if (bin < HIST_BINS) atomicAdd(reinterpret_cast<unsigned long long *>(&bins[bin]), (unsigned long long)w);
+        }
+    });
+}
+// Maximum and flag over the parts of a row, in every lane of the wavefront.
+__device__ __forceinline__ void split_top(const SplitPart *parts, int n, uint32_t &top, uint32_t &bad) {
+    top = bad = 0;
+    for (int i = int(threadIdx.x) & (kWave - 1); i < n; i += kWave) {
+        top = parts[i].top > top ? parts[i].top : top;
+        bad |= parts[i].bad;
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+        const uint32_t o = __shfl_xor(top, off, kWave);
+        top = o > top ? o : top;
+        bad |= __shfl_xor(bad, off, kWave);
+    }
+}
+
+// `parts`: what verify_split_top and verify_split_mass found about the row (n_parts of them, and its bins), or null.
+template <typename T>
+__device__ __forceinline__ bool coarse_cut(CoarseRow &h, const typename T::raw_t *rp, int vocab, const Filter &f, bool want_lse,
+                                           const SplitPart *parts, int n_parts, const uint64_t *bins) {
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    for (int i = tid; i < HIST_BINS; i += S_THREADS) h.mass[i] = 0;
+    const bool ahead = parts != nullptr;  // (never with top-k)
+    for (int i = tid; i < HIST_BINS; i += S_THREADS) h.mass[i] = ahead && f.use_p ? bins[i] : 0;
     if (tid == 0) { h.n_list = h.give_up = h.max_key = h.ok = 0; }
     __syncthreads();
     auto last_u64 = [&](uint64_t v) {
@@ -634,7 +686,11 @@ __device__ __forceinline__ bool coarse_cut(CoarseRow &h, const typename T::raw_t
                uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), kWave - 1));
     };
     // ---- first pass: the maximum, and with top-k the counts ----------------------------------
-    {
+    if (ahead) {
+        uint32_t top, bad;
+        split_top(parts, n_parts, top, bad);
+        if (tid == 0) { h.max_key = top; h.give_up = bad; }
+    } else {
         uint32_t top = 0, bad = 0;
         each_entry<T, true>(rp, vocab, [&](typename T::raw_t raw) {
             const float x = T::widen(raw);
@@ -656,7 +712,7 @@ __device__ __forceinline__ bool coarse_cut(CoarseRow &h, const typename T::raw_t
     }
     __syncthreads();
     const float xmax = value_of<T>(h.max_key);
-    if (h.give_up != 0 || h.max_key == 0 || !(xmax >= 0x1p-11f || xmax <= -0x1p-11f) || !(xmax > -256.0f)) return false;
+    if (h.give_up != 0 || h.max_key == 0 || !coarse_top(xmax)) return false;
     const uint32_t kmax = elem_key<T>(raw_of_key<T>(h.max_key), f.temp, f.has_t);
     const float vmax = value_of<T>(kmax);
     auto weight_of = [&](uint32_t key) { return weight_fix(key == kmax ? 0.0f : value_of<T>(key) - vmax); };
@@ -690,42 +746,38 @@ __device__ __forceinline__ bool coarse_cut(CoarseRow &h, const typename T::raw_t
     uint64_t z_all = 0;
     double raw_sum = 0.0;
     {
-        uint64_t all = 0;
+        uint64_t all = 0, raw = 0;
         const float low = f.use_k ? h.edge_low : 0.0f;
-        if (f.use_k) {
-            each_entry<T, true>(rp, vocab, [&](typename T::raw_t raw) {
-                const float x = T::widen(raw);
-                if (want_lse) raw_sum += double(fast_exp2((x - xmax) * kLseLog2e));
+        if (ahead) {
+            for (int i = tid; i < n_parts; i += S_THREADS) {
+                all += parts[i].mass;
+                raw += parts[i].raw;
+            }
+        } else if (f.use_k) {
+            each_entry<T, true>(rp, vocab, [&](typename T::raw_t r) {
+                const float x = T::widen(r);
+                if (want_lse) raw += raw_fix(x, xmax);
                 if (x >= low) {
                     const uint32_t at = atomicAdd(&h.n_list, 1u);
-                    if (at < uint32_t(LIST_CAP)) h.key[at] = elem_key<T>(raw, f.temp, f.has_t);
+                    if (at < uint32_t(LIST_CAP)) h.key[at] = elem_key<T>(r, f.temp, f.has_t);
                 }
             });
         } else {
-            each_entry<T, false>(rp, vocab, [&](typename T::raw_t raw) {
-                const float x = T::widen(raw);
-                if (want_lse) raw_sum += double(fast_exp2((x - xmax) * kLseLog2e));
-                const uint64_t w = weight_of(elem_key<T>(raw, f.temp, f.has_t));
-                all += w;
-                if (f.use_p && w != 0) {
-                    const int bin = coarse_bin(x);
-                    if (bin < HIST_BINS) atomicAdd(reinterpret_cast<unsigned long long *>(&h.mass[bin]), (unsigned long long)w);
-                }
-            });
+            coarse_masses<T>(rp, vocab, f, want_lse, xmax, kmax, h.mass, all, raw);
         }
         all = wave_sum_u64_of(all);
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) raw_sum += __shfl_xor(raw_sum, off, kWave);
+        raw = wave_sum_u64_of(raw);
         if (lane == 0) {
-            h.sums[wave] = all;
-            h.raw_sums[wave] = raw_sum;
+            h.sums[wave][0] = all;
+            h.sums[wave][1] = raw;
         }
         __syncthreads();
-        raw_sum = 0.0;
+        raw = 0;
         for (int w = 0; w < S_WAVES; ++w) {
-            z_all += h.sums[w];
-            raw_sum += h.raw_sums[w];
+            z_all += h.sums[w][0];
+            raw += h.sums[w][1];
         }
+        raw_sum = double(raw) * 0x1p-40;
         if (f.use_p && !f.use_k) {
             // ---- the bin where the mass before an entry passes theta; the list: it and its two neighbours ----
             if (wave == 0) {
@@ -862,18 +914,127 @@ __device__ __forceinline__ bool coarse_cut(CoarseRow &h, const typename T::raw_t
     return (f.use_k || f.use_p) ? ok : true;
 }
 
+// Row r of a call (target rows first), and whether it counts: target rows 0 .. len, draft rows 0 .. len - 1.
+struct RowRef { int b, j, len; bool target, counts; };
+__device__ __forceinline__ RowRef row_ref(const VerifyParams &p, int64_t r) {
+    const int64_t n_target = int64_t(p.batch) * (p.k + 1);
+    RowRef x;
+    x.target = r < n_target;
+    const int per = x.target ? p.k + 1 : p.k;
+    const int64_t q = x.target ? r : r - n_target;
+    x.b = int(q / per);
+    x.j = int(q % per);
+    x.len = draft_len(p, x.b);
+    x.counts = x.target ? x.j <= x.len : x.j < x.len;
+    return x;
+}
+
+// ---------------------------------------------------------------------------
+// fp16 and fp32 rows without top-k, in calls of few rows: the maximum, then the masses (which are 60 instructions an entry: one
+// CU takes 50 us for a row of 128,256), by a workgroup per 32 KB of every row.  grid (rows, parts) each; verify_rows goes on from the
+// bins.  8 requests x 2 drafts, fp32, top-p 0.9, 128,256 entries: 134 us in verify_rows alone, 6.6 + 28 + 26
+// us so; verify_split_mass is bound by its arithmetic.
+// ---------------------------------------------------------------------------
+constexpr int SPLIT_BYTES = 32768;
+// Up to how many rows: fp32, top-p 0.9, 128,256 entries, a call of 5 / 40 / 120 / 250 rows: 156 / 165 / 175 / 187 us by a workgroup per
+// row, 70 / 95 / 136 / 200 us split; fp16, 50,257 entries: 83 / 105 / 105 / 112 and 67 / 90 / 99 / 124 us.
+constexpr int64_t SPLIT_ROWS = 160;
+template <typename T> __device__ __forceinline__ int split_span(const VerifyParams &p, int &first) {
+    first = int(blockIdx.y) * p.split_entries;
+    return p.vocab - first < p.split_entries ? p.vocab - first : p.split_entries;
+}
+template <typename T> __global__ __launch_bounds__(S_THREADS) void verify_split_top(VerifyParams p) {
+    __shared__ uint32_t tops[S_WAVES], bads[S_WAVES];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    if (int(blockIdx.x) >= p.n_rows) return;
+    const RowRef x = row_ref(p, blockIdx.x);
+    if (!x.counts) return;
+    const Filter f = filter_of(p, x.b);
+    if (f.use_k) return;
+    int first;
+    const int count = split_span<T>(p, first);
+    uint32_t top = 0, bad = 0;
+    each_entry<T, true>((x.target ? target_row<T>(p, x.b, x.j) : draft_row<T>(p, x.b, x.j)) + first, count, [&](typename T::raw_t raw) {
+        const float v = T::widen(raw);
+        const uint32_t key = masked_key<T>(v);
+        top = key > top && v == v ? key : top;
+        bad |= !(v < 256.0f) ? 1u : 0u;
+    });
+    if (f.use_p)  // the row's bins, for the kernel behind to add to
+        for (int i = int(blockIdx.y) * S_THREADS + tid; i < HIST_BINS; i += p.split_parts * S_THREADS)
+            p.split_bins[int64_t(blockIdx.x) * HIST_BINS + i] = 0;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+        const uint32_t o = __shfl_xor(top, off, kWave);
+        top = o > top ? o : top;
+        bad |= __shfl_xor(bad, off, kWave);
+    }
+    if (lane == 0) {
+        tops[wave] = top;
+        bads[wave] = bad;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < S_WAVES; ++w) {
+            top = tops[w] > top ? tops[w] : top;
+            bad |= bads[w];
+        }
+        SplitPart &part = p.split[int64_t(blockIdx.x) * p.split_parts + blockIdx.y];
+        part.top = top;
+        part.bad = bad;
+    }
+}
+template <typename T> __global__ __launch_bounds__(S_THREADS) void verify_split_mass(VerifyParams p) {
+    __shared__ uint64_t mass[HIST_BINS];
+    __shared__ uint64_t sums[S_WAVES][2];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    if (int(blockIdx.x) >= p.n_rows) return;
+    const RowRef x = row_ref(p, blockIdx.x);
+    if (!x.counts) return;
+    const Filter f = filter_of(p, x.b);
+    if (f.use_k) return;
+    SplitPart *const parts = p.split + int64_t(blockIdx.x) * p.split_parts;
+    uint32_t top, bad;
+    split_top(parts, p.split_parts, top, bad);
+    if (bad != 0 || top == 0 || !coarse_top(value_of<T>(top))) return;  // (verify_rows sees the same, and takes the radix path)
+    if (f.use_p)
+        for (int i = tid; i < HIST_BINS; i += S_THREADS) mass[i] = 0;
+    __syncthreads();
+    int first;
+    const int count = split_span<T>(p, first);
+    uint64_t all = 0, raw = 0;
+    coarse_masses<T>((x.target ? target_row<T>(p, x.b, x.j) : draft_row<T>(p, x.b, x.j)) + first, count, f, x.target && p.out_policy != nullptr,
+                     value_of<T>(top), elem_key<T>(raw_of_key<T>(top), f.temp, f.has_t), mass, all, raw);
+    all = wave_sum_u64_of(all);
+    raw = wave_sum_u64_of(raw);
+    if (lane == 0) {
+        sums[wave][0] = all;
+        sums[wave][1] = raw;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < S_WAVES; ++w) {
+            all += sums[w][0];
+            raw += sums[w][1];
+        }
+        parts[blockIdx.y].mass = all;
+        parts[blockIdx.y].raw = raw;
+    }
+    if (f.use_p)
+        for (int i = tid; i < HIST_BINS; i += S_THREADS)
+            if (mass[i] != 0)
+                atomicAdd(reinterpret_cast<unsigned long long *>(&p.split_bins[int64_t(blockIdx.x) * HIST_BINS + i]), (unsigned long long)mass[i]);
+}
+
 template <typename T>
 __global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(6, 6))) void verify_rows(VerifyParams p) {
     __shared__ VerifyShared<T> lds;
     const int tid = threadIdx.x;
-    const int64_t n_target = int64_t(p.batch) * (p.k + 1);
     const int64_t r = blockIdx.x;
-    const bool is_target = r < n_target;
-    const int per = is_target ? p.k + 1 : p.k;
-    const int64_t q = is_target ? r : r - n_target;
-    const int b = int(q / per), j = int(q % per);
-    const int len = draft_len(p, b);
-    if (j > len || (!is_target && j == len)) return;  // the whole workgroup: nobody reads this row's summary
+    const RowRef ref = row_ref(p, r);
+    const bool is_target = ref.target;
+    const int b = ref.b, j = ref.j, len = ref.len;
+    if (!ref.counts) return;  // the whole workgroup: nobody reads this row's summary
     const typename T::raw_t *rp = is_target ? target_row<T>(p, b, j) : draft_row<T>(p, b, j);
     const bool vec = (is_target ? p.vec_target : p.vec_draft) != 0;
     const Filter f = filter_of(p, b);
@@ -887,7 +1048,8 @@ __global__ __launch_bounds__(S_THREADS) __attribute__((amdgpu_waves_per_eu(6, 6)
     float raw_top = 0.0f;
     bool done = false;
     if constexpr (T::kDtype == KA_DTYPE_BF16) done = hist_cut(lds.row, rp, p.vocab, f, want_lse);
-    else done = coarse_cut<T>(lds.row, rp, p.vocab, f, want_lse);
+    else done = coarse_cut<T>(lds.row, rp, p.vocab, f, want_lse, p.split_parts > 0 && !f.use_k ? p.split + r * p.split_parts : nullptr,
+                              p.split_parts, p.split_bins + r * HIST_BINS);
     if (done) {
         cut = lds.row.cut;
         raw_sum = lds.row.raw_sum;
@@ -1413,8 +1575,20 @@ inline int reserve_table_lds() {
 
 template <typename T> int launch_verify(const VerifyParams &p, hipStream_t stream) {
     const int64_t rows = int64_t(p.batch) * (p.k + 1) + (p.draft != nullptr ? int64_t(p.batch) * p.k : 0);
+    int rc = KA_OK;
+    if constexpr (T::kDtype != KA_DTYPE_BF16) {
+        if (p.split_parts > 0) {
+            const dim3 grid{unsigned((rows + 7) / 8 * 8), unsigned(p.split_parts)};  // all parts of a row on one XCD
+            hipLaunchKernelGGL((verify_split_top<T>), grid, dim3(S_THREADS), 0, stream, p);
+            rc = check_hip(hipGetLastError(), "verify launch (maxima)");
+            if (rc != KA_OK) return rc;
+            hipLaunchKernelGGL((verify_split_mass<T>), grid, dim3(S_THREADS), 0, stream, p);
+            rc = check_hip(hipGetLastError(), "verify launch (masses)");
+            if (rc != KA_OK) return rc;
+        }
+    }
     hipLaunchKernelGGL((verify_rows<T>), dim3(unsigned(rows)), dim3(S_THREADS), 0, stream, p);
-    int rc = check_hip(hipGetLastError(), "verify launch (rows)");
+    rc = check_hip(hipGetLastError(), "verify launch (rows)");
     if (rc != KA_OK) return rc;
     if (T::kDtype == KA_DTYPE_BF16 && p.shares_per_group > 0) {
         rc = reserve_table_lds();
@@ -1433,8 +1607,8 @@ template <typename T> int launch_verify(const VerifyParams &p, hipStream_t strea
 inline size_t align_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
 struct VerifyLayout {
-    int64_t n_shares;
-    size_t rows, shares, total;
+    int64_t n_shares, split_parts;
+    size_t rows, shares, split, split_bins, total;
 };
 inline VerifyLayout verify_layout(int dtype, int64_t batch, int64_t k, int64_t vocab) {
     VerifyLayout l;
@@ -1443,6 +1617,11 @@ inline VerifyLayout verify_layout(int dtype, int64_t batch, int64_t k, int64_t v
     l.rows = 0;
     l.shares = align_up(size_t(batch) * size_t(2 * k + 1) * sizeof(RowSummary), 256);
     l.total = l.shares + size_t(batch) * size_t(l.n_shares) * sizeof(ShareSums);
+    l.split = align_up(l.total, 256);
+    const int64_t n_rows = batch * (2 * k + 1), parts = (vocab + SPLIT_BYTES / (16 / epv) - 1) / (SPLIT_BYTES / (16 / epv));
+    l.split_parts = dtype != KA_DTYPE_BF16 && parts > 1 && n_rows <= SPLIT_ROWS ? parts : 0;
+    l.split_bins = align_up(l.split + size_t(n_rows) * size_t(l.split_parts) * sizeof(SplitPart), 256);
+    if (l.split_parts > 0) l.total = l.split_bins + size_t(n_rows) * HIST_BINS * sizeof(uint64_t);
     return l;
 }
 
@@ -1519,6 +1698,13 @@ KA_EXPORT int ka_verify_draft(int dtype, const void *target_logits, int64_t targ
     p.rows = reinterpret_cast<RowSummary *>(ws + l.rows);
     p.shares = reinterpret_cast<ShareSums *>(ws + l.shares);
     p.n_shares = int32_t(l.n_shares);
+    if (l.split_parts > 0 && (top_k_rows != nullptr || top_k == 0 || top_k >= vocab)) {
+        p.n_rows = int32_t(batch * (max_draft + 1) + (p.draft != nullptr ? batch * max_draft : 0));
+        p.split_parts = int32_t(l.split_parts);
+        p.split_entries = int32_t(SPLIT_BYTES / esize);
+        p.split = reinterpret_cast<SplitPart *>(ws + l.split);
+        p.split_bins = reinterpret_cast<uint64_t *>(ws + l.split_bins);
+    }
     // Tables pay where most entries may have mass: two of them cost 9728 evaluations, a share of 2048 entries 4096 without.
     // Enough groups to fill the device twice, of at least eight shares (one per wavefront).
     const bool many = top_k_rows != nullptr || top_k == 0 || top_k > 1024;

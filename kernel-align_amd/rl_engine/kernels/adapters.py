@@ -28,28 +28,7 @@ def _stride(rows):
     return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
 
 
-class _OwnScratch:
-    """Scratch from torch's stream-ordered allocator, held until the launches on the current stream are enqueued."""
-
-    __slots__ = ("_memory",)
-
-    def __init__(self, nbytes, device):
-        self._memory = torch.empty(nbytes, dtype=torch.uint8, device=device)
-
-    def __enter__(self):
-        return self._memory.data_ptr()
-
-    def __exit__(self, *exc):
-        self._memory = None
-        return False
-
-
 class AdapterOps:
-    def _scratch(self, nbytes, device):
-        """Device pointer of scratch for launches on the current stream: the pool where it is large enough, memory of its own
-        where the partial sums of a large call are not."""
-        return self._workspace(nbytes, device) if nbytes <= self.pool.capacity else _OwnScratch(nbytes, device)
-
     def _check_adapters(self, hidden, lora_a, lora_b, adapter_ids, scaling):
         """Shapes of one call: (hidden rows, A, B, ids, scaling tensor or None, scaling number)."""
         for t, name in ((hidden, "hidden"), (lora_a, "lora_a"), (lora_b, "lora_b")):

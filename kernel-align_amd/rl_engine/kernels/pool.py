@@ -146,3 +146,19 @@ class _Lease:
         finally:
             pool._lock.release()
         return False
+
+
+class OwnScratch:
+    """Scratch from torch's stream-ordered allocator, held until the launches on the current stream are enqueued."""
+
+    __slots__ = ("_memory",)
+
+    def __init__(self, nbytes, device):
+        self._memory = torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+    def __enter__(self):
+        return self._memory.data_ptr()
+
+    def __exit__(self, *exc):
+        self._memory = None
+        return False

@@ -16,7 +16,7 @@ import torch.nn as nn
 from rl_engine.kernels import _hip
 from rl_engine.kernels._launch import _on_device, _raw_stream, _require_gpu
 from rl_engine.kernels.adapters import AdapterOps
-from rl_engine.kernels.pool import PoolExhausted, WorkspacePool
+from rl_engine.kernels.pool import OwnScratch, PoolExhausted, WorkspacePool
 from rl_engine.kernels.speculative import SpeculativeOps
 from rl_engine.platforms.constants import constants
 from rl_engine.utils.logger import logger
@@ -80,6 +80,11 @@ class SamplerBackend(AdapterOps, SpeculativeOps, nn.Module):
         """Device pointer of `nbytes` of scratch for launches on the current stream (None for no bytes).  The
         pool orders users of different streams and threads, so one SamplerBackend may be shared by them."""
         return nullcontext() if nbytes == 0 else self.pool.lease_pointer(nbytes, device)
+
+    def _scratch(self, nbytes, device):
+        """Device pointer of scratch for launches on the current stream: the pool where it is large enough, memory of its own
+        where the partial sums of a large call are not."""
+        return self._workspace(nbytes, device) if nbytes <= self.pool.capacity else OwnScratch(nbytes, device)
 
     # ------------------------------------------------------------------ logprob
     @torch.inference_mode()

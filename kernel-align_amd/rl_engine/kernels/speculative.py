@@ -90,7 +90,7 @@ class SpeculativeOps:
             ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
             with _on_device(dev):
                 ws_bytes = self._lib.ka_verify_workspace_bytes(code, batch, k, vocab)
-                with self._workspace(ws_bytes, dev) as ws_ptr:
+                with self._scratch(ws_bytes, dev) as ws_ptr:
                     status = self._lib.ka_verify_draft(
                         code, target.data_ptr(), *t_strides, ptr(draft), *d_strides, ids.data_ptr(), ptr(lens),
                         uniforms.data_ptr(), batch, k, vocab, float(temp), ptr(temp_rows), int(kk), ptr(kk_rows),

@@ -171,6 +171,9 @@ def test_verify_argument_checks_and_workspace_size():
     up = lambda n: (n + 255) // 256 * 256  # noqa: E731
     assert ws(0, 64, 4, 128256) == up(64 * 9 * 48) + 64 * 63 * 40
     assert ws(2, 3, 0, 4097) == up(3 * 48) + 3 * 5 * 40
+    # fp16 / fp32 rows of more than 32 KB, in calls of up to 160: bins (4864 masses) and 24 bytes per part of every row
+    assert ws(2, 8, 2, 128256) == up(up(8 * 5 * 48) + 8 * 126 * 40) + up(40 * 16 * 24) + 40 * 4864 * 8
+    assert ws(1, 54, 1, 16385) == up(162 * 48) + 54 * 9 * 40 and ws(1, 53, 1, 16385) > 159 * 4864 * 8
     assert ws(0, 0, 4, 128256) == 0 and ws(0, 4, 65, 100) == 0 and ws(0, 4, 4, 1 << 22) == 0
 
     def call(dtype=0, target=p, tb=500, tp=100, draft=p, db=400, dp=100, ids=p, lens=None, u=p, batch=2, k=4, vocab=100,

@@ -286,3 +286,32 @@ def test_generator_and_empty_batch(sampler):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     e = sampler.verify_draft(t[:0].cuda(), ids[:0].cuda(), u[:0], return_policy_logprob=True)
     assert e[0].shape == (0, 3) and e[1].shape == (0,) and e[2].shape == (0, 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_rows_worked_on_by_several_workgroups(sampler, dtype):
+    """A call of few long rows and the same requests inside a call of many take different routes to the same bits, for requests with
+    and without top-k side by side, odd lengths, masked entries, and rows that the bins do not describe."""
+    vocab, k = 40003, 3
+    target, ids, u, q, lens = _inputs(60, k, vocab, dtype, 31, ragged=True)
+    target[1, 0, 7:20000] = -float("inf")
+    target[2, 1, :] = torch.finfo(dtype).min
+    target[2, 1, 11] = 3.0
+    target[3, 0, 5] = float("nan")
+    target[4, 1, 9] = 1000.0
+    top_k = torch.zeros(60, dtype=torch.int32)
+    top_k[::3] = 40
+    top_p = torch.linspace(0.3, 1.0, 60)
+    kw = dict(top_k=top_k, top_p=top_p, temperature=0.8)
+    d = [None if t is None else t.cuda() for t in (target, ids, u, q, lens)]
+    few = [slice(0, 6), slice(6, 7), slice(40, 60)]
+    many = sampler.verify_draft(d[0], d[1], d[2], draft_logits=d[3], draft_lens=d[4], return_policy_logprob=True, **kw)
+    for part in few:
+        sub = dict(kw, top_k=top_k[part], top_p=top_p[part])
+        got = sampler.verify_draft(d[0][part], d[1][part], d[2][part], draft_logits=d[3][part], draft_lens=d[4][part],
+                                   return_policy_logprob=True, **sub)
+        assert torch.equal(got[0], many[0][part]) and torch.equal(got[1], many[1][part])
+        assert torch.equal(got[2].view(torch.int32), many[2][part].view(torch.int32))
+    part = slice(0, 6)
+    want = verify_ref.verify(target[part], ids[part], u[part], q[part], lens[part], temperature=0.8, top_k=top_k[part], top_p=top_p[part])
+    assert torch.equal(many[0][part].cpu(), want[0]) and torch.equal(many[1][part].cpu(), want[1])
