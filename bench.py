@@ -35,22 +35,22 @@ BYTES_PER_TOKEN = 2 * V + 8 + 4
 # hex digits of the SHA-256 of those files (concatenated in that order) at the time of the counter runs.
 CSRC = REPO / "kernel-align_amd" / "csrc"
 _SAMPLING_SOURCES = ("ka_common.h", "ka_sampling_common.h", "ka_sampling_topk.h", "ka_sampling_dense.h", "ka_sampling_draw.h",
-                     "ka_sampling_kernel.h", "ka_sampling.hip", "ka_sampling_half.hip")
+                     "ka_sampling_kernel.h", "ka_sampling_radix.h", "ka_sampling.hip", "ka_sampling_half.hip")
 _LMHEAD_SOURCES = ("ka_common.h", "ka_lmhead.hip", "ka_lmhead_narrow.h")
 STATIC_TRAFFIC = {
     "logprob_rows": ((2 * 16425200 + 4317.5) * 1024, "profiles/logprob_rows_bf16_G256_L512_V128256.txt",         # 131072 rows
                      ("ka_common.h", "ka_logprob.hip"), "d3ed0936386075a5"),
     "logprob_backward_rows": ((2 * 4108350 + 8208390) * 1024, "profiles/logprob_backward_rows_bf16_G64_L512_V128256.txt",  # 32768 rows
                               ("ka_common.h", "ka_logprob.hip"), "d3ed0936386075a5"),
-    "sample_rows": ((2 * 32831.5 + 10.3) * 1024, "profiles/sample_rows_bf16_B64-1024_V128256.txt",                     # B = 256
-                    _SAMPLING_SOURCES, "817959ab3c8df18c"),
+    "sample_rows": ((2 * 32842.9 + 8.0) * 1024, "profiles/sample_rows_bf16_B64-1024_V128256.txt",                     # B = 256
+                    _SAMPLING_SOURCES, "5a715c73a294257e"),
     "lmhead_partials": ((2 * 3.176e7 + 121088) * 1024, "profiles/lmhead_partials_bf16_H4096_V128256.txt",            # N = 32768; L2 misses: varies +-50 % between calls
                         _LMHEAD_SOURCES, "793ffdf2d7810fe0"),
     "lmhead_n64": ((2 * 517332 + 256) * 1024, "profiles/lmhead_partials_bf16_H4096_V128256.txt", _LMHEAD_SOURCES, "793ffdf2d7810fe0"),
     "lmhead_n256": ((2 * 532202 + 9216) * 1024, "profiles/lmhead_partials_bf16_H4096_V128256.txt", _LMHEAD_SOURCES, "793ffdf2d7810fe0"),
 }
 # FETCH_SIZE / WRITE_SIZE KiB per dispatch of sample_rows by batch, from the same counter runs as the B = 256 entry above
-_SAMPLING_KIB = {64: (8268.3, 2.6), 128: (16314.7, 5.3), 256: (32831.5, 10.3), 512: (65957.6, 21.0), 1024: (131641.0, 42.9)}
+_SAMPLING_KIB = {64: (8278.2, 2.6), 128: (16325.7, 5.3), 256: (32842.9, 8.0), 512: (65965.1, 21.0), 1024: (131680.2, 42.7)}
 PARITY_TOL = 1e-4
 
 
