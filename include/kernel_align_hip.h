@@ -249,7 +249,7 @@ int ka_verify_draft(int dtype, const void *target_logits, int64_t target_batch_s
  */
 #define KA_LORA_MAX_RANK 128
 #define KA_LORA_MAX_ADAPTERS 1023
-#define KA_LORA_MAX_TOKENS (1 << 21)
+#define KA_LORA_MAX_TOKENS (1 << 20)
 size_t ka_lora_workspace_bytes(int64_t n_tokens, int64_t in_dim, int64_t out_dim, int64_t rank, int64_t n_adapters,
                                int backward);
 int ka_lora_linear(int dtype, const void *base, int64_t base_stride, const void *hidden, int64_t hidden_stride,

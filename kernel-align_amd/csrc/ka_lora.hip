@@ -31,6 +31,7 @@ constexpr int THREADS = 256;
 constexpr int WAVES = THREADS / kWave;
 constexpr int FWD_TILE = 32;    // tokens per tile of the forward: two groups of sixteen
 constexpr int FWD_SUBS = FWD_TILE / 16;
+static_assert(KA_LORA_MAX_TOKENS / FWD_TILE + MAX_ADAPTERS + 1 <= 65535, "the tiles are the second dimension of a grid");
 constexpr int BWD_TILE_MAX = 1024;  // ... of the backward at most (a multiple of 32)
 
 struct LoraTile {

@@ -31,7 +31,7 @@
 #define KA_SAMPLING_THREADS 512
 #include <stddef.h>
 
-#include <mutex>
+#include <atomic>
 #include <type_traits>
 
 #include "ka_sampling_common.h"
@@ -1556,19 +1556,17 @@ __global__ __launch_bounds__(SHARE_VECS) void verify_draw(VerifyParams p) {
     if (tid == 0) p.out_accepted[b] = n;
 }
 
-// verify_shares_table uses 78 KB of LDS: the attribute belongs to the device, set once for each.
+// verify_shares_table uses 78 KB of LDS: the attribute belongs to the device, set once for each (or twice, by two threads at once).
 inline int reserve_table_lds() {
-    static std::mutex mutex;
-    static bool done[64] = {};
+    static std::atomic<bool> done[64];
     int device = 0;
     hipError_t rc = hipGetDevice(&device);
     if (rc != hipSuccess) return check_hip(rc, "verify: hipGetDevice");
     if (device < 0 || device >= 64) return fail(KA_ERR_UNSUPPORTED, "verify: device index %d", device);
-    std::lock_guard<std::mutex> lock(mutex);
-    if (!done[device]) {
+    if (!done[device].load(std::memory_order_acquire)) {
         rc = hipFuncSetAttribute(reinterpret_cast<const void *>(verify_shares_table), hipFuncAttributeMaxDynamicSharedMemorySize, int(TABLE_LDS_BYTES));
         if (rc != hipSuccess) return check_hip(rc, "verify: reserving LDS for the tables");
-        done[device] = true;
+        done[device].store(true, std::memory_order_release);
     }
     return KA_OK;
 }
@@ -1655,6 +1653,8 @@ KA_EXPORT int ka_verify_draft(int dtype, const void *target_logits, int64_t targ
     if (vocab >= (int64_t(1) << 22))
         return fail(KA_ERR_UNSUPPORTED, "verify: vocab %lld >= 2^22 (integer masses would overflow)", (long long)vocab);
     if (batch > 65535) return fail(KA_ERR_UNSUPPORTED, "verify: batch %lld > 65535", (long long)batch);
+    if (batch * (2 * max_draft + 1) >= (int64_t(1) << 32) / S_THREADS)
+        return fail(KA_ERR_UNSUPPORTED, "verify: %lld rows in one call", (long long)(batch * (2 * max_draft + 1)));
     // (a stride counts only where there is a second row to step to)
     if ((batch > 1 && target_batch_stride < vocab) || (max_draft > 0 && target_pos_stride < vocab))
         return fail(KA_ERR_BAD_ARG, "verify: a target stride is smaller than the vocabulary");

@@ -13,7 +13,7 @@ from rl_engine.kernels._launch import _on_device, _raw_stream, _require_gpu
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1}
 MAX_RANK = 128         # KA_LORA_MAX_RANK
 MAX_ADAPTERS = 1023    # KA_LORA_MAX_ADAPTERS
-MAX_TOKENS = 1 << 21   # KA_LORA_MAX_TOKENS
+MAX_TOKENS = 1 << 20   # KA_LORA_MAX_TOKENS
 
 
 def _flat_rows(t):

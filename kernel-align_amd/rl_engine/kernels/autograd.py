@@ -123,7 +123,8 @@ class _LoraLinearLogp(torch.autograd.Function):
             logp = sampler._compute_logp(logits, tokens[part])
             dlogits = sampler._compute_logp_backward(logits, tokens[part], logp, grads[part], inplace=True)
             dhidden[part], da_part, db_part = sampler._lora_linear_backward(
-                dlogits, rows[part], lora_a, lora_b, adapters[part], scaling, shrunk, torch.matmul(dlogits, weight))
+                dlogits, rows[part], lora_a, lora_b, adapters[part], scaling, shrunk,
+                torch.matmul(dlogits, weight) if ctx.needs_input_grad[1] else None)
             da += da_part
             db += db_part
             del logits, dlogits

@@ -27,7 +27,7 @@ class SpeculativeOps:
         K = 0 is ``sample``.
 
         Both rows of a position are taken through the same temperature -> top-k -> top-p as in ``sample`` (scalars, or [B]
-        tensors of per-request values): P from the target, Q from the draft (one-hot without draft logits).  Draft j is
+        tensors of per-request values, where a top_k of 0 filters nothing): P from the target, Q from the draft (one-hot without draft logits).  Draft j is
         accepted iff ``uniforms[:, j] * Q(d) < P(d)``; the first position that is not is redrawn from max(P - Q, 0), and
         when all are accepted the position behind them is drawn from P, both by the inverse CDF in index order that
         ``uniforms[:, K]`` drives.  All of it is decided on the sampling operator's integer masses: the ids are a function of the

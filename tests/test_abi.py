@@ -187,7 +187,7 @@ def test_verify_argument_checks_and_workspace_size():
                 dict(vocab=0), dict(t=0.0), dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.5), dict(tp=99), dict(tb=99),
                 dict(dp=99), dict(db=99), dict(ws_ptr=ctypes.c_void_p(4104)), dict(target=ctypes.c_void_p(4097))):
         assert call(**bad) == _hip.KA_ERR_BAD_ARG, bad
-    for far in (dict(k=65), dict(vocab=1 << 22, tb=1 << 30, tp=1 << 23, db=1 << 30, dp=1 << 23), dict(batch=65536)):
+    for far in (dict(k=65), dict(vocab=1 << 22, tb=1 << 30, tp=1 << 23, db=1 << 30, dp=1 << 23), dict(batch=65536), dict(batch=65535, k=64)):
         assert call(**far) == _hip.KA_ERR_UNSUPPORTED, far
     assert call(ws_bytes=ws(0, 2, 4, 100) - 1) == _hip.KA_ERR_WORKSPACE
     assert call(ws_ptr=None) == _hip.KA_ERR_WORKSPACE and b"workspace" in lib.ka_last_error()

@@ -244,3 +244,34 @@ def test_graph_replay_and_two_streams(sampler):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
         assert all(torch.equal(a, b) for a, b in zip(other, want[(i + 1) % 3]))
+
+
+def test_the_largest_number_of_tokens(sampler):
+    """2^20 tokens: every tile list at its longest; a second call of the same tokens in another order gives every token the same bits."""
+    n, h, o, r, s = 1 << 20, 8, 16, 4, 1023
+    g = torch.Generator(device="cuda").manual_seed(21)
+    rnd = lambda *shape: torch.randn(*shape, generator=g, device="cuda").bfloat16()  # noqa: E731
+    base, hidden, a, b = rnd(n, o), rnd(n, h), rnd(s, r, h), rnd(s, o, r)
+    ids = torch.randint(-1, s + 1, (n,), generator=g, device="cuda")
+    out, u = sampler.lora_linear(base, hidden, a, b, ids, 0.5, return_shrunk=True)
+    some = torch.randint(0, n, (4000,), generator=g, device="cuda")
+    some[0], some[1] = 0, n - 1
+    pick = lambda t: t[some].cpu()  # noqa: E731
+    y, want_u, ey, eu = lora_ref.forward(pick(base), pick(hidden), a.cpu(), b.cpu(), pick(ids), torch.full((s,), 0.5))
+    _within(out[some], y, ey, "out")
+    _within(u[some], want_u, eu, "shrunk")
+    order = torch.randperm(n, generator=g, device="cuda")
+    assert torch.equal(sampler.lora_linear(base[order], hidden[order], a, b, ids[order], 0.5), out[order])
+    dx, da, db = sampler.lora_linear_backward(base, hidden, a, b, ids, 0.5, u)
+    got = [x.clone() for x in (da, db)]
+    # an adapter's gradients are sums over its tokens alone: those of a few adapters, in fp64
+    for i in (0, 511, 1022):
+        mine = ids == i
+        c = [t[mine].cpu() for t in (base, hidden, u)]
+        want, bound = lora_ref.backward(c[0], c[1], a[i:i + 1].cpu(), b[i:i + 1].cpu(), torch.zeros(len(c[0]), dtype=torch.int64),
+                                        torch.full((1,), 0.5), c[2], None)
+        _within(dx[mine], want[0], bound[0], "dhidden")
+        _within(got[0][i:i + 1], want[1], bound[1], "dlora_a")
+        _within(got[1][i:i + 1], want[2], bound[2], "dlora_b")
+    with pytest.raises(ValueError, match="tokens"):
+        sampler.lora_linear(rnd(n + 1, 1), rnd(n + 1, 1), rnd(1, 1, 1), rnd(1, 1, 1), torch.zeros(n + 1, dtype=torch.int64, device="cuda"))
