@@ -820,6 +820,20 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
 }
 
 // ---------------------------------------------------------------------------
+// lora_fold_parts: grid (elements / 256, groups).  Sums of 32 neighbouring partial results, all requested together, where there
+// are so many that the few workgroups of lora_pack would wait for them one after the other (512 tokens, rank 128, 501 parts: 235 us in
+// lora_pack alone, @FOLD@ so).
+// ---------------------------------------------------------------------------
+constexpr int FOLD_PARTS = 32;
+__global__ __launch_bounds__(THREADS) void lora_fold_parts(const float *__restrict__ part, int parts, int64_t elements, float *__restrict__ out) {
+    const int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x;
+    if (i >= elements) return;
+    const int first = int(blockIdx.y) * FOLD_PARTS;
+    const float *at = part + int64_t(first) * elements + i;
+    out[int64_t(blockIdx.y) * elements + i] = add_some<FOLD_PARTS>(0.0f, at, parts - first, elements);
+}
+
+// ---------------------------------------------------------------------------
 // lora_pack: grid (tiles of the first list).  u, or the sum of the partial results of dy B times s_a, for every 32 tokens of an
 // adapter in the layout and precision the matrix cores take it in, so that the workgroups of the two passes over the data load
 // fragments and split nothing:
@@ -1269,7 +1283,7 @@ inline FwdLayout fwd_layout(const Shape &d) {
 }
 
 // The backward: outputs per wavefront (64 G) of the first pass, tokens per tile of both.
-struct BwdLayout { PlanLayout plan; int64_t slots[2], blocks[2]; int groups; size_t packed, du_part, db_part, da_part, total; };
+struct BwdLayout { PlanLayout plan; int64_t slots[2], blocks[2], folded; int groups; size_t packed, du_part, du_fold, db_part, da_part, total; };
 // Tokens per tile such that `blocks` times the tiles make about `want` workgroups.
 inline int64_t bwd_tile(int64_t n, int64_t blocks, int64_t want) {
     const int64_t tiles = ceil_div(want, blocks);
@@ -1283,16 +1297,20 @@ inline BwdLayout bwd_layout(const Shape &d) {
     l.groups = padded_rank(d.r) == 16 && ceil_div(d.n, 64) * ceil_div(small_blocks, 4) >= 512 ? 4 : 1;
     l.blocks[0] = ceil_div(d.o, 64 * WAVES * l.groups);
     l.blocks[1] = ceil_div(d.h, 64 * WAVES);
-    const int64_t tile0 = bwd_tile(d.n, l.blocks[0], 1024), tile1 = bwd_tile(d.n, l.blocks[1], 512);
+    // as many workgroups as the registers of the two kernels let reside at once
+    const int64_t rp = padded_rank(d.r);
+    const int64_t tile0 = bwd_tile(d.n, l.blocks[0], rp == 16 ? 1024 : (rp == 32 ? 512 : 256));
+    const int64_t tile1 = bwd_tile(d.n, l.blocks[1], rp == 128 ? 256 : 512);
     l.slots[0] = d.n / tile0;
     l.slots[1] = d.n / tile1;
     l.plan = plan_layout(d.n, d.s, tile0, tile1);
     // fragments of u, then of dy B in the same place: 3 + 2 (or 4) KB per 32 tokens and 16 (or 32) ranks
-    const int64_t rp = padded_rank(d.r);
     const size_t chunk = size_t(rp) / 16 * 3 * 1024 + (rp == 16 ? 2048 : size_t(rp) / 32 * 4 * 1024);
     l.packed = l.plan.total;
     l.du_part = l.packed + align_up(size_t(d.n / 32 + d.s + 1) * chunk);
-    l.db_part = l.du_part + align_up(size_t(l.blocks[0]) * d.n * d.r * 4);
+    l.du_fold = l.du_part + align_up(size_t(l.blocks[0]) * d.n * d.r * 4);
+    l.folded = l.blocks[0] > FOLD_PARTS ? ceil_div(l.blocks[0], FOLD_PARTS) : 0;
+    l.db_part = l.du_fold + align_up(size_t(l.folded) * d.n * d.r * 4);
     l.da_part = l.db_part + align_up(size_t(l.slots[0]) * d.o * d.r * 4);
     l.total = l.da_part + align_up(size_t(l.slots[1]) * d.h * d.r * 4);
     return l;
@@ -1534,7 +1552,14 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     });
     rc = check_hip(hipGetLastError(), "lora backward launch (out)");
     if (rc != KA_OK) return rc;
-    rc = pack(du_part, l.blocks[0], true);
+    float *du_fold = reinterpret_cast<float *>(ws + l.du_fold);
+    if (l.folded > 0) {
+        hipLaunchKernelGGL(lora_fold_parts, dim3(unsigned(ceil_div(n_tokens * rank, THREADS)), unsigned(l.folded)), dim3(THREADS), 0, stream,
+                           du_part, int(l.blocks[0]), n_tokens * rank, du_fold);
+        rc = check_hip(hipGetLastError(), "lora backward launch (fold)");
+        if (rc != KA_OK) return rc;
+    }
+    rc = l.folded > 0 ? pack(du_fold, l.folded, true) : pack(du_part, l.blocks[0], true);
     if (rc != KA_OK) return rc;
     BwdInArgs ia{};
     ia.x = hidden;
