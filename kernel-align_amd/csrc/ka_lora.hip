@@ -24,6 +24,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int MAX_RANK = KA_LORA_MAX_RANK;
 constexpr int MAX_ADAPTERS = KA_LORA_MAX_ADAPTERS;
@@ -943,6 +944,8 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
     constexpr int RED = RF < 4 ? RF : 4;  // groups of sixteen ranks that cross the wavefronts at a time
     __shared__ __attribute__((aligned(16))) int32_t tokens[BWD_TILE_MAX];
     __shared__ f32x4 red[WAVES][32][RED * 4];
+    constexpr int US = RF * 3 * kWave, US_PER = (US + THREADS - 1) / THREADS;
+    __shared__ u32x4 us[US];  // fragments of u for the step, the same for every wavefront
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
     if (int(blockIdx.y) >= *p.plan.list[0].count) return;
     const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];
@@ -982,7 +985,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) col8[g][ks] = lane_column<MODE>(o0 + g * 64 + ks * 32 + 8 * quad, p.o);
     }
-    const uint4 *const packed = p.u + int64_t(tile.start / 32 + tile.adapter) * Packed<RP>::kColumns + lane;
+    const u32x4 *const packed = reinterpret_cast<const u32x4 *>(p.u) + int64_t(tile.start / 32 + tile.adapter) * Packed<RP>::kColumns + tid;
     auto request = [&](int c, uint2 (&w)[G][8]) {
         int32_t tk[8];
         eight_tokens(tokens + c + 8 * quad, tk);
@@ -994,8 +997,10 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
         }
     };
     auto step = [&](int c, const uint2 (&w)[G][8], uint2 (&next)[G][8]) {
-        // the step's own remaining loads first (they come from cache), then the next step's
-        uint4 fy[G][2][2], v[RF][3];
+        // the step's own remaining loads first (they come from cache), then the next step's; none behind those, since loads are
+        // waited for in their order
+        uint4 fy[G][2][2];
+        u32x4 next_u[US_PER];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const row_offset_t<MODE> at = row_offset<MODE>(tokens[c + 16 * s + col], p.dy_stride);
@@ -1004,12 +1009,10 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) fy[g][ks][s] = row_load8<T, MODE>(p.dy, at, col8[g][ks], p.o);
         }
-        const uint4 *pu = packed + int64_t(c / 32) * Packed<RP>::kColumns;
+        const int then = c + 32 < tile.count ? c + 32 : c;
 #pragma unroll
-        for (int f = 0; f < RF; ++f)
-#pragma unroll
-            for (int k = 0; k < 3; ++k) v[f][k] = pu[(f * 3 + k) * kWave];
-        request(c + 32 < tile.count ? c + 32 : c, next);
+        for (int i = 0; i < US_PER; ++i) next_u[i] = packed[int64_t(then / 32) * Packed<RP>::kColumns + i * THREADS];
+        request(then, next);
         f32x4 du[2][RF];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -1022,9 +1025,13 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) as_bf16<T>(frag[e], part[e]);
 #pragma unroll
-            for (int f = 0; f < RF; ++f)
+            for (int f = 0; f < RF; ++f) {
+                uint4 v[3];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[g][f][e] = outer<T>(part[e], v[f], acc[g][f][e]);
+                for (int k = 0; k < 3; ++k) v[k] = __builtin_bit_cast(uint4, us[(f * 3 + k) * kWave + lane]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[g][f][e] = outer<T>(part[e], v, acc[g][f][e]);
+            }
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -1033,9 +1040,13 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
                     for (int f = 0; f < RF; ++f) du[s][f] = mfma<T>(fb[g][ks][f], fy[g][ks][s], du[s][f]);
         }
         // dy B of the workgroup's outputs: the wavefronts' parts in their order
+        lds_barrier();  // the previous sums and the step's u are read
+#pragma unroll
+        for (int i = 0; i < US_PER; ++i)
+            if (i * THREADS + tid < US) us[i * THREADS + tid] = next_u[i];
 #pragma unroll
         for (int f0 = 0; f0 < RF; f0 += RED) {
-            lds_barrier();  // the previous sums are read
+            if (f0 > 0) lds_barrier();
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -1056,7 +1067,16 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
         }
     };
     uint2 even[G][8], odd[G][8];
-    request(0, even);
+    {
+        u32x4 first_u[US_PER];
+#pragma unroll
+        for (int i = 0; i < US_PER; ++i) first_u[i] = packed[i * THREADS];
+        request(0, even);
+#pragma unroll
+        for (int i = 0; i < US_PER; ++i)
+            if (i * THREADS + tid < US) us[i * THREADS + tid] = first_u[i];
+        lds_barrier();
+    }
     for (int c = 0; c < tile.count; c += 64) {
         step(c, even, odd);
         if (c + 32 >= tile.count) break;
