@@ -823,7 +823,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
 // ---------------------------------------------------------------------------
 // lora_fold_parts: grid (elements / 256, groups).  Sums of 32 neighbouring partial results, all requested together, where there
 // are so many that the few workgroups of lora_pack would wait for them one after the other (512 tokens, rank 128, 501 parts: 235 us in
-// lora_pack alone, @FOLD@ so).
+// lora_pack alone, 21 + 10 us so).
 // ---------------------------------------------------------------------------
 constexpr int FOLD_PARTS = 32;
 __global__ __launch_bounds__(THREADS) void lora_fold_parts(const float *__restrict__ part, int parts, int64_t elements, float *__restrict__ out) {
@@ -1292,7 +1292,9 @@ inline FwdLayout fwd_layout(const Shape &d) {
     FwdLayout l;
     l.plan = plan_layout(d.n, d.s, FWD_TILE, 0);
     l.segments = ceil_div(d.h, SEG_STEPS * 32);
-    l.split = l.segments > 1 && l.plan.max_tiles[0] < 256;
+    // a workgroup per segment of H where the tiles alone are fewer than two per CU: 32 tokens, rank 64, H = O = 4096: 24 us a call,
+    // 33 without; 8192 tokens, rank 16: 71 and 77
+    l.split = l.segments > 1 && l.plan.max_tiles[0] < 512;
     l.part = l.plan.total;
     l.u = l.part + (l.split ? align_up(size_t(l.segments) * d.n * d.r * 4) : 0);
     l.packed = l.u + align_up(size_t(d.n) * d.r * 4);
@@ -1313,8 +1315,10 @@ inline int64_t bwd_tile(int64_t n, int64_t blocks, int64_t want) {
 inline BwdLayout bwd_layout(const Shape &d) {
     BwdLayout l;
     const int64_t small_blocks = ceil_div(d.o, 64 * WAVES);
-    // 1024 outputs per workgroup where that leaves work for every CU: fewer partial sums of dy B
-    l.groups = padded_rank(d.r) == 16 && ceil_div(d.n, 64) * ceil_div(small_blocks, 4) >= 512 ? 4 : 1;
+    // 1024 outputs per workgroup instead of 256 where there are several rounds of workgroups all the same: fewer partial sums of
+    // dy B, fewer wavefronts at a time.  us a call with 1024 and 256, rank 16: 1024 tokens x 128,256 outputs 145 / 135, 8192 x 14,336
+    // 194 / 181, 2048 x 128,256 224 / 230, 8192 x 32,000 258 / 268, 4096 x 128,256 369 / 403.
+    l.groups = padded_rank(d.r) == 16 && ceil_div(d.n, 64) * ceil_div(small_blocks, 4) >= 4000 ? 4 : 1;
     l.blocks[0] = ceil_div(d.o, 64 * WAVES * l.groups);
     l.blocks[1] = ceil_div(d.h, 64 * WAVES);
     // as many workgroups as the registers of the two kernels let reside at once
@@ -1394,8 +1398,10 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     const LoraPlan plan = plan_at(ws, l.plan);
-    // one workgroup per token and segment, and the plan made by one more: up to 2 MB of A per 16 KB of x, all from L2
-    const bool one = n_tokens * rank <= 2048 && n_tokens <= 256;
+    // Few tokens: one workgroup per token and segment, which needs no plan, and the plan made by one more beside them; every token
+    // reads its A from L2.  H = O = 4096, us a call with and without: 1 token, rank 16: 23 / 29; 512, rank 16: 26 / 30;
+    // 1024, rank 16: 41 / 28; 128, rank 64: 25 / 31; 512, rank 32: 35 / 29.
+    const bool one = n_tokens * rank <= 8192 && n_tokens <= 512;
     if (!one) {
         hipLaunchKernelGGL(lora_plan, dim3(1), dim3(PLAN_THREADS), 0, stream, adapter_ids, int(n_tokens), int(n_adapters), 1, plan);
         rc = check_hip(hipGetLastError(), "lora launch (plan)");
