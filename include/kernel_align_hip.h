@@ -212,9 +212,9 @@ int ka_sample_mass_fixed(const float *d, int64_t n, uint64_t *out, void *hip_str
  * decided exactly, on integers of up to 126 bits.  uniforms: fp32 [batch, max_draft + 1] in [0, 1).
  * out_policy_logprob (optional, fp32 [batch, max_draft + 1]): log-probability of every emitted token under the unfiltered
  * softmax of its target row (to 1e-5 what ka_logprob_* returns), 0 behind the last.
- * Limits: max_draft <= KA_VERIFY_MAX_DRAFT, vocab < 2^22, batch <= 65535.  The workspace is 16-byte aligned, of
+ * Limits: max_draft <= KA_VERIFY_MAX_DRAFT, vocab < 2^22, batch <= 65535, batch (2 max_draft + 1) < 2^23.  The workspace is 16-byte aligned, of
  * ka_verify_workspace_bytes (0 for arguments the call refuses): 48 bytes per row and 40 per request and share of 256
- * 16-byte vectors.  Any alignment of the rows is taken.  No counterpart in the reference, whose sampler draws one token per
+ * 16-byte vectors, and for up to 160 fp16 / fp32 rows of more than 32 KB another 39 KB each.  Any alignment of the rows is taken.  No counterpart in the reference, whose sampler draws one token per
  * forward pass (rl_engine/kernels/sampling.py:39-88).
  */
 #define KA_VERIFY_MAX_DRAFT 64
@@ -243,9 +243,9 @@ int ka_verify_draft(int dtype, const void *target_logits, int64_t target_batch_s
  *     dlora_b[a]    = sum over the adapter's tokens of grad_out[n, :]^T u[n, :]         fp32 [n_adapters, out_dim, rank]
  * Sums run in a fixed order (a function of the shapes and the ids); an adapter without tokens gets zeros.
  *
- * Any alignment and any rank, width and token count up to the limits; multiples of eight on 16-byte aligned rows take
- * 16-byte accesses.  The workspace is 16-byte aligned, of ka_lora_workspace_bytes (0 for arguments the calls refuse).  No
- * counterpart in the reference, which names no adapters.
+ * Any alignment and any rank, width and token count up to the limits (multiples of eight on 16-byte aligned rows cost the
+ * fewest instructions).  The workspace is 16-byte aligned, of ka_lora_workspace_bytes (0 for arguments the calls refuse); the
+ * backward's holds 4 rank bytes per token and 256 outputs, and partial gradients.  No counterpart in the reference, which names no adapters.
  */
 #define KA_LORA_MAX_RANK 128
 #define KA_LORA_MAX_ADAPTERS 1023

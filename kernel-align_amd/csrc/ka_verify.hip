@@ -224,7 +224,8 @@ template <typename T> __device__ __forceinline__ float cut_value(uint32_t raw_cu
 // ordinary maximum.  Masses are then evaluated once per occupied bin instead of once per entry (by all threads where a sum
 // over the whole row is needed), and one wavefront walks the bins from the largest value down to the cuts, 64 at a time.  Rows
 // it cannot describe (values of 2^8 and above, NaN, a maximum or a cut among the small values, dropped values that would
-// count) take the radix path.
+// count) take the radix path.  Measured, bf16, 128,256 entries: 576 rows (64 requests x 4 drafts, 148 MB) 50 - 52 us, 2.9 TB/s, of which
+// the stream takes about 30 and the masses and the walk behind it, which all rows reach together, the rest; 2304 rows, ragged: 109 us.
 // ---------------------------------------------------------------------------
 constexpr uint32_t MAG_LOW = 0x3A00u, MAG_HIGH = 0x4380u;  // bits of 2^-11 and 2^8
 constexpr int HIST_SIDE = int(MAG_HIGH - MAG_LOW);         // values of one sign: 19 octaves of 128
@@ -1310,7 +1311,7 @@ __global__ __launch_bounds__(SHARE_THREADS) void verify_shares(VerifyParams p) {
 // The same for bf16 rows of which many entries survive (no top-k, or a large one): the masses come from two tables in LDS, one
 // value per bin of verify_rows, so that an entry costs two reads of LDS instead of two evaluations of the mass polynomial.
 // Entries outside the bins (about one in 10^4) are evaluated.  A workgroup builds the tables (9728 evaluations) for
-// shares_per_group shares.  grid (groups, B)
+// shares_per_group shares.  grid (groups, B)  64 requests, two rows of 128,256 each (66 MB): 26 us, a third of it the tables.
 constexpr int TABLE_THREADS = 512;
 constexpr size_t TABLE_LDS_BYTES = size_t(2) * HIST_BINS * sizeof(double);
 __global__ __launch_bounds__(TABLE_THREADS) void verify_shares_table(VerifyParams p) {
@@ -1417,6 +1418,8 @@ template <typename T> __device__ __forceinline__ int exact_draw(Residual<T> res,
 }
 
 // grid B; a thread per vector of the share that holds the draw
+// verify_draw: grid (B).  Bound by its chain of waits, not by what it reads: the request's summaries, its shares, two vectors; 7.5 us for
+// one request, 11.5 for 64, 14.5 where top-p cuts inside tie groups, 17 for 256.
 template <typename T>
 __global__ __launch_bounds__(SHARE_VECS) void verify_draw(VerifyParams p) {
     constexpr int WAVES = SHARE_VECS / kWave, EPV = T::kPerVec;
