@@ -801,6 +801,11 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[e] = mfma<T>(st.b[ks][e], f, acc[e]);
                 }
+            // (0 times an infinity of the rows that were read in their place would not be 0)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[e][i] = tile.adapter >= 0 ? acc[e][i] : 0.0f;
             if constexpr (T::kDtype == KA_DTYPE_F16) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[e] *= up[s];
@@ -1193,14 +1198,16 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
             f32x4 sum[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum[e] = f32x4{0, 0, 0, 0};
+            if (has) {  // (A of another adapter was read in its place: 0 times its infinities would not be 0)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+                for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int k = 0; k < HL; ++k)
+                    for (int k = 0; k < HL; ++k)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
+                        for (int e = 0; e < 4; ++e)
 #pragma unroll
-                        for (int q = 0; q < NP; ++q) sum[e] = mfma<Bf16>(fa[ks][e][q], rows[s][ks][k], sum[e]);
+                            for (int q = 0; q < NP; ++q) sum[e] = mfma<Bf16>(fa[ks][e][q], rows[s][ks][k], sum[e]);
+            }
             if (c + 16 * s + col < tile.count)
                 base[s].store(static_cast<typename T::raw_t *>(p.dx) + int64_t(tokens[c + 16 * s + col]) * p.dx_stride, out_col, p.h, sum);
         }
@@ -1398,6 +1405,9 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
     if (hidden == nullptr || lora_a == nullptr || adapter_ids == nullptr || (out != nullptr && (base == nullptr || lora_b == nullptr)) ||
         (out == nullptr && out_shrunk == nullptr))
         return fail(KA_ERR_BAD_ARG, "lora: null base / hidden / lora_a / lora_b / adapter_ids / out pointer");
+    if ((reinterpret_cast<uintptr_t>(base) | reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(lora_a) |
+         reinterpret_cast<uintptr_t>(lora_b) | reinterpret_cast<uintptr_t>(out)) % 2 != 0)
+        return fail(KA_ERR_BAD_ARG, "lora: a matrix is not aligned to its elements");
     if ((out != nullptr && (base_stride < out_dim || out_stride < out_dim)) || hidden_stride < in_dim)
         return fail(KA_ERR_BAD_ARG, "lora: a row stride is smaller than its row");
     const FwdLayout l = fwd_layout(d);
@@ -1522,6 +1532,9 @@ KA_EXPORT int ka_lora_linear_backward(int dtype, const void *grad_out, int64_t g
     if (grad_out == nullptr || hidden == nullptr || lora_a == nullptr || lora_b == nullptr || adapter_ids == nullptr ||
         shrunk == nullptr || dhidden == nullptr || dlora_a == nullptr || dlora_b == nullptr)
         return fail(KA_ERR_BAD_ARG, "lora backward: null grad_out / hidden / lora_a / lora_b / adapter_ids / shrunk / result pointer");
+    if ((reinterpret_cast<uintptr_t>(grad_out) | reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(lora_a) |
+         reinterpret_cast<uintptr_t>(lora_b) | reinterpret_cast<uintptr_t>(dhidden_base) | reinterpret_cast<uintptr_t>(dhidden)) % 2 != 0)
+        return fail(KA_ERR_BAD_ARG, "lora backward: a matrix is not aligned to its elements");
     if (grad_stride < out_dim || hidden_stride < in_dim || dhidden_stride < in_dim || (dhidden_base != nullptr && dhidden_base_stride < in_dim))
         return fail(KA_ERR_BAD_ARG, "lora backward: a row stride is smaller than its row");
     const BwdLayout l = bwd_layout(d);

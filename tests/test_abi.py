@@ -195,7 +195,7 @@ def test_verify_argument_checks_and_workspace_size():
 
 def test_lora_argument_checks_and_workspace_size():
     lib = _hip.load()
-    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4104)
+    p, odd, half = ctypes.c_void_p(4096), ctypes.c_void_p(4104), ctypes.c_void_p(4097)
     ws = lib.ka_lora_workspace_bytes
     assert ws(0, 64, 64, 16, 1, 0) == 0 and ws(8, 64, 64, 129, 1, 0) == 0 and ws(8, 64, 64, 16, 1024, 1) == 0
     assert ws(8, 64, 64, 16, 1, 0) > 0 and ws(8, 64, 64, 16, 1, 1) > 0
@@ -210,14 +210,16 @@ def test_lora_argument_checks_and_workspace_size():
 
     assert fwd(n=0, base=None) == _hip.KA_OK
     for bad in (dict(dtype=2), dict(n=-1), dict(h=0), dict(o=0), dict(r=0), dict(s=0), dict(base=None), dict(hid=None),
-                dict(a=None), dict(b=None), dict(ids=None), dict(out=None), dict(bs=63), dict(os=63), dict(hs=31), dict(w=odd)):
+                dict(a=None), dict(b=None), dict(ids=None), dict(out=None), dict(bs=63), dict(os=63), dict(hs=31), dict(w=odd),
+                dict(base=half), dict(hid=half), dict(a=half), dict(b=half), dict(out=half)):
         assert fwd(**bad) == _hip.KA_ERR_BAD_ARG, bad
     for bad in (dict(dtype=2), dict(n=0), dict(n=-1), dict(g=None), dict(hid=None), dict(a=None), dict(b=None), dict(ids=None),
                 dict(u=None), dict(dx=None), dict(da=None), dict(db=None), dict(gs=63), dict(hs=31), dict(dxs=31),
-                dict(xb=p, xbs=31), dict(w=odd)):
+                dict(xb=p, xbs=31), dict(w=odd), dict(g=half), dict(hid=half), dict(a=half), dict(b=half), dict(dx=half),
+                dict(xb=half, xbs=32)):
         assert bwd(**bad) == _hip.KA_ERR_BAD_ARG, bad
     for call in (fwd, bwd):
-        for far in (dict(r=129), dict(s=1024), dict(n=(1 << 21) + 1), dict(h=1 << 24), dict(o=1 << 24)):
+        for far in (dict(r=129), dict(s=1024), dict(n=(1 << 20) + 1), dict(h=1 << 24), dict(o=1 << 24)):
             assert call(**far) == _hip.KA_ERR_UNSUPPORTED, far
         assert call(w=None) == _hip.KA_ERR_WORKSPACE
     assert fwd(wb=ws(4, 32, 64, 8, 2, 0) - 1) == _hip.KA_ERR_WORKSPACE

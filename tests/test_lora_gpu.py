@@ -275,3 +275,30 @@ def test_the_largest_number_of_tokens(sampler):
         _within(got[1][i:i + 1], want[2], bound[2], "dlora_b")
     with pytest.raises(ValueError, match="tokens"):
         sampler.lora_linear(rnd(n + 1, 1), rnd(n + 1, 1), rnd(1, 1, 1), rnd(1, 1, 1), torch.zeros(n + 1, dtype=torch.int64, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [5, 700])
+@pytest.mark.parametrize("o", [136, 139])
+def test_infinities_of_an_adapter_stay_with_its_tokens(sampler, dtype, n, o):
+    """Adapter 0 diverged (infinities and NaN in both matrices): tokens of other adapters, and those without one, keep their results."""
+    c = _inputs(n, 72, o, 12, 3, dtype, seed=n)
+    c["ids"] = torch.arange(n) % 4 - 1
+    d = {k: v.cuda() for k, v in c.items()}
+    run = lambda a, b: (sampler.lora_linear(d["base"], d["hidden"], a, b, d["ids"], d["scaling"], return_shrunk=True))  # noqa: E731
+    back = lambda a, b, u: sampler.lora_linear_backward(d["dy"], d["hidden"], a, b, d["ids"], d["scaling"], u, d["dx"])  # noqa: E731
+    want, u = run(d["a"], d["b"])
+    grads = back(d["a"], d["b"], u)
+    a, b = d["a"].clone(), d["b"].clone()
+    a[0, 0, :] = float("inf")
+    a[0, :, 3] = float("nan")
+    b[0, :, 0] = float("inf")
+    b[0, 5, :] = float("nan")
+    out, u_bad = run(a, b)
+    bad = back(a, b, u_bad)
+    others = d["ids"] != 0
+    assert torch.equal(out[others], want[others]) and torch.equal(bad[0][others], grads[0][others])
+    assert torch.equal(out[d["ids"] < 0], d["base"][d["ids"] < 0]) and torch.equal(bad[0][d["ids"] < 0], d["dx"][d["ids"] < 0])
+    for got, w in zip(bad[1:], grads[1:]):
+        assert torch.equal(got[1:], w[1:])
+    assert not torch.isfinite(out[d["ids"] == 0]).any(1).all()
