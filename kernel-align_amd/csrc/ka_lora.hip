@@ -164,26 +164,8 @@ __device__ __forceinline__ void make_plan(PlanShared<PLAN_THREADS> &sh, const in
     }
     if (tid < lists) *plan.list[tid].count = total[tid];
     __syncthreads();
-    // up to 64 groups: lane l keeps the next position of group l in a register
-    const bool in_lanes = s + 1 <= kWave;
-    int next = in_lanes && lane <= s ? at[wave][lane] : 0;
     for (int st = s0; st < s1; st += U) {
         if (per > U) load(st);
-        if (in_lanes) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                uint64_t left = __ballot(a[u] >= 0);
-                while (left != 0) {  // one turn per adapter that occurs in the step
-                    const int want = __builtin_amdgcn_readlane(a[u], __ffsll((long long)left) - 1);
-                    const uint64_t same = __ballot(a[u] == want);
-                    const int base = __builtin_amdgcn_readlane(next, want);
-                    if (a[u] == want) plan.order[base + __popcll(same & ((uint64_t(1) << lane) - 1))] = (st + u) * kWave + lane;
-                    next += lane == want ? __popcll(same) : 0;
-                    left &= ~same;
-                }
-            }
-            continue;
-        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             uint64_t left = __ballot(a[u] >= 0);
