@@ -12,6 +12,7 @@
 // Numbers.  Products of two 16-bit matrices (x A^T, dy B) run in their own type with fp32 accumulation.  u and du are fp32 and
 // stay so: an operand of a product with them is split into bf16 parts, high + low (17 bits: for results that are rounded
 // to 16 bits) or high + middle + low (24 bits: for the fp32 gradients); an fp16 operand next to them is split into two bf16 (11 bits, exact).
+// The forward of fp16 splits u into two fp16 instead, after a power of two per token (22 bits), and multiplies fp16 by fp16.
 // Every sum runs in a fixed order: no atomics on floating-point values.
 #include <type_traits>
 
@@ -1342,7 +1343,7 @@ inline BwdLayout bwd_layout(const Shape &d) {
 
 inline bool aligned16(const void *p, int64_t stride) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0); }
 
-// Calls launch(type, padded rank, vector accesses), each as a compile-time value.
+// Calls launch(type, padded rank[, row mode]), each as a compile-time value.
 template <typename F> void with_types(int dtype, int rp, F &&launch) {
     auto ranks = [&](auto type) {
         if (rp == 16) launch(type, std::integral_constant<int, 16>{});

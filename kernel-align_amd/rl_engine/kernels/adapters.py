@@ -5,6 +5,8 @@ token adds its own adapter's product.  The reference has no counterpart.  ``Samp
 """
 from __future__ import annotations
 
+from functools import cached_property, lru_cache
+
 import torch
 
 from rl_engine.kernels import _hip
@@ -29,6 +31,11 @@ def _stride(rows):
 
 
 class AdapterOps:
+    @cached_property
+    def _lora_workspace_bytes(self):
+        """The library's query, remembered by shape: a call of it costs as much host time as a kernel launch."""
+        return lru_cache(maxsize=1024)(self._lib.ka_lora_workspace_bytes)
+
     def _check_adapters(self, hidden, lora_a, lora_b, adapter_ids, scaling):
         """Shapes of one call: (hidden rows, A, B, ids, scaling tensor or None, scaling number)."""
         for t, name in ((hidden, "hidden"), (lora_a, "lora_a"), (lora_b, "lora_b")):
@@ -75,7 +82,7 @@ class AdapterOps:
         n, (s, r, h), o = hidden.shape[0], a.shape, b.shape[1]
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         with _on_device(hidden.device):
-            ws_bytes = self._lib.ka_lora_workspace_bytes(n, h, o, r, s, 0)
+            ws_bytes = self._lora_workspace_bytes(n, h, o, r, s, 0)
             with self._scratch(ws_bytes, hidden.device) as ws_ptr:
                 status = self._lib.ka_lora_linear(
                     _DTYPE_CODE[hidden.dtype], ptr(base), 0 if base is None else _stride(base), hidden.data_ptr(),
@@ -168,7 +175,7 @@ class AdapterOps:
         da = torch.empty(s, r, h, dtype=torch.float32, device=dev)
         db = torch.empty(s, o, r, dtype=torch.float32, device=dev)
         with _on_device(dev):
-            ws_bytes = self._lib.ka_lora_workspace_bytes(n, h, o, r, s, 1)
+            ws_bytes = self._lora_workspace_bytes(n, h, o, r, s, 1)
             with self._scratch(ws_bytes, dev) as ws_ptr:
                 status = self._lib.ka_lora_linear_backward(
                     _DTYPE_CODE[hidden.dtype], dy.data_ptr(), _stride(dy), rows.data_ptr(), _stride(rows), a.data_ptr(),

@@ -5,6 +5,8 @@ The reference has no counterpart: its ``sample`` (rl_engine/kernels/sampling.py:
 """
 from __future__ import annotations
 
+from functools import cached_property, lru_cache
+
 import torch
 
 from rl_engine.kernels import _hip
@@ -15,6 +17,11 @@ MAX_DRAFT = 64  # KA_VERIFY_MAX_DRAFT
 
 
 class SpeculativeOps:
+    @cached_property
+    def _verify_workspace_bytes(self):
+        """The library's query, remembered by shape."""
+        return lru_cache(maxsize=1024)(self._lib.ka_verify_workspace_bytes)
+
     @torch.inference_mode()
     def verify_draft(self, target_logits, draft_ids, uniforms=None, draft_logits=None, draft_lens=None, top_k=None,
                      top_p=None, temperature=1.0, generator=None, return_policy_logprob=False):
@@ -89,7 +96,7 @@ class SpeculativeOps:
             code = _DTYPE_CODE[target_logits.dtype]
             ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
             with _on_device(dev):
-                ws_bytes = self._lib.ka_verify_workspace_bytes(code, batch, k, vocab)
+                ws_bytes = self._verify_workspace_bytes(code, batch, k, vocab)
                 with self._scratch(ws_bytes, dev) as ws_ptr:
                     status = self._lib.ka_verify_draft(
                         code, target.data_ptr(), *t_strides, ptr(draft), *d_strides, ids.data_ptr(), ptr(lens),

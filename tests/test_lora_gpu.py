@@ -302,3 +302,58 @@ def test_infinities_of_an_adapter_stay_with_its_tokens(sampler, dtype, n, o):
     for got, w in zip(bad[1:], grads[1:]):
         assert torch.equal(got[1:], w[1:])
     assert not torch.isfinite(out[d["ids"] == 0]).any(1).all()
+
+
+def test_scratch_beyond_the_pool():
+    """Calls whose scratch does not fit the pool take memory of their own: the same bits, eager, on two streams at once and captured."""
+    from rl_engine.kernels.sampling import SamplerBackend
+
+    small, large = SamplerBackend(pool_bytes=1 << 16), SamplerBackend()
+    c = {k: v.cuda() for k, v in _inputs(300, 1100, 2000, 40, 3, torch.bfloat16, seed=23).items()}
+    args = (c["hidden"], c["a"], c["b"], c["ids"], c["scaling"])
+    assert small._lora_workspace_bytes(300, 1100, 2000, 40, 3, 1) > 1 << 20
+
+    def both(backend):
+        out, u = backend.lora_linear(c["base"], *args, return_shrunk=True)
+        return (out, u, *backend.lora_linear_backward(c["dy"], *args, u, c["dx"]))
+
+    want = both(large)
+    side, results = torch.cuda.Stream(), []
+    side.wait_stream(torch.cuda.current_stream())
+    for i in range(6):
+        with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
+            results.append(both(small))
+    torch.cuda.synchronize()
+    for got in results:
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both(small)
+    for _ in range(3):
+        with torch.inference_mode():
+            for x in got:
+                x.zero_()
+        both(small)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("o", [65544, 65541])
+def test_many_tokens_in_front_of_a_wide_output(sampler, dtype, o):
+    """The size from which the backward takes 1024 outputs per workgroup; the fp64 statement is evaluated on the GPU here."""
+    n, h, r, s = 4100, 72, 11, 2
+    g = torch.Generator(device="cuda").manual_seed(o)
+    rnd = lambda std, *shape: (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)  # noqa: E731
+    dy, hidden, a, b, dx_base = rnd(0.1, n, o), rnd(1.0, n, h), rnd(0.1, s, r, h), rnd(0.3, s, o, r), rnd(0.5, n, h)
+    ids = torch.randint(-1, s, (n,), generator=g, device="cuda")
+    scaling = torch.tensor([0.75, 1.25], device="cuda")
+    u = torch.randn(n, r, generator=g, device="cuda")
+    got = sampler.lora_linear_backward(dy, hidden, a, b, ids, scaling, u, dx_base)
+    with torch.device("cuda"):
+        want, bound = lora_ref.backward(dy, hidden, a, b, ids, scaling, u, dx_base)
+    for x, w, e, what in zip(got, want, bound, ("dhidden", "dlora_a", "dlora_b")):
+        assert ((x.double() - w).abs() - e).max().item() <= 0, what
+    again = sampler.lora_linear_backward(dy, hidden, a, b, ids, scaling, u, dx_base)
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
