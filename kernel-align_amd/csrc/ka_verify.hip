@@ -583,8 +583,7 @@ template <typename T> __device__ __forceinline__ uint32_t raw_key_of_cut(uint32_
 // values below 2^-11 or at the edge of the list, more than 2048 entries in it) takes the radix path.
 // ---------------------------------------------------------------------------
 // f(entry) for every entry of the row by the whole block, in any order; eight vectors in flight per lane, any alignment.
-// UNROLL: f is short enough to be written out for each of the eight.
-template <typename T, bool UNROLL, typename F> __device__ __forceinline__ void each_entry(const typename T::raw_t *rp, int vocab, F &&f) {
+template <typename T, typename F> __device__ __forceinline__ void each_entry(const typename T::raw_t *rp, int vocab, F &&f) {
     constexpr int EPV = T::kPerVec, U = 8;
     const int tid = threadIdx.x;
     int head = int((16 - (reinterpret_cast<uintptr_t>(rp) & 15)) & 15) / T::kBytes;
@@ -597,22 +596,11 @@ template <typename T, bool UNROLL, typename F> __device__ __forceinline__ void e
         uint4 q[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) q[u] = vp[v + u * S_THREADS < nvec ? v + u * S_THREADS : v];
-        if constexpr (UNROLL) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (v + u * S_THREADS >= nvec) continue;
+        for (int u = 0; u < U; ++u) {
+            if (v + u * S_THREADS >= nvec) continue;
 #pragma unroll
-                for (int j = 0; j < EPV; ++j) f(entry_of<T>(q[u], j));
-            }
-        } else {
-#pragma unroll 1
-            for (int u = 0; u < U; ++u) {
-                if (v + u * S_THREADS >= nvec) break;
-#pragma unroll
-                for (int j = 0; j < EPV; ++j) f(entry_of<T>(q[0], j));
-#pragma unroll
-                for (int t = 0; t + 1 < U; ++t) q[t] = q[t + 1];
-            }
+            for (int j = 0; j < EPV; ++j) f(entry_of<T>(q[u], j));
         }
     }
 }
@@ -646,7 +634,7 @@ template <typename T>
 __device__ __forceinline__ void coarse_masses(const typename T::raw_t *rp, int count, const Filter &f, bool want_lse, float xmax, uint32_t kmax,
                                               uint64_t *bins, uint64_t &all, uint64_t &raw) {
     const float vmax = value_of<T>(kmax);
-    each_entry<T, false>(rp, count, [&](typename T::raw_t r) {
+    each_entry<T>(rp, count, [&](typename T::raw_t r) {
         const float x = T::widen(r);
         if (want_lse) raw += raw_fix(x, xmax);
         const uint32_t key = elem_key<T>(r, f.temp, f.has_t);
@@ -693,7 +681,7 @@ __device__ __forceinline__ bool coarse_cut(CoarseRow &h, const typename T::raw_t
         if (tid == 0) { h.max_key = top; h.give_up = bad; }
     } else {
         uint32_t top = 0, bad = 0;
-        each_entry<T, true>(rp, vocab, [&](typename T::raw_t raw) {
+        each_entry<T>(rp, vocab, [&](typename T::raw_t raw) {
             const float x = T::widen(raw);
             const uint32_t key = masked_key<T>(x);
             top = key > top && x == x ? key : top;
@@ -755,7 +743,7 @@ __device__ __forceinline__ bool coarse_cut(CoarseRow &h, const typename T::raw_t
                 raw += parts[i].raw;
             }
         } else if (f.use_k) {
-            each_entry<T, true>(rp, vocab, [&](typename T::raw_t r) {
+            each_entry<T>(rp, vocab, [&](typename T::raw_t r) {
                 const float x = T::widen(r);
                 if (want_lse) raw += raw_fix(x, xmax);
                 if (x >= low) {
@@ -814,7 +802,7 @@ __device__ __forceinline__ bool coarse_cut(CoarseRow &h, const typename T::raw_t
             __syncthreads();
             if (h.ok == 0) return false;
             const float lo = h.edge_low, hi = h.edge_high;
-            each_entry<T, true>(rp, vocab, [&](typename T::raw_t raw) {
+            each_entry<T>(rp, vocab, [&](typename T::raw_t raw) {
                 const float x = T::widen(raw);
                 if (x >= lo && x < hi) {
                     const uint32_t at = atomicAdd(&h.n_list, 1u);
@@ -933,7 +921,7 @@ __device__ __forceinline__ RowRef row_ref(const VerifyParams &p, int64_t r) {
 // ---------------------------------------------------------------------------
 // fp16 and fp32 rows without top-k, in calls of few rows: the maximum, then the masses (which are 60 instructions an entry: one
 // CU takes 50 us for a row of 128,256), by a workgroup per 32 KB of every row.  grid (rows, parts) each; verify_rows goes on from the
-// bins.  8 requests x 2 drafts, fp32, top-p 0.9, 128,256 entries: 134 us in verify_rows alone, 6.6 + 28 + 26
+// bins.  8 requests x 2 drafts, fp32, top-p 0.9, 128,256 entries: 134 us in verify_rows alone, 6 + 26 + 26
 // us so; verify_split_mass is bound by its arithmetic.
 // ---------------------------------------------------------------------------
 constexpr int SPLIT_BYTES = 32768;
@@ -955,7 +943,7 @@ template <typename T> __global__ __launch_bounds__(S_THREADS) void verify_split_
     int first;
     const int count = split_span<T>(p, first);
     uint32_t top = 0, bad = 0;
-    each_entry<T, true>((x.target ? target_row<T>(p, x.b, x.j) : draft_row<T>(p, x.b, x.j)) + first, count, [&](typename T::raw_t raw) {
+    each_entry<T>((x.target ? target_row<T>(p, x.b, x.j) : draft_row<T>(p, x.b, x.j)) + first, count, [&](typename T::raw_t raw) {
         const float v = T::widen(raw);
         const uint32_t key = masked_key<T>(v);
         top = key > top && v == v ? key : top;
