@@ -1417,6 +1417,16 @@ __global__ __launch_bounds__(SHARE_VECS) void verify_draw(VerifyParams p) {
     __shared__ uint32_t s_rank[2];
     const int b = blockIdx.x, tid = threadIdx.x;
     const int len = draft_len(p, b);
+    // what thread j needs for its output at position j, ahead of the draw: the draft, its logit and the row's log-sum-exp
+    const bool has_row = tid <= len, has_draft = tid < len;
+    const int64_t drafted = has_draft ? p.draft_ids[int64_t(b) * p.k + tid] : -1;
+    double lse = 0.0;
+    float logit = 0.0f;
+    if (p.out_policy != nullptr && has_row) {
+        const RowSummary &row = p.rows[int64_t(b) * (p.k + 1) + tid];
+        if (drafted >= 0 && drafted < p.vocab) logit = T::widen(target_row<T>(p, b, tid)[drafted]);
+        lse = double(row.raw_top) + log(row.raw_sum);
+    }
     const int n = accepted_prefix(p, b, len);
     if (tid == 0) { s_share = s_hit = -1; s_cut[0] = s_cut[1] = -1; s_limit[0] = s_limit[1] = 0x7fffffff; }
     const float u = clean_uniform(p.uniforms[int64_t(b) * (p.k + 1) + p.k]);
@@ -1531,15 +1541,15 @@ __global__ __launch_bounds__(SHARE_VECS) void verify_draw(VerifyParams p) {
         hit = exact_draw<T>(res, u, p.n_shares, wave_buf.w, &s_hit);
     }
     // outputs: thread j writes position j
-    for (int j = tid; j <= p.k; j += SHARE_VECS) {
-        const int64_t at = int64_t(b) * (p.k + 1) + j;
-        const int64_t id = j < n ? p.draft_ids[int64_t(b) * p.k + j] : (j == n ? int64_t(hit) : int64_t(-1));
+    if (tid <= p.k) {
+        const int64_t at = int64_t(b) * (p.k + 1) + tid;
+        const int64_t id = tid < n ? drafted : (tid == n ? int64_t(hit) : int64_t(-1));
         p.out_ids[at] = id;
         if (p.out_policy != nullptr) {
             float lp = 0.0f;
-            if (j <= n) {
-                const double lse = double(p.rows[at].raw_top) + log(p.rows[at].raw_sum);
-                lp = id >= 0 ? float(double(T::widen(target_row<T>(p, b, j)[id])) - lse) : __builtin_nanf("");
+            if (tid <= n) {
+                if (tid == n && id >= 0) logit = T::widen(target_row<T>(p, b, tid)[id]);
+                lp = id >= 0 ? float(double(logit) - lse) : __builtin_nanf("");
             }
             p.out_policy[at] = lp;
         }
