@@ -1406,8 +1406,8 @@ template <typename T> __device__ __forceinline__ int exact_draw(Residual<T> res,
 }
 
 // grid B; a thread per vector of the share that holds the draw
-// verify_draw: grid (B).  Bound by its chain of waits, not by what it reads: the request's summaries, its shares, two vectors; 7.5 us for
-// one request, 11.5 for 64, 14.5 where top-p cuts inside tie groups, 17 for 256.
+// verify_draw: grid (B).  Bound by its chain of waits, not by what it reads: the request's summaries, its shares, two vectors; 8 us for one
+// request, 11 for 64, 13.5 where top-p cuts inside tie groups, 16 for 256.
 template <typename T>
 __global__ __launch_bounds__(SHARE_VECS) void verify_draw(VerifyParams p) {
     constexpr int WAVES = SHARE_VECS / kWave, EPV = T::kPerVec;
@@ -1417,6 +1417,12 @@ __global__ __launch_bounds__(SHARE_VECS) void verify_draw(VerifyParams p) {
     __shared__ uint32_t s_rank[2];
     const int b = blockIdx.x, tid = threadIdx.x;
     const int len = draft_len(p, b);
+    // thread t takes a run of shares, as a rule one; it is requested ahead of the positions' decision
+    const ShareSums *const shares = p.shares + int64_t(b) * p.n_shares;
+    const int per = (p.n_shares + SHARE_VECS - 1) / SHARE_VECS;
+    const int s0 = tid * per, s1 = s0 + per < p.n_shares ? s0 + per : p.n_shares;
+    const ShareSums first = shares[s0 < p.n_shares ? s0 : 0];
+    auto share_at = [&](int s) { return s == s0 ? first : shares[s]; };
     // what thread j needs for its output at position j, ahead of the draw: the draft, its logit and the row's log-sum-exp
     const bool has_row = tid <= len, has_draft = tid < len;
     const int64_t drafted = has_draft ? p.draft_ids[int64_t(b) * p.k + tid] : -1;
@@ -1432,26 +1438,24 @@ __global__ __launch_bounds__(SHARE_VECS) void verify_draw(VerifyParams p) {
     const float u = clean_uniform(p.uniforms[int64_t(b) * (p.k + 1) + p.k]);
     Residual<T> res;
     res.setup(p, b, n, len);
-    const ShareSums *const shares = p.shares + int64_t(b) * p.n_shares;
     const bool parts = res.p.partial() || res.q.partial();
-    const int per = (p.n_shares + SHARE_VECS - 1) / SHARE_VECS;  // thread t takes a run of shares
-    const int s0 = tid * per, s1 = s0 + per < p.n_shares ? s0 + per : p.n_shares;
     uint32_t before_p = 0, before_q = 0;  // ties in front of the thread's shares
     if (parts) {
         // ---- the shares and the indices at which the groups are cut ----
         uint32_t cp = 0, cq = 0;
-        for (int s = s0; s < s1; ++s) { cp += shares[s].ties_p; cq += shares[s].ties_q; }
+        for (int s = s0; s < s1; ++s) { cp += share_at(s).ties_p; cq += share_at(s).ties_q; }
         uint64_t total;
         const uint64_t both = block_excl_scan_of<WAVES, uint64_t>((uint64_t(cq) << 32) | cp, wave_buf.u, &total);
         before_p = uint32_t(both);
         before_q = uint32_t(both >> 32);
         uint32_t rp = before_p, rq = before_q;
         for (int s = s0; s < s1; ++s) {
+            const uint32_t ties_p = share_at(s).ties_p, ties_q = share_at(s).ties_q;
             // the share that holds the last survivor, and how many of its entries survive
-            if (res.p.partial() && rp < res.p.r_cut && res.p.r_cut <= rp + shares[s].ties_p) { s_cut[0] = s; s_rank[0] = res.p.r_cut - rp; }
-            if (res.q.partial() && rq < res.q.r_cut && res.q.r_cut <= rq + shares[s].ties_q) { s_cut[1] = s; s_rank[1] = res.q.r_cut - rq; }
-            rp += shares[s].ties_p;
-            rq += shares[s].ties_q;
+            if (res.p.partial() && rp < res.p.r_cut && res.p.r_cut <= rp + ties_p) { s_cut[0] = s; s_rank[0] = res.p.r_cut - rp; }
+            if (res.q.partial() && rq < res.q.r_cut && res.q.r_cut <= rq + ties_q) { s_cut[1] = s; s_rank[1] = res.q.r_cut - rq; }
+            rp += ties_p;
+            rq += ties_q;
         }
         __syncthreads();
 #pragma unroll 1
@@ -1483,7 +1487,7 @@ __global__ __launch_bounds__(SHARE_VECS) void verify_draw(VerifyParams p) {
     }
     // a share's sum, given the ties in front of it
     auto share_sum = [&](int s, uint32_t &rp, uint32_t &rq) {
-        const ShareSums &x = shares[s];
+        const ShareSums x = share_at(s);
         if (!parts) return x.all;
         const bool out_p = res.p.partial() && rp >= res.p.r_cut, out_q = res.q.partial() && rq >= res.q.r_cut;
         rp += x.ties_p;
