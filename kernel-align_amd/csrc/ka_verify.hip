@@ -440,7 +440,8 @@ __device__ __forceinline__ bool hist_cut(HistRow &h, const uint16_t *rp, int voc
     bool ok = true;
     if (dropped) {
         key_dropped = key_of_raw(0x8000u | MAG_HIGH);
-        ok = weight_fix(value_of<Bf16>(key_dropped) - vmax) == 0 && weight_fix(-256.0f - xmax) == 0;
+        // (a temperature that takes every value of the row to -infinity makes them all its maximum)
+        ok = weight_of(key_dropped) == 0 && weight_fix(-256.0f - xmax) == 0;
     }
     if (f.use_k || f.use_p) {
         key_tiny = key_of_raw(MAG_LOW - 1);

@@ -1,0 +1,49 @@
+"""verify_draft at the edges of its parameters, against its exact statement in integers (oracle/verify_ref.py)."""
+import pytest
+import torch
+
+from oracle import verify_ref
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _equal(sampler, target, ids, u, q, **kw):
+    move = lambda t: t.cuda() if isinstance(t, torch.Tensor) else t  # noqa: E731
+    got = sampler.verify_draft(target.cuda(), ids.cuda(), u.cuda(), draft_logits=move(q), **{k: move(v) for k, v in kw.items()})
+    want = verify_ref.verify(target, ids, u, q, **kw)
+    assert torch.equal(got[1].cpu(), want[1]) and torch.equal(got[0].cpu(), want[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kw", [{}, {"top_p": 0.5}, {"top_k": 9}])
+@pytest.mark.parametrize("temperature", [1e-37, 2e-38, 1e-3])
+def test_temperatures_that_fold_a_row(sampler, dtype, kw, temperature):
+    """Rows of negative logits at a temperature so small that every scaled value is -infinity: all of them equal the maximum, those
+    of -256 and below and the masked ones too.  A row with a larger entry has that one alone left."""
+    vocab, g = 1200, torch.Generator().manual_seed(3)
+    pick = torch.tensor([-100.0, -300.0, -float("inf"), -60.0, -90.5])
+    row = lambda few: pick[torch.randint(0, len(pick), (vocab,), generator=g)] if few else torch.full((vocab,), -70.0)  # noqa: E731
+    for first in (-100.0, -0.25, 0.5):
+        for few in (True, False):
+            target = torch.stack([torch.stack([row(few) for _ in range(3)]) for _ in range(8)]).to(dtype)
+            draft = torch.stack([torch.stack([row(not few) for _ in range(2)]) for _ in range(8)]).to(dtype)
+            target[:, :, 5] = first
+            ids = torch.randint(0, vocab, (8, 2), generator=g)
+            u = torch.rand(8, 3, generator=g)
+            _equal(sampler, target, ids, u, draft, temperature=temperature, **kw)
+            u[:, :2] *= 3.0 / vocab                           # a looked-up draft is accepted with its probability
+            _equal(sampler, target, ids, u, None, temperature=temperature, **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kw", [{}, {"top_k": 50, "top_p": 0.9}, {"top_p": 0.9}])
+def test_uniforms_of_zero(sampler, dtype, kw):
+    """u = 0 takes the first entry with mass, by way of the 128-bit draw."""
+    g = torch.Generator().manual_seed(6)
+    target = (torch.randn(5, 3, 4100, generator=g) * 2).to(dtype)
+    draft = (target[:, :2].float() + 0.5 * torch.randn(5, 2, 4100, generator=g)).to(dtype)
+    ids = torch.randint(0, 4100, (5, 2), generator=g)
+    for q in (draft, None):
+        _equal(sampler, target, ids, torch.zeros(5, 3), q, **kw)
