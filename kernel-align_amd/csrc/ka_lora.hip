@@ -10,9 +10,10 @@
 // 2 R (H + O) flop, 16 flop per byte at R = 16, against about 300 that the matrix cores could do.
 //
 // Numbers.  Products of two 16-bit matrices (x A^T, dy B) run in their own type with fp32 accumulation.  u and du are fp32 and
-// stay so: an operand of a product with them is split into bf16 parts, high + low (17 bits: for results that are rounded
-// to 16 bits) or high + middle + low (24 bits: for the fp32 gradients); an fp16 operand next to them is split into two bf16 (11 bits, exact).
-// The forward of fp16 splits u into two fp16 instead, after a power of two per token (22 bits), and multiplies fp16 by fp16.
+// stay so: next to a 16-bit matrix they are split into bf16 parts, high + low (17 bits: for results that are rounded
+// to 16 bits) or high + middle + low (24 bits: for the fp32 gradients), and an fp16 matrix into the two bf16 that hold it exactly (11
+// bits).  bf16 has fp32's range, so the bits are each entry's own: fp16 parts of u would share one scale per token, and a small
+// u_r beside a large one would lose its bits however large its column of B.
 // Every sum runs in a fixed order: no atomics on floating-point values.
 #include <type_traits>
 
@@ -23,6 +24,7 @@ namespace {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -230,20 +232,6 @@ template <int PARTS> __device__ __forceinline__ void split(const float (&v)[8], 
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) part[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
 }
-// v * down = part[0] + part[1] in fp16, |v * down| < 2: to 2^-22 of it, or 2^-25
-__device__ __forceinline__ void split_f16(const float (&v)[8], float down, uint4 (&part)[2]) {
-    uint32_t w[2][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float x = v[j] * down;
-        const _Float16 hi = _Float16(x), lo = _Float16(rest(x, float(hi)));
-        const uint32_t h = __builtin_bit_cast(uint16_t, hi), l = __builtin_bit_cast(uint16_t, lo);
-        w[0][j / 2] = j & 1 ? w[0][j / 2] | h << 16 : h;
-        w[1][j / 2] = j & 1 ? w[1][j / 2] | l << 16 : l;
-    }
-#pragma unroll
-    for (int p = 0; p < 2; ++p) part[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
-}
 __device__ __forceinline__ uint4 choose(bool first, const uint4 &a, const uint4 &b) {
     return make_uint4(first ? a.x : b.x, first ? a.y : b.y, first ? a.z : b.z, first ? a.w : b.w);
 }
@@ -253,9 +241,17 @@ template <typename T> __device__ __forceinline__ void as_bf16(const uint4 &f, ui
     if constexpr (T::kDtype == KA_DTYPE_BF16) {
         part[0] = f;
     } else {
-        float v[8];
-        F16::unpack(f, v);
-        split<2>(v, part);
+        // an fp16 without its last three bits has the 8 that a bf16 holds; the difference has three, and fp16's subtraction is exact
+        const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f16x2 h = __builtin_bit_cast(f16x2, w[j] & 0xfff8fff8u), l = __builtin_bit_cast(f16x2, w[j]) - h;
+            hi[j] = __builtin_amdgcn_perm(__float_as_uint(float(h[1])), __float_as_uint(float(h[0])), 0x07060302u);
+            lo[j] = __builtin_amdgcn_perm(__float_as_uint(float(l[1])), __float_as_uint(float(l[0])), 0x07060302u);
+        }
+        part[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        part[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
 }
 
@@ -565,39 +561,26 @@ __global__ __launch_bounds__(THREADS) void lora_fold_rows(const float *__restric
 // ---------------------------------------------------------------------------
 // lora_expand: grid (blocks of O, tiles).  y = base + u B^T for the tokens of a tile.
 //
-// u enters as fragments (column = token, contraction index = rank) in B's own type: bf16 has fp32's range, for fp16 a token's u is
-// brought to [1, 2) by a power of two, and its products back by it.  High + low parts then hold 17 (bf16) or 22 (fp16)
-// bits.  They come packed from lora_pack_rows, or in calls of few tokens (PARTS) from the segments of lora_shrink.
+// u enters as fragments (column = token, contraction index = rank) of its high and low bf16 parts, 17 bits of every entry.
+// They come packed from lora_pack_rows, or in calls of few tokens (PARTS) from the segments of lora_shrink.
 // Bound by memory, base in and out through: 64 tokens x 128,256 outputs, 16 adapters of rank 16 (99 MB): 19.5 us, 5.1 TB/s; 5003 tokens x
 // 4096, rank 64 (82 MB): 23 us, 3.5 TB/s.  Tiles of 32 tokens: at 64 an adapter with a few tokens left half of the products empty
 // and the registers let two workgroups reside instead of four.
 // ---------------------------------------------------------------------------
-template <int RP> struct RowFragments {  // of 32 tokens, in uint4: [group of 16][step][high, low][lane], then 32 powers of two
+template <int RP> struct RowFragments {  // of 32 tokens, in uint4: [group of 16][step][high, low][lane]
     static constexpr int kSteps = Steps<RP>::kCount, kParts = RP <= 16 ? 1 : 2;
-    static constexpr int kFragments = FWD_SUBS * kSteps * kParts * kWave;
-    static constexpr int kTotal = kFragments + 8;
+    static constexpr int kTotal = FWD_SUBS * kSteps * kParts * kWave;
 };
-// The fragment of group s, step ks (both parts) from eight values of u a lane, and the token's power of two (1 for bf16).
-// `big`: the largest |u| of the token.
-template <typename T, int RP>
-__device__ __forceinline__ float row_fragment(const float (&v)[8], float big, uint4 *out, int lane) {
+// The fragment of a group and step (both parts) from eight values of u a lane.
+template <int RP> __device__ __forceinline__ void row_fragment(const float (&v)[8], uint4 *out, int lane) {
     uint4 hl[2];
-    float up = 1.0f;
-    if constexpr (T::kDtype == KA_DTYPE_F16) {
-        const uint32_t exponent = __float_as_uint(big) & 0x7f800000u;
-        const bool plain = exponent == 0u || exponent >= 0x7e000000u;  // nothing to bring to range, or infinite
-        up = plain ? 1.0f : __uint_as_float(exponent);
-        split_f16(v, plain ? 1.0f : __uint_as_float(0x7f000000u - exponent), hl);
-    } else {
-        split<2>(v, hl);
-    }
+    split<2>(v, hl);
     if (RP <= 16) {
         out[lane] = choose((lane >> 4) < 2, hl[0], hl[1]);
     } else {
         out[lane] = hl[0];
         out[kWave + lane] = hl[1];
     }
-    return up;
 }
 
 // grid (tiles): u of a tile's tokens from `parts` segments, added in order and scaled; also to out_shrunk.
@@ -611,7 +594,7 @@ struct PackRowsArgs {
     uint4 *out;
     LoraPlan plan;
 };
-template <typename T, int RP>
+template <int RP>
 __global__ __launch_bounds__(THREADS) void lora_pack_rows(PackRowsArgs p) {
     constexpr int KS = Steps<RP>::kCount, LD = RP + 1;
     __shared__ float v[FWD_TILE * LD];
@@ -638,13 +621,10 @@ __global__ __launch_bounds__(THREADS) void lora_pack_rows(PackRowsArgs p) {
         const int s = q / KS, ks = q % KS;
         const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
         const float *row = v + (16 * s + col) * LD;
-        float x[8], big = 0.0f;
+        float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = row[r0 + j];
-        if (T::kDtype == KA_DTYPE_F16)
-            for (int j = 0; j < RP; ++j) big = fmaxf(big, fabsf(row[j]));
-        const float up = row_fragment<T, RP>(x, big, out + q * RowFragments<RP>::kParts * kWave, lane);
-        if (ks == 0 && quad == 0) reinterpret_cast<float *>(out + RowFragments<RP>::kFragments)[s * 16 + col] = up;
+        row_fragment<RP>(x, out + q * RowFragments<RP>::kParts * kWave, lane);
     }
 }
 
@@ -663,9 +643,8 @@ struct ExpandArgs {
 };
 template <typename T, int RP, int MODE, bool PARTS>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 32 ? 4 : 2))) void lora_expand(ExpandArgs p) {
-    constexpr int KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2;
+    constexpr int KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, NP = Parts<T>::kCount;
     __shared__ uint4 uf[PARTS ? FWD_SUBS * KS * HL * kWave : 1];
-    __shared__ float back[FWD_SUBS][16];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
     const LoraTile tile = p.plan.list[0].tiles[blockIdx.y];  // (in the list's memory also where there is no such tile)
     if (int(blockIdx.y) >= *p.plan.list[0].count) return;
@@ -700,17 +679,14 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
     Stage even;
     request(0, even);
     uint4 fu[PARTS ? 1 : FWD_SUBS][KS][HL];
-    float up[FWD_SUBS];
     if constexpr (!PARTS) {
         const uint4 *packed = p.packed + int64_t(blockIdx.y) * RowFragments<RP>::kTotal;
 #pragma unroll
-        for (int s = 0; s < FWD_SUBS; ++s) {
+        for (int s = 0; s < FWD_SUBS; ++s)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int k = 0; k < HL; ++k) fu[s][ks][k] = packed[((s * KS + ks) * HL + k) * kWave + lane];
-            up[s] = T::kDtype == KA_DTYPE_F16 ? reinterpret_cast<const float *>(packed + RowFragments<RP>::kFragments)[s * 16 + col] : 1.0f;
-        }
     } else {
         const float scale = tile.adapter < 0 ? 0.0f : (p.scaling != nullptr ? p.scaling[tile.adapter] : p.scale);
         for (int q = wave; q < FWD_SUBS * KS; q += WAVES) {
@@ -739,64 +715,76 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
                 for (int j = 0; j < 8; ++j) v[j] = mine && r0 + j < p.r ? v[j] * scale : 0.0f;
             };
             const int r0 = RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad;
-            float own[8], big = 0.0f;
-            if constexpr (T::kDtype == KA_DTYPE_F16) {  // the largest of the token's whole row
-#pragma unroll 1
-                for (int k = 0; k < KS; ++k) {
-                    load_u(RP <= 16 ? r0 : 32 * k + 8 * quad, own);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(own[j]));
-                }
-                big = fmaxf(big, __shfl_xor(big, 16, kWave));
-                big = fmaxf(big, __shfl_xor(big, 32, kWave));
-            }
+            float own[8];
             load_u(r0, own);
             if (shrunk_out && (s == 0 ? live[0] : live[1]) && (RP > 16 || quad < 2)) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (r0 + j < p.r) p.out_shrunk[row + r0 + j] = own[j];
             }
-            const float power = row_fragment<T, RP>(own, big, uf + (s * KS + ks) * HL * kWave, lane);
-            if (ks == 0 && quad == 0) back[s][col] = power;
+            row_fragment<RP>(own, uf + (s * KS + ks) * HL * kWave, lane);
         }
         lds_barrier();
-#pragma unroll
-        for (int s = 0; s < FWD_SUBS; ++s) up[s] = T::kDtype == KA_DTYPE_F16 ? back[s][col] : 1.0f;
     }
     if (tile.adapter < 0 && p.in_place) return;
     typename T::raw_t *out = static_cast<typename T::raw_t *>(p.out);
+    // Groups whose products run side by side: both for fp16, so that the parts of a fragment of B are made once and kept for no longer.
+    constexpr int SIDE = NP == 1 ? 1 : FWD_SUBS;
     auto finish = [&](int g, const Stage &st) {
         const int o0 = first_of(g);
         if (o0 >= p.o) return;
 #pragma unroll
-        for (int s = 0; s < FWD_SUBS; ++s) {
-            if (s == 1 && !two) continue;
-            f32x4 acc[4];
+        for (int s0 = 0; s0 < FWD_SUBS; s0 += SIDE) {
+            if (s0 == 1 && !two) continue;
+            f32x4 acc[SIDE][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = f32x4{0, 0, 0, 0};
+            for (int s = 0; s < SIDE; ++s)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+                for (int e = 0; e < 4; ++e) acc[s][e] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int k = 0; k < HL; ++k) {
-                    uint4 f;
-                    if constexpr (PARTS) f = uf[((s * KS + ks) * HL + k) * kWave + lane];
-                    else f = fu[s][ks][k];
+            for (int ks = 0; ks < KS; ++ks) {
+                uint4 f[SIDE][HL];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[e] = mfma<T>(st.b[ks][e], f, acc[e]);
+                for (int s = 0; s < SIDE; ++s)
+#pragma unroll
+                    for (int k = 0; k < HL; ++k) {
+                        if constexpr (PARTS) f[s][k] = uf[(((s0 + s) * KS + ks) * HL + k) * kWave + lane];
+                        else f[s][k] = fu[s0 + s][ks][k];
+                    }
+                if constexpr (NP == 1) {
+#pragma unroll
+                    for (int k = 0; k < HL; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[0][e] = mfma<Bf16>(st.b[ks][e], f[0][k], acc[0][e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint4 part[NP];
+                        as_bf16<T>(st.b[ks][e], part);
+#pragma unroll
+                        for (int q = NP - 1; q >= 0; --q)
+#pragma unroll
+                            for (int s = 0; s < SIDE; ++s)
+#pragma unroll
+                                for (int k = HL - 1; k >= 0; --k) acc[s][e] = mfma<Bf16>(part[q], f[s][k], acc[s][e]);
+                    }
                 }
-            // (0 times an infinity of the rows that were read in their place would not be 0)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[e][i] = tile.adapter >= 0 ? acc[e][i] : 0.0f;
-            if constexpr (T::kDtype == KA_DTYPE_F16) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[e] *= up[s];
             }
-            if (live[s]) st.row[s].store(out + token[s] * p.out_stride, o0 + 8 * quad, p.o, acc);
+#pragma unroll
+            for (int s = 0; s < SIDE; ++s) {
+                // (0 times an infinity of the rows that were read in their place would not be 0)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[s][e][i] = tile.adapter >= 0 ? acc[s][e][i] : 0.0f;
+                if (live[s0 + s]) st.row[s0 + s].store(out + token[s0 + s] * p.out_stride, o0 + 8 * quad, p.o, acc[s]);
+            }
         }
     };
-    if constexpr (RP <= 32) {
+    // Two stages of outputs where the registers of four wavefronts per SIMD hold them (fp16 keeps the parts of a fragment of B and both
+    // groups' sums beside them).  fp16, us a call with two stages and one: rank 32, 64 tokens x 16 adapters x 128,256 outputs 51.5 / 48.5,
+    // 5003 x 4096 75 / 67; rank 16, 64 x 128,255 (any address) 47 / 47, 512 x 4096 24.5 / 25.3 (two of aligned rows are kept).
+    if constexpr (RP <= (NP == 1 ? 32 : (MODE == ROWS_ALIGNED ? 16 : 0))) {
         // what the next 64 outputs need is requested before the products of the present ones
         Stage odd;
         for (int g = 0; g < p.groups; g += 2) {
@@ -807,7 +795,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
                 finish(g + 1, odd);
             }
         }
-    } else {  // (two stages of B would take the registers of half the wavefronts)
+    } else {
         for (int g = 0; g < p.groups; ++g) {
             if (g > 0) request(g, even);
             finish(g, even);
@@ -1460,10 +1448,9 @@ KA_EXPORT int ka_lora_linear(int dtype, const void *base, int64_t base_stride, c
         pa.n = n_tokens;
         pa.out = packed;
         pa.plan = plan;
-        with_types(dtype, rp, [&](auto type, auto rank_c) {
-            using T = decltype(type);
+        with_types(dtype, rp, [&](auto, auto rank_c) {
             constexpr int RP = decltype(rank_c)::value;
-            hipLaunchKernelGGL((lora_pack_rows<T, RP>), dim3(unsigned(l.plan.max_tiles[0])), dim3(THREADS), 0, stream, pa);
+            hipLaunchKernelGGL((lora_pack_rows<RP>), dim3(unsigned(l.plan.max_tiles[0])), dim3(THREADS), 0, stream, pa);
         });
         rc = check_hip(hipGetLastError(), "lora launch (pack)");
         if (rc != KA_OK) return rc;
