@@ -46,7 +46,7 @@ const char *ka_version(void);
  * Result bits of the floating-point operators (fixed summation orders) are stable within one revision of the library,
  * not across revisions; token ids are defined exactly and never change.
  */
-#define KA_ABI_REVISION 4
+#define KA_ABI_REVISION 5
 int ka_abi_revision(void);
 /* Message of the last error on the calling thread ("" if none). */
 const char *ka_last_error(void);
