@@ -242,6 +242,7 @@ int ka_verify_draft(int dtype, const void *target_logits, int64_t target_batch_s
  *     dlora_a[a]    = sum over the adapter's tokens of du[n, :]^T hidden[n, :]          fp32 [n_adapters, rank, in_dim]
  *     dlora_b[a]    = sum over the adapter's tokens of grad_out[n, :]^T u[n, :]         fp32 [n_adapters, out_dim, rank]
  * Sums run in a fixed order (a function of the shapes and the ids); an adapter without tokens gets zeros.
+ * Infinities and NaN of the inputs come out of both calls as the formulas give them (of the same sign, in the same entries).
  *
  * Any alignment and any rank, width and token count up to the limits (multiples of eight on 16-byte aligned rows cost the
  * fewest instructions).  The workspace is 16-byte aligned, of ka_lora_workspace_bytes (0 for arguments the calls refuse); the

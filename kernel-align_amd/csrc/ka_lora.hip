@@ -15,6 +15,10 @@
 // bits).  bf16 has fp32's range, so the bits are each entry's own: fp16 parts of u would share one scale per token, and a small
 // u_r beside a large one would lose its bits however large its column of B.
 // Every sum runs in a fixed order: no atomics on floating-point values.
+// Infinities come out as in the definition.  The low parts of a number are 0 or of either sign, so that a product of parts with an
+// infinity is no number; where such a sum is not finite it is formed again from the leading parts alone, which are 0, infinite and of
+// a sign as the numbers are, without the places that a lane without work reads (leading_kind).  To see that nothing has to be costs
+// one instruction a sum: backward of 2048 x 4096, us a call without and with it, rank 16 57.1 / 57.7, rank 128 164 / 170.
 #include <type_traits>
 
 #include "ka_common.h"
@@ -255,9 +259,41 @@ template <typename T> __device__ __forceinline__ void as_bf16(const uint4 &f, ui
     }
 }
 
+// The leading part of each entry: 0 where the entry is, of its sign, infinite or no number where it is.
+template <typename T> __device__ __forceinline__ uint4 leading(const uint4 (&part)[Parts<T>::kCount]) {
+    if constexpr (T::kDtype == KA_DTYPE_BF16) {
+        return part[0];
+    } else {  // (of the smallest fp16 only the second part is left)
+        const uint32_t h[4] = {part[0].x, part[0].y, part[0].z, part[0].w}, l[4] = {part[1].x, part[1].y, part[1].z, part[1].w};
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t low = (h[j] & 0x7fffu) != 0 ? h[j] : l[j], high = (h[j] & 0x7fff0000u) != 0 ? h[j] : l[j];
+            w[j] = (low & 0xffffu) | (high & 0xffff0000u);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+// Whether a sum of some lane of the wavefront is not finite (the same in every lane).
+__device__ __forceinline__ bool any_odd(const f32x4 (&acc)[4]) {
+    float odd[4];  // (four chains: one of sixteen is waited for)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd[e] = fmaf(acc[e][3], 0.0f, fmaf(acc[e][2], 0.0f, fmaf(acc[e][1], 0.0f, acc[e][0] * 0.0f)));
+    const float all = (odd[0] + odd[1]) + (odd[2] + odd[3]);
+    return __ballot(all != all) != 0;
+}
+// Sums that are not finite become those of the leading parts, if these are not either.
+__device__ __forceinline__ void leading_kind(f32x4 &acc, const f32x4 &kind) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (!(fabsf(acc[i]) < __builtin_inff()) && !(fabsf(kind[i]) < __builtin_inff())) acc[i] = kind[i];
+    __builtin_amdgcn_sched_barrier(0);  // (one after the other: what is rare takes few registers)
+}
+
 // Loads are never conditional: a lane without work of its own reads a place that exists (another row of the tile, the
 // start of a row), so that all loads of a step are in flight together, and what it read meets a zero in the other operand or a
-// result that is not stored.  (An infinity read that way belongs to the same token or adapter.)
+// result that is not stored.  (An infinity read that way belongs to the same token or adapter; the product with zero is then formed
+// again without it, or it is cleared where the columns end.)
 //
 // How a kernel reaches the rows of its matrices:
 //   ROWS_ALIGNED  16-byte vectors at 16-byte addresses, widths multiples of 8; the backward's kernels then step through the matrix they
@@ -512,6 +548,12 @@ __global__ __launch_bounds__(THREADS) void lora_shrink(ShrinkArgs p) {
 #pragma unroll
                     for (int s = 0; s < SUBS; ++s) fx[t][s] = load8<T, MODE>(rows[s], k, p.h);
                 }
+                if ((st + 2) * 32 > p.h) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int s = 0; s < SUBS; ++s) fx[t][s] = first_entries(fx[t][s], p.h - (st + t) * 32 - 8 * quad);
+                }
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -664,15 +706,16 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
         uint4 b[KS][4];
     };
     auto first_of = [&](int g) { return ((int(blockIdx.x) * p.groups + g) * WAVES + wave) * 64; };
+    auto b_fragment = [&](int o0, int ks, int e) {
+        const int o = o0 + 32 * (e / 2) + 8 * (col / 4) + 4 * (e & 1) + (col & 3);
+        return dense_load8<T, MODE>(bw, o < p.o ? o : 0, p.o, RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad, p.r);
+    };
     auto request = [&](int g, Stage &st) {
         const int o0 = first_of(g) < p.o ? first_of(g) : 0;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int o = o0 + 32 * (e / 2) + 8 * (col / 4) + 4 * (e & 1) + (col & 3);
-                st.b[ks][e] = dense_load8<T, MODE>(bw, o < p.o ? o : 0, p.o, RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad, p.r);
-            }
+            for (int e = 0; e < 4; ++e) st.b[ks][e] = b_fragment(o0, ks, e);
         st.row[0].load(p.base, token[0] * p.base_stride, o0 + 8 * quad, p.o);
         if (two) st.row[1].load(p.base, token[1] * p.base_stride, o0 + 8 * quad, p.o);
     };
@@ -772,6 +815,23 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
             }
 #pragma unroll
             for (int s = 0; s < SIDE; ++s) {
+                if (tile.adapter >= 0 && any_odd(acc[s])) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        f32x4 kind = {0, 0, 0, 0};
+#pragma unroll
+                        for (int ks = 0; ks < KS; ++ks) {
+                            // (ranks of this lane; with R <= 16 the second half of the lanes holds low parts)
+                            const int ranks = RP <= 16 ? (quad < 2 ? p.r - 8 * quad : 0) : p.r - 32 * ks - 8 * quad;
+                            uint4 f, part[NP];
+                            if constexpr (PARTS) f = uf[((s0 + s) * KS + ks) * HL * kWave + lane];
+                            else f = p.packed[int64_t(blockIdx.y) * RowFragments<RP>::kTotal + ((s0 + s) * KS + ks) * HL * kWave + lane];
+                            as_bf16<T>(b_fragment(o0, ks, e), part);  // (read again, so that the products above need not keep it)
+                            kind = mfma<Bf16>(first_entries(leading<T>(part), ranks), first_entries(f, ranks), kind);
+                        }
+                        leading_kind(acc[s][e], kind);
+                    }
+                }
                 // (0 times an infinity of the rows that were read in their place would not be 0)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -781,10 +841,10 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
             }
         }
     };
-    // Two stages of outputs where the registers of four wavefronts per SIMD hold them (fp16 keeps the parts of a fragment of B and both
-    // groups' sums beside them).  fp16, us a call with two stages and one: rank 32, 64 tokens x 16 adapters x 128,256 outputs 51.5 / 48.5,
-    // 5003 x 4096 75 / 67; rank 16, 64 x 128,255 (any address) 47 / 47, 512 x 4096 24.5 / 25.3 (two of aligned rows are kept).
-    if constexpr (RP <= (NP == 1 ? 32 : (MODE == ROWS_ALIGNED ? 16 : 0))) {
+    // Two stages of outputs where the registers of four wavefronts per SIMD hold them.  fp16 keeps the parts of a fragment of B and both
+    // groups' sums beside them and would spill; us a call with two stages and with one: rank 16, 64 tokens x 128,256 outputs 42.6 / 39.3,
+    // 8192 x 4096 94 / 83; rank 32, 5003 x 4096 75 / 67.
+    if constexpr (RP <= 32 && NP == 1) {
         // what the next 64 outputs need is requested before the products of the present ones
         Stage odd;
         for (int g = 0; g < p.groups; g += 2) {
@@ -924,6 +984,27 @@ template <typename T> __device__ __forceinline__ f32x4 outer(const uint4 (&data)
     acc = mfma<Bf16>(data[0], v[1], acc);
     return mfma<Bf16>(data[0], v[0], acc);
 }
+// What a gradient's sums are by their leading parts: data(c, j) loads four columns of token 8 quad + j of the 32 at c, `v` the leading parts of
+// the other operand for the first 32 tokens, `step` further for the next.
+template <typename T, typename F>
+__device__ __forceinline__ void gradient_kind(f32x4 (&acc)[4], int count, const uint4 *v, int step, F &&data) {
+    const int quad = (int(threadIdx.x) & (kWave - 1)) >> 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f32x4 kind = {0, 0, 0, 0};
+#pragma unroll 1
+        for (int c = 0; c < count; c += 32) {
+            uint2 w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = c + 8 * quad + j < count ? data(c, j) : make_uint2(0, 0);
+            uint4 frag[4], part[Parts<T>::kCount];
+            transpose(w, frag);
+            as_bf16<T>(frag[e], part);
+            kind = mfma<Bf16>(leading<T>(part), v[int64_t(c / 32) * step], kind);
+        }
+        leading_kind(acc[e], kind);
+    }
+}
 template <typename T, int RP, int G, int MODE>
 __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
     constexpr int RF = RP / 16, NP = Parts<T>::kCount;
@@ -939,6 +1020,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
     load_tokens(p.plan.order, tile, tokens);
     const typename T::raw_t *bw = static_cast<const typename T::raw_t *>(p.b) + int64_t(tile.adapter) * p.o * p.r;
     const int o0 = (int(blockIdx.x) * WAVES + wave) * 64 * G;
+    const bool cut_short = (int(blockIdx.x) + 1) * WAVES * 64 * G > p.o;  // of the workgroup's outputs some do not exist
     // B^T fragments: row = rank, contraction index = output
     uint4 fb[G][2][RF];
 #pragma unroll
@@ -1044,6 +1126,15 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
                     f32x4 sum = red[0][i][r4];
 #pragma unroll
                     for (int k = 1; k < WAVES; ++k) sum += red[k][i][r4];
+                    if (cut_short && !(fabsf(sum[0] * 0.0f + sum[1] * 0.0f + sum[2] * 0.0f + sum[3] * 0.0f) < 1.0f)) {
+                        // a lane behind the last output read another one, of which an infinity times 0 is no number: entry by entry
+                        const typename T::raw_t *row = row_at<T, MODE>(p.dy, row_offset<MODE>(tokens[c + i], p.dy_stride));
+                        sum = f32x4{0, 0, 0, 0};
+#pragma unroll 1
+                        for (int o = int(blockIdx.x) * WAVES * 64 * G; o < p.o; ++o)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) sum[j] += T::widen(row[o]) * T::widen(bw[int64_t(o) * p.r + (r0 + j < p.r ? r0 + j : r0)]);
+                    }
                     float *out = p.du_part + (int64_t(blockIdx.x) * p.n + tokens[c + i]) * p.r + r0;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -1068,6 +1159,16 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
         if (c + 32 >= tile.count) break;
         step(c + 32, odd, even);
     }
+    // sums of tokens that are not finite, once more from the leading parts
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int f = 0; f < RF; ++f)
+            if (any_odd(acc[g][f]))
+                gradient_kind<T>(acc[g][f], tile.count, reinterpret_cast<const uint4 *>(packed) - tid + f * 3 * kWave + lane, Packed<RP>::kColumns,
+                                 [&](int c, int j) {
+                                     return row_load4<T, MODE>(p.dy, row_offset<MODE>(tokens[c + 8 * quad + j], p.dy_stride), col4[g], p.o);
+                                 });
     float *db = tile.slot < 0 ? p.db + int64_t(tile.adapter) * p.o * p.r : p.db_part + int64_t(tile.slot) * p.o * p.r;
 #pragma unroll
     for (int g = 0; g < G; ++g)
@@ -1096,7 +1197,8 @@ struct BwdInArgs {
     LoraPlan plan;
 };
 template <typename T, int RP, int MODE>
-__global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
+// (three wavefronts per SIMD at rank 16, as many as the hot loop alone would have: 2048 x 4096, fp16 57.6 us a call, with two 61.5)
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 16 ? 3 : RP <= 32 ? 2 : 1))) void lora_bwd_in(BwdInArgs p) {
     constexpr int RF = RP / 16, KS = Steps<RP>::kCount, HL = RP <= 16 ? 1 : 2, NP = Parts<T>::kCount;
     __shared__ __attribute__((aligned(16))) int32_t tokens[BWD_TILE_MAX];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, col = lane & 15, quad = lane >> 4;
@@ -1119,6 +1221,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
         for (int j = 0; j < 8; ++j) {
             const int rank = (RP <= 16 ? 8 * (quad & 1) : 32 * ks + 8 * quad) + j;
             w[j] = load4<T, MODE>(aw + int64_t(rank < p.r ? rank : 0) * p.h, h0 + permuted(col), p.h);
+            if (rank >= p.r) w[j] = make_uint2(0, 0);
         }
         uint4 frag[4];
         transpose(w, frag);
@@ -1178,6 +1281,19 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
                         for (int e = 0; e < 4; ++e)
 #pragma unroll
                             for (int q = 0; q < NP; ++q) sum[e] = mfma<Bf16>(fa[ks][e][q], rows[s][ks][k], sum[e]);
+                if (any_odd(sum)) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        f32x4 kind = {0, 0, 0, 0};
+#pragma unroll
+                        for (int ks = 0; ks < KS; ++ks) {
+                            const int ranks = RP <= 16 && quad >= 2 ? 0 : 8;  // (with R <= 16 the second half of the lanes holds low parts)
+                            kind = mfma<Bf16>(first_entries(leading<T>(fa[ks][e]), ranks),
+                                              first_entries(pu[Packed<RP>::kColumns + (s * KS + ks) * HL * kWave], ranks), kind);
+                        }
+                        leading_kind(sum[e], kind);
+                    }
+                }
             }
             if (c + 16 * s + col < tile.count)
                 base[s].store(static_cast<typename T::raw_t *>(p.dx) + int64_t(tokens[c + 16 * s + col]) * p.dx_stride, out_col, p.h, sum);
@@ -1191,6 +1307,12 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_in(BwdInArgs p) {
         step(c + 32, odd, even);
     }
     if (!has) return;
+#pragma unroll
+    for (int f = 0; f < RF; ++f)
+        if (any_odd(acc[f]))
+            gradient_kind<T>(acc[f], tile.count, packed + f * 3 * kWave, Packed<RP>::kColumns + Packed<RP>::kRows, [&](int c, int j) {
+                return row_load4<T, MODE>(p.x, row_offset<MODE>(tokens[c + 8 * quad + j], p.x_stride), col4, p.h);
+            });
     float *da = tile.slot < 0 ? p.da + int64_t(tile.adapter) * p.r * p.h : p.da_part + int64_t(tile.slot) * p.r * p.h;
 #pragma unroll
     for (int f = 0; f < RF; ++f) {

@@ -103,6 +103,7 @@ class AdapterOps:
         base: [.., O], the projection's output (``F.linear(hidden, weight)``); hidden: [.., H]; lora_a: [S, R, H]; lora_b:
         [S, O, R]; all bf16 or all fp16, R <= 128, S <= 1023.  adapter_ids: integer tensor of shape hidden.shape[:-1], in any
         order; scaling: a number or one per adapter ([S]).  Accumulates in fp32 and rounds once, when the sum is written.
+        Infinities and NaN come out as the formula gives them.
         With ``inplace=True`` the result overwrites ``base`` (whose rows must be views of one [N, O] layout).  With
         ``return_shrunk=True`` the result is ``(out, shrunk)``, shrunk fp32 [.., R] the scaled product with lora_a, which
         ``lora_linear_backward`` takes.

@@ -1,4 +1,4 @@
-"""lora_linear and its backward where numbers are hardest: ranks of unlike magnitude, and the batch a token comes in."""
+"""lora_linear and its backward where numbers are hardest: ranks of unlike magnitude, infinities, and the batch a token comes in."""
 import pytest
 import torch
 
@@ -40,6 +40,80 @@ def test_a_small_rank_alone_in_a_column(sampler, dtype, n):
     c = [t.to(dtype) for t in (torch.zeros(n, 16), hidden, a, b)] + [torch.zeros(n, dtype=torch.int64)]
     y, _, bound, _ = lora_ref.forward(*c, torch.ones(1))
     _within(sampler.lora_linear(*[t.cuda() for t in c]), y, bound, "out")
+
+
+def _kinds(got, want, what):
+    """The same entries are not a number, infinite and of either sign."""
+    got, want = got.double().cpu(), want.double()
+    for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+        wrong = kind(got) != kind(want)
+        assert not wrong.any(), f"{what}: {kind.__name__} in {wrong.nonzero()[:4].tolist()}, {int(wrong.sum())} entries"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [5, 700])
+@pytest.mark.parametrize("h, o", [(72, 136), (75, 139), (5, 6), (300, 600)])
+@pytest.mark.parametrize("r", [1, 8, 12, 24, 64, 72, 128])
+def test_infinities_of_the_definition(sampler, dtype, n, h, o, r):
+    """An infinity anywhere gives what the definition has there: infinities of its sign, or no number where two meet or one
+    meets a zero; fp64 says which.  Several come one at a time, since two in one sum mostly cancel to no number."""
+    inf = float("inf")
+    clean = _inputs(n, h, o, r, 2, dtype, seed=n + h + r, ids=torch.arange(n) % 3 - 1)
+    last = int((clean["ids"] == 0).nonzero()[-1])             # the last token of adapter 0, which may fill up a tile
+    places = [("hidden", (1, 0), inf), ("hidden", (last, h - 1), -inf), ("a", (0, 0, 0), inf), ("a", (0, r - 1, h - 1), -inf),
+              ("b", (0, 0, 0), inf), ("b", (0, o - 1, r - 1), -inf), ("dy", (1, 0), inf), ("dy", (last, o - 1), -inf), ("dy", (last, 3), inf),
+              ("base", (1, 2), -inf), ("dx", (1, 2), inf)]
+    for name, at, value in places:
+        c = dict(clean, **{name: clean[name].clone()})
+        c[name][at] = value
+        d = {k: v.cuda() for k, v in c.items()}
+        out, u = sampler.lora_linear(d["base"], d["hidden"], d["a"], d["b"], d["ids"], d["scaling"], return_shrunk=True)
+        want, want_u, _, _ = lora_ref.forward(c["base"], c["hidden"], c["a"], c["b"], c["ids"], c["scaling"])
+        _kinds(u, want_u, f"{name}{at}: shrunk")
+        _kinds(out, want, f"{name}{at}: out")
+        got = sampler.lora_linear_backward(d["dy"], d["hidden"], d["a"], d["b"], d["ids"], d["scaling"], u, d["dx"])
+        want, _ = lora_ref.backward(c["dy"], c["hidden"], c["a"], c["b"], c["ids"], c["scaling"], u.cpu(), c["dx"])
+        for x, w, what in zip(got, want, ("dhidden", "dlora_a", "dlora_b")):
+            _kinds(x, w, f"{name}{at}: {what}")
+
+
+@pytest.mark.parametrize("n", [3, 600])
+@pytest.mark.parametrize("r", [1, 40])
+def test_infinities_beside_the_smallest_numbers(sampler, n, r):
+    """The smallest fp16 numbers are all in the second of their two parts: an infinity times them is one all the same."""
+    tiny, inf = 2.0 ** -24, float("inf")
+    full = lambda v, *shape: torch.full(shape, v, dtype=torch.float16)  # noqa: E731
+    c = dict(base=full(0.0, n, 24), hidden=full(3 * tiny, n, 16), a=full(-tiny, 1, r, 16), b=full(5 * tiny, 1, 24, r),
+             ids=torch.zeros(n, dtype=torch.int64), scaling=torch.ones(1), dy=full(-7 * tiny, n, 24))
+    for name in ("hidden", "dy", "a", "b"):
+        x = dict(c, **{name: c[name].clone()})
+        x[name].view(-1)[1] = inf
+        d = {k: v.cuda() for k, v in x.items()}
+        out, u = sampler.lora_linear(d["base"], d["hidden"], d["a"], d["b"], d["ids"], d["scaling"], return_shrunk=True)
+        want, want_u, _, _ = lora_ref.forward(x["base"], x["hidden"], x["a"], x["b"], x["ids"], x["scaling"])
+        _kinds(u, want_u, f"{name}: shrunk")
+        _kinds(out, want, f"{name}: out")
+        got = sampler.lora_linear_backward(d["dy"], d["hidden"], d["a"], d["b"], d["ids"], d["scaling"], u)
+        want, _ = lora_ref.backward(x["dy"], x["hidden"], x["a"], x["b"], x["ids"], x["scaling"], u.cpu(), None)
+        for y, w, what in zip(got, want, ("dhidden", "dlora_a", "dlora_b")):
+            _kinds(y, w, f"{name}: {what}")
+
+
+def test_infinities_in_front_of_a_wide_output(sampler):
+    """The same in the blocks of 1024 outputs, of which the last is cut short."""
+    n, h, o, r, s, inf = 4100, 72, 65560, 11, 2, float("inf")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rnd = lambda std, *shape: (torch.randn(*shape, generator=g, device="cuda") * std).bfloat16()  # noqa: E731
+    dy, hidden, a, b = rnd(0.1, n, o), rnd(1.0, n, h), rnd(0.1, s, r, h), rnd(0.3, s, o, r)
+    ids = torch.arange(n, device="cuda") % 3 - 1
+    u = torch.randn(n, r, generator=g, device="cuda")
+    scaling = torch.ones(s, device="cuda")
+    dy[1, 65536], dy[4, 0], dy[4099, 65559], dy[2, 7] = inf, -inf, inf, -inf
+    got = sampler.lora_linear_backward(dy, hidden, a, b, ids, scaling, u)
+    with torch.device("cuda"):
+        want, _ = lora_ref.backward(dy, hidden, a, b, ids, scaling, u, None)
+    for x, w, what in zip(got, want, ("dhidden", "dlora_a", "dlora_b")):
+        _kinds(x, w.cpu(), what)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
