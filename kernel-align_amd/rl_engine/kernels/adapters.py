@@ -104,8 +104,9 @@ class AdapterOps:
         [S, O, R]; all bf16 or all fp16, R <= 128, S <= 1023.  adapter_ids: integer tensor of shape hidden.shape[:-1], in any
         order; scaling: a number or one per adapter ([S]).  Accumulates in fp32 and rounds once, when the sum is written.
         Infinities and NaN come out as the formula gives them.
-        With ``inplace=True`` the result overwrites ``base`` (whose rows must be views of one [N, O] layout).  With
-        ``return_shrunk=True`` the result is ``(out, shrunk)``, shrunk fp32 [.., R] the scaled product with lora_a, which
+        With ``inplace=True`` the result overwrites ``base`` (whose rows must be views of one [N, O] layout, and which must not
+        be a leaf that requires grad); autograd sees that as it does torch's in-place operators, and a backward that needs the
+        overwritten values raises.  With ``return_shrunk=True`` the result is ``(out, shrunk)``, shrunk fp32 [.., R] the scaled product with lora_a, which
         ``lora_linear_backward`` takes.
         """
         _require_gpu(base, "base")
@@ -120,10 +121,14 @@ class AdapterOps:
         base_rows = _flat_rows(base)
         if inplace and base_rows.data_ptr() != base.data_ptr():
             raise ValueError("inplace=True needs base as rows of one [N, O] layout")
+        if inplace and base.requires_grad and (base.is_leaf or (base._is_view() and base._base.is_leaf)):
+            raise ValueError("inplace=True cannot overwrite a leaf that requires grad, or a view of one: pass it detached")
         n = rows.shape[0]
         out = base if inplace else torch.empty(lead + (o,), dtype=base.dtype, device=base.device)
         shrunk = torch.empty(lead + (r,), dtype=torch.float32, device=base.device) if return_shrunk else None
         if n > 0:
+            if inplace and not base.is_inference():
+                torch.autograd.graph.increment_version(base)  # the kernel writes through a pointer, which autograd does not see
             self._launch_lora(base_rows, rows, a, b, ids, scaling, scale, out, _stride(base_rows) if inplace else o, shrunk)
         return (out, shrunk) if return_shrunk else out
 

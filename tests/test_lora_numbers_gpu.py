@@ -1,4 +1,5 @@
-"""lora_linear and its backward where numbers are hardest: ranks of unlike magnitude, infinities, and the batch a token comes in."""
+"""lora_linear and its backward where numbers are hardest: ranks of unlike magnitude, infinities, the batch a token comes in, and
+in-place results that autograd has seen."""
 import pytest
 import torch
 
@@ -129,3 +130,29 @@ def test_bits_of_a_token_whatever_the_batch(sampler, dtype, r, h):
               slice(19999, 20000), torch.tensor([5, 19000, 64, 3], device="cuda")):
         part = call(i)
         assert torch.equal(part[0], whole[0][i]) and torch.equal(part[1], whole[1][i])
+
+
+def test_in_place_is_seen_by_autograd(sampler):
+    """A base that autograd has saved must not be overwritten unseen: the backward refuses it, as after torch's own in-place operators."""
+    c = {k: v.cuda() for k, v in _inputs(9, 24, 40, 8, 2, torch.bfloat16, seed=2).items()}
+    args = (c["hidden"], c["a"], c["b"], c["ids"])
+    weight = torch.randn(40, 24, device="cuda").bfloat16().requires_grad_()
+    base = torch.nn.functional.linear(c["hidden"], weight)
+    loss = base.square().sum()                                # saves base
+    before = base._version
+    assert sampler.lora_linear(base, *args, inplace=True) is base
+    assert base._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    # rows of a larger tensor share its version; inference tensors have none
+    store = torch.zeros(9, 64, device="cuda", dtype=torch.bfloat16)
+    before = store._version
+    sampler.lora_linear(store[:, 8:48], *args, inplace=True)
+    assert store._version > before
+    with torch.inference_mode():
+        inside = c["base"].clone()
+        sampler.lora_linear(inside, *args, inplace=True)
+    assert torch.equal(inside, sampler.lora_linear(c["base"], *args))
+    before = base._version
+    sampler.lora_linear(base, *args)                          # out of place: nothing to see
+    assert base._version == before

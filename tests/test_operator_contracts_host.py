@@ -1,0 +1,26 @@
+"""What the entry points around verification, adapters and the registry promise, as far as the host decides it."""
+import pytest
+import torch
+
+from rl_engine.kernels.sampling import SamplerBackend
+
+
+class _OnGpu(torch.Tensor):
+    """A CPU tensor that says it lives on the GPU, so that the checks behind the device check can be reached without one."""
+    is_cuda = True
+
+
+def _fake(*shape, dtype=torch.bfloat16, grad=False):
+    return torch.zeros(*shape, dtype=dtype).requires_grad_(grad).as_subclass(_OnGpu)
+
+
+def test_in_place_refuses_a_leaf_that_requires_grad():
+    args = (_fake(4, 5), _fake(2, 3, 5), _fake(2, 6, 3), torch.zeros(4, dtype=torch.int64))
+    leaf = torch.zeros(4, 6, dtype=torch.bfloat16, requires_grad=True)
+    leaf.__class__ = _OnGpu
+    assert leaf.is_leaf and leaf.requires_grad
+    view = torch.zeros(4, 8, dtype=torch.bfloat16, requires_grad=True)[:, :6]
+    view.__class__ = _OnGpu
+    for base in (leaf, view):
+        with pytest.raises(ValueError, match="leaf"):
+            SamplerBackend().lora_linear(base, *args, inplace=True)
