@@ -7,6 +7,7 @@ now points at code that exists: the HIP-backed methods of SamplerBackend.
 """
 from __future__ import annotations
 
+import re
 from enum import Enum, EnumMeta
 from typing import Callable, Dict
 
@@ -42,8 +43,10 @@ class KernelRegistry:
         logger.info(f"KernelRegistry initialized for {device_ctx.device_type}")
 
     def dispatch(self, op_type: str) -> str:
-        """Name of the backend serving `op_type` (substring match, as in registry.py:41-55)."""
-        if "lora" in op_type or "adapter" in op_type:
+        """Name of the backend serving `op_type` (substring match, as in registry.py:41-55; the adapters by whole words, and only
+        where the name asks for no log-probability or sampling operator)."""
+        words = re.split(r"[^a-z0-9]+", op_type)
+        if any(w in words for w in ("lora", "adapter", "adapters")) and "logp" not in op_type and "sampl" not in op_type:
             return OpBackend.HIP_LORA_LINEAR.name
         if "lm_head" in op_type or "linear" in op_type:
             return OpBackend.HIP_FUSED_LMHEAD_LOGPROB.name

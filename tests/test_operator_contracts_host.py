@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from rl_engine.kernels.registry import kernel_registry
 from rl_engine.kernels.sampling import SamplerBackend
 
 
@@ -12,6 +13,16 @@ class _OnGpu(torch.Tensor):
 
 def _fake(*shape, dtype=torch.bfloat16, grad=False):
     return torch.zeros(*shape, dtype=dtype).requires_grad_(grad).as_subclass(_OnGpu)
+
+
+def test_names_of_other_operators_keep_their_answers():
+    """A name is the adapters' where one of its words says so, and none of the operators around them does."""
+    for name, want in (("exploration_logp", "HIP_LOGPROB"), ("exploration_linear", "HIP_FUSED_LMHEAD_LOGPROB"),
+                       ("adapter_linear_logp", "HIP_FUSED_LMHEAD_LOGPROB"), ("lora_linear_logp", "HIP_FUSED_LMHEAD_LOGPROB"),
+                       ("adapter_logp", "HIP_LOGPROB"), ("adapter_sampling", "HIP_SAMPLING"), ("exploration_sampling", "HIP_SAMPLING"),
+                       ("exploration", "NOT_ON_HIP_PATH"), ("lora", "HIP_LORA_LINEAR"), ("multi-lora", "HIP_LORA_LINEAR"),
+                       ("adapters", "HIP_LORA_LINEAR"), ("lora.linear", "HIP_LORA_LINEAR")):
+        assert kernel_registry.dispatch(name) == want, name
 
 
 def test_in_place_refuses_a_leaf_that_requires_grad():
