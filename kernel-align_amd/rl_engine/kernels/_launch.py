@@ -1,4 +1,4 @@
-"""What every operator does around a launch: the device check, the device guard and the stream lookup."""
+"""What every operator does around a launch: the device check, the device guard, the stream lookup and per-row parameters."""
 from __future__ import annotations
 
 import torch
@@ -35,3 +35,12 @@ def _on_device(device):
 def _raw_stream() -> int:
     """Handle of the current HIP stream of the current device (what torch.cuda.current_stream().cuda_stream returns)."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def to_rows(values: torch.Tensor, device, dtype) -> torch.Tensor:
+    """Per-row parameters in the type the kernels read.  Integers beyond 32 bits become the largest that fit, instead of what their
+    low bits say (a top_k beyond the vocabulary filters nothing, however large)."""
+    if dtype == torch.int32 and values.dtype != torch.int32:
+        limits = torch.iinfo(torch.int32)
+        values = values.clamp(limits.min, limits.max)
+    return values.to(device=device, dtype=dtype).contiguous()

@@ -14,7 +14,7 @@ import torch
 import torch.nn as nn
 
 from rl_engine.kernels import _hip
-from rl_engine.kernels._launch import _on_device, _raw_stream, _require_gpu
+from rl_engine.kernels._launch import _on_device, _raw_stream, _require_gpu, to_rows
 from rl_engine.kernels.adapters import AdapterOps
 from rl_engine.kernels.pool import OwnScratch, PoolExhausted, WorkspacePool
 from rl_engine.kernels.speculative import SpeculativeOps
@@ -277,7 +277,7 @@ class SamplerBackend(AdapterOps, SpeculativeOps, nn.Module):
             if isinstance(value, torch.Tensor):
                 if tuple(value.shape) != (batch,):
                     raise ValueError(f"{name} tensor must have shape ({batch},)")
-                return default, value.to(device=dev, dtype=dtype).contiguous()
+                return default, to_rows(value, dev, dtype)
             scalar = default if value is None else value
             check(scalar)
             return scalar, None
@@ -297,7 +297,7 @@ class SamplerBackend(AdapterOps, SpeculativeOps, nn.Module):
         k, k_rows = rows_or_scalar(top_k, "top_k", torch.int32, 0, check_k)
         p, p_rows = rows_or_scalar(top_p, "top_p", torch.float32, 1.0, check_p)
         t, t_rows = rows_or_scalar(temperature, "temperature", torch.float32, 1.0, check_t)
-        k, p, t = int(k), float(p), float(t)
+        k, p, t = min(int(k), vocab), float(p), float(t)
         rows = _rows_view(logits)
         if uniforms is None:
             uniforms = torch.rand(batch, generator=generator, device=dev, dtype=torch.float32)

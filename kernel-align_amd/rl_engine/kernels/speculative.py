@@ -10,7 +10,7 @@ from functools import cached_property, lru_cache
 import torch
 
 from rl_engine.kernels import _hip
-from rl_engine.kernels._launch import _on_device, _raw_stream, _require_gpu
+from rl_engine.kernels._launch import _on_device, _raw_stream, _require_gpu, to_rows
 
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_DRAFT = 64  # KA_VERIFY_MAX_DRAFT
@@ -79,6 +79,7 @@ class SpeculativeOps:
         temp, temp_rows = _per_request(temperature, "temperature", batch, dev, torch.float32, 1.0, lambda v: v > 0.0,
                                        "must be > 0")
         kk, kk_rows = _per_request(top_k, "top_k", batch, dev, torch.int32, 0, lambda v: int(v) >= 1, "must be >= 1")
+        kk = min(int(kk), vocab)
         pp, pp_rows = _per_request(top_p, "top_p", batch, dev, torch.float32, 1.0, lambda v: 0.0 < v <= 1.0,
                                    "must be in (0, 1]")
         if uniforms is None:
@@ -100,7 +101,7 @@ class SpeculativeOps:
                 with self._scratch(ws_bytes, dev) as ws_ptr:
                     status = self._lib.ka_verify_draft(
                         code, target.data_ptr(), *t_strides, ptr(draft), *d_strides, ids.data_ptr(), ptr(lens),
-                        uniforms.data_ptr(), batch, k, vocab, float(temp), ptr(temp_rows), int(kk), ptr(kk_rows),
+                        uniforms.data_ptr(), batch, k, vocab, float(temp), ptr(temp_rows), kk, ptr(kk_rows),
                         float(pp), ptr(pp_rows), out.data_ptr(), accepted.data_ptr(), ptr(policy), ws_ptr, ws_bytes,
                         _raw_stream())
             _hip.check(status, "ka_verify_draft")
@@ -112,7 +113,7 @@ def _per_request(value, name, batch, dev, dtype, default, valid, rule):
     if isinstance(value, torch.Tensor):
         if tuple(value.shape) != (batch,):
             raise ValueError(f"{name} tensor must have shape ({batch},)")
-        return default, value.to(device=dev, dtype=dtype).contiguous()
+        return default, to_rows(value, dev, dtype)
     if value is None:
         return default, None
     if not valid(value):

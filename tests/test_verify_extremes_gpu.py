@@ -37,6 +37,20 @@ def test_temperatures_that_fold_a_row(sampler, dtype, kw, temperature):
             _equal(sampler, target, ids, u, None, temperature=temperature, **kw)
 
 
+@pytest.mark.parametrize("top_k", [1 << 31, (1 << 32) + 5, (1 << 40) + 1])
+def test_top_k_beyond_32_bits_filters_nothing(sampler, top_k):
+    g = torch.Generator().manual_seed(4)
+    target = torch.randn(6, 3, 500, generator=g).bfloat16()
+    draft = torch.randn(6, 2, 500, generator=g).bfloat16()
+    ids, u = torch.randint(0, 500, (6, 2), generator=g), torch.rand(6, 3, generator=g)
+    plain = sampler.verify_draft(target.cuda(), ids.cuda(), u.cuda(), draft_logits=draft.cuda())
+    sampled = sampler.sample(target[:, 0].cuda(), uniforms=u[:, 0].cuda())
+    for k in (top_k, torch.full((6,), top_k, dtype=torch.int64, device="cuda")):
+        got = sampler.verify_draft(target.cuda(), ids.cuda(), u.cuda(), draft_logits=draft.cuda(), top_k=k)
+        assert torch.equal(got[0], plain[0]) and torch.equal(got[1], plain[1])
+        assert torch.equal(sampler.sample(target[:, 0].cuda(), top_k=k, uniforms=u[:, 0].cuda()), sampled)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kw", [{}, {"top_k": 50, "top_p": 0.9}, {"top_p": 0.9}])
 def test_uniforms_of_zero(sampler, dtype, kw):
