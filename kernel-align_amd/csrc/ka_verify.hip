@@ -44,6 +44,9 @@ typedef unsigned __int128 u128;
 
 constexpr int VERIFY_MAX_DRAFT = KA_VERIFY_MAX_DRAFT;
 static_assert(VERIFY_MAX_DRAFT <= kWave, "one lane decides one position");
+constexpr int64_t VERIFY_MAX_VOCAB = int64_t(1) << 22;           // below it: masses of 2^40 add up to less than 2^62
+constexpr int64_t VERIFY_MAX_BATCH = 65535;                      // the second dimension of a grid
+constexpr int64_t VERIFY_MAX_ROWS = (int64_t(1) << 32) / S_THREADS;  // below it: a grid of a workgroup per row
 constexpr int SHARE_VECS = 256;    // 16-byte vectors of a row in one share; verify_draw has a thread for each
 constexpr int SHARE_THREADS = 256;
 
@@ -1633,7 +1636,10 @@ inline VerifyLayout verify_layout(int dtype, int64_t batch, int64_t k, int64_t v
 }  // namespace ka
 
 KA_EXPORT size_t ka_verify_workspace_bytes(int dtype, int64_t batch, int64_t max_draft, int64_t vocab) {
-    if (batch <= 0 || max_draft < 0 || max_draft > ka::VERIFY_MAX_DRAFT || vocab < 1 || vocab >= (int64_t(1) << 22)) return 0;
+    if ((dtype != KA_DTYPE_BF16 && dtype != KA_DTYPE_F16 && dtype != KA_DTYPE_F32) || batch <= 0 || max_draft < 0 ||
+        max_draft > ka::VERIFY_MAX_DRAFT || vocab < 1 || vocab >= ka::VERIFY_MAX_VOCAB || batch > ka::VERIFY_MAX_BATCH ||
+        batch * (2 * max_draft + 1) >= ka::VERIFY_MAX_ROWS)
+        return 0;
     return ka::verify_layout(dtype, batch, max_draft, vocab).total;
 }
 
@@ -1656,10 +1662,10 @@ KA_EXPORT int ka_verify_draft(int dtype, const void *target_logits, int64_t targ
         (draft_ids == nullptr && max_draft > 0))
         return fail(KA_ERR_BAD_ARG, "verify: null target_logits / draft_ids / uniforms / out_ids / out_accepted pointer");
     if (vocab < 1) return fail(KA_ERR_BAD_ARG, "verify: vocab %lld < 1", (long long)vocab);
-    if (vocab >= (int64_t(1) << 22))
+    if (vocab >= VERIFY_MAX_VOCAB)
         return fail(KA_ERR_UNSUPPORTED, "verify: vocab %lld >= 2^22 (integer masses would overflow)", (long long)vocab);
-    if (batch > 65535) return fail(KA_ERR_UNSUPPORTED, "verify: batch %lld > 65535", (long long)batch);
-    if (batch * (2 * max_draft + 1) >= (int64_t(1) << 32) / S_THREADS)
+    if (batch > VERIFY_MAX_BATCH) return fail(KA_ERR_UNSUPPORTED, "verify: batch %lld > %lld", (long long)batch, (long long)VERIFY_MAX_BATCH);
+    if (batch * (2 * max_draft + 1) >= VERIFY_MAX_ROWS)
         return fail(KA_ERR_UNSUPPORTED, "verify: %lld rows in one call", (long long)(batch * (2 * max_draft + 1)));
     // (a stride counts only where there is a second row to step to)
     if ((batch > 1 && target_batch_stride < vocab) || (max_draft > 0 && target_pos_stride < vocab))

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from rl_engine.kernels import _hip
 from rl_engine.kernels.registry import kernel_registry
 from rl_engine.kernels.sampling import SamplerBackend
 
@@ -35,3 +36,10 @@ def test_in_place_refuses_a_leaf_that_requires_grad():
     for base in (leaf, view):
         with pytest.raises(ValueError, match="leaf"):
             SamplerBackend().lora_linear(base, *args, inplace=True)
+
+
+def test_verify_workspace_query_refuses_what_the_call_refuses():
+    ws = _hip.load().ka_verify_workspace_bytes
+    assert ws(0, 65535, 1, 100) > 0 and ws(2, 4, 64, 100) > 0
+    assert ws(3, 4, 4, 100) == 0 and ws(-1, 4, 4, 100) == 0              # no such type
+    assert ws(0, 65536, 1, 100) == 0 and ws(0, 65535, 64, 100) == 0      # more requests, more rows than a call takes
