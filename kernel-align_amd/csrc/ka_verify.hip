@@ -242,8 +242,8 @@ struct HistRow {
     uint32_t bin[HIST_BINS];
     uint16_t tiny[TINY_CAP];
     uint32_t n_tiny, n_zero, give_up, dropped, first;
-    uint64_t sums[S_WAVES][2];  // per wavefront: mass of all entries, and of the small ones
-    double raw_sums[S_WAVES];   // sum of exp(x - max) over the unscaled row
+    uint64_t sums[S_WAVES][3];  // per wavefront: mass of all entries, of the small ones, and raw_fix of these
+    double raw_sums[S_WAVES];   // sum of exp(x - max) over the unscaled row's bins
     uint64_t win_mass[WINDOW];  // mass and scaled key of the positions from the first occupied one on
     uint32_t win_key[WINDOW];
     RowCut cut;
@@ -288,6 +288,11 @@ __device__ __forceinline__ uint64_t wave_sum_u64_of(uint64_t v) {
            uint32_t(__builtin_amdgcn_readlane(int(uint32_t(inc)), kWave - 1));
 }
 
+// exp(x - xmax) in 2^-40, rounded: sums of it do not depend on their order, and are off by V 2^-41 + 2^-22 of themselves.
+__device__ __forceinline__ uint64_t raw_fix(float x, float xmax) {
+    const double e = double(fast_exp2((x - xmax) * kLseLog2e)) + 4096.0;  // (its last bit is 2^-40)
+    return uint64_t(__double_as_longlong(e)) & 0x000fffffffffffffull;
+}
 // Counts the row into h.bin / h.tiny.  A barrier must follow.
 __device__ __forceinline__ void hist_count(HistRow &h, const uint16_t *rp, int vocab) {
     const int tid = threadIdx.x;
@@ -384,7 +389,7 @@ __device__ __forceinline__ bool hist_cut(HistRow &h, const uint16_t *rp, int voc
     // ---- masses: of all positions where a total is needed, else of the window -------------------
     const bool total = !f.use_k;
     {
-        uint64_t all = 0, mid = 0;
+        uint64_t all = 0, mid = 0, mid_raw = 0;
         double raw_sum = 0.0;
         // (without branches on empty bins, two at a time: the chain of fused multiply-adds is what takes the time)
         const int end = total ? HIST_POS : (first + WINDOW < HIST_POS ? first + WINDOW : HIST_POS);
@@ -410,15 +415,17 @@ __device__ __forceinline__ bool hist_cut(HistRow &h, const uint16_t *rp, int voc
                 const uint32_t c = i < int(n_tiny) ? 1u : n_zero;
                 const uint32_t raw = i < int(n_tiny) ? uint32_t(h.tiny[i]) : 0u;
                 if (total) mid += weight_of(key_of_raw(raw)) * c;
-                if (want_lse) raw_sum += double(float(c) * fast_exp2((Bf16::widen(uint16_t(raw)) - xmax) * kLseLog2e));
+                if (want_lse) mid_raw += raw_fix(Bf16::widen(uint16_t(raw)), xmax) * c;  // (integers: the list's order is the atomics')
             }
             all = wave_sum_u64_of(all);
             mid = wave_sum_u64_of(mid);
+            mid_raw = wave_sum_u64_of(mid_raw);
 #pragma unroll
             for (int off = 32; off >= 1; off >>= 1) raw_sum += __shfl_xor(raw_sum, off, kWave);
             if (lane == 0) {
                 h.sums[wave][0] = all;
                 h.sums[wave][1] = mid;
+                h.sums[wave][2] = mid_raw;
                 h.raw_sums[wave] = raw_sum;
             }
         }
@@ -429,15 +436,17 @@ __device__ __forceinline__ bool hist_cut(HistRow &h, const uint16_t *rp, int voc
         return h.ok != 0;
     }
     // ---- the first wavefront finishes the row --------------------------------------------------
-    uint64_t z_all = 0, z_mid = 0;
+    uint64_t z_all = 0, z_mid = 0, mid_raw = 0;
     double raw_sum = 0.0;
     if (total || want_lse)
         for (int w = 0; w < S_WAVES; ++w) {
             z_all += h.sums[w][0];
             z_mid += h.sums[w][1];
+            mid_raw += h.sums[w][2];
             raw_sum += h.raw_sums[w];
         }
     z_all += z_mid;
+    raw_sum += double(mid_raw) * 0x1p-40;
     const bool dropped = h.dropped != 0;
     uint32_t key_dropped = 0, key_tiny = 0, key_tiny_neg = 0;
     bool ok = true;
@@ -626,11 +635,6 @@ __device__ __forceinline__ float lower_edge(int bin) {
     return bin >= HIST_SIDE ? bin_value(bin) : __uint_as_float(__float_as_uint(bin_value(bin - 1)) - 1u);
 }
 
-// exp(x - xmax) in 2^-40, rounded: sums of it do not depend on their order, and are off by V 2^-41 + 2^-22 of themselves.
-__device__ __forceinline__ uint64_t raw_fix(float x, float xmax) {
-    const double e = double(fast_exp2((x - xmax) * kLseLog2e)) + 4096.0;  // (its last bit is 2^-40)
-    return uint64_t(__double_as_longlong(e)) & 0x000fffffffffffffull;
-}
 // The maxima at which the bins describe a row.
 __device__ __forceinline__ bool coarse_top(float xmax) { return (xmax >= 0x1p-11f || xmax <= -0x1p-11f) && xmax > -256.0f && xmax < 256.0f; }
 // Mass and raw_fix of entries of a row, and the bins' masses (added to `bins` where `use_p`).

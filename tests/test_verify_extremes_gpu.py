@@ -61,3 +61,26 @@ def test_uniforms_of_zero(sampler, dtype, kw):
     ids = torch.randint(0, 4100, (5, 2), generator=g)
     for q in (draft, None):
         _equal(sampler, target, ids, torch.zeros(5, 3), q, **kw)
+
+
+def test_log_probability_whatever_the_order_of_the_entries(sampler):
+    """Rows with some thousand entries next to zero, which the kernel collects in no fixed order: the same bits for every call and
+    for every order of the row's entries."""
+    g = torch.Generator().manual_seed(8)
+    vocab = 20000
+    row = torch.randn(24, vocab, generator=g) * 2
+    small = torch.rand(24, vocab, generator=g)
+    row = torch.where(small < 0.04, row * 1e-4, torch.where(small < 0.05, torch.zeros(()), row)).bfloat16()
+    token = torch.randint(0, vocab, (24, 1), generator=g)
+    want = None
+    for turn in range(6):
+        order = torch.stack([torch.randperm(vocab, generator=g) if turn > 1 else torch.arange(vocab) for _ in range(24)])
+        target = row.gather(1, order).unsqueeze(1).expand(24, 2, vocab).contiguous()
+        draft = (order == token).nonzero()[:, 1:]
+        ids, accepted, lp = sampler.verify_draft(target.cuda(), draft.cuda(), torch.zeros(24, 2).cuda(), return_policy_logprob=True)
+        assert (accepted == 1).all() and torch.equal(ids[:, :1].cpu(), draft)
+        want = lp[:, 0] if want is None else want
+        assert torch.equal(lp[:, 0], want)
+    rows = row.double()
+    exact = rows.gather(1, token).squeeze(1) - torch.logsumexp(rows, 1)
+    assert (want.cpu().double() - exact).abs().max().item() <= 2e-5
