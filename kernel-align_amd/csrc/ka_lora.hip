@@ -62,7 +62,7 @@ struct LoraPlan {          // device pointers into the workspace
 // lora_plan: one workgroup sorts the tokens.  Every wavefront takes a contiguous share of them: counts, a prefix over
 // (adapter, wavefront), then the ranks inside a step of 64 tokens from ballots.  The ids of eight steps are requested together.
 // One workgroup, since a sort over several would need launches of its own: bound by its chain of waits, 6 us for 777 tokens, 8 for
-// 2048, 14 for 5003.
+// 2048, 15 for 5003.
 // ---------------------------------------------------------------------------
 template <int PLAN_THREADS> struct PlanShared {
     int32_t at[PLAN_THREADS / kWave][MAX_ADAPTERS + 1];  // counts, then the next position of the wavefront's tokens
@@ -482,8 +482,8 @@ __device__ __forceinline__ float add_parts(float first, const float *__restrict_
 // partial result per segment (grid (segments, tiles)) where the tiles alone would leave CUs idle.  The bits of a token's u
 // do not depend on which of the two runs, nor on the other tokens.
 // ONE: a call of few tokens, one per workgroup, which need no plan; one more workgroup makes it for the kernel behind.
-// Bound by the reads of x and, with many adapters, of A: 64 tokens over 16 adapters of rank 16, H 4096: 5.5 us; 5003 tokens, rank 64
-// (fp16, 41 MB): 19 us, 2.2 TB/s.
+// Bound by the reads of x and, with many adapters, of A: 64 tokens over 16 adapters of rank 16, H 4096: 5.8 us; 5003 tokens, rank 64
+// (fp16, 41 MB): 22 us, 1.9 TB/s (data that no cache holds, here and below).
 // ---------------------------------------------------------------------------
 constexpr int SEG_STEPS = 32;  // steps of 32 per segment
 struct ShrinkArgs {
@@ -605,9 +605,10 @@ __global__ __launch_bounds__(THREADS) void lora_fold_rows(const float *__restric
 //
 // u enters as fragments (column = token, contraction index = rank) of its high and low bf16 parts, 17 bits of every entry.
 // They come packed from lora_pack_rows, or in calls of few tokens (PARTS) from the segments of lora_shrink.
-// Bound by memory, base in and out through: 64 tokens x 128,256 outputs, 16 adapters of rank 16 (99 MB): 19.5 us, 5.1 TB/s; 5003 tokens x
-// 4096, rank 64 (82 MB): 23 us, 3.5 TB/s.  Tiles of 32 tokens: at 64 an adapter with a few tokens left half of the products empty
-// and the registers let two workgroups reside instead of four.
+// Bound by memory, base in and out through: 64 tokens x 128,256 outputs, 16 adapters of rank 16 (99 MB): 26 us, 3.9 TB/s, fp16 29;
+// 5003 tokens x 4096, rank 64 (82 MB): 29 us, 2.8 TB/s, fp16 33.  Tiles of 32 tokens: at 64 an adapter with a few tokens left half of the
+// products empty and the registers let two workgroups reside instead of four.  The builds for aligned rows hold everything in
+// registers; those for any address spill up to 10 of them.
 // ---------------------------------------------------------------------------
 template <int RP> struct RowFragments {  // of 32 tokens, in uint4: [group of 16][step][high, low][lane]
     static constexpr int kSteps = Steps<RP>::kCount, kParts = RP <= 16 ? 1 : 2;
@@ -952,9 +953,9 @@ __global__ __launch_bounds__(THREADS) void lora_pack(PackArgs p) {
 // lora_bwd_out: grid (blocks of O, tiles).  One pass over dy: the tile's part of dB, and dy B over the block's outputs.
 // A wavefront owns 64 G outputs; per 32 tokens it reads them twice (once from HBM, once from cache): transposed for dB, as
 // they are for dy B.  What a step needs from HBM is requested a step ahead (two steps ahead measured slower: 301 -> 335 us below).
-// Bound by the wait for those rows with one wavefront per SIMD (rank 16 with G = 4, rank 64 and 128): 4096 tokens x 128,256 outputs,
-// rank 16 (1.05 GB): 301 us, 3.5 TB/s; 2048 x 4096: 12 us; rank 64, 1024 x 128,256: 201 us; rank 128, 512 x 128,256: 193 us, of which the
-// three products of the gradient's split take about 40.
+// Bound by the wait for those rows with one wavefront per SIMD (rank 16 with G = 4, rank 128; two at rank 64): 4096 tokens x 128,256
+// outputs, rank 16 (1.05 GB): 297 us, 3.5 TB/s; 2048 x 4096: 12 us; rank 64, 1024 x 128,256: 166 us; rank 128, 512 x 128,256: 180 us, of
+// which the three products of the gradient's split take about 40.
 // ---------------------------------------------------------------------------
 struct BwdOutArgs {
     const void *dy, *b;
@@ -1185,7 +1186,7 @@ __global__ __launch_bounds__(THREADS) void lora_bwd_out(BwdOutArgs p) {
 
 // ---------------------------------------------------------------------------
 // lora_bwd_in: grid (blocks of H, tiles).  One pass over x: the tile's part of dA, and dx = dx_base + du A.  Bound by memory:
-// 4096 tokens x 4096 (100 MB): 33 us, 3.0 TB/s; 2048 x 4096: 19.6 us.
+// 4096 tokens x 4096 (100 MB): 30 us, 3.3 TB/s; 2048 x 4096: 22 us.
 // ---------------------------------------------------------------------------
 struct BwdInArgs {
     const void *x, *a, *dx_base;

@@ -15,13 +15,14 @@
 // The acceptance is evaluated in those integers.  The draw is first evaluated in fp64, with a bound of its error: each P_i =
 // W^p_i / Z^p is off by 3 * 2^-53 of itself, R_i by 2^-51 (P_i + Q_i), and a sum of them, added in runs and trees of fewer than
 // 2^12 terms, by 2^-41 in all (P and Q sum to one).  An entry whose prefix sums lie more than DRAW_MARGIN = 2^-38 on either side of u R is the
-// integers' answer too; otherwise (about one draw in 10^6, and u = 0) the workgroup repeats the draw in 128-bit integers.
+// integers' answer too; otherwise (about one draw in 10^6, and u = 0) the workgroup repeats the draw in 128-bit integers, two passes over the
+// row by one workgroup: 64 requests x 4 drafts with u = 0 everywhere take 215 us instead of 80 with top-k and 480 instead of 91 without.
 //
 // Three launches, five where rows are split, no host synchronisation:
 //   verify_split_top, verify_split_mass   few fp16 / fp32 rows without top-k only: maxima and masses by several workgroups per row
 //   verify_rows    one workgroup per row that counts (target rows 0 .. len, draft rows 0 .. len - 1): the cut of the row's
 //                  distribution, its total mass, the draft token's mass, the log-sum-exp of the raw row.  This is the pass over
-//                  the data: bound by HBM, 2 V (2 K + 1) bytes per request.
+//                  the data, 2 V (2 K + 1) bytes per request.
 //   verify_shares  residual mass of every share of 256 vectors of the stopping position, a wavefront each
 //   verify_draw    one workgroup per request: the share, the vector and the entry that hold the draw; all outputs
 // Where top-p cuts inside a group of equal logits, the first r of the group survive, in index order.  verify_shares cannot know
@@ -227,8 +228,11 @@ template <typename T> __device__ __forceinline__ float cut_value(uint32_t raw_cu
 // ordinary maximum.  Masses are then evaluated once per occupied bin instead of once per entry (by all threads where a sum
 // over the whole row is needed), and one wavefront walks the bins from the largest value down to the cuts, 64 at a time.  Rows
 // it cannot describe (values of 2^8 and above, NaN, a maximum or a cut among the small values, dropped values that would
-// count) take the radix path.  Measured, bf16, 128,256 entries: 576 rows (64 requests x 4 drafts, 148 MB) 50 - 52 us, 2.9 TB/s, of which
-// the stream takes about 30 and the masses and the walk behind it, which all rows reach together, the rest; 2304 rows, ragged: 109 us.
+// count) take the radix path.  Measured, bf16, 128,256 entries: 576 rows (64 requests x 4 drafts, 148 MB) 50 us, 2.9 TB/s, of which
+// the stream takes about 30 (an atomic on LDS per entry) and the masses and the walk behind it, which all rows reach together, the rest;
+// 2304 rows, of which about 56 % count: 106 us.  (A plain read of the 148 MB takes 21 us, and the sampling operator's short top-k route summarises
+// 512 such rows in 28: most entries that are counted here do not survive.)  At the six wavefronts per SIMD that let three bf16
+// workgroups share a CU, 30 registers are spilled; the fp16 and fp32 builds have 56 KB of LDS, two workgroups a CU.
 // ---------------------------------------------------------------------------
 constexpr uint32_t MAG_LOW = 0x3A00u, MAG_HIGH = 0x4380u;  // bits of 2^-11 and 2^8
 constexpr int HIST_SIDE = int(MAG_HIGH - MAG_LOW);         // values of one sign: 19 octaves of 128
@@ -930,11 +934,13 @@ __device__ __forceinline__ RowRef row_ref(const VerifyParams &p, int64_t r) {
 // fp16 and fp32 rows without top-k, in calls of few rows: the maximum, then the masses (which are 60 instructions an entry: one
 // CU takes 50 us for a row of 128,256), by a workgroup per 32 KB of every row.  grid (rows, parts) each; verify_rows goes on from the
 // bins.  8 requests x 2 drafts, fp32, top-p 0.9, 128,256 entries: 134 us in verify_rows alone, 6 + 26 + 26
-// us so; verify_split_mass is bound by its arithmetic.
+// us so.  What bounds verify_split_mass was not measured: its 60 instructions an entry would take about a third of its time, 64-bit LDS
+// atomics on the few bins that hold most entries, and 39 KB of bins cleared and added per 32 KB of the row, are the rest of what it does.
 // ---------------------------------------------------------------------------
 constexpr int SPLIT_BYTES = 32768;
 // Up to how many rows: fp32, top-p 0.9, 128,256 entries, a call of 5 / 40 / 120 / 250 rows: 156 / 165 / 175 / 187 us by a workgroup per
 // row, 70 / 95 / 136 / 200 us split; fp16, 50,257 entries: 83 / 105 / 105 / 112 and 67 / 90 / 99 / 124 us.
+// (Counted as if every draft had logits: the workspace query does not know.  Looked-up drafts stop being split at little more than half as many rows.)
 constexpr int64_t SPLIT_ROWS = 160;
 template <typename T> __device__ __forceinline__ int split_span(const VerifyParams &p, int &first) {
     first = int(blockIdx.y) * p.split_entries;
@@ -1307,7 +1313,7 @@ __global__ __launch_bounds__(SHARE_THREADS) void verify_shares(VerifyParams p) {
 // The same for bf16 rows of which many entries survive (no top-k, or a large one): the masses come from two tables in LDS, one
 // value per bin of verify_rows, so that an entry costs two reads of LDS instead of two evaluations of the mass polynomial.
 // Entries outside the bins (about one in 10^4) are evaluated.  A workgroup builds the tables (9728 evaluations) for
-// shares_per_group shares.  grid (groups, B)  64 requests, two rows of 128,256 each (66 MB): 26 us, a third of it the tables.
+// shares_per_group shares.  grid (groups, B).  64 requests, two rows of 128,256 each (33 MB): 25 us, 1.3 TB/s, a third of it the tables.
 constexpr int TABLE_THREADS = 512;
 constexpr size_t TABLE_LDS_BYTES = size_t(2) * HIST_BINS * sizeof(double);
 __global__ __launch_bounds__(TABLE_THREADS) void verify_shares_table(VerifyParams p) {

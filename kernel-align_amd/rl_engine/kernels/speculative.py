@@ -34,11 +34,14 @@ class SpeculativeOps:
         K = 0 is ``sample``.
 
         Both rows of a position are taken through the same temperature -> top-k -> top-p as in ``sample`` (scalars, or [B]
-        tensors of per-request values, where a top_k of 0 filters nothing): P from the target, Q from the draft (one-hot without draft logits).  Draft j is
-        accepted iff ``uniforms[:, j] * Q(d) < P(d)``; the first position that is not is redrawn from max(P - Q, 0), and
-        when all are accepted the position behind them is drawn from P, both by the inverse CDF in index order that
-        ``uniforms[:, K]`` drives.  All of it is decided on the sampling operator's integer masses: the ids are a function of the
-        request alone.  uniforms: fp32 [B, K + 1] in [0, 1); None takes them from ``torch.rand(generator=generator)``.
+        tensors of per-request values, where a top_k of 0 filters nothing): P from the target, Q from the draft (one-hot without
+        draft logits).  There is one set of parameters, one dtype and one vocabulary for both models: a drafter that sampled at
+        another temperature or with other filters is not described by Q exactly (scale its logits beforehand, which rounds them;
+        or draft under the target's parameters).  Draft j is accepted iff ``uniforms[:, j] * Q(d) < P(d)``; the first position that
+        is not is redrawn from max(P - Q, 0), and when all are accepted the position behind them is drawn from P, both by the
+        inverse CDF in index order that ``uniforms[:, K]`` drives.  All of it is decided on the sampling operator's integer masses:
+        the ids are a function of the request alone.  uniforms: fp32 [B, K + 1] in [0, 1) (a last one of exactly 0 costs the
+        request two serial passes over a row in 128-bit integers); None takes them from ``torch.rand(generator=generator)``.
         A draft id outside [0, V) has P = 0 and is never accepted.  (A draft that Q cannot have drawn may leave no residual,
         where P = Q: the token then comes from P.)
 
