@@ -40,7 +40,7 @@ def _raw_stream() -> int:
 def to_rows(values: torch.Tensor, device, dtype) -> torch.Tensor:
     """Per-row parameters in the type the kernels read.  Integers beyond 32 bits become the largest that fit, instead of what their
     low bits say (a top_k beyond the vocabulary filters nothing, however large)."""
-    if dtype == torch.int32 and values.dtype != torch.int32:
+    if dtype == torch.int32 and values.dtype in (torch.int64, torch.uint32, torch.uint64):
         limits = torch.iinfo(torch.int32)
-        values = values.clamp(limits.min, limits.max)
+        values = values.to(torch.int64).clamp(limits.min, limits.max)
     return values.to(device=device, dtype=dtype).contiguous()

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from rl_engine.kernels import _hip
+from rl_engine.kernels._launch import to_rows
 from rl_engine.kernels.registry import kernel_registry
 from rl_engine.kernels.sampling import SamplerBackend
 
@@ -43,3 +44,17 @@ def test_verify_workspace_query_refuses_what_the_call_refuses():
     assert ws(0, 65535, 1, 100) > 0 and ws(2, 4, 64, 100) > 0
     assert ws(3, 4, 4, 100) == 0 and ws(-1, 4, 4, 100) == 0              # no such type
     assert ws(0, 65536, 1, 100) == 0 and ws(0, 65535, 64, 100) == 0      # more requests, more rows than a call takes
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.int16, torch.uint8, torch.uint16, torch.uint32, torch.uint64, torch.float32,
+                                   torch.float16])
+def test_row_parameters_of_every_type(dtype):
+    """Small values as they are, in any type; those beyond 32 bits as the largest that fit."""
+    got = to_rows(torch.tensor([0, 5, 100], dtype=torch.int64).to(dtype), torch.device("cpu"), torch.int32)
+    assert got.dtype == torch.int32 and got.tolist() == [0, 5, 100]
+    if dtype in (torch.int64, torch.uint32):
+        big = torch.tensor([(1 << 31) + 5, 7], dtype=torch.int64).to(dtype)
+        assert to_rows(big, torch.device("cpu"), torch.int32).tolist() == [(1 << 31) - 1, 7]
+    if dtype == torch.int64:
+        wide = torch.tensor([(1 << 32) + 5, -(1 << 40)])
+        assert to_rows(wide, torch.device("cpu"), torch.int32).tolist() == [(1 << 31) - 1, -(1 << 31)]
