@@ -28,7 +28,6 @@ namespace {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -245,35 +244,21 @@ template <typename T> __device__ __forceinline__ void as_bf16(const uint4 &f, ui
     if constexpr (T::kDtype == KA_DTYPE_BF16) {
         part[0] = f;
     } else {
-        // an fp16 without its last three bits has the 8 that a bf16 holds; the difference has three, and fp16's subtraction is exact
-        const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+        // an fp16 has 11 bits: the 8 of its first half as fp32, and the 3 that are left, which fp32's subtraction gives exactly
+        float v[8];
+        F16::unpack(f, v);
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const f16x2 h = __builtin_bit_cast(f16x2, w[j] & 0xfff8fff8u), l = __builtin_bit_cast(f16x2, w[j]) - h;
-            hi[j] = __builtin_amdgcn_perm(__float_as_uint(float(h[1])), __float_as_uint(float(h[0])), 0x07060302u);
-            lo[j] = __builtin_amdgcn_perm(__float_as_uint(float(l[1])), __float_as_uint(float(l[0])), 0x07060302u);
+            const uint32_t a = __float_as_uint(v[2 * j]), b = __float_as_uint(v[2 * j + 1]);
+            hi[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            lo[j] = __builtin_amdgcn_perm(__float_as_uint(v[2 * j + 1] - high_half(b)), __float_as_uint(v[2 * j] - high_half(a)), 0x07060302u);
         }
         part[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         part[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
 }
 
-// The leading part of each entry: 0 where the entry is, of its sign, infinite or no number where it is.
-template <typename T> __device__ __forceinline__ uint4 leading(const uint4 (&part)[Parts<T>::kCount]) {
-    if constexpr (T::kDtype == KA_DTYPE_BF16) {
-        return part[0];
-    } else {  // (of the smallest fp16 only the second part is left)
-        const uint32_t h[4] = {part[0].x, part[0].y, part[0].z, part[0].w}, l[4] = {part[1].x, part[1].y, part[1].z, part[1].w};
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t low = (h[j] & 0x7fffu) != 0 ? h[j] : l[j], high = (h[j] & 0x7fff0000u) != 0 ? h[j] : l[j];
-            w[j] = (low & 0xffffu) | (high & 0xffff0000u);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-}
 // Whether a sum of some lane of the wavefront is not finite (the same in every lane).
 __device__ __forceinline__ bool any_odd(const f32x4 (&acc)[4]) {
     float odd[4];  // (four chains: one of sixteen is waited for)
@@ -828,7 +813,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 3
                             if constexpr (PARTS) f = uf[((s0 + s) * KS + ks) * HL * kWave + lane];
                             else f = p.packed[int64_t(blockIdx.y) * RowFragments<RP>::kTotal + ((s0 + s) * KS + ks) * HL * kWave + lane];
                             as_bf16<T>(b_fragment(o0, ks, e), part);  // (read again, so that the products above need not keep it)
-                            kind = mfma<Bf16>(first_entries(leading<T>(part), ranks), first_entries(f, ranks), kind);
+                            kind = mfma<Bf16>(first_entries(part[0], ranks), first_entries(f, ranks), kind);
                         }
                         leading_kind(acc[s][e], kind);
                     }
@@ -1001,7 +986,7 @@ __device__ __forceinline__ void gradient_kind(f32x4 (&acc)[4], int count, const 
             uint4 frag[4], part[Parts<T>::kCount];
             transpose(w, frag);
             as_bf16<T>(frag[e], part);
-            kind = mfma<Bf16>(leading<T>(part), v[int64_t(c / 32) * step], kind);
+            kind = mfma<Bf16>(part[0], v[int64_t(c / 32) * step], kind);
         }
         leading_kind(acc[e], kind);
     }
@@ -1289,7 +1274,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(RP <= 1
 #pragma unroll
                         for (int ks = 0; ks < KS; ++ks) {
                             const int ranks = RP <= 16 && quad >= 2 ? 0 : 8;  // (with R <= 16 the second half of the lanes holds low parts)
-                            kind = mfma<Bf16>(first_entries(leading<T>(fa[ks][e]), ranks),
+                            kind = mfma<Bf16>(first_entries(fa[ks][e][0], ranks),
                                               first_entries(pu[Packed<RP>::kColumns + (s * KS + ks) * HL * kWave], ranks), kind);
                         }
                         leading_kind(sum[e], kind);

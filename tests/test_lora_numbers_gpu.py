@@ -81,7 +81,7 @@ def test_infinities_of_the_definition(sampler, dtype, n, h, o, r):
 @pytest.mark.parametrize("n", [3, 600])
 @pytest.mark.parametrize("r", [1, 40])
 def test_infinities_beside_the_smallest_numbers(sampler, n, r):
-    """The smallest fp16 numbers are all in the second of their two parts: an infinity times them is one all the same."""
+    """An infinity times the smallest fp16 numbers is one all the same."""
     tiny, inf = 2.0 ** -24, float("inf")
     full = lambda v, *shape: torch.full(shape, v, dtype=torch.float16)  # noqa: E731
     c = dict(base=full(0.0, n, 24), hidden=full(3 * tiny, n, 16), a=full(-tiny, 1, r, 16), b=full(5 * tiny, 1, 24, r),
@@ -115,6 +115,22 @@ def test_infinities_in_front_of_a_wide_output(sampler):
         want, _ = lora_ref.backward(dy, hidden, a, b, ids, scaling, u, None)
     for x, w, what in zip(got, want, ("dhidden", "dlora_a", "dlora_b")):
         _kinds(x, w.cpu(), what)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_gradients_of_the_smallest_numbers(sampler, dtype, n):
+    """dy and hidden of a few steps of fp16's smallest number, one token or a few: every product counts to its last bit."""
+    c = _inputs(n, 72, 136, 12, 2, dtype, seed=n, ids=torch.arange(n) % 2)
+    g = torch.Generator().manual_seed(n)
+    for name in ("dy", "hidden"):
+        c[name] = (torch.randint(-40, 41, c[name].shape, generator=g) * 2.0 ** -24).to(dtype)
+    u = torch.randn(n, 12, generator=g)
+    d = {k: v.cuda() for k, v in c.items()}
+    got = sampler.lora_linear_backward(d["dy"], d["hidden"], d["a"], d["b"], d["ids"], d["scaling"], u.cuda(), d["dx"])
+    want, bound = lora_ref.backward(c["dy"], c["hidden"], c["a"], c["b"], c["ids"], c["scaling"], u, c["dx"])
+    for x, w, e, what in zip(got, want, bound, ("dhidden", "dlora_a", "dlora_b")):
+        _within(x, w, e, what)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
