@@ -84,3 +84,22 @@ def test_log_probability_whatever_the_order_of_the_entries(sampler):
     rows = row.double()
     exact = rows.gather(1, token).squeeze(1) - torch.logsumexp(rows, 1)
     assert (want.cpu().double() - exact).abs().max().item() <= 2e-5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_log_probabilities_of_rows_far_from_zero(sampler, dtype):
+    """Rows whose maximum is some hundreds or thousands, of either sign: to 1e-5 what compute_logp returns, so that a ratio of the two is
+    one.  (Both multiply by log2(e) as fp32 and by ln(2) at the end, whose product is off from 1 by 1.3e-8 < 2^-26: against fp64 they are
+    off by that much of the row's maximum, beside the tolerance of rows near zero.)"""
+    g = torch.Generator().manual_seed(12)
+    for top in (300.0, 2000.0, 20000.0, -300.0, -2000.0, -20000.0):
+        for vocab in (1, 2, 700, 5000):
+            step = 2.0 ** (torch.tensor(abs(top)).log2().floor() - (7 if dtype == torch.bfloat16 else 10))  # of the type, there
+            target = (top - step * torch.randint(0, 6, (5, 2, vocab), generator=g)).to(dtype)
+            ids = target[:, :1].float().argmax(-1)
+            got = sampler.verify_draft(target.cuda(), ids.cuda(), torch.zeros(5, 2).cuda(), return_policy_logprob=True)
+            assert torch.equal(got[0][:, :1].cpu(), ids)
+            rows = target.double()
+            want = rows.gather(2, got[0].cpu().unsqueeze(2)).squeeze(2) - torch.logsumexp(rows, 2)
+            assert (got[2].cpu().double() - want).abs().max().item() <= 2e-5 + 2.0 ** -26 * abs(top)
+            assert (got[2] - sampler.compute_logp(target.cuda(), got[0])).abs().max().item() <= 1e-5
